@@ -495,11 +495,13 @@ def triu(t, diagonal=0): return _op(b"triu", [_t(t)], i=(int(diagonal),))
 def tril(t, diagonal=0): return _op(b"tril", [_t(t)], i=(int(diagonal),))
 
 
+_ACTS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 2, "gelu_exact": 3}
+
+
 def linear(x, weight, bias=None, activation=None):
     """y = act(x @ weight^T + bias) in one GEMM (weight in torch layout [out, in])."""
-    acts = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 2, "gelu_exact": 3}
     ins = [_t(x), _t(weight)] + ([_t(bias)] if bias is not None else [])
-    return _op(b"linear", ins, i=(acts[activation],))
+    return _op(b"linear", ins, i=(_ACTS[activation],))
 
 
 # backward helpers
@@ -639,6 +641,55 @@ def linear_int8(x, q, scale):
     return _op(b"linear_int8", [_t(x), _t(q), _t(scale)])
 
 
+def quantize_int4(w, group=128):
+    """W [out, in] (float32, float16 or bfloat16) in 4 bits with a scale for
+    each row and group of 32, 64 or 128 columns: (packed uint8 [ceil(out / 16),
+    ceil(in / 128), 64, 16], scales [ceil(in / group), out] of W's dtype).
+    scale = the group's largest magnitude / 7, rounded to that dtype; codes =
+    W / scale, rounded half to even, within -7 .. 7.  Packed tiles hold 16
+    rows by 128 columns: byte run l the 32 codes of row l % 16 from column
+    32 (l // 16) on, eight codes to each 4 bytes, as code + 8, nibble j
+    (lowest first) code 2 j for j < 4 and code 2 (j - 4) + 1 for the others."""
+    return _op(b"quantize_int4", [_t(w)], i=(int(group),), nout=2)
+
+
+def dequantize_int4(packed, scales, in_features, group=128):
+    """The values [out, in_features] that 4-bit weights stand for, in the
+    scales' dtype."""
+    return _op(b"dequantize_int4", [_t(packed), _t(scales)], i=(int(in_features), int(group)))
+
+
+def linear_int4(x, packed, scales, bias=None, activation=None, group=128):
+    """y = act(x @ W^T + bias) with the 4-bit weights of quantize_int4(W,
+    group): x [..., in] of the scales' dtype, any number of rows, summed in
+    float32.  Decode steps and prompts take the same call."""
+    if activation not in _ACTS:
+        raise ValueError(f"linear_int4: unknown activation {activation!r}")
+    ins = [_t(x), _t(packed), _t(scales)] + ([_t(bias)] if bias is not None else [])
+    return _op(b"linear_int4", ins, i=(int(group), _ACTS[activation]))
+
+
+def token_logprobs(logits, tokens, top_k=0):
+    """Of logits [..., V] and the tokens [...] (int32 or int64) that were
+    given or picked: (logprobs, entropy, lse), float32 [...], where logprobs =
+    log softmax(logits)[token], entropy is that of the whole distribution and
+    lse = log sum exp(logits); with top_k (up to 32) also (top_logprobs
+    float32, top_ids int32), [..., top_k], the most likely tokens in order,
+    equal logits by index.  A token outside [0, V) (padding) has logprob 0.  A
+    row of -inf only has lse and logprobs -inf and entropy 0; one with NaN or
+    +inf gives NaN."""
+    return _op(b"token_logprobs", [_t(logits), _t(tokens)], i=(int(top_k),), nout=5 if top_k else 3)
+
+
+def token_logprobs_backward(grad_logprobs, grad_entropy, logits, tokens, entropy, lse):
+    """The gradient with respect to the logits, in their dtype, of
+    token_logprobs' logprobs and entropy, from their gradients (float32 [...];
+    grad_entropy may be None) and the entropy and lse it returned.  Rows whose
+    token is outside [0, V) get the entropy's part only."""
+    ins = [_t(grad_logprobs), _t(logits), _t(tokens), _t(entropy), _t(lse)]
+    return _op(b"token_logprobs_backward", ins + ([_t(grad_entropy)] if grad_entropy is not None else []))
+
+
 def blit_copy(src, dst):
     """dst = src on the device, at once; dst may be a view (a slice of a
     larger tensor, any strides), which is then written in place."""
@@ -679,6 +730,44 @@ def decode_attention(q, k_cache, v_cache, lens, k_new=None, v_new=None):
     if k_new is not None or v_new is not None:
         ins += [_t(k_new), _t(v_new)]
     return _op(b"decode_attention", ins)
+
+
+def kv_write_int8(k_codes, k_scales, v_codes, v_scales, k_rows, v_rows, pos, block=16):
+    """kv_write_pair for a cache held in 8 bits, in place, at once: codes int8
+    [B, H, Tmax, D] (D 32, 64 or 128) and a float32 scale for each head and
+    block of 16, 32, 64 or 128 rows, [B, H, ceil(Tmax / block)]; value = code *
+    scale.
+
+    Rows [B, H, T, D] become cache rows pos[b] .. pos[b] + T; what the cache
+    held from row pos[b] on is dropped.  A block's scale is its largest
+    magnitude / 127.  The rows that the first touched block holds before
+    pos[b] keep their values, to half a step of its scale where that grows.  A
+    block given an infinity or NaN reads as NaN.  Rows that would land outside
+    the cache are not written."""
+    ids = [_t(t)._id for t in (k_codes, k_scales, v_codes, v_scales, k_rows, v_rows, pos)]
+    if lib.applegpu_kv_write_int8(*ids, int(block)) != 0:
+        raise ValueError(ffi_error())
+
+
+def kv_read_int8(k_codes, k_scales, v_codes, v_scales, pos, rows, block=16, dtype="float32"):
+    """(K, V) rows pos[b] .. pos[b] + rows of an 8-bit cache as values,
+    [B, H, rows, D] each; zeros for rows outside the cache."""
+    return _op(b"kv_read_int8", [_t(k_codes), _t(k_scales), _t(v_codes), _t(v_scales), _t(pos)],
+               i=(int(rows), int(block), DTYPE_CODES[canon_dtype(dtype)]), nout=2)
+
+
+def decode_attention_int8(q, k_codes, k_scales, v_codes, v_scales, lens, block=16, scale=None, k_new=None, v_new=None):
+    """decode_attention over a cache held in 8 bits (kv_write_int8): q [B, Hq,
+    Tq, D], the caches' H heads each serving Hq / H query heads in a row; query
+    row i of sequence b sees cache rows j <= lens[b] - Tq + i, and a row that
+    sees none gets zeros.  The softmax scale is 1 / sqrt(D) by default.
+
+    k_new, v_new ([B, H, 1, D], Tq = 1): the step's own K and V rows, appended
+    as row lens[b] - 1 when the result is evaluated, before it attends."""
+    ins = [_t(q), _t(k_codes), _t(k_scales), _t(v_codes), _t(v_scales), _t(lens)]
+    if k_new is not None or v_new is not None:
+        ins += [_t(k_new), _t(v_new)]
+    return _op(b"decode_attention_int8", ins, f=() if scale is None else (float(scale),), i=(int(block),))
 
 
 # ── graph capture ────────────────────────────────────────────────────────────

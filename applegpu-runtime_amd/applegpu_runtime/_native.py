@@ -105,6 +105,7 @@ _SIGS = {
     "applegpu_ffi_inject_alloc_failures": (None, [c_int32]),
     "applegpu_kv_write": (c_int32, [c_uint64, c_uint64, c_uint64]),
     "applegpu_kv_write_pair": (c_int32, [c_uint64, c_uint64, c_uint64, c_uint64, c_uint64]),
+    "applegpu_kv_write_int8": (c_int32, [c_uint64] * 7 + [c_int64]),
     "applegpu_capture_begin": (c_int32, []),
     "applegpu_capture_end": (c_int64, []),
     "applegpu_capture_abort": (c_int32, []),

@@ -295,6 +295,16 @@ int32_t applegpu_kv_write_pair(uint64_t k_cache_id, uint64_t v_cache_id, uint64_
   });
 }
 
+int32_t applegpu_kv_write_int8(uint64_t k_codes_id, uint64_t k_scales_id, uint64_t v_codes_id, uint64_t v_scales_id,
+                               uint64_t k_rows_id, uint64_t v_rows_id, uint64_t pos_id, int64_t block) {
+  return guarded<int32_t>(kFfi, -1, [&]() -> int32_t {
+    TensorP kr = kv_operand(k_rows_id), vr = kv_operand(v_rows_id), pos = kv_operand(pos_id);
+    ops::kv_write_int8({kv_cache_operand(k_codes_id), kv_cache_operand(k_scales_id), kv_cache_operand(v_codes_id),
+                        kv_cache_operand(v_scales_id), block}, kr, vr, pos);
+    return 0;
+  });
+}
+
 uint8_t* applegpu_ffi_add_out(uint64_t a, uint64_t b, uint64_t* o) { return lazy_out("add", {a, b}, {}, o); }
 uint8_t* applegpu_ffi_mul_out(uint64_t a, uint64_t b, uint64_t* o) { return lazy_out("mul", {a, b}, {}, o); }
 uint8_t* applegpu_ffi_sub_out(uint64_t a, uint64_t b, uint64_t* o) { return lazy_out("sub", {a, b}, {}, o); }

@@ -36,6 +36,8 @@ enum Op : int {
   OP_EMBEDDING_BACKWARD, OP_PACK_WEIGHT_X3, OP_PACK_ROWS_X3, OP_MATMUL_PP, OP_ROW_STATS_X3, OP_MATMUL_PP_NORM,
   OP_LINEAR_BACKWARD_SGD, OP_LINEAR_MSE_BACKWARD_SGD, OP_MLP2_SGD_STEP, OP_LINEAR_BACKWARD_SGD_PAIR,
   OP_LINEAR_RELU_MSE_BACKWARD_SGD, OP_ATTENTION_BACKWARD, OP_LAYER_NORM_STATS,
+  OP_KV_READ_INT8, OP_DECODE_ATTENTION_INT8, OP_QUANTIZE_INT4, OP_DEQUANTIZE_INT4, OP_LINEAR_INT4,
+  OP_TOKEN_LOGPROBS, OP_TOKEN_LOGPROBS_BACKWARD,
   OP_COUNT
 };
 
@@ -58,6 +60,8 @@ static const char* kNames[OP_COUNT] = {
     "embedding_backward", "pack_weight_x3", "pack_rows_x3", "matmul_pp", "row_stats_x3", "matmul_pp_norm",
     "linear_backward_sgd_", "linear_mse_backward_sgd_", "mlp2_sgd_step_", "linear_backward_sgd_pair_",
     "linear_relu_mse_backward_sgd_", "attention_backward", "layer_norm_stats",
+    "kv_read_int8", "decode_attention_int8", "quantize_int4", "dequantize_int4", "linear_int4",
+    "token_logprobs", "token_logprobs_backward",
 };
 
 int op_code(const char* name) {
@@ -77,7 +81,9 @@ int op_code(const char* name) {
 const char* op_name(int code) { return code >= 0 && code < OP_COUNT ? kNames[code] : "?"; }
 int op_outputs(int code) {
   if (code == OP_LAYER_NORM_GRADS || code == OP_ATTENTION_BACKWARD || code == OP_LAYER_NORM_STATS) return 3;
-  return code == OP_QUANTIZE_PER_ROW || code == OP_MSE_LOSS_GRAD ? 2 : 1;
+  if (code == OP_TOKEN_LOGPROBS) return 3;  // 5 with alternatives
+  return code == OP_QUANTIZE_PER_ROW || code == OP_MSE_LOSS_GRAD || code == OP_KV_READ_INT8 || code == OP_QUANTIZE_INT4
+             ? 2 : 1;
 }
 
 static void need(const std::vector<TensorP>& in, size_t n, int code) {
@@ -236,6 +242,34 @@ std::vector<TensorP> run_op(int code, const std::vector<TensorP>& in, const std:
       if (in.size() == 6) return {decode_attention(in[0], in[1], in[2], in[3], in[4], in[5])};
       need(in, 4, code);
       return {decode_attention(in[0], in[1], in[2], in[3])};
+    case OP_KV_READ_INT8:
+      // (k_codes, k_scales, v_codes, v_scales, pos); iv: rows, block, dtype
+      need(in, 5, code);
+      return kv_read_int8({in[0], in[1], in[2], in[3], ip(iv, 1, code)}, in[4], ip(iv, 0, code),
+                          dt_param(ip(iv, 2, code)));
+    case OP_DECODE_ATTENTION_INT8: {
+      // (q, k_codes, k_scales, v_codes, v_scales, lens[, k_new, v_new]); iv:
+      // block; f: the softmax scale (default 1/sqrt(D))
+      if (in.size() != 8) need(in, 6, code);
+      const float scale = !f.empty() ? (float)f[0]
+                          : in[0]->ndim == 4 ? 1.0f / std::sqrt((float)in[0]->shape[3]) : 1.f;
+      return {decode_attention_int8(in[0], {in[1], in[2], in[3], in[4], ip(iv, 0, code)}, in[5], scale,
+                                    in.size() == 8 ? in[6] : nullptr, in.size() == 8 ? in[7] : nullptr)};
+    }
+    case OP_QUANTIZE_INT4: need(in, 1, code); return quantize_int4(in[0], ip(iv, 0, code));
+    case OP_DEQUANTIZE_INT4:
+      need(in, 2, code);
+      return {dequantize_int4(in[0], in[1], ip(iv, 0, code), ip(iv, 1, code))};
+    case OP_LINEAR_INT4:
+      // (x, packed, scales[, bias]); iv: group, activation
+      if (in.size() != 4) need(in, 3, code);
+      return {linear_int4(in[0], in[1], in[2], in.size() == 4 ? in[3] : nullptr, ip(iv, 0, code),
+                          (int)ip(iv, 1, code))};
+    case OP_TOKEN_LOGPROBS: need(in, 2, code); return token_logprobs(in[0], in[1], ip(iv, 0, code));
+    case OP_TOKEN_LOGPROBS_BACKWARD:
+      // (grad_logprobs, logits, tokens, entropy, lse[, grad_entropy])
+      if (in.size() != 6) need(in, 5, code);
+      return {token_logprobs_backward(in[0], in.size() == 6 ? in[5] : nullptr, in[1], in[2], in[3], in[4])};
     case OP_PACK_WEIGHT: need(in, 1, code); return {pack_weight(in[0])};
     case OP_PACK_WEIGHT_X3: need(in, 1, code); return {pack_weight_x3(in[0])};
     case OP_MATMUL_PACKED: need(in, 2, code); return {matmul_packed(in[0], in[1], ip(iv, 0, code))};

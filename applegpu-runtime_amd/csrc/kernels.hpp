@@ -476,6 +476,101 @@ struct KvWrite {
   const int32_t* pos = nullptr;
 };
 void kv_write(const KvWrite& a, hipStream_t s);
+// ── cache in 8 bits ───────────────────────────────────────────────────────
+// A K or V cache held as int8 codes [B, H, Tmax, D] with one fp32 scale per
+// (sequence, head, block of `block` consecutive rows): value = code * scale.
+// Strides: codes (batch, head, row), scales (batch, head, block), unit stride
+// along D; every codes row starts at a 16-byte boundary.
+struct Int8Cache {
+  int8_t* codes = nullptr; int64_t cs[3] = {0, 0, 0};
+  float* scales = nullptr; int64_t ss[3] = {0, 0, 0};
+};
+// Rows pos[b] .. pos[b] + T of the K and the V cache = rows [B, H, T, D] of
+// dtype dt (strides batch, head, token; 16-byte aligned rows), one launch.
+// A block's scale is its largest magnitude / 127; the rows that the first
+// touched block holds before pos[b] keep their values, to half a step of a
+// scale that grows.  Rows outside [0, Tmax) are dropped.  pos is int32 [B] in
+// device memory, pos_off is added to it.
+struct KvInt8 {
+  DType dt = DType::F16;
+  int64_t B = 1, H = 1, T = 0, D = 0, Tmax = 0;
+  int block = 16;
+  Int8Cache c[2];
+  const void* x[2] = {nullptr, nullptr}; int64_t xs[2][3] = {{0, 0, 0}, {0, 0, 0}};
+  const int32_t* pos = nullptr;
+  int pos_off = 0;
+};
+bool kv_int8_supported(int64_t D, int64_t block);
+void kv_write_int8(const KvInt8& a, hipStream_t s);
+// y[j] = the values of rows pos[b] .. pos[b] + T of cache j, contiguous
+// [B, H, T, D] of dtype dt, zeros for rows outside [0, Tmax).
+void kv_read_int8(const KvInt8& a, void* const y[2], hipStream_t s);
+// softmax(q K^T scale) V of q [B, H * G, Tq, D] over such caches of H heads
+// (query head h reads cache head h / G); query row i of sequence b sees rows
+// j <= lens[b] - Tq + i, and zeros come out where it sees none.
+struct DecodeInt8 {
+  DType dt = DType::F16;
+  int64_t B = 1, H = 1, G = 1, Tq = 1, Tmax = 0, D = 0;
+  int block = 16;
+  const void* q = nullptr; int64_t q_sb = 0, q_sh = 0, q_st = 0;  // 16-byte aligned rows
+  Int8Cache k, v;
+  void* o = nullptr; int64_t o_sb = 0, o_sh = 0, o_st = 0;
+  const int32_t* lens = nullptr;
+  float scale = 1.f;
+};
+size_t decode_int8_ws_bytes(const DecodeInt8& a);
+void decode_attention_int8(const DecodeInt8& a, void* ws, hipStream_t s);
+
+// ── 4-bit weights ─────────────────────────────────────────────────────────
+// W [N, K] in 4 bits: packed [ceil(N/16), ceil(K/128), 64, 16] bytes, tiles
+// of 16 rows x 128 columns whose byte run l holds the 32 codes of row l % 16
+// from column 32 (l / 16) on; the eight codes of a 4-byte word as code + 8,
+// nibble j (lowest first) code 2j for j < 4 and code 2(j - 4) + 1 for the
+// others; padding has code 0.  Scales [ceil(K / group), N] of dtype dt:
+// value = code * scale.
+int64_t int4_bytes(int64_t N, int64_t K);
+// Scale = largest magnitude of the group / 7 rounded to dt, codes = value /
+// scale rounded half to even, within -7 .. 7; w [N, K] read through strides.
+void quantize_int4(DType dt, const void* w, int64_t sn, int64_t sk, int64_t N, int64_t K, int64_t group,
+                   uint8_t* packed, void* scales, hipStream_t s);
+// out [N, K] = the values, of the scales' dtype, row stride ld.
+void dequantize_int4(DType dt, const uint8_t* packed, const void* scales, int64_t N, int64_t K, int64_t group,
+                     void* out, int64_t ld, hipStream_t s);
+// out [M, N] = act(x [M, K] W^T + bias); x rows contiguous along K.
+struct LinearInt4 {
+  DType dt = DType::F16;
+  int64_t M = 0, N = 0, K = 0, group = 128;
+  const void* x = nullptr; int64_t x_sm = 0;
+  const uint8_t* packed = nullptr;
+  const void* scales = nullptr;
+  const void* bias = nullptr;
+  int act = 0;
+  void* out = nullptr;
+};
+void linear_int4(const LinearInt4& a, hipStream_t s);
+
+// ── log probabilities of given tokens ─────────────────────────────────────
+// For each row of logits [R, V] (row stride ld): lp[r] = log p(token r) (0
+// where the token is outside [0, V)), the row's entropy and log sum of
+// exponentials, and its top_k largest logits as log probabilities with their
+// indices, equal ones by index, NaN first.
+struct TokenLogprobs {
+  DType dt = DType::F32;
+  int64_t R = 0, V = 0, ld = 0;
+  const void* z = nullptr;
+  DType idx_dt = DType::I32;
+  const void* tokens = nullptr;
+  int top_k = 0;
+  float* lp = nullptr; float* entropy = nullptr; float* lse = nullptr;
+  float* top_lp = nullptr; int32_t* top_ids = nullptr;
+};
+constexpr int kTopKMax = 32;
+size_t token_logprobs_ws_bytes(const TokenLogprobs& a);
+void token_logprobs(const TokenLogprobs& a, void* ws, hipStream_t s);
+// dz[r, j] = g_lp[r] (1[j = token r] - p_j) - g_H[r] p_j (log p_j + H[r]),
+// p from the logits and lse; g_H may be null.  dz contiguous [R, V].
+void token_logprobs_backward(const TokenLogprobs& a, const float* g_lp, const float* g_H, void* dz, hipStream_t s);
+
 // o = x elementwise with dtype conversion, o written through the strides of
 // `so` (shape and destination strides) and x read through `sx`.
 void copy_strided(DType in, DType out, const void* x, const ND& sx, void* o, const ND& so, hipStream_t s);

@@ -1926,5 +1926,310 @@ void kv_write(const TensorP& cache, const TensorP& rows, const TensorP& pos, con
   LAUNCH k::kv_write(a, rt().stream());
 }
 
+// ── K/V cache in 8 bits ────────────────────────────────────────────────────
+static k::Int8Cache int8_cache(const char* name, const char* what, const TensorP& codes, const TensorP& scales,
+                               int64_t block) {
+  if (codes->dtype != DType::I8) fail("%s: %s codes must be int8, got %s", name, what, dtype_name(codes->dtype));
+  if (scales->dtype != DType::F32) fail("%s: %s scales must be float32, got %s", name, what, dtype_name(scales->dtype));
+  check_bhtd(name, what, *codes);
+  const int64_t B = codes->shape[0], H = codes->shape[1], Tmax = codes->shape[2], D = codes->shape[3];
+  if (!k::kv_int8_supported(D, block))
+    fail("%s: head dim %lld (32, 64 or 128) or block %lld (16, 32, 64 or 128) not supported", name, (long long)D,
+         (long long)block);
+  if (Tmax < 1) fail("%s: empty cache", name);
+  if (scales->ndim != 3 || scales->shape[0] != B || scales->shape[1] != H || scales->shape[2] != (Tmax + block - 1) / block)
+    fail("%s: %s scales must be [%lld, %lld, %lld] for blocks of %lld rows, got %s", name, what, (long long)B,
+         (long long)H, (long long)((Tmax + block - 1) / block), (long long)block, shape_str(scales->dims()).c_str());
+  for (int i = 0; i < 3; ++i) {
+    if ((codes->shape[i] > 1 && codes->strides[i] == 0) || (scales->shape[i] > 1 && scales->strides[i] == 0))
+      fail("%s: the %s cache has overlapping rows", name, what);
+    if (codes->shape[i] > 1 && codes->strides[i] % 16 != 0)
+      fail("%s: rows of the %s codes must start at 16-byte boundaries", name, what);
+  }
+  if ((uintptr_t)codes->data() & 15) fail("%s: rows of the %s codes must start at 16-byte boundaries", name, what);
+  k::Int8Cache c;
+  c.codes = (int8_t*)codes->data();
+  c.scales = (float*)scales->data();
+  for (int i = 0; i < 3; ++i) { c.cs[i] = codes->strides[i]; c.ss[i] = scales->strides[i]; }
+  return c;
+}
+
+// The pair's sizes and pointers, checked.
+static k::KvInt8 int8_pair(const char* name, const Int8KV& c) {
+  k::KvInt8 a;
+  a.c[0] = int8_cache(name, "k", c.kc, c.ks, c.block);
+  a.c[1] = int8_cache(name, "v", c.vc, c.vs, c.block);
+  if (c.kc->dims() != c.vc->dims())
+    fail("%s: the K codes %s and the V codes %s differ in shape", name, shape_str(c.kc->dims()).c_str(),
+         shape_str(c.vc->dims()).c_str());
+  a.B = c.kc->shape[0]; a.H = c.kc->shape[1]; a.Tmax = c.kc->shape[2]; a.D = c.kc->shape[3];
+  a.block = (int)c.block;
+  return a;
+}
+
+// Rows [B, H, T, D] to append; copied when a row is not 16-byte aligned.
+static TensorP int8_rows(const char* name, const TensorP& rows, const k::KvInt8& a, DType dt) {
+  check_dtype(name, kFloatOnly, rows->dtype);
+  if (rows->dtype != dt) fail("%s: the K and V rows must share a dtype", name);
+  if (rows->ndim != 4 || rows->shape[0] != a.B || rows->shape[1] != a.H || rows->shape[3] != a.D)
+    fail("%s: rows %s do not match a cache of [%lld, %lld, %lld, %lld]", name, shape_str(rows->dims()).c_str(),
+         (long long)a.B, (long long)a.H, (long long)a.Tmax, (long long)a.D);
+  if (meta_mode()) return rows;
+  const int64_t es = (int64_t)dtype_size(dt);
+  bool ok = rows->strides[3] == 1 && ((uintptr_t)rows->data() & 15) == 0;
+  for (int i = 0; i < 3; ++i) ok = ok && (rows->shape[i] <= 1 || rows->strides[i] * es % 16 == 0);
+  return ok ? rows : materialize(rows);
+}
+
+static void append_int8(const char* name, k::KvInt8 a, const Int8KV& c, const TensorP& k_rows, const TensorP& v_rows,
+                        const TensorP& pos, int pos_off) {
+  if (c.kc->data() && c.kc->data() == c.vc->data()) fail("%s: K and V need codes of their own", name);
+  if (c.ks->data() && c.ks->data() == c.vs->data()) fail("%s: K and V need scales of their own", name);
+  a.dt = k_rows->dtype;
+  a.T = k_rows->ndim == 4 ? k_rows->shape[2] : 0;
+  TensorP r[2] = {int8_rows(name, k_rows, a, a.dt), int8_rows(name, v_rows, a, a.dt)};
+  if (r[1]->shape[2] != a.T) fail("%s: the K and V rows differ in number", name);
+  if (a.T > a.Tmax) fail("%s: %lld rows exceed the cache length %lld", name, (long long)a.T, (long long)a.Tmax);
+  TensorP pc = check_lens(name, "positions", pos, a.B);
+  for (int j = 0; j < 2; ++j) {
+    a.x[j] = r[j]->data();
+    for (int i = 0; i < 3; ++i) a.xs[j][i] = r[j]->strides[i];
+  }
+  a.pos = (const int32_t*)pc->data();
+  a.pos_off = pos_off;
+  LAUNCH k::kv_write_int8(a, rt().stream());
+}
+
+void kv_write_int8(const Int8KV& c, const TensorP& k_rows, const TensorP& v_rows, const TensorP& pos) {
+  append_int8("kv_write_int8", int8_pair("kv_write_int8", c), c, k_rows, v_rows, pos, 0);
+}
+
+std::vector<TensorP> kv_read_int8(const Int8KV& c, const TensorP& pos, int64_t T, DType dt) {
+  const char* name = "kv_read_int8";
+  k::KvInt8 a = int8_pair(name, c);
+  check_dtype(name, kFloatOnly, dt);
+  if (T < 0) fail("%s: negative row count", name);
+  a.dt = dt;
+  a.T = T;
+  TensorP pc = check_lens(name, "positions", pos, a.B);
+  a.pos = (const int32_t*)pc->data();
+  std::vector<TensorP> out{alloc_out(dt, {a.B, a.H, T, a.D}), alloc_out(dt, {a.B, a.H, T, a.D})};
+  void* const y[2] = {out[0]->data(), out[1]->data()};
+  LAUNCH k::kv_read_int8(a, y, rt().stream());
+  return out;
+}
+
+TensorP decode_attention_int8(const TensorP& q_in, const Int8KV& c, const TensorP& lens, float scale,
+                              const TensorP& k_new, const TensorP& v_new) {
+  const char* name = "decode_attention_int8";
+  check_dtype(name, kFloatOnly, q_in->dtype);
+  const k::KvInt8 p = int8_pair(name, c);
+  if (q_in->ndim != 4) fail("%s: q must be 4-D [batch, heads, tokens, head_dim], got %s", name,
+                            shape_str(q_in->dims()).c_str());
+  const int64_t B = q_in->shape[0], Hq = q_in->shape[1], Tq = q_in->shape[2], D = q_in->shape[3];
+  if (B != p.B || D != p.D || p.H < 1 || Hq % p.H != 0 || Hq < 1)
+    fail("%s: q %s does not match a cache of %s (its heads must be a multiple of the cache's)", name,
+         shape_str(q_in->dims()).c_str(), shape_str(c.kc->dims()).c_str());
+  if (Tq > p.Tmax) fail("%s: %lld query rows exceed the cache length %lld", name, (long long)Tq, (long long)p.Tmax);
+  if (!(scale > 0.f) || !std::isfinite(scale)) fail("%s: the scale must be positive and finite", name);
+  TensorP lc = check_lens(name, "lens", lens, B);
+  TensorP q = q_in;
+  if (!meta_mode()) {
+    const int64_t es = (int64_t)dtype_size(q->dtype);
+    bool ok = q->strides[3] == 1 && ((uintptr_t)q->data() & 15) == 0;
+    for (int i = 0; i < 3; ++i) ok = ok && (q->shape[i] <= 1 || q->strides[i] * es % 16 == 0);
+    if (!ok) q = materialize(q);
+  }
+  if (k_new || v_new) {
+    if (!k_new || !v_new) fail("%s: new K and V rows come together", name);
+    if (Tq != 1) fail("%s: appending new rows needs one query row per sequence, got %lld", name, (long long)Tq);
+    if (k_new->dtype != q->dtype) fail("%s: new rows must share q's dtype", name);
+    if (k_new->ndim == 4 && k_new->shape[2] != 1) fail("%s: new rows must hold one token", name);
+    append_int8(name, p, c, k_new, v_new, lc, -1);
+  }
+  k::DecodeInt8 a;
+  a.dt = q->dtype;
+  a.B = B; a.H = p.H; a.G = Hq / p.H; a.Tq = Tq; a.Tmax = p.Tmax; a.D = D;
+  a.block = p.block;
+  a.q = q->data(); a.q_sb = q->strides[0]; a.q_sh = q->strides[1]; a.q_st = q->strides[2];
+  a.k = p.c[0]; a.v = p.c[1];
+  a.lens = (const int32_t*)lc->data();
+  a.scale = scale;
+  // physical [B, Tq, Hq, D], logical [B, Hq, Tq, D]
+  TensorP base = alloc_out(q->dtype, {B, Tq, Hq, D});
+  TensorP out = make_meta(q->dtype, q->dims());
+  out->buf = base->buf;
+  out->offset = base->offset;
+  out->strides[0] = Tq * Hq * D; out->strides[1] = D; out->strides[2] = Hq * D; out->strides[3] = 1;
+  a.o = out->data(); a.o_sb = out->strides[0]; a.o_sh = out->strides[1]; a.o_st = out->strides[2];
+  const size_t wsb = meta_mode() ? 0 : k::decode_int8_ws_bytes(a);
+  BufferP ws;
+  if (wsb) ws = scratch(wsb);
+  LAUNCH k::decode_attention_int8(a, ws ? ws->ptr : nullptr, rt().stream());
+  return out;
+}
+
+// ── 4-bit weights ──────────────────────────────────────────────────────────
+static void check_group(const char* name, int64_t group) {
+  if (group != 32 && group != 64 && group != 128) fail("%s: group %lld not supported (32, 64 or 128)", name, (long long)group);
+}
+
+// The checked codes (contiguous, 16-byte aligned) of [N, K] weights.
+static TensorP int4_codes(const char* name, const TensorP& packed, const TensorP& scales, int64_t K, int64_t group) {
+  check_group(name, group);
+  if (K < 1) fail("%s: needs at least one input feature", name);
+  if (packed->dtype != DType::U8 || packed->ndim != 4 || packed->shape[2] != 64 || packed->shape[3] != 16)
+    fail("%s: weights are not packed (quantize_int4)", name);
+  check_dtype(name, kFloatOnly, scales->dtype);
+  if (scales->ndim != 2 || scales->shape[1] < 1) fail("%s: scales must be [groups, out]", name);
+  const int64_t N = scales->shape[1];
+  if (packed->shape[0] != (N + 15) / 16 || packed->shape[1] != (K + 127) / 128 || scales->shape[0] != (K + group - 1) / group)
+    fail("%s: packed weights %s and scales %s do not hold [out %lld, in %lld] in groups of %lld", name,
+         shape_str(packed->dims()).c_str(), shape_str(scales->dims()).c_str(), (long long)N, (long long)K,
+         (long long)group);
+  TensorP pc = contiguous(packed);
+  if (!meta_mode() && ((uintptr_t)pc->data() & 15)) pc = materialize(pc);
+  return pc;
+}
+
+std::vector<TensorP> quantize_int4(const TensorP& w, int64_t group) {
+  const char* name = "quantize_int4";
+  check_dtype(name, kFloatOnly, w->dtype);
+  check_group(name, group);
+  if (w->ndim != 2 || w->shape[0] < 1 || w->shape[1] < 1) fail("%s: weights must be 2-D [out, in], got %s", name,
+                                                               shape_str(w->dims()).c_str());
+  const int64_t N = w->shape[0], K = w->shape[1];
+  TensorP packed = alloc_out(DType::U8, {(N + 15) / 16, (K + 127) / 128, 64, 16});
+  TensorP scales = alloc_out(w->dtype, {(K + group - 1) / group, N});
+  LAUNCH k::quantize_int4(w->dtype, w->data(), w->strides[0], w->strides[1], N, K, group, (uint8_t*)packed->data(),
+                          scales->data(), rt().stream());
+  return {packed, scales};
+}
+
+TensorP dequantize_int4(const TensorP& packed, const TensorP& scales, int64_t K, int64_t group) {
+  TensorP pc = int4_codes("dequantize_int4", packed, scales, K, group), sc = contiguous(scales);
+  const int64_t N = scales->shape[1];
+  TensorP out = alloc_out(scales->dtype, {N, K});
+  LAUNCH k::dequantize_int4(scales->dtype, (const uint8_t*)pc->data(), sc->data(), N, K, group, out->data(), K,
+                            rt().stream());
+  return out;
+}
+
+TensorP linear_int4(const TensorP& x, const TensorP& packed, const TensorP& scales, const TensorP& bias, int64_t group,
+                    int act) {
+  const char* name = "linear_int4";
+  check_dtype(name, kFloatOnly, x->dtype);
+  if (x->ndim < 1) fail("%s requires at least 1D input", name);
+  if (act < k::kActNone || act > k::kActGeluExact) fail("%s: unknown activation %d", name, act);
+  const int64_t K = x->shape[x->ndim - 1];
+  TensorP pc = int4_codes(name, packed, scales, K, group), sc = contiguous(scales);
+  const int64_t N = scales->shape[1], M = x->numel() / K;
+  if (scales->dtype != x->dtype) fail("Dtype mismatch: %s vs %s", dtype_name(x->dtype), dtype_name(scales->dtype));
+  TensorP bc;
+  if (bias) {
+    if (bias->dtype != x->dtype) fail("Dtype mismatch: %s vs %s", dtype_name(x->dtype), dtype_name(bias->dtype));
+    if (bias->numel() != N || bias->ndim != 1) fail("%s: bias must be [%lld], got %s", name, (long long)N,
+                                                    shape_str(bias->dims()).c_str());
+    bc = contiguous(bias);
+  }
+  TensorP xc = contiguous(x);
+  std::vector<int64_t> od = x->dims();
+  od.back() = N;
+  TensorP out = alloc_out(x->dtype, od);
+  k::LinearInt4 a;
+  a.dt = x->dtype;
+  a.M = M; a.N = N; a.K = K; a.group = group;
+  a.x = xc->data(); a.x_sm = K;
+  a.packed = (const uint8_t*)pc->data();
+  a.scales = sc->data();
+  a.bias = bc ? bc->data() : nullptr;
+  a.act = act;
+  a.out = out->data();
+  LAUNCH k::linear_int4(a, rt().stream());
+  return out;
+}
+
+// ── log probabilities of given tokens ──────────────────────────────────────
+// Logits as rows with a unit stride along V, and the checked tokens.
+static k::TokenLogprobs logprob_rows(const char* name, const TensorP& logits, const TensorP& tokens, TensorP* zc,
+                                     TensorP* tc, std::vector<int64_t>* lead) {
+  check_dtype(name, kFloatOnly, logits->dtype);
+  if (logits->ndim < 1) fail("%s requires at least 1D logits", name);
+  *lead = logits->dims();
+  lead->pop_back();
+  if (lead->empty()) *lead = {1};
+  const int64_t V = logits->shape[logits->ndim - 1];
+  if (V < 1 || V > 0x7fffffffLL) fail("%s: %lld logits in a row", name, (long long)V);
+  if (tokens->dtype != DType::I32 && tokens->dtype != DType::I64)
+    fail("%s: tokens must be int32 or int64, got %s", name, dtype_name(tokens->dtype));
+  k::TokenLogprobs a;
+  a.dt = logits->dtype;
+  a.V = V;
+  a.R = logits->numel() / V;
+  if (tokens->numel() != a.R || (logits->ndim > 1 && tokens->dims() != *lead))
+    fail("%s: tokens %s do not match logits %s", name, shape_str(tokens->dims()).c_str(),
+         shape_str(logits->dims()).c_str());
+  *zc = logits;
+  if (!as_rows(*logits, &a.R, &a.ld)) {
+    *zc = contiguous(logits);
+    if (!meta_mode()) as_rows(**zc, &a.R, &a.ld);
+  }
+  a.R = logits->numel() / V;
+  *tc = contiguous(tokens);
+  a.z = (*zc)->data();
+  a.idx_dt = tokens->dtype;
+  a.tokens = (*tc)->data();
+  return a;
+}
+
+std::vector<TensorP> token_logprobs(const TensorP& logits, const TensorP& tokens, int64_t top_k) {
+  const char* name = "token_logprobs";
+  TensorP zc, tc;
+  std::vector<int64_t> lead;
+  k::TokenLogprobs a = logprob_rows(name, logits, tokens, &zc, &tc, &lead);
+  if (top_k < 0 || top_k > k::kTopKMax || top_k > a.V)
+    fail("%s: %lld alternatives of %lld (at most %d)", name, (long long)top_k, (long long)a.V, k::kTopKMax);
+  a.top_k = (int)top_k;
+  std::vector<TensorP> out;
+  for (int i = 0; i < 3; ++i) out.push_back(alloc_out(DType::F32, lead));
+  a.lp = (float*)out[0]->data(); a.entropy = (float*)out[1]->data(); a.lse = (float*)out[2]->data();
+  if (top_k > 0) {
+    std::vector<int64_t> td = lead;
+    td.push_back(top_k);
+    out.push_back(alloc_out(DType::F32, td));
+    out.push_back(alloc_out(DType::I32, td));
+    a.top_lp = (float*)out[3]->data();
+    a.top_ids = (int32_t*)out[4]->data();
+  }
+  const size_t wsb = meta_mode() ? 0 : k::token_logprobs_ws_bytes(a);
+  BufferP ws;
+  if (wsb) ws = scratch(wsb);
+  LAUNCH k::token_logprobs(a, ws ? ws->ptr : nullptr, rt().stream());
+  return out;
+}
+
+TensorP token_logprobs_backward(const TensorP& g_lp, const TensorP& g_H, const TensorP& logits, const TensorP& tokens,
+                                const TensorP& entropy, const TensorP& lse) {
+  const char* name = "token_logprobs_backward";
+  TensorP zc, tc;
+  std::vector<int64_t> lead;
+  k::TokenLogprobs a = logprob_rows(name, logits, tokens, &zc, &tc, &lead);
+  std::vector<TensorP> keep;
+  auto row = [&](const char* what, const TensorP& t) -> float* {
+    if (t->dtype != DType::F32 || t->numel() != a.R)
+      fail("%s: %s must be float32 with one value a row (%lld), got %s %s", name, what, (long long)a.R,
+           dtype_name(t->dtype), shape_str(t->dims()).c_str());
+    keep.push_back(contiguous(t));
+    return (float*)keep.back()->data();
+  };
+  const float* gl = row("grad_logprobs", g_lp);
+  const float* gh = g_H ? row("grad_entropy", g_H) : nullptr;
+  a.entropy = row("entropy", entropy);
+  a.lse = row("lse", lse);
+  TensorP out = alloc_out(logits->dtype, logits->dims());
+  LAUNCH k::token_logprobs_backward(a, gl, gh, out->data(), rt().stream());
+  return out;
+}
+
 }  // namespace ops
 }  // namespace agpu

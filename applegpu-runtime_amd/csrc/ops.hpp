@@ -264,5 +264,38 @@ TensorP decode_attention(const TensorP& q, const TensorP& k_cache, const TensorP
 void kv_write(const TensorP& cache, const TensorP& rows, const TensorP& pos, const TensorP& cache2 = nullptr,
               const TensorP& rows2 = nullptr);
 
+// ── few bits ───────────────────────────────────────────────────────────────
+// A K/V cache in 8 bits: codes int8 [B, H, Tmax, D] (in place; views with a
+// unit stride along D and 16-byte aligned rows) and scales fp32 [B, H,
+// ceil(Tmax / block)], a scale for each block of rows and head (D 32, 64 or
+// 128; block 16, 32, 64 or 128).
+struct Int8KV {
+  TensorP kc, ks, vc, vs;
+  int64_t block = 16;
+};
+// Appends rows [B, H, T, D] at row pos[b] (k::KvInt8 says how scales grow).
+void kv_write_int8(const Int8KV& c, const TensorP& k_rows, const TensorP& v_rows, const TensorP& pos);
+// {K, V} rows pos[b] .. pos[b] + T as values of dtype dt, [B, H, T, D].
+std::vector<TensorP> kv_read_int8(const Int8KV& c, const TensorP& pos, int64_t T, DType dt);
+// Attention of q [B, Hq, Tq, D] (Hq a multiple of H) over the first lens[b]
+// rows; the output is logically [B, Hq, Tq, D], stored as [B, Tq, Hq, D].
+// With k_new / v_new ([B, H, 1, D], Tq == 1) the step's own rows are appended
+// as cache row lens[b] - 1 first.
+TensorP decode_attention_int8(const TensorP& q, const Int8KV& c, const TensorP& lens, float scale,
+                              const TensorP& k_new = nullptr, const TensorP& v_new = nullptr);
+// {packed, scales} of W [N, K] in 4 bits (k::quantize_int4 has the layout),
+// and its values again ([N, K], the scales' dtype).
+std::vector<TensorP> quantize_int4(const TensorP& w, int64_t group);
+TensorP dequantize_int4(const TensorP& packed, const TensorP& scales, int64_t K, int64_t group);
+// act(x W^T + bias) over the last dim of x; bias may be null.
+TensorP linear_int4(const TensorP& x, const TensorP& packed, const TensorP& scales, const TensorP& bias, int64_t group,
+                    int act);
+// {lp, entropy, lse} of logits [..., V] and int32/int64 tokens [...], fp32,
+// and with top_k > 0 also {top log probabilities, int32 indices} [..., top_k].
+std::vector<TensorP> token_logprobs(const TensorP& logits, const TensorP& tokens, int64_t top_k);
+// The gradient of lp and entropy (g_H may be null) with respect to the logits.
+TensorP token_logprobs_backward(const TensorP& g_lp, const TensorP& g_H, const TensorP& logits, const TensorP& tokens,
+                                const TensorP& entropy, const TensorP& lse);
+
 }  // namespace ops
 }  // namespace agpu

@@ -234,6 +234,23 @@ int32_t applegpu_kv_write(uint64_t cache_id, uint64_t rows_id, uint64_t pos_id);
  * have the same shapes and dtype. */
 int32_t applegpu_kv_write_pair(uint64_t k_cache_id, uint64_t v_cache_id, uint64_t k_rows_id, uint64_t v_rows_id,
                                uint64_t pos_id);
+/* The same append to a cache held in 8 bits: codes int8 [B, H, Tmax, D] (D 32,
+ * 64 or 128; rows 16-byte aligned) with one float32 scale per head and block
+ * of `block` (16, 32, 64 or 128) rows, scales [B, H, ceil(Tmax / block)];
+ * value = code * scale.  Rows [B, H, T, D] (float32, float16 or bfloat16)
+ * become cache rows pos[b] .. pos[b] + T; what the cache held from row pos[b]
+ * on is dropped.  A block's scale is its largest magnitude / 127 and codes
+ * are rounded half to even; the rows that the first touched block holds
+ * before pos[b] keep their values, to half a step of a scale that grows.  A
+ * block given an infinity or NaN reads as NaN.  Rows outside [0, Tmax) are
+ * not written.  Readers: the lazy ops "kv_read_int8" (k_codes, k_scales,
+ * v_codes, v_scales, pos; ints rows, block, dtype code: the rows' values) and
+ * "decode_attention_int8" (q [B, Hq, Tq, D] with Hq a multiple of H, k_codes,
+ * k_scales, v_codes, v_scales, lens[, k_new, v_new]; int block; optional
+ * float scale), which attends and appends as "decode_attention" does.
+ * Returns 0, or -1 with the error set. */
+int32_t applegpu_kv_write_int8(uint64_t k_codes_id, uint64_t k_scales_id, uint64_t v_codes_id, uint64_t v_scales_id,
+                               uint64_t k_rows_id, uint64_t v_rows_id, uint64_t pos_id, int64_t block);
 
 int32_t applegpu_capture_begin(void);
 int64_t applegpu_capture_end(void);

@@ -1,0 +1,216 @@
+"""Linear layers with 4-bit weights on the device, against float64.
+
+Bars.  Codes, scales and dequantised values: none.  Products: codes are taken
+as code + 16 in the matrix units and 24 of them is subtracted again, so that a
+group of at most 128 terms loses at most 16 roundings of sums of 24 |x| s; the
+groups, waves and the bias are added in float32, at most K / 32 + 32 of them:
+2^-24 (16 * 24 + K / 32 + 32) sum |x| s.  float32 activations are split into
+three 8-bit parts (2^-24 relative).  16-bit weights of prompts (more than 64
+rows) are rounded to the type once: half a step of sum |x| |w|.  gelu has a
+slope of at most 1.13.  The output is rounded once."""
+import numpy as np
+import pytest
+
+from oracle import few_bits as O
+
+pytestmark = pytest.mark.gpu
+
+HALF_STEP = {"float32": 2.0 ** -24, "float16": 2.0 ** -11, "bfloat16": 2.0 ** -8}
+
+
+def _dev(gpu, a, dtype="float32"):
+    t = gpu.from_numpy(np.ascontiguousarray(a, np.float32))
+    return t if dtype == "float32" else gpu.cast(t, dtype)
+
+
+def _weights(rng, N, K, dtype):
+    """Rows of unlike size, a row of zeros among them."""
+    w = rng.standard_normal((N, K)).astype(np.float32) * np.exp(rng.standard_normal((N, 1))).astype(np.float32) * 0.05
+    w[N // 2] = 0
+    return O.round_to(w, dtype)
+
+
+def _pack(codes):
+    """O.pack_int4 without its loops."""
+    N, K = codes.shape
+    T, S = -(-N // 16), -(-K // 128)
+    u = np.full((T * 16, S * 128), 8, np.uint8)
+    u[:N, :K] = codes + 8
+    u = u.reshape(T, 16, S, 4, 4, 4, 2).transpose(0, 2, 3, 1, 4, 6, 5).reshape(T, S, 64, 16, 2)
+    return u[..., 0] | u[..., 1] << 4
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("N,K,group", [(1, 1, 32), (16, 128, 128), (17, 33, 32), (40, 200, 64), (130, 259, 128),
+                                       (33, 1280, 128)])
+def test_quantize_bit_exact(gpu, dtype, N, K, group):
+    rng = np.random.default_rng(N + K)
+    w = _weights(rng, N, K, dtype)
+    codes, scales = O.quantize_int4(w, group, dtype)
+    for t in (_dev(gpu, w, dtype), gpu.transpose(_dev(gpu, w.T, dtype))):   # also read through strides
+        packed, s = gpu.quantize_int4(t, group)
+        assert packed.dtype == "uint8" and s.dtype == dtype
+        np.testing.assert_array_equal(s.to_numpy().astype(np.float32), scales)
+        np.testing.assert_array_equal(packed.to_numpy(), _pack(codes))
+        if N * K < 20000:
+            np.testing.assert_array_equal(packed.to_numpy(), O.pack_int4(codes))
+        back = gpu.dequantize_int4(packed, s, K, group)
+        assert back.dtype == dtype
+        want = O.round_to(O.values_int4(codes, scales, group).astype(np.float32), dtype)
+        np.testing.assert_array_equal(back.to_numpy().astype(np.float32), want)
+
+
+def test_quantize_infinities(gpu):
+    w = np.ones((20, 70), np.float32)
+    w[3, 40], w[5, 2] = np.inf, np.nan
+    packed, s = gpu.quantize_int4(gpu.from_numpy(w), 32)
+    back = gpu.dequantize_int4(packed, s, 70, 32).to_numpy()
+    bad = np.zeros((20, 70), bool)
+    bad[3, 32:64] = bad[5, :32] = True
+    np.testing.assert_array_equal(np.isnan(back), bad)
+    assert np.abs(back[~bad] - 1).max() <= 2.0 ** -22
+    x = np.ones((2, 70), np.float32)
+    y = gpu.linear_int4(gpu.from_numpy(x), packed, s, group=32).to_numpy()
+    np.testing.assert_array_equal(np.isnan(y).all(0), np.isin(np.arange(20), (3, 5)))
+    assert not np.isnan(np.delete(y, (3, 5), 1)).any()
+
+
+def _check(gpu, rng, dtype, M, N, K, group, act=None, bias=True, lead=None):
+    w = _weights(rng, N, K, dtype)
+    codes, scales = O.quantize_int4(w, group, dtype)
+    x = O.round_to(rng.standard_normal((M, K)).astype(np.float32), dtype)
+    b = O.round_to(rng.standard_normal(N).astype(np.float32), dtype) if bias else None
+    packed, s = gpu.from_numpy(_pack(codes)), _dev(gpu, scales, dtype)
+    xt = _dev(gpu, x.reshape(lead + [K]) if lead else x, dtype)
+    y = gpu.linear_int4(xt, packed, s, _dev(gpu, b, dtype) if bias else None, act, group=group)
+    assert y.shape == (lead or [M]) + [N] and y.dtype == dtype
+    got = y.to_numpy().reshape(M, N).astype(np.float64)
+    wv = O.values_int4(codes, scales, group)
+    want = O.linear(x, wv, b, act)
+    step = np.repeat(scales.T.astype(np.float64), group, 1)[:, :K]
+    ax = np.abs(x).astype(np.float64)
+    bar = 2.0 ** -24 * (16 * 24 + K / 32 + 32) * (ax @ step.T) + 2.0 ** -22 * (np.abs(b) if bias else 0)
+    if dtype != "float32" and M > 64:
+        bar += HALF_STEP[dtype] * (ax @ np.abs(wv).T)
+    bar = 1.13 * bar + (HALF_STEP[dtype] + 2.0 ** -20) * np.abs(want) + (2.0 ** -25 if dtype == "float16" else 0)
+    assert np.isfinite(got).all()
+    over = np.abs(got - want) - bar
+    assert over.max() <= 0, (np.abs(got - want).max(), over.max(), np.unravel_index(over.argmax(), over.shape))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("M", [1, 2, 15, 16, 17, 33, 64, 65, 130])
+@pytest.mark.parametrize("N,K,group", [(48, 256, 128), (33, 321, 32), (17, 64, 64)])
+def test_rows_and_odd_sizes(gpu, dtype, M, N, K, group):
+    _check(gpu, np.random.default_rng(M * N), dtype, M, N, K, group)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (3, 5, 7), (1, 16, 31), (5, 15, 129), (1, 1000, 4100), (8, 3840, 1280),
+                                   (1, 50257, 64), (4, 100, 8192)])
+def test_sizes(gpu, dtype, M, N, K):
+    for group in (32, 64, 128):
+        _check(gpu, np.random.default_rng(N + K), dtype, M, N, K, group, bias=group != 64)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("act", [None, "relu", "gelu", "gelu_exact"])
+@pytest.mark.parametrize("M", [1, 20, 100])
+def test_epilogues(gpu, dtype, act, M):
+    _check(gpu, np.random.default_rng(7), dtype, M, 70, 300, 64, act, bias=act != "relu")
+
+
+def test_leading_dims_and_views(gpu):
+    rng = np.random.default_rng(11)
+    _check(gpu, rng, "float16", 6, 40, 96, 32, lead=[2, 3])
+    _check(gpu, rng, "float16", 1, 40, 96, 32, lead=[])
+    # rows that are a slice at an offset 16 bytes do not divide, and a transposed view
+    w = _weights(rng, 40, 96, "float16")
+    packed, s = gpu.quantize_int4(_dev(gpu, w, "float16"), 32)
+    wv = gpu.dequantize_int4(packed, s, 96, 32).to_numpy().astype(np.float64)
+    big = rng.standard_normal((5, 103)).astype(np.float16)
+    for off in (0, 3, 7):
+        y = gpu.linear_int4(gpu.slice(gpu.from_numpy(big), 1, off, off + 96), packed, s, group=32).to_numpy()
+        want = big[:, off:off + 96].astype(np.float64) @ wv.T
+        assert np.abs(y - want).max() <= 2.0 ** -11 * np.abs(want).max() + 1e-4
+    t = gpu.linear_int4(gpu.transpose(gpu.from_numpy(np.ascontiguousarray(big[:, :96].T))), packed, s, group=32)
+    np.testing.assert_array_equal(t.to_numpy(), gpu.linear_int4(gpu.from_numpy(big[:, :96].copy()), packed, s,
+                                                                group=32).to_numpy())
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16", "float32"])
+@pytest.mark.parametrize("M", [1, 16, 80])
+def test_magnitudes_and_infinities_in_rows(gpu, dtype, M):
+    """Rows of unlike size; an infinity or NaN in one row stays in that row."""
+    rng = np.random.default_rng(M)
+    N, K, group = 50, 160, 32
+    w = _weights(rng, N, K, dtype)
+    w[N // 2] = w[0]
+    codes, scales = O.quantize_int4(w, group, dtype)
+    x = rng.standard_normal((M, K)) * np.exp(rng.uniform(-8, 8, (M, 1)))
+    x = O.round_to(x.astype(np.float32), dtype)
+    wv = O.values_int4(codes, scales, group)
+    want = O.linear(x, wv)
+    if M > 1:
+        x[1, 3], x[M - 1, 5] = np.inf, np.nan
+    y = gpu.linear_int4(_dev(gpu, x, dtype), gpu.from_numpy(_pack(codes)), _dev(gpu, scales, dtype), group=group)
+    y = y.to_numpy().astype(np.float64)
+    good = np.ones(M, bool)
+    if M > 1:
+        good[[1, M - 1]] = False
+        assert not np.isfinite(y[~good]).any()
+    ax = np.abs(np.where(np.isfinite(x), x, 0)).astype(np.float64)
+    step = np.repeat(scales.T.astype(np.float64), group, 1)[:, :K]
+    bar = 2.0 ** -24 * (16 * 24 + K / 32 + 32) * (ax @ step.T) + (HALF_STEP[dtype] + 2.0 ** -20) * np.abs(want)
+    bar = bar + (HALF_STEP[dtype] * (ax @ np.abs(wv).T) if M > 64 else 0) + (2.0 ** -25 if dtype == "float16" else 0)
+    assert (np.abs(y - want) <= bar)[good].all()
+
+
+def test_captured_and_replayed(gpu):
+    rng = np.random.default_rng(0)
+    w = _weights(rng, 96, 256, "float16")
+    packed, s = gpu.quantize_int4(_dev(gpu, w, "float16"), 64)
+    gpu.eval_many([packed, s])
+    graphs = []
+    for M in (4, 100):
+        x = gpu.zeros([M, 256], "float16")
+        graphs.append((x, gpu.capture(lambda x=x: gpu.linear_int4(x, packed, s, group=64))))
+    for _ in range(4):
+        for x, g in graphs:
+            a = rng.standard_normal(x.shape).astype(np.float16)
+            x.write(a)
+            g.replay()
+            np.testing.assert_array_equal(g.outputs.to_numpy(),
+                                          gpu.linear_int4(gpu.from_numpy(a), packed, s, group=64).to_numpy())
+    for _, g in graphs:
+        g.destroy()
+
+
+def test_empty_rows(gpu):
+    packed, s = gpu.quantize_int4(gpu.from_numpy(np.ones((16, 128), np.float32)))
+    assert gpu.linear_int4(gpu.zeros([0, 128]), packed, s).to_numpy().shape == (0, 16)
+
+
+def test_refusals(gpu):
+    w = gpu.zeros([40, 200], "float16")
+    packed, s = gpu.quantize_int4(w, 64)
+    x = gpu.zeros([2, 200], "float16")
+    for bad in (0, 16, 48, 256):
+        with pytest.raises(ValueError, match="quantize_int4"):
+            gpu.quantize_int4(w, bad)
+    with pytest.raises(ValueError, match="quantize_int4"):
+        gpu.quantize_int4(gpu.zeros([4], "float16"))
+    with pytest.raises(ValueError):
+        gpu.quantize_int4(gpu.zeros([4, 32], "int32"))
+    with pytest.raises(ValueError):
+        gpu.quantize_int4(gpu.zeros([4, 0], "float16"))
+    call = lambda x=x, p=packed, s=s, b=None, act=None, g=64: gpu.linear_int4(x, p, s, b, act, group=g)  # noqa: E731
+    for bad in [dict(g=32), dict(g=128), dict(g=7), dict(x=gpu.zeros([2, 300], "float16")),
+                dict(x=gpu.zeros([2, 257], "float16")), dict(x=gpu.zeros([2, 200])), dict(x=gpu.zeros([2, 0], "float16")),
+                dict(p=gpu.zeros([3, 2, 64, 16], "int8")), dict(p=gpu.zeros([2, 2, 64, 16], "uint8")),
+                dict(p=gpu.zeros([40, 100], "uint8")), dict(s=gpu.zeros([4, 64], "float16")), dict(s=gpu.zeros([4, 40])),
+                dict(b=gpu.zeros([39], "float16")), dict(b=gpu.zeros([40])), dict(act="tanh")]:
+        with pytest.raises(ValueError):
+            call(**bad)
+    with pytest.raises(ValueError, match="dequantize_int4"):
+        gpu.dequantize_int4(packed, s, 300, 64)
