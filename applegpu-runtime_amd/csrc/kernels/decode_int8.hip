@@ -2,8 +2,36 @@
 // block of rows and head):
 //   s_j = scale ks[j / block] sum_d q_d kc[j, d],   j < visible rows
 //   o_d = sum_j e^{s_j - m} vs[j / block] vc[j, d] / sum_j e^{s_j - m}
-// One pass over the cache with a running maximum and sum (online softmax).
-// A row that sees no key gets zeros.
+// One pass over the cache with a running maximum and sum; a row that sees no
+// key gets zeros.
+//
+// Everything GEMM-shaped is on v_mfma_f32_16x16x32_f16 with 16 query rows
+// (the query heads of one cache head, and their Tq rows) as columns, so that
+// a read of the cache serves them all; with one query row the 15 idle columns
+// cost nothing that the loads do not hide.
+//  - Scores: S^T = K Q^T.  Lane l owns key l % 16 of a 16-key tile and reads
+//    its codes 16 bytes at a time (a wave instruction is 1 KB in a row); the
+//    order of d inside the product is free as long as Q has the same.
+//  - Codes become f16 without a conversion: byte u = code + 128 under the
+//    byte 0x64 is 1024 + u.  For K the 1152 too many are taken off through
+//    the accumulator's initial value, -1152 sum_d q_d (fp32 queries: off the
+//    f16 itself, since scores must be good to fp32); for V always off the
+//    f16, because there the sum over a long context would lose the difference.
+//  - Queries are scaled by a power of two per row so that the largest is in
+//    [128, 256): any type then fits f16, bf16 exactly; fp32 as hi + lo (2^-22).
+//  - Weights: the accumulators of S^T hold, for a query (lane l % 16), keys
+//    4 (l / 16) .. + 3 of each tile, which is the layout of the B operand of
+//    O^T = V^T P^T for 32 keys: they are exponentiated, scaled by the block's
+//    vs and packed in place, with no exchange between lanes.  V^T's operand
+//    is read 4 bytes of 8 keys a lane (D = 64) and its bytes interleaved by
+//    v_perm, which the conversion needs anyway.
+//  - Weights are rounded to f16 (2^-11 relative, against 2^-8 .. 2^-11 of the
+//    output's own rounding), hi + lo for fp32 outputs; they are kept within
+//    2^15 of a reference maximum that moves only when a score exceeds it by
+//    2^8, so that the exchange between lanes that a new maximum needs is rare,
+//    and within f16's normal range for 2^-21 of the maximum.
+// Work: waves of a block take 32-key steps in turn; a context is split over
+// blocks while these leave CUs idle, and the splits' (O, m, l) are merged.
 #include "device.hpp"
 
 namespace agpu {
@@ -12,105 +40,378 @@ using namespace dev;
 
 namespace {
 
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+
+constexpr int kNW = 4;           // waves of a block
+constexpr int kStep = 32;        // keys of a wave's step
+constexpr int kIter = kNW * kStep;
+constexpr float kLift = 7.f;     // log2 of the weight at the reference maximum
+constexpr float kSlack = 8.f;    // log2 by which a weight may exceed that
+
 struct D8Args {
   DecodeInt8 a;
-  int lg_block;
+  int lg_block, splits, q_tiles;
+  int64_t chunk;  // keys of a split, a multiple of kIter
+  float* part;     // [units][splits][16 (D + 2)]: O, m, l of each query column
 };
 
-// One block of 4 waves per query row: D/16 lanes own one key, 16 codes each
-// (one 16-byte load).
+// 1024 + (code + 128) of the codes in bytes SEL of w ^ 0x80808080, as f16.
+__device__ __forceinline__ uint32_t lift(uint32_t u, uint32_t sel) { return __builtin_amdgcn_perm(0x64646464u, u, sel); }
+__device__ __forceinline__ uint32_t drop(uint32_t h) {
+  const h2 c = {(_Float16)-1152.f, (_Float16)-1152.f};
+  return __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, h) + c);
+}
+
+// 8 codes in two words as an MFMA operand; EXACT: codes, else codes + 1152.
+template <bool EXACT>
+__device__ __forceinline__ h8 codes8(uint32_t w0, uint32_t w1) {
+  w0 ^= 0x80808080u;
+  w1 ^= 0x80808080u;
+  uint32_t r[4] = {lift(w0, 0x04010400u), lift(w0, 0x04030402u), lift(w1, 0x04010400u), lift(w1, 0x04030402u)};
+  if constexpr (EXACT) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = drop(r[i]);
+  }
+  h8 o;
+  __builtin_memcpy(&o, r, 16);
+  return o;
+}
+
+// A wave's codes of one 32-key step.
+template <int D>
+struct Step {
+  static constexpr int KW = D / 16;   // words of a K row that a lane holds (two tiles of them)
+  uint32_t k[2][KW];
+  static constexpr int VB = D / 16;   // bytes of a V row that a lane holds (8 keys of them)
+  uint32_t v[8][VB < 4 ? 1 : VB / 4];
+  float ks[2], vs[2];
+};
+
 template <typename T, int D>
-__global__ void __launch_bounds__(256) decode_int8_row(D8Args g) {
-  constexpr int LPK = D / 16, KPS = 64 / LPK;
+__global__ void __launch_bounds__(64 * kNW) decode_int8_mfma(D8Args g) {
+  constexpr bool F32 = sizeof(T) == 4;
+  constexpr int NK = D / 32;     // MFMAs of a score tile
+  constexpr int ND = D / 16;     // tiles of the output's D
+  constexpr int LD = D + 4;      // padding of a query's row in LDS
+  __shared__ float sm_o[kNW][16][LD];
+  __shared__ float sm_m[kNW][16], sm_l[kNW][16];
   const DecodeInt8& a = g.a;
-  __shared__ float sm_acc[4][D], sm_m[4], sm_l[4];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, grp = lane / LPK, sub = lane % LPK;
-  const int64_t row = blockIdx.x, i = row % a.Tq, bh = row / a.Tq, hq = bh % (a.H * a.G), b = bh / (a.H * a.G);
-  const int64_t h = hq / a.G;
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, q4 = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int split = (int)(blockIdx.x % (unsigned)g.splits);
+  const int64_t unit = blockIdx.x / (unsigned)g.splits;
+  const int qt = (int)(unit % g.q_tiles);
+  const int64_t bh = unit / g.q_tiles, h = bh % a.H, b = bh / a.H;
+  const int R = (int)(a.G * a.Tq);
   int64_t len = a.lens[b];
   len = len < 0 ? 0 : len > a.Tmax ? a.Tmax : len;
-  const int64_t vis = len - a.Tq + i + 1;
-  const T* q = (const T*)a.q + b * a.q_sb + hq * a.q_sh + i * a.q_st + sub * 16;
-  float qf[16], acc[16];
+
+  // the query rows of this tile, r = (query head of the group, token)
+  const int r0 = qt * 16, r1 = r0 + 15 < R ? r0 + 15 : R - 1, Tq = (int)a.Tq;
+  const bool one_head = r0 / Tq == r1 / Tq;
+  const int64_t vis_lo = len - Tq + (one_head ? r0 % Tq : 0) + 1, vis_hi = len - Tq + (one_head ? r1 % Tq : Tq - 1) + 1;
+  const int r = r0 + n < R ? r0 + n : R - 1, i_q = r % Tq;
+  const int64_t vis = r0 + n < R ? len - Tq + i_q + 1 : 0;
+
+  const int64_t j_lo = split * g.chunk;
+  const int64_t j_hi = j_lo + g.chunk < vis_hi ? j_lo + g.chunk : vis_hi;
+
+  // queries as MFMA operands: lane (n, q4) holds d = 64 c + 16 q4 + 8 x + e of
+  // row n (D = 32: d = 8 q4 + e), scaled to [128, 256) at the row's largest
+  h8 qh[NK], ql[F32 ? NK : 1];
+  float corr = 0.f, cq;
+  {
+    const T* q = (const T*)a.q + b * a.q_sb + (h * a.G + r / Tq) * a.q_sh + i_q * a.q_st;
+    float x[NK][8];
+    uint32_t top = 0;
 #pragma unroll
-  for (int e = 0; e < 16; ++e) { qf[e] = to_f(q[e]) * a.scale * 1.4426950408889634f; acc[e] = 0.f; }
-  const int8_t* K = a.k.codes + b * a.k.cs[0] + h * a.k.cs[1] + sub * 16;
-  const int8_t* V = a.v.codes + b * a.v.cs[0] + h * a.v.cs[1] + sub * 16;
-  const float* ks = a.k.scales + b * a.k.ss[0] + h * a.k.ss[1];
-  const float* vs = a.v.scales + b * a.v.ss[0] + h * a.v.ss[1];
-  float m = -INFINITY, l = 0.f;
-  for (int64_t j = w * KPS + grp; j < vis; j += 4 * KPS) {
-    const uint4 kr = *(const uint4*)(K + j * a.k.cs[2]), vr = *(const uint4*)(V + j * a.v.cs[2]);
-    int8_t kc[16], vc[16];
-    __builtin_memcpy(kc, &kr, 16);
-    __builtin_memcpy(vc, &vr, 16);
-    float d = 0.f;
+    for (int t = 0; t < NK; ++t) {
+      const int d = D == 32 ? 8 * q4 : 64 * (t >> 1) + 16 * q4 + 8 * (t & 1);
 #pragma unroll
-    for (int e = 0; e < 16; ++e) d += qf[e] * (float)kc[e];
+      for (int e = 0; e < 8; ++e) {
+        x[t][e] = to_f(q[d + e]);
+        const uint32_t m = __float_as_uint(x[t][e]) & 0x7fffffffu;
+        top = m > top ? m : top;
+      }
+    }
 #pragma unroll
-    for (int x = 1; x < LPK; x <<= 1) d += __shfl_xor(d, x, 64);
-    d *= ks[(j >> g.lg_block) * a.k.ss[2]];
-    const float M = fmaxf(m, d), f = m == -INFINITY ? 0.f : exp2f(m - M), pe = exp2f(d - M);
-    const float pv = pe * vs[(j >> g.lg_block) * a.v.ss[2]];
-    l = l * f + pe;
+    for (int s = 16; s <= 32; s <<= 1) {
+      const uint32_t o = (uint32_t)__shfl_xor((int)top, s, 64);
+      top = o > top ? o : top;
+    }
+    // an infinity or NaN makes its row NaN
+    int ex = (int)(top >> 23) - 127;
+    ex = ex < -100 ? -100 : ex;
+    const float up = top >= 0x7f800000u ? NAN : __uint_as_float((uint32_t)(7 - ex + 127) << 23);
+    float sum = 0.f;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) acc[e] = acc[e] * f + pv * (float)vc[e];
-    m = M;
+    for (int t = 0; t < NK; ++t)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float y = x[t][e] * up;
+        qh[t][e] = (_Float16)y;
+        if constexpr (F32) ql[t][e] = (_Float16)(y - (float)qh[t][e]);
+        else sum += (float)qh[t][e];
+      }
+    if constexpr (!F32) {
+      sum += __shfl_xor(sum, 16, 64);
+      sum += __shfl_xor(sum, 32, 64);
+      corr = -1152.f * sum;
+    }
+    // log2 domain: score = cq ks acc
+    cq = a.scale * 1.4426950408889634f * __uint_as_float((uint32_t)(ex - 7 + 127) << 23);
   }
-  auto merge = [](float& m1, float& l1, float m2, float l2, float& f1, float& f2) {
-    // a NaN maximum wins, so that it reaches the output
-    const float M = m1 != m1 ? m1 : m2 != m2 ? m2 : fmaxf(m1, m2);
-    f1 = m1 == -INFINITY ? 0.f : exp2f(m1 - M);
-    f2 = m2 == -INFINITY ? 0.f : exp2f(m2 - M);
-    l1 = l1 * f1 + l2 * f2;
-    m1 = M;
+
+  const int8_t* K = a.k.codes + b * a.k.cs[0] + h * a.k.cs[1] + (D == 32 ? 8 : 16) * q4;
+  const int8_t* V = a.v.codes + b * a.v.cs[0] + h * a.v.cs[1] + (D / 16) * n;
+  const float* KS = a.k.scales + b * a.k.ss[0] + h * a.k.ss[1];
+  const float* VS = a.v.scales + b * a.v.ss[0] + h * a.v.ss[1];
+
+  auto load = [&](Step<D>& s, int64_t j0) __attribute__((always_inline)) {
+    const int64_t last = a.Tmax - 1;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      int64_t row = j0 + 16 * t + n;
+      row = row < last ? row : last;
+      const int8_t* p = K + row * a.k.cs[2];
+      if constexpr (D == 32) {
+        const uint2 x = *(const uint2*)p;
+        s.k[t][0] = x.x; s.k[t][1] = x.y;
+      } else {
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) {
+          const uint4 x = *(const uint4*)(p + 64 * c);
+          s.k[t][4 * c] = x.x; s.k[t][4 * c + 1] = x.y; s.k[t][4 * c + 2] = x.z; s.k[t][4 * c + 3] = x.w;
+        }
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      int64_t row = j0 + 16 * (e >> 2) + 4 * q4 + (e & 3);
+      row = row < last ? row : last;
+      const int8_t* p = V + row * a.v.cs[2];
+      if constexpr (D == 32) s.v[e][0] = *(const uint16_t*)p;
+      else if constexpr (D == 64) s.v[e][0] = *(const uint32_t*)p;
+      else {
+        const uint2 x = *(const uint2*)p;
+        s.v[e][0] = x.x; s.v[e][1] = x.y;
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      // (a tile that no query sees may be past the cache, or of a block that
+      // holds nothing yet: its scales are not read)
+      const bool seen = j0 + 16 * t < j_hi;
+      const int64_t blk = seen ? (j0 + 16 * t) >> g.lg_block : 0;
+      const float ks = KS[blk * a.k.ss[2]], vs = VS[blk * a.v.ss[2]];
+      s.ks[t] = seen ? ks : 0.f;
+      s.vs[t] = seen ? vs : 0.f;
+    }
   };
+
+  f4 acc[ND];
 #pragma unroll
-  for (int x = LPK; x < 64; x <<= 1) {
-    const float om = __shfl_xor(m, x, 64), ol = __shfl_xor(l, x, 64);
-    float f1, f2;
-    merge(m, l, om, ol, f1, f2);
+  for (int c = 0; c < ND; ++c) acc[c] = f4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
+  int E = -126;          // O is kept in units of 2^E, at least the largest vs so far
+  float vinv = 0x1p126f;
+
+  Step<D> cur, nxt;
+  int64_t j0 = j_lo + w * kStep;
+  if (j0 < j_hi) load(cur, j0);
+  for (; j0 < j_hi; j0 += kIter) {
+    if (j0 + kIter < j_hi) load(nxt, j0 + kIter);
+    // scores of keys 16 t + 4 q4 + i for query n
+    float s[8];
+    float top = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const float oa = __shfl_xor(acc[e], x, 64);
-      acc[e] = acc[e] * f1 + oa * f2;
+    for (int t = 0; t < 2; ++t) {
+      f4 x = f4{corr, corr, corr, corr};
+#pragma unroll
+      for (int c = 0; c < NK; ++c) {
+        const h8 kf = codes8<F32>(cur.k[t][2 * c], cur.k[t][2 * c + 1]);
+        x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[c], x, 0, 0, 0);
+        if constexpr (F32) x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[c], x, 0, 0, 0);
+      }
+      const float f = cq * cur.ks[t];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[4 * t + i] = x[i] * f;
+    }
+    if (j0 + kStep > vis_lo) {
+      const int left = (int)(vis - j0 < 64 ? vis - j0 : 64);  // this query's keys of the step
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (16 * (e >> 2) + 4 * q4 + (e & 3) >= left) s[e] = -INFINITY;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = fmaxf(top, s[e]);
+    if (__any(top > m + kSlack)) {
+      top = fmaxf(top, __shfl_xor(top, 16, 64));
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      const float M = fmaxf(m, top);
+      const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
+      l *= f;
+#pragma unroll
+      for (int c = 0; c < ND; ++c) acc[c] *= f;
+      m = M;
+    }
+    const float v0 = fabsf(cur.vs[0]), v1 = fabsf(cur.vs[1]);
+    const float v_top = fmaxf(v0 < INFINITY ? v0 : 0.f, v1 < INFINITY ? v1 : 0.f);
+    if (v_top * vinv > 1.f) {
+      const int e1 = (int)(__float_as_uint(v_top) >> 23) - 126;
+#pragma unroll
+      for (int c = 0; c < ND; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[c][i] = ldexpf(acc[c][i], E - e1);
+      E = e1;
+      vinv = ldexpf(1.f, -E);
+    }
+    const float ref = m == -INFINITY ? 0.f : m - kLift;
+    float p[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float x = __builtin_amdgcn_exp2f(s[e] - ref);
+      l += x;
+      // a hidden key adds nothing, whatever its block's scale is
+      p[e] = s[e] == -INFINITY ? 0.f : x * (cur.vs[e >> 2] * vinv);
+    }
+    h8 ph, pl;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      ph[e] = (_Float16)p[e];
+      if constexpr (F32) pl[e] = (_Float16)(p[e] - (float)ph[e]);
+    }
+    // V^T operands: byte c of the 8 keys' words, pairs of keys together
+#pragma unroll
+    for (int wd = 0; wd < (D < 64 ? 1 : D / 64); ++wd) {
+      uint32_t f[4][4];
+#pragma unroll
+      for (int pr = 0; pr < 4; ++pr) {
+        const uint32_t x = cur.v[2 * pr][wd] ^ 0x80808080u, y = cur.v[2 * pr + 1][wd] ^ 0x80808080u;
+        const uint32_t a01 = __builtin_amdgcn_perm(y, x, 0x05010400u);  // x0 y0 x1 y1
+        f[0][pr] = drop(lift(a01, 0x04010400u));
+        f[1][pr] = drop(lift(a01, 0x04030402u));
+        if constexpr (D >= 64) {
+          const uint32_t a23 = __builtin_amdgcn_perm(y, x, 0x07030602u);
+          f[2][pr] = drop(lift(a23, 0x04010400u));
+          f[3][pr] = drop(lift(a23, 0x04030402u));
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < (D < 64 ? 2 : 4); ++c) {
+        h8 vf;
+        __builtin_memcpy(&vf, f[c], 16);
+        f4& o = acc[4 * wd + c];
+        o = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph, o, 0, 0, 0);
+        if constexpr (F32) o = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl, o, 0, 0, 0);
+      }
+    }
+    cur = nxt;
+  }
+
+  // the waves' states meet in LDS; lane (n, q4) holds d = (D/4) q4 + (D/16) i + c
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+#pragma unroll
+  for (int c = 0; c < ND; ++c)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sm_o[w][n][(D / 4) * q4 + (D / 16) * i + c] = ldexpf(acc[c][i], E);
+  if (q4 == 0) { sm_m[w][n] = m; sm_l[w][n] = l; }
+  __syncthreads();
+  const int rows = r1 - r0 + 1;
+  for (int idx = tid; idx < rows * D; idx += 64 * kNW) {
+    const int qr = idx / D, d = idx % D, rr = r0 + qr, iq = rr % Tq;
+    float M = sm_m[0][qr];
+#pragma unroll
+    for (int x = 1; x < kNW; ++x) M = fmaxf(M, sm_m[x][qr]);
+    float L = 0.f, A = 0.f;
+#pragma unroll
+    for (int x = 0; x < kNW; ++x) {
+      const float mx = sm_m[x][qr], f = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - M);
+      L += sm_l[x][qr] * f;
+      A += sm_o[x][qr][d] * f;
+    }
+    if (g.splits == 1) {
+      T* o = (T*)a.o + b * a.o_sb + (h * a.G + rr / Tq) * a.o_sh + iq * a.o_st;
+      o[d] = from_f<T>(len - Tq + iq + 1 > 0 ? A / L : 0.f);
+    } else {
+      float* P = g.part + ((unit * g.splits + split) * 16 + qr) * (D + 2);
+      P[d] = A;
+      if (d == 0) { P[D] = M; P[D + 1] = L; }
     }
   }
-  if (grp == 0) {
-#pragma unroll
-    for (int e = 0; e < 16; ++e) sm_acc[w][sub * 16 + e] = acc[e];
-    if (sub == 0) { sm_m[w] = m; sm_l[w] = l; }
+}
+
+// One block of D threads per query row: merges its splits.
+template <typename T, int D>
+__global__ void __launch_bounds__(D < 64 ? 64 : D) decode_int8_merge(D8Args g) {
+  const DecodeInt8& a = g.a;
+  const int d = threadIdx.x, Tq = (int)a.Tq, R = (int)(a.G * a.Tq);
+  const int64_t row = blockIdx.x, bh = row / R, h = bh % a.H, b = bh / a.H;
+  const int rr = (int)(row % R), iq = rr % Tq;
+  if (d >= D) return;
+  const float* P = g.part + ((bh * g.q_tiles + rr / 16) * g.splits * 16 + rr % 16) * (D + 2);
+  const int64_t st = 16 * (D + 2);
+  float M = -INFINITY;
+  for (int s = 0; s < g.splits; ++s) M = fmaxf(M, P[s * st + D]);
+  float L = 0.f, A = 0.f;
+  for (int s = 0; s < g.splits; ++s) {
+    const float m = P[s * st + D], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
+    L += P[s * st + D + 1] * f;
+    A += P[s * st + d] * f;
   }
-  __syncthreads();
-  if (tid >= D) return;
-  float M = sm_m[0], L = sm_l[0], A = sm_acc[0][tid];
-  for (int x = 1; x < 4; ++x) {
-    float f1, f2;
-    merge(M, L, sm_m[x], sm_l[x], f1, f2);
-    A = A * f1 + sm_acc[x][tid] * f2;
-  }
-  T* o = (T*)a.o + b * a.o_sb + hq * a.o_sh + i * a.o_st;
-  o[tid] = from_f<T>(vis > 0 ? A / L : 0.f);
+  int64_t len = a.lens[b];
+  len = len < 0 ? 0 : len > a.Tmax ? a.Tmax : len;
+  T* o = (T*)a.o + b * a.o_sb + (h * a.G + rr / Tq) * a.o_sh + iq * a.o_st;
+  o[d] = from_f<T>(len - Tq + iq + 1 > 0 ? A / L : 0.f);
+}
+
+D8Args plan(const DecodeInt8& a) {
+  D8Args g;
+  g.a = a;
+  g.lg_block = a.block == 16 ? 4 : a.block == 32 ? 5 : a.block == 64 ? 6 : 7;
+  g.q_tiles = (int)((a.G * a.Tq + 15) / 16);
+  const int64_t units = a.B * a.H * g.q_tiles, most = (a.Tmax + kIter - 1) / kIter;
+  int64_t want = units > 0 ? (1024 + units - 1) / units : 1;
+  if (want > most) want = most;
+  g.chunk = ((a.Tmax + want - 1) / want + kIter - 1) / kIter * kIter;
+  g.splits = (int)((a.Tmax + g.chunk - 1) / g.chunk);
+  g.part = nullptr;
+  return g;
+}
+
+template <typename T, int D>
+void launch(const D8Args& g, hipStream_t s) {
+  const int64_t units = g.a.B * g.a.H * g.q_tiles;
+  hipLaunchKernelGGL((decode_int8_mfma<T, D>), dim3((unsigned)(units * g.splits)), dim3(64 * kNW), 0, s, g);
+  if (g.splits > 1)
+    hipLaunchKernelGGL((decode_int8_merge<T, D>), dim3((unsigned)(g.a.B * g.a.H * g.a.G * g.a.Tq)),
+                       dim3(D < 64 ? 64 : D), 0, s, g);
 }
 
 }  // namespace
 
-size_t decode_int8_ws_bytes(const DecodeInt8&) { return 0; }
+size_t decode_int8_ws_bytes(const DecodeInt8& a) {
+  const D8Args g = plan(a);
+  if (g.splits <= 1) return 0;
+  return (size_t)(a.B * a.H * g.q_tiles) * g.splits * 16 * (a.D + 2) * sizeof(float);
+}
 
 void decode_attention_int8(const DecodeInt8& a, void* ws, hipStream_t s) {
-  (void)ws;
   if (!kv_int8_supported(a.D, a.block))
     fail("decode_attention_int8: head dim %lld or block %d not supported", (long long)a.D, a.block);
-  const int64_t rows = a.B * a.H * a.G * a.Tq;
-  if (rows == 0) return;
-  if (rows > 0x7fffffffLL) fail("decode_attention_int8: too many rows");
-  D8Args g;
-  g.a = a;
-  g.lg_block = a.block == 16 ? 4 : a.block == 32 ? 5 : a.block == 64 ? 6 : 7;
+  if (a.B * a.H * a.G * a.Tq == 0) return;
+  D8Args g = plan(a);
+  if (a.G * a.Tq > 0x7fffffffLL / 2 || a.B * a.H * a.G * a.Tq > 0x7fffffffLL || a.B * a.H * g.q_tiles * g.splits > 0x7fffffffLL)
+    fail("decode_attention_int8: too many query rows");
+  if (g.splits > 1 && !ws) fail("decode_attention_int8: workspace missing");
+  g.part = (float*)ws;
   AGPU_FLOAT_SWITCH(a.dt, {
-    if (a.D == 32) hipLaunchKernelGGL((decode_int8_row<T, 32>), dim3((unsigned)rows), dim3(256), 0, s, g);
-    else if (a.D == 64) hipLaunchKernelGGL((decode_int8_row<T, 64>), dim3((unsigned)rows), dim3(256), 0, s, g);
-    else hipLaunchKernelGGL((decode_int8_row<T, 128>), dim3((unsigned)rows), dim3(256), 0, s, g);
+    if (a.D == 32) launch<T, 32>(g, s);
+    else if (a.D == 64) launch<T, 64>(g, s);
+    else launch<T, 128>(g, s);
   });
   check_launch("decode_attention_int8");
 }
