@@ -536,7 +536,9 @@ void quantize_int4(DType dt, const void* w, int64_t sn, int64_t sk, int64_t N, i
 // out [N, K] = the values, of the scales' dtype, row stride ld.
 void dequantize_int4(DType dt, const uint8_t* packed, const void* scales, int64_t N, int64_t K, int64_t group,
                      void* out, int64_t ld, hipStream_t s);
-// out [M, N] = act(x [M, K] W^T + bias); x rows contiguous along K.
+// out [M, N] = act(x [M, K] W^T + bias) for M up to kInt4Rows; x rows
+// contiguous along K.
+constexpr int64_t kInt4Rows = 64;
 struct LinearInt4 {
   DType dt = DType::F16;
   int64_t M = 0, N = 0, K = 0, group = 128;

@@ -73,11 +73,6 @@ __global__ void __launch_bounds__(256) dequantize_int4_kernel(const uint32_t* __
   }
 }
 
-struct L4Args {
-  LinearInt4 a;
-  int64_t steps;
-};
-
 __device__ __forceinline__ float act_of(float v, int act) {
   if (act == kActRelu) return v > 0.f ? v : (v != v ? v : 0.f);
   if (act == kActGelu) return gelu_tanh(v);
@@ -85,35 +80,243 @@ __device__ __forceinline__ float act_of(float v, int act) {
   return v;
 }
 
-// One wave per 16 columns of the output and row of x: lane l sums the codes
-// of its run (row l % 16 of the tile) against x.
+// ── few rows: codes straight into the matrix units ─────────────────────────
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+
+// The 16-bit type that the codes take, and the parts that a row's value is
+// split into: fp32 rows become three bf16 (24 bits).
+template <typename T> struct In4 {
+  typedef b8 vec;
+  static constexpr int P = sizeof(T) == 4 ? 3 : 1;
+  // code + 24 of nibble i of a word: 16 + (code + 8), exact in 8 bits
+  static constexpr uint32_t kMask = 0x00780078u, kBase = 0x41804180u;
+  template <int I> static __device__ __forceinline__ uint32_t pair(uint32_t w) {
+    const uint32_t v = I == 0 ? w << 3 : w >> (4 * I - 3);
+    return (v & kMask) | kBase;
+  }
+  static __device__ __forceinline__ f4 mfma(vec a, vec b, f4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <> struct In4<half_t> {
+  typedef h8 vec;
+  static constexpr int P = 1;
+  static constexpr uint32_t kMask = 0x03c003c0u, kBase = 0x4c004c00u;
+  template <int I> static __device__ __forceinline__ uint32_t pair(uint32_t w) {
+    const uint32_t v = I == 0 ? w << 6 : I == 1 ? w << 2 : w >> (4 * I - 6);
+    return (v & kMask) | kBase;
+  }
+  static __device__ __forceinline__ f4 mfma(vec a, vec b, f4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+};
+
 template <typename T>
-__global__ void __launch_bounds__(64) linear_int4_row(L4Args g) {
+__device__ __forceinline__ typename In4<T>::vec codes24(uint32_t w) {
+  const uint32_t r[4] = {In4<T>::template pair<0>(w), In4<T>::template pair<1>(w), In4<T>::template pair<2>(w),
+                         In4<T>::template pair<3>(w)};
+  typename In4<T>::vec o;
+  __builtin_memcpy(&o, r, 16);
+  return o;
+}
+
+struct L4Args {
+  LinearInt4 a;
+  int64_t steps;
+  int nw;  // waves of a block
+};
+
+// Steps of 128 columns whose codes a wave has in flight (one where a step is
+// much work: the registers go to the tiles).
+template <int MT> struct InFlight { static constexpr int value = MT == 1 ? 4 : 1; };
+
+// MT tiles of 16 rows of x by NT tiles of 16 columns of the output; the waves
+// of a block take 128-deep steps of K in turn.  G: columns of a scale.  XVEC:
+// K and the rows of x are such that 8 columns are one aligned load.
+template <typename T, int MT, int NT, int G, bool XVEC>
+__global__ void __launch_bounds__(MT == 1 ? 1024 : 512) linear_int4_mfma(L4Args g) {
+  typedef In4<T> I;
+  typedef typename I::vec V;
+  constexpr int NG = 128 / G, kUn = InFlight<MT>::value;
+  extern __shared__ float red[];  // [nw][MT][NT][16][16]
   const LinearInt4& a = g.a;
-  const int lane = threadIdx.x;
-  const int64_t tile = blockIdx.y, m = blockIdx.x, n = tile * 16 + (lane & 15);
-  const T* x = (const T*)a.x + m * a.x_sm;
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, q = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t tiles = (a.N + 15) / 16, tile0 = (int64_t)blockIdx.x * NT, m0 = (int64_t)blockIdx.y * (16 * MT);
   const T* sc = (const T*)a.scales;
-  float acc = 0.f;
-  for (int64_t st = 0; st < g.steps; ++st) {
-    const uint4 w = *(const uint4*)(a.packed + ((tile * g.steps + st) * 64 + lane) * 16);
-    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-    const int64_t k0 = st * 128 + (lane >> 4) * 32;
-    if (k0 >= a.K || n >= a.N) continue;
-    float part = 0.f;
-    for (int i = 0; i < 4; ++i)
-      for (int e = 0; e < 8; ++e) {
-        const int64_t k = k0 + i * 8 + e;
-        if (k < a.K) part += to_f(x[k]) * (float)((int)((ws[i] >> (4 * nibble_of(e))) & 15) - 8);
+  const int64_t groups = (a.K + G - 1) / G;
+
+  V minus;  // -24: takes off what the codes are too large by
+#pragma unroll
+  for (int e = 0; e < 8; ++e) minus[e] = -24.f;
+
+  const T* x[MT];
+  bool row_ok[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const int64_t m = m0 + 16 * i + c;
+    row_ok[i] = m < a.M;
+    x[i] = (const T*)a.x + (row_ok[i] ? m : 0) * a.x_sm;
+  }
+  const uint4* wp[NT];
+  int64_t col[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const int64_t t = tile0 + j < tiles ? tile0 + j : tiles - 1;
+    wp[j] = (const uint4*)a.packed + t * g.steps * 64 + lane;
+    col[j] = t * 16 + c < a.N ? t * 16 + c : a.N - 1;
+  }
+
+  f4 tot[MT][NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) tot[i][j] = f4{0.f, 0.f, 0.f, 0.f};
+
+  for (int64_t s0 = w; s0 < g.steps; s0 += (int64_t)g.nw * kUn) {
+    uint4 wv[kUn][NT];
+    T sv[kUn][NT][NG];
+#pragma unroll
+    for (int u = 0; u < kUn; ++u) {
+      int64_t st = s0 + (int64_t)u * g.nw;
+      st = st < g.steps ? st : s0;
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        wv[u][j] = wp[j][st * 64];
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+          const int64_t gr = st * NG + i < groups ? st * NG + i : groups - 1;
+          sv[u][j][i] = sc[gr * a.N + col[j]];
+        }
       }
-    acc += part * to_f(sc[k0 / a.group * a.N + n]);
+    }
+#pragma unroll
+    for (int u = 0; u < kUn; ++u) {
+      const int64_t st = s0 + (int64_t)u * g.nw;
+      if (st >= g.steps) break;
+      uint32_t word[NT][4];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        word[j][0] = wv[u][j].x; word[j][1] = wv[u][j].y; word[j][2] = wv[u][j].z; word[j][3] = wv[u][j].w;
+        if constexpr (G < 128) {
+          // lane (c, q) holds columns 32 q + 8 t of word t: exchanged between
+          // the four lanes of a row so that word t holds 32 t + 8 q, and one
+          // product covers 32 columns in a row, of one scale
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const auto r = __builtin_amdgcn_permlane32_swap(word[j][t], word[j][t + 2], false, false);
+            word[j][t] = r[0]; word[j][t + 2] = r[1];
+          }
+#pragma unroll
+          for (int t = 0; t < 4; t += 2) {
+            const auto r = __builtin_amdgcn_permlane16_swap(word[j][t], word[j][t + 1], false, false);
+            word[j][t] = r[0]; word[j][t + 1] = r[1];
+          }
+        }
+      }
+#pragma unroll
+      for (int gr = 0; gr < NG; ++gr) {
+        f4 acc[MT][NT], cor[MT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          cor[i] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int j = 0; j < NT; ++j) acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
+        }
+#pragma unroll
+        for (int t = gr * 4 / NG; t < (gr + 1) * 4 / NG; ++t) {
+          const int64_t k = st * 128 + (G < 128 ? 32 * t + 8 * q : 32 * q + 8 * t);
+          V wf[NT];
+#pragma unroll
+          for (int j = 0; j < NT; ++j) wf[j] = codes24<T>(word[j][t]);
+#pragma unroll
+          for (int i = 0; i < MT; ++i) {
+            T xr[8];
+            if constexpr (XVEC) {
+              constexpr int NV = sizeof(T) / 2;
+              uint4 raw[NV];
+              const bool ok = row_ok[i] && k < a.K;
+#pragma unroll
+              for (int e = 0; e < NV; ++e) raw[e] = ok ? ((const uint4*)(x[i] + k))[e] : uint4{0, 0, 0, 0};
+              __builtin_memcpy(xr, raw, sizeof(xr));
+            } else {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) xr[e] = row_ok[i] && k + e < a.K ? x[i][k + e] : (T)0.f;
+            }
+            if constexpr (I::P == 1) {
+              V xf;
+              __builtin_memcpy(&xf, xr, 16);
+              cor[i] = I::mfma(xf, minus, cor[i]);
+#pragma unroll
+              for (int j = 0; j < NT; ++j) acc[i][j] = I::mfma(xf, wf[j], acc[i][j]);
+            } else {
+              float f[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) f[e] = to_f(xr[e]);
+#pragma unroll
+              for (int p = 0; p < 3; ++p) {
+                V xf;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                  xf[e] = (__bf16)f[e];
+                  f[e] -= (float)xf[e];
+                }
+                cor[i] = I::mfma(xf, minus, cor[i]);
+#pragma unroll
+                for (int j = 0; j < NT; ++j) acc[i][j] = I::mfma(xf, wf[j], acc[i][j]);
+              }
+            }
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          const float s = to_f(sv[u][j][gr]);
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) tot[i][j][e] += s * (acc[i][j][e] + cor[i][e]);
+        }
+      }
+    }
   }
-  acc += __shfl_xor(acc, 16, 64);
-  acc += __shfl_xor(acc, 32, 64);
-  if (lane < 16 && n < a.N) {
-    if (a.bias) acc += to_f(((const T*)a.bias)[n]);
-    ((T*)a.out)[m * a.N + n] = from_f<T>(act_of(acc, a.act));
+
+  // lane (c, q) holds rows 4 q + e, column c of each tile; the waves' sums
+  // are added in wave order
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) red[((w * MT + i) * NT + j) * 256 + (4 * q + e) * 16 + c] = tot[i][j][e];
+  __syncthreads();
+  for (int idx = tid; idx < MT * NT * 256; idx += 64 * g.nw) {
+    const int cc = idx & 15, j = (idx >> 4) % NT, mm = idx / (16 * NT);
+    const int64_t m = m0 + mm, n = (tile0 + j) * 16 + cc;
+    if (m >= a.M || n >= a.N) continue;
+    const int at = ((mm >> 4) * NT + j) * 256 + (mm & 15) * 16 + cc;
+    float v = 0.f;
+    for (int i = 0; i < g.nw; ++i) v += red[i * MT * NT * 256 + at];
+    if (a.bias) v += to_f(((const T*)a.bias)[n]);
+    ((T*)a.out)[m * a.N + n] = from_f<T>(act_of(v, a.act));
   }
+}
+
+template <typename T, int MT, int NT, int G>
+void launch_int4(const L4Args& g, bool xvec, hipStream_t s) {
+  const int64_t tiles = (g.a.N + 15) / 16, bx = (tiles + NT - 1) / NT, by = (g.a.M + 16 * MT - 1) / (16 * MT);
+  const dim3 grid((unsigned)bx, (unsigned)by);
+  const size_t lds = (size_t)g.nw * MT * NT * 256 * sizeof(float);
+  if (xvec) hipLaunchKernelGGL((linear_int4_mfma<T, MT, NT, G, true>), grid, dim3(64 * g.nw), lds, s, g);
+  else hipLaunchKernelGGL((linear_int4_mfma<T, MT, NT, G, false>), grid, dim3(64 * g.nw), lds, s, g);
+}
+
+template <typename T, int MT, int NT>
+void launch_int4_g(const L4Args& g, bool xvec, hipStream_t s) {
+  if (g.a.group == 32) launch_int4<T, MT, NT, 32>(g, xvec, s);
+  else if (g.a.group == 64) launch_int4<T, MT, NT, 64>(g, xvec, s);
+  else launch_int4<T, MT, NT, 128>(g, xvec, s);
 }
 
 }  // namespace
@@ -148,12 +351,20 @@ void dequantize_int4(DType dt, const uint8_t* packed, const void* scales, int64_
 
 void linear_int4(const LinearInt4& a, hipStream_t s) {
   if (a.M == 0) return;
+  if (a.M > kInt4Rows || (a.N + 15) / 16 > 0x7fffffffLL) fail("linear_int4: too many rows or columns");
   L4Args g;
   g.a = a;
   g.steps = (a.K + 127) / 128;
-  if (a.M > 0x7fffffffLL || a.N > 65535 * 16) fail("linear_int4: too many rows or columns");
-  const dim3 grid((unsigned)a.M, (unsigned)((a.N + 15) / 16));
-  AGPU_FLOAT_SWITCH(a.dt, hipLaunchKernelGGL((linear_int4_row<T>), grid, dim3(64), 0, s, g));
+  const int es = (int)dtype_size(a.dt);
+  const bool xvec = a.K % 8 == 0 && ((uintptr_t)a.x & 15) == 0 && (a.M == 1 || a.x_sm * es % 16 == 0);
+  const int mt = a.M <= 16 ? 1 : a.M <= 32 ? 2 : 4;
+  const int most = mt == 1 ? 16 : 8;
+  g.nw = (int)(g.steps < most ? g.steps : most);
+  AGPU_FLOAT_SWITCH(a.dt, {
+    if (mt == 1) launch_int4_g<T, 1, 1>(g, xvec, s);
+    else if (mt == 2) launch_int4_g<T, 2, 2>(g, xvec, s);
+    else launch_int4_g<T, 4, 2>(g, xvec, s);
+  });
   check_launch("linear_int4");
 }
 

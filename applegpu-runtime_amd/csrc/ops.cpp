@@ -2132,9 +2132,21 @@ TensorP linear_int4(const TensorP& x, const TensorP& packed, const TensorP& scal
                                                     shape_str(bias->dims()).c_str());
     bc = contiguous(bias);
   }
-  TensorP xc = contiguous(x);
   std::vector<int64_t> od = x->dims();
   od.back() = N;
+  if (M > k::kInt4Rows && !meta_mode()) {
+    // Many rows: the product is what counts, so the weights become values of
+    // x's dtype once (rounded to it) and the GEMM multiplies them; rows of a
+    // multiple of 8 values keep its loads aligned.
+    const int64_t ld = (K + 7) / 8 * 8;
+    TensorP w = rt().alloc(x->dtype, {N, ld});
+    k::dequantize_int4(x->dtype, (const uint8_t*)pc->data(), sc->data(), N, K, group, w->data(), ld, rt().stream());
+    Epilogue e;
+    e.bias = bc;
+    e.act = act;
+    return reshape(matmul(reshape(contiguous(x), {M, K}), view(w, {N, K}, {ld, 1}, 0), false, true, &e), od);
+  }
+  TensorP xc = contiguous(x);
   TensorP out = alloc_out(x->dtype, od);
   k::LinearInt4 a;
   a.dt = x->dtype;
