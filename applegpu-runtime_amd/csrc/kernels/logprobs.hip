@@ -8,6 +8,11 @@
 // digits where one token has nearly all of the probability.
 // A row of -inf only has no distribution: lse and lp are -inf, H 0, and its
 // gradient is 0.
+//
+// Both directions are bound by the read (and write) of the logits: one pass,
+// each thread with a running maximum that moves its sums, 16 elements a step
+// as 16-byte loads whose next ones are in flight.  Few rows are split over
+// blocks, whose states a second launch merges.
 #include "device.hpp"
 
 namespace agpu {
@@ -16,8 +21,18 @@ using namespace dev;
 
 namespace {
 
+constexpr int kNT = 512, kNW = kNT / 64;  // threads and waves of a block
+constexpr int kCh = 16;                   // elements of a thread's step
+constexpr int kCap = 2560;                // alternatives that a block sorts at most
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
+constexpr float kLowest = -3.402823466e38f;
+
 struct LpArgs {
   TokenLogprobs a;
+  int splits;
+  int64_t chunk;    // logits of a split
+  float4* stats;    // [R][splits]: maximum, elements at it, sum of the others, sum of e d
+  uint64_t* keys;   // [R][splits][top_k]
 };
 
 // Unsigned integers in the order of the floats, -0 as 0, NaN above all.
@@ -31,137 +46,414 @@ __device__ __forceinline__ uint32_t order_of(float z) {
 __device__ __forceinline__ uint64_t key_of(float z, uint32_t j) {
   return ((uint64_t)order_of(z) << 32) | (0xffffffffu - j);
 }
-
-__device__ __forceinline__ uint64_t wave_kmax(uint64_t v) {
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) {
-    const uint64_t o = ((uint64_t)(uint32_t)__shfl_xor((int)(v >> 32), m, 64) << 32) |
-                       (uint32_t)__shfl_xor((int)(uint32_t)v, m, 64);
-    v = o > v ? o : v;
-  }
-  return v;
-}
-
-template <int NW>
-__device__ __forceinline__ uint64_t block_kmax(uint64_t v, uint64_t* sh) {
-  v = wave_kmax(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
-  __syncthreads();
-  uint64_t r = sh[0];
-#pragma unroll
-  for (int i = 1; i < NW; ++i) r = sh[i] > r ? sh[i] : r;
-  return r;
-}
-
-template <int NW>
-__device__ __forceinline__ float block_add(float v, float* sh) {
-  v = wave_sum(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
-  __syncthreads();
-  float r = 0.f;
-#pragma unroll
-  for (int i = 0; i < NW; ++i) r += sh[i];
-  return r;
-}
+__device__ __forceinline__ uint32_t index_of(uint64_t k) { return 0xffffffffu - (uint32_t)k; }
 
 __device__ __forceinline__ int64_t token_at(const TokenLogprobs& a, int64_t r) {
   return a.idx_dt == DType::I64 ? ((const int64_t*)a.tokens)[r] : (int64_t)((const int32_t*)a.tokens)[r];
 }
 
-// One block per row: a pass for the maximum, one for the sums, one for each
-// alternative.
+// Part of a row as 16-byte vectors at 16-byte boundaries: vector v holds
+// elements v VE - mis ..; those outside [0, n) read as -inf.
 template <typename T>
-__global__ void __launch_bounds__(256) token_logprobs_row(LpArgs g) {
-  const TokenLogprobs& a = g.a;
-  __shared__ uint64_t shk[4];
-  __shared__ float shf[4];
-  const int64_t r = blockIdx.x;
-  const T* z = (const T*)a.z + r * a.ld;
-  const int tid = threadIdx.x;
-  uint64_t best = 0;
-  for (int64_t j = tid; j < a.V; j += 256) {
-    const uint64_t k = key_of(to_f(z[j]), (uint32_t)j);
-    best = k > best ? k : best;
+struct Span {
+  static constexpr int VE = 16 / (int)sizeof(T), NV = kCh / VE;
+  const T* z;
+  int64_t n;
+  int mis;
+  __device__ __forceinline__ Span(const T* p, int64_t len) : z(p), n(len) {
+    mis = (int)(((uintptr_t)p & 15) / sizeof(T));
   }
-  best = block_kmax<4>(best, shk);
-  const float m = to_f(z[0xffffffffu - (uint32_t)best]);
-  float ones = 0.f, rest = 0.f, dot = 0.f;
-  for (int64_t j = tid; j < a.V; j += 256) {
-    const float d = to_f(z[j]) - m, e = expf(d);
-    ones += d == 0.f ? 1.f : 0.f;
-    rest += d == 0.f ? 0.f : e;
-    dot += e == 0.f ? 0.f : e * d;
+  __device__ __forceinline__ int64_t steps() const { return (n + mis + (int64_t)kNT * kCh - 1) / ((int64_t)kNT * kCh); }
+  // element 0 of this thread's vector u of step c
+  __device__ __forceinline__ int64_t at(int64_t c, int u) const {
+    return ((c * NV + u) * kNT + threadIdx.x) * VE - mis;
   }
-  ones = block_add<4>(ones, shf);
-  rest = block_add<4>(rest, shf);
-  dot = block_add<4>(dot, shf);
-  const bool none = m == -INFINITY;
-  const float logl = none ? 0.f : log1pf((ones - 1.f) + rest), lse = none ? m : m + logl;
-  if (tid == 0) {
-    const int64_t t = token_at(a, r);
-    a.lp[r] = t < 0 || t >= a.V ? 0.f : none ? m : (to_f(z[t]) - m) - logl;
-    a.entropy[r] = none ? 0.f : logl - dot / (ones + rest);
-    a.lse[r] = lse;
-  }
-  for (int i = 0; i < a.top_k; ++i) {
-    if (i > 0) {
-      uint64_t next = 0;
-      for (int64_t j = tid; j < a.V; j += 256) {
-        const uint64_t k = key_of(to_f(z[j]), (uint32_t)j);
-        if (k < best && k > next) next = k;
+  __device__ __forceinline__ void load(int64_t c, uint4 (&raw)[NV]) const {
+    // the first and the last step reach over the ends
+    if (c > 0 && (c + 1) * kNT * kCh - mis <= n) {
+#pragma unroll
+      for (int u = 0; u < NV; ++u) raw[u] = *(const uint4*)(z + at(c, u));
+    } else {
+#pragma unroll
+      for (int u = 0; u < NV; ++u) {
+        const int64_t j = at(c, u);
+        T e[VE];
+        if (j >= 0 && j + VE <= n) {
+          const uint4 x = *(const uint4*)(z + j);
+          __builtin_memcpy(e, &x, 16);
+        } else {
+#pragma unroll
+          for (int i = 0; i < VE; ++i) e[i] = j + i >= 0 && j + i < n ? z[j + i] : from_f<T>(-INFINITY);
+        }
+        __builtin_memcpy(&raw[u], e, 16);
       }
-      best = block_kmax<4>(next, shk);
     }
-    if (tid == 0) {
-      const uint32_t j = 0xffffffffu - (uint32_t)best;
-      a.top_ids[r * a.top_k + i] = (int32_t)j;
-      a.top_lp[r * a.top_k + i] = none ? m : (to_f(z[j]) - m) - logl;
+  }
+  static __device__ __forceinline__ void floats(const uint4 (&raw)[NV], float (&f)[kCh]) {
+    T e[kCh];
+    __builtin_memcpy(e, raw, sizeof(e));
+#pragma unroll
+    for (int i = 0; i < kCh; ++i) f[i] = to_f(e[i]);
+  }
+};
+
+struct Stats {
+  float m, ones, rest, dot;  // maximum; number of elements at it; sums over the others, dot in log2 units
+};
+
+// One more part of the row.
+__device__ __forceinline__ void add_stats(Stats& s, const Stats& o) {
+  const float M = fmaxf(s.m, o.m);
+  const float d1 = s.m == M ? 0.f : fmaxf((s.m - M) * kLog2e, -200.f), d2 = o.m == M ? 0.f : fmaxf((o.m - M) * kLog2e, -200.f);
+  const float f1 = __builtin_amdgcn_exp2f(d1), f2 = __builtin_amdgcn_exp2f(d2);
+  const float l1 = s.ones + s.rest, l2 = o.ones + o.rest;
+  s.dot = f1 * (s.dot + l1 * d1) + f2 * (o.dot + l2 * d2);
+  s.rest = (d1 == 0.f ? s.rest : f1 * l1) + (d2 == 0.f ? o.rest : f2 * l2);
+  s.ones = (d1 == 0.f ? s.ones : 0.f) + (d2 == 0.f ? o.ones : 0.f);
+  s.m = M;
+}
+
+__device__ __forceinline__ Stats wave_stats(Stats s) {
+#pragma unroll
+  for (int x = 32; x >= 1; x >>= 1) {
+    const Stats o{__shfl_xor(s.m, x, 64), __shfl_xor(s.ones, x, 64), __shfl_xor(s.rest, x, 64), __shfl_xor(s.dot, x, 64)};
+    add_stats(s, o);
+  }
+  return s;
+}
+
+// The outputs of row r from the whole row's statistics; returns what is
+// taken from a logit for its log probability.
+__device__ __forceinline__ void finish_row(const TokenLogprobs& a, int64_t r, float z_t, int64_t t, const Stats& s,
+                                           float* m_out, float* logl_out) {
+  const bool none = s.ones + s.rest == 0.f;  // every logit is -inf
+  const float m = none ? -INFINITY : s.m;
+  const float logl = none ? 0.f : log1pf((s.ones - 1.f) + s.rest);
+  if (threadIdx.x == 0) {
+    a.lp[r] = t < 0 || t >= a.V ? 0.f : none ? m : (z_t - m) - logl;
+    a.entropy[r] = none ? 0.f : logl - s.dot * kLn2 / (s.ones + s.rest);
+    a.lse[r] = m + logl;
+  }
+  *m_out = m;
+  *logl_out = logl;
+}
+
+__device__ __forceinline__ float logp_of(float z, float m, float logl) { return m == -INFINITY ? m : (z - m) - logl; }
+
+struct TopShared {
+  uint64_t list[kCap];
+  uint64_t group[64], red[kNW], floor;
+  int count;
+};
+
+__device__ __forceinline__ uint64_t shfl64(uint64_t v, int x) {
+  return ((uint64_t)(uint32_t)__shfl_xor((int)(v >> 32), x, 64) << 32) | (uint32_t)__shfl_xor((int)(uint32_t)v, x, 64);
+}
+
+// The n keys in list, sorted: those of rank < k go to put(rank, key).
+template <typename F>
+__device__ __forceinline__ void rank_keys(const uint64_t* list, int n, int k, F&& put) {
+  for (int i = threadIdx.x; i < n; i += blockDim.x) {
+    const uint64_t me = list[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += list[j] > me ? 1 : 0;
+    if (rank < k) put(rank, me);
+  }
+}
+
+// f(key) for each element of this thread's step c that lies in the span.
+template <typename T, typename F>
+__device__ __forceinline__ void keys_of_step(const Span<T>& sp, uint32_t j0, int64_t c, F&& f) {
+  uint4 raw[Span<T>::NV];
+  float x[kCh];
+  sp.load(c, raw);
+  Span<T>::floats(raw, x);
+#pragma unroll
+  for (int i = 0; i < kCh; ++i) {
+    const int64_t j = sp.at(c, i / Span<T>::VE) + i % Span<T>::VE;
+    if (j >= 0 && j < sp.n) f(key_of(x[i], (uint32_t)j + j0));
+  }
+}
+
+// The k largest keys of the span (indices from j0) in order, by put(rank,
+// key).  best_step: the step of this thread's first largest element; plain:
+// no NaN or +inf among the elements.
+//
+// A lower bound of the k-th largest key is the k-th largest of the maxima of
+// 64 groups of threads.  Only threads whose own maximum reaches it look at
+// their elements again (the L2 has them), and what reaches it, little more
+// than k elements of an ordinary row, is sorted by counting.  Where more than
+// kCap do (the largest of a row gathered in a few threads' elements), and in
+// rows that are not plain, one maximum after another is searched.
+template <typename T, typename F>
+__device__ void top_keys(const Span<T>& sp, uint32_t j0, int k, int64_t best_step, bool plain, TopShared& sh, F&& put) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t steps = sp.steps();
+  bool one_by_one = !plain;
+  if (plain) {
+    constexpr int GL = kNT / 64;  // threads of a group
+    uint64_t mine = 0;
+    keys_of_step(sp, j0, best_step, [&](uint64_t key) { mine = key > mine ? key : mine; });
+    uint64_t gm = mine;
+#pragma unroll
+    for (int x = 1; x < GL; x <<= 1) {
+      const uint64_t o = shfl64(gm, x);
+      gm = o > gm ? o : gm;
+    }
+    if (lane % GL == 0) sh.group[tid / GL] = gm;
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
+    if (wave == 0) {
+      const uint64_t v = sh.group[lane];
+      int rank = 0;
+      for (int i = 0; i < 64; ++i) {
+        const uint64_t o = sh.group[i];
+        rank += o > v || (o == v && i < lane) ? 1 : 0;
+      }
+      if (rank == k - 1) sh.floor = v;
+    }
+    __syncthreads();
+    const uint64_t floor = sh.floor;
+    if (mine >= floor)
+      for (int64_t c = 0; c < steps; ++c)
+        keys_of_step(sp, j0, c, [&](uint64_t key) {
+          if (key >= floor) {
+            const int at = atomicAdd(&sh.count, 1);
+            if (at < kCap) sh.list[at] = key;
+          }
+        });
+    __syncthreads();
+    const int n = sh.count;
+    if (n <= kCap) {
+      rank_keys(sh.list, n, k, put);
+      for (int i = n + tid; i < k; i += kNT) put(i, 0);  // a span of fewer than k elements
+    } else {
+      one_by_one = true;
+    }
+  }
+  if (one_by_one) {
+    uint64_t last = ~0ull;
+    for (int i = 0; i < k; ++i) {
+      uint64_t next = 0;
+      if (last)
+        for (int64_t c = 0; c < steps; ++c)
+          keys_of_step(sp, j0, c, [&](uint64_t key) {
+            if (key < last && key > next) next = key;
+          });
+#pragma unroll
+      for (int x = 32; x >= 1; x >>= 1) {
+        const uint64_t o = shfl64(next, x);
+        next = o > next ? o : next;
+      }
+      __syncthreads();
+      if (lane == 0) sh.red[wave] = next;
+      __syncthreads();
+      last = sh.red[0];
+      for (int x = 1; x < kNW; ++x) last = sh.red[x] > last ? sh.red[x] : last;
+      if (tid == 0) put(i, last);
     }
   }
 }
 
+// log p of a key's element: z - lse in the form that lp has.
+__device__ __forceinline__ float logp_of(uint64_t key, float m, float logl) {
+  const uint32_t o = (uint32_t)(key >> 32);
+  const float z = o == 0xffffffffu ? NAN : __uint_as_float((o >> 31) ? o & 0x7fffffffu : ~o);
+  return m == -INFINITY ? m : (z - m) - logl;
+}
+
 template <typename T>
+__global__ void __launch_bounds__(kNT, 4) token_logprobs_kernel(LpArgs g) {
+  const TokenLogprobs& a = g.a;
+  __shared__ TopShared sh;
+  __shared__ Stats wave_s[kNW];
+  const int tid = threadIdx.x;
+  const int split = (int)(blockIdx.x % (unsigned)g.splits);
+  const int64_t r = blockIdx.x / (unsigned)g.splits, j0 = split * g.chunk;
+  const int64_t n = j0 + g.chunk < a.V ? g.chunk : a.V - j0;
+  const T* z = (const T*)a.z + r * a.ld;
+  const Span<T> sp(z + j0, n);
+  const int64_t steps = sp.steps();
+
+  float m = kLowest, l = 0.f, rest = 0.f, dot = 0.f, best = -INFINITY;
+  int64_t best_step = 0;
+  uint4 cur[Span<T>::NV], nxt[Span<T>::NV];
+  sp.load(0, cur);
+  for (int64_t c = 0; c < steps; ++c) {
+    if (c + 1 < steps) sp.load(c + 1, nxt);
+    float x[kCh];
+    Span<T>::floats(cur, x);
+    float top = x[0];
+#pragma unroll
+    for (int i = 1; i < kCh; ++i) top = fmaxf(top, x[i]);
+    if (top > best) { best = top; best_step = c; }
+    if (top > m) {
+      const float d = fmaxf((m - top) * kLog2e, -200.f), f = __builtin_amdgcn_exp2f(d);
+      dot = f * (dot + l * d);
+      l *= f;
+      rest = l;
+      m = top;
+    }
+#pragma unroll
+    for (int i = 0; i < kCh; ++i) {
+      // (a NaN stays one; -inf gives e = 0 and 0 to the sum of e d)
+      const float d = __builtin_elementwise_maximum((x[i] - m) * kLog2e, -200.f);
+      const float e = __builtin_amdgcn_exp2f(d);
+      l += e;
+      rest += __builtin_amdgcn_fractf(e);  // 0 for the elements at the maximum
+      dot += e * d;
+    }
+#pragma unroll
+    for (int u = 0; u < Span<T>::NV; ++u) cur[u] = nxt[u];
+  }
+  Stats s = wave_stats(Stats{m, rintf(l - rest), rest, dot});
+  if ((tid & 63) == 0) wave_s[tid >> 6] = s;
+  __syncthreads();
+  s = wave_s[0];
+#pragma unroll
+  for (int w = 1; w < kNW; ++w) add_stats(s, wave_s[w]);
+  const bool plain = s.dot == s.dot && s.rest == s.rest;
+
+  if (g.splits == 1) {
+    const int64_t t = token_at(a, r);
+    float mm, logl;
+    finish_row(a, r, t >= 0 && t < a.V ? to_f(z[t]) : 0.f, t, s, &mm, &logl);
+    if (a.top_k)
+      top_keys(sp, 0u, a.top_k, best_step, plain, sh, [&](int rank, uint64_t key) {
+        a.top_ids[r * a.top_k + rank] = (int32_t)index_of(key);
+        a.top_lp[r * a.top_k + rank] = logp_of(key, mm, logl);
+      });
+  } else {
+    const int64_t at = r * g.splits + split;
+    if (tid == 0) g.stats[at] = float4{s.m, s.ones, s.rest, s.dot};
+    if (a.top_k)
+      top_keys(sp, (uint32_t)j0, a.top_k, best_step, plain, sh,
+               [&](int rank, uint64_t key) { g.keys[at * a.top_k + rank] = key; });
+  }
+}
+
+// One block per row: its splits' statistics in order, and the largest of
+// their keys.
+template <typename T>
+__global__ void __launch_bounds__(256) token_logprobs_merge(LpArgs g) {
+  const TokenLogprobs& a = g.a;
+  __shared__ uint64_t list[64 * kTopKMax];
+  const int64_t r = blockIdx.x, t = token_at(a, r);
+  Stats s{kLowest, 0.f, 0.f, 0.f};
+  for (int i = 0; i < g.splits; ++i) {
+    const float4 x = g.stats[r * g.splits + i];
+    add_stats(s, Stats{x.x, x.y, x.z, x.w});
+  }
+  const T* z = (const T*)a.z + r * a.ld;
+  float mm, logl;
+  finish_row(a, r, t >= 0 && t < a.V ? to_f(z[t]) : 0.f, t, s, &mm, &logl);
+  if (!a.top_k) return;
+  const int n = g.splits * a.top_k;
+  for (int i = threadIdx.x; i < n; i += 256) list[i] = g.keys[r * n + i];
+  __syncthreads();
+  rank_keys(list, n, a.top_k, [&](int rank, uint64_t key) {
+    if (key == 0) return;  // (a row has at least top_k elements)
+    a.top_ids[r * a.top_k + rank] = (int32_t)index_of(key);
+    a.top_lp[r * a.top_k + rank] = logp_of(key, mm, logl);
+  });
+}
+
+// 16 logits a thread; VEC: the rows of z and dz are aligned alike.
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) token_logprobs_grad(LpArgs g, const float* __restrict__ g_lp,
                                                            const float* __restrict__ g_h, T* __restrict__ dz) {
   const TokenLogprobs& a = g.a;
+  constexpr int VE = 16 / (int)sizeof(T);
   const int64_t r = blockIdx.x, t = token_at(a, r);
   const T* z = (const T*)a.z + r * a.ld;
+  T* out = dz + r * a.V;
   const float lse = a.lse[r];
+  const bool none = lse == -INFINITY;
   const float gl = t >= 0 && t < a.V ? g_lp[r] : 0.f, gh = g_h ? g_h[r] : 0.f, H = g_h ? a.entropy[r] : 0.f;
-  for (int64_t j = (int64_t)blockIdx.y * 256 + threadIdx.x; j < a.V; j += (int64_t)gridDim.y * 256) {
-    float v = 0.f;
-    if (lse != -INFINITY) {
-      const float lp = to_f(z[j]) - lse, p = expf(lp);
-      v = (j == t ? gl : 0.f) - p * gl;
-      if (p != 0.f) v -= gh * p * (lp + H);
+  const float c0 = gl + gh * H, c1 = gh * kLn2;
+  // -p (g_lp + g_H (log p + H)), + g_lp at the token
+  auto grad = [&](float x, int64_t j) __attribute__((always_inline)) {
+    const float d = __builtin_elementwise_maximum((x - lse) * kLog2e, -200.f);
+    const float v = -__builtin_amdgcn_exp2f(d) * (c0 + c1 * d);
+    return none ? 0.f : j == t ? v + gl : v;
+  };
+  if constexpr (VEC) {
+    const int mis = (int)(((uintptr_t)z & 15) / sizeof(T));
+    const int64_t vecs = (a.V + mis + VE - 1) / VE;
+    for (int64_t v = (int64_t)blockIdx.y * 256 + threadIdx.x; v < vecs; v += (int64_t)gridDim.y * 256) {
+      const int64_t j = v * VE - mis;
+      if (j >= 0 && j + VE <= a.V) {
+        const uint4 raw = *(const uint4*)(z + j);
+        T e[VE];
+        __builtin_memcpy(e, &raw, 16);
+#pragma unroll
+        for (int i = 0; i < VE; ++i) e[i] = from_f<T>(grad(to_f(e[i]), j + i));
+        uint4 o;
+        __builtin_memcpy(&o, e, 16);
+        *(uint4*)(out + j) = o;
+      } else {
+        for (int i = 0; i < VE; ++i)
+          if (j + i >= 0 && j + i < a.V) out[j + i] = from_f<T>(grad(to_f(z[j + i]), j + i));
+      }
     }
-    dz[r * a.V + j] = from_f<T>(v);
+  } else {
+    for (int64_t j = (int64_t)blockIdx.y * 256 + threadIdx.x; j < a.V; j += (int64_t)gridDim.y * 256)
+      out[j] = from_f<T>(grad(to_f(z[j]), j));
   }
+}
+
+LpArgs plan(const TokenLogprobs& a) {
+  LpArgs g{};
+  g.a = a;
+  // rows that fill the CUs take a block each; fewer are split, in parts of at
+  // least 4096 logits
+  int64_t want = a.R > 0 && a.R < 512 ? (512 + a.R - 1) / a.R : 1;
+  const int64_t most = (a.V + 4095) / 4096;
+  if (want > most) want = most;
+  if (want > 64) want = 64;
+  g.chunk = ((a.V + want - 1) / want + 4095) / 4096 * 4096;
+  g.splits = (int)((a.V + g.chunk - 1) / g.chunk);
+  return g;
 }
 
 }  // namespace
 
-size_t token_logprobs_ws_bytes(const TokenLogprobs&) { return 0; }
+size_t token_logprobs_ws_bytes(const TokenLogprobs& a) {
+  const LpArgs g = plan(a);
+  return g.splits <= 1 ? 0 : (size_t)a.R * g.splits * (sizeof(float4) + a.top_k * sizeof(uint64_t));
+}
 
 void token_logprobs(const TokenLogprobs& a, void* ws, hipStream_t s) {
-  (void)ws;
   if (a.R == 0) return;
-  if (a.R > 0x7fffffffLL) fail("token_logprobs: too many rows");
-  LpArgs g{a};
-  AGPU_FLOAT_SWITCH(a.dt, hipLaunchKernelGGL((token_logprobs_row<T>), dim3((unsigned)a.R), dim3(256), 0, s, g));
+  LpArgs g = plan(a);
+  if (a.R * g.splits > 0x7fffffffLL) fail("token_logprobs: too many rows");
+  if (g.splits > 1) {
+    if (!ws) fail("token_logprobs: workspace missing");
+    g.stats = (float4*)ws;
+    g.keys = (uint64_t*)(g.stats + a.R * g.splits);
+  }
+  AGPU_FLOAT_SWITCH(a.dt, {
+    hipLaunchKernelGGL((token_logprobs_kernel<T>), dim3((unsigned)(a.R * g.splits)), dim3(kNT), 0, s, g);
+    if (g.splits > 1) hipLaunchKernelGGL((token_logprobs_merge<T>), dim3((unsigned)a.R), dim3(256), 0, s, g);
+  });
   check_launch("token_logprobs");
 }
 
 void token_logprobs_backward(const TokenLogprobs& a, const float* g_lp, const float* g_H, void* dz, hipStream_t s) {
   if (a.R == 0) return;
-  LpArgs g{a};
-  int64_t by = (a.V + 2047) / 2048;
-  if (by > 65535) by = 65535;
   if (a.R > 0x7fffffffLL) fail("token_logprobs_backward: too many rows");
-  AGPU_FLOAT_SWITCH(a.dt, hipLaunchKernelGGL((token_logprobs_grad<T>), dim3((unsigned)a.R, (unsigned)by), dim3(256), 0,
-                                             s, g, g_lp, g_H, (T*)dz));
+  LpArgs g{};
+  g.a = a;
+  const int64_t es = (int64_t)dtype_size(a.dt);
+  const bool vec = ((uintptr_t)a.z & 15) == ((uintptr_t)dz & 15) && (a.ld - a.V) * es % 16 == 0;
+  const int64_t per = 256 * 16 / es * 2;
+  int64_t by = (a.V + per - 1) / per;
+  if (by > 65535) by = 65535;
+  const dim3 grid((unsigned)a.R, (unsigned)by);
+  AGPU_FLOAT_SWITCH(a.dt, {
+    if (vec) hipLaunchKernelGGL((token_logprobs_grad<T, true>), grid, dim3(256), 0, s, g, g_lp, g_H, (T*)dz);
+    else hipLaunchKernelGGL((token_logprobs_grad<T, false>), grid, dim3(256), 0, s, g, g_lp, g_H, (T*)dz);
+  });
   check_launch("token_logprobs_backward");
 }
 
