@@ -567,6 +567,7 @@ struct TokenLogprobs {
   float* top_lp = nullptr; int32_t* top_ids = nullptr;
 };
 constexpr int kTopKMax = 32;
+constexpr int64_t kLogitsMax = (int64_t)1 << 30;  // V
 size_t token_logprobs_ws_bytes(const TokenLogprobs& a);
 void token_logprobs(const TokenLogprobs& a, void* ws, hipStream_t s);
 // dz[r, j] = g_lp[r] (1[j = token r] - p_j) - g_H[r] p_j (log p_j + H[r]),

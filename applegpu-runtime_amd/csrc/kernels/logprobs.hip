@@ -52,41 +52,37 @@ __device__ __forceinline__ int64_t token_at(const TokenLogprobs& a, int64_t r) {
   return a.idx_dt == DType::I64 ? ((const int64_t*)a.tokens)[r] : (int64_t)((const int32_t*)a.tokens)[r];
 }
 
-// Part of a row as 16-byte vectors at 16-byte boundaries: vector v holds
-// elements v VE - mis ..; those outside [0, n) read as -inf.
+// Part of a row as 16-byte vectors at 16-byte boundaries, and the few elements
+// before the first and behind the last of them, one each for the first threads.
 template <typename T>
 struct Span {
   static constexpr int VE = 16 / (int)sizeof(T), NV = kCh / VE;
-  const T* z;
-  int64_t n;
-  int mis;
-  __device__ __forceinline__ Span(const T* p, int64_t len) : z(p), n(len) {
-    mis = (int)(((uintptr_t)p & 15) / sizeof(T));
+  const T* z;      // the first vector
+  int head, vecs;  // elements before it; vectors
+  int edge;        // index of this thread's single element, or -1
+  __device__ __forceinline__ Span(const T* p, int n) {
+    const int mis = (int)(((uintptr_t)p & 15) / sizeof(T));
+    head = mis ? VE - mis : 0;
+    head = head < n ? head : n;
+    z = p + head;
+    vecs = (n - head) / VE;
+    const int tid = (int)threadIdx.x, tail = n - head - vecs * VE;
+    edge = tid < head ? tid : tid < head + tail ? vecs * VE + tid : -1;
   }
-  __device__ __forceinline__ int64_t steps() const { return (n + mis + (int64_t)kNT * kCh - 1) / ((int64_t)kNT * kCh); }
-  // element 0 of this thread's vector u of step c
-  __device__ __forceinline__ int64_t at(int64_t c, int u) const {
-    return ((c * NV + u) * kNT + threadIdx.x) * VE - mis;
-  }
-  __device__ __forceinline__ void load(int64_t c, uint4 (&raw)[NV]) const {
-    // the first and the last step reach over the ends
-    if (c > 0 && (c + 1) * kNT * kCh - mis <= n) {
+  __device__ __forceinline__ int steps() const { return (vecs + kNT * NV - 1) / (kNT * NV); }
+  // this thread's vector u of step c
+  static __device__ __forceinline__ int vec(int c, int u) { return (c * NV + u) * kNT + (int)threadIdx.x; }
+  // index of element i of its step c
+  __device__ __forceinline__ int at(int c, int i) const { return head + vec(c, i / VE) * VE + i % VE; }
+  __device__ __forceinline__ void load(int c, uint4 (&raw)[NV]) const {
 #pragma unroll
-      for (int u = 0; u < NV; ++u) raw[u] = *(const uint4*)(z + at(c, u));
-    } else {
+    for (int u = 0; u < NV; ++u) {
+      const int v = vec(c, u);
+      T e[VE];
 #pragma unroll
-      for (int u = 0; u < NV; ++u) {
-        const int64_t j = at(c, u);
-        T e[VE];
-        if (j >= 0 && j + VE <= n) {
-          const uint4 x = *(const uint4*)(z + j);
-          __builtin_memcpy(e, &x, 16);
-        } else {
-#pragma unroll
-          for (int i = 0; i < VE; ++i) e[i] = j + i >= 0 && j + i < n ? z[j + i] : from_f<T>(-INFINITY);
-        }
-        __builtin_memcpy(&raw[u], e, 16);
-      }
+      for (int i = 0; i < VE; ++i) e[i] = from_f<T>(-INFINITY);
+      __builtin_memcpy(&raw[u], e, 16);
+      if (v < vecs) raw[u] = *(const uint4*)(z + (int64_t)v * VE);
     }
   }
   static __device__ __forceinline__ void floats(const uint4 (&raw)[NV], float (&f)[kCh]) {
@@ -140,9 +136,24 @@ __device__ __forceinline__ void finish_row(const TokenLogprobs& a, int64_t r, fl
 
 __device__ __forceinline__ float logp_of(float z, float m, float logl) { return m == -INFINITY ? m : (z - m) - logl; }
 
+// The logit of a key.
+__device__ __forceinline__ float value_of(uint64_t key) {
+  const uint32_t o = (uint32_t)(key >> 32);
+  return o == 0xffffffffu ? NAN : __uint_as_float((o >> 31) ? o & 0x7fffffffu : ~o);
+}
+
+// log p of a key's element: z - lse in the form that lp has.
+__device__ __forceinline__ float logp_of(uint64_t key, float m, float logl) {
+  return m == -INFINITY ? m : (value_of(key) - m) - logl;
+}
+
+constexpr int kSlots = 8;  // maxima of a thread's steps that are kept, step c in slot c % kSlots
+
 struct TopShared {
   uint64_t list[kCap];
-  uint64_t group[64], red[kNW], floor;
+  float top[kSlots][kNT];
+  uint64_t group[kNW][64], red[kNW], floor;
+  int rank[64];
   int count;
 };
 
@@ -156,74 +167,105 @@ __device__ __forceinline__ void rank_keys(const uint64_t* list, int n, int k, F&
   for (int i = threadIdx.x; i < n; i += blockDim.x) {
     const uint64_t me = list[i];
     int rank = 0;
+#pragma unroll 8
     for (int j = 0; j < n; ++j) rank += list[j] > me ? 1 : 0;
     if (rank < k) put(rank, me);
   }
 }
 
-// f(key) for each element of this thread's step c that lies in the span.
+// f(key) for each element of this thread's step c that is not below `least`.
 template <typename T, typename F>
-__device__ __forceinline__ void keys_of_step(const Span<T>& sp, uint32_t j0, int64_t c, F&& f) {
+__device__ __forceinline__ void keys_of_step(const Span<T>& sp, uint32_t j0, int c, float least, F&& f) {
   uint4 raw[Span<T>::NV];
   float x[kCh];
   sp.load(c, raw);
   Span<T>::floats(raw, x);
+  float top = x[0];
+#pragma unroll
+  for (int i = 1; i < kCh; ++i) top = fmaxf(top, x[i]);
+  if (top < least) return;
 #pragma unroll
   for (int i = 0; i < kCh; ++i) {
-    const int64_t j = sp.at(c, i / Span<T>::VE) + i % Span<T>::VE;
-    if (j >= 0 && j < sp.n) f(key_of(x[i], (uint32_t)j + j0));
+    if (!(x[i] < least) && sp.vec(c, i / Span<T>::VE) < sp.vecs) f(key_of(x[i], (uint32_t)sp.at(c, i) + j0));
   }
 }
 
-// The k largest keys of the span (indices from j0) in order, by put(rank,
-// key).  best_step: the step of this thread's first largest element; plain:
-// no NaN or +inf among the elements.
-//
-// A lower bound of the k-th largest key is the k-th largest of the maxima of
-// 64 groups of threads.  Only threads whose own maximum reaches it look at
-// their elements again (the L2 has them), and what reaches it, little more
-// than k elements of an ordinary row, is sorted by counting.  Where more than
-// kCap do (the largest of a row gathered in a few threads' elements), and in
-// rows that are not plain, one maximum after another is searched.
-template <typename T, typename F>
-__device__ void top_keys(const Span<T>& sp, uint32_t j0, int k, int64_t best_step, bool plain, TopShared& sh, F&& put) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t steps = sp.steps();
-  bool one_by_one = !plain;
-  if (plain) {
-    constexpr int GL = kNT / 64;  // threads of a group
-    uint64_t mine = 0;
-    keys_of_step(sp, j0, best_step, [&](uint64_t key) { mine = key > mine ? key : mine; });
-    uint64_t gm = mine;
+// In sh.floor the k-th largest of the keys that 64 groups of threads have, a
+// group being the threads of one lane of each wave (mine: the largest of this
+// thread); ends with a barrier.
+__device__ __forceinline__ void group_floor(TopShared& sh, uint64_t mine, int k) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  sh.group[wave][lane] = mine;
+  if (tid < 64) sh.rank[tid] = 0;
+  if (tid == 0) sh.count = 0;
+  __syncthreads();
+  uint64_t v = sh.group[0][lane];
 #pragma unroll
-    for (int x = 1; x < GL; x <<= 1) {
-      const uint64_t o = shfl64(gm, x);
-      gm = o > gm ? o : gm;
+  for (int w = 1; w < kNW; ++w) v = sh.group[w][lane] > v ? sh.group[w][lane] : v;
+  int rank = 0;   // this wave's share of the groups
+#pragma unroll
+  for (int i = 0; i < 64 / kNW; ++i) {
+    const int at = wave * (64 / kNW) + i;
+    const uint64_t o = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), at) << 32) |
+                       (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, at);
+    rank += o > v || (o == v && at < lane) ? 1 : 0;
+  }
+  if (rank) atomicAdd(&sh.rank[lane], rank);
+  __syncthreads();
+  if (wave == 0 && sh.rank[lane] == k - 1) sh.floor = v;
+  __syncthreads();
+}
+
+// The k largest keys of the span (indices from j0) in order, by put(rank,
+// key).  edge: the thread's single element; best: its largest (the maxima of
+// its steps are in sh.top); plain: no NaN or +inf among the elements.
+//
+// A lower bound of the k-th largest is the k-th largest of the maxima of 64
+// groups of threads.  Only the steps whose own maximum reaches it are looked
+// at again, and what reaches it, little more than k elements of an ordinary
+// row, is sorted by counting.  Rows in which more than kCap elements do are
+// those with many equal to the bound: they are bounded once more, with the
+// index as part of the order.  Where that leaves too many as well (the
+// largest of a row gathered in a few threads' elements), and in rows that are
+// not plain, one maximum after another is searched.
+template <typename T, typename F>
+__device__ __forceinline__ void top_keys(const Span<T>& sp, uint32_t j0, int k, float edge, float best, bool plain,
+                                         TopShared& sh, F&& put) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int steps = sp.steps();
+  bool one_by_one = !plain;
+  const uint64_t edge_key = sp.edge >= 0 ? key_of(edge, (uint32_t)sp.edge + j0) : 0;
+  auto add = [&](uint64_t key) {
+    const int at = atomicAdd(&sh.count, 1);
+    if (at < kCap) sh.list[at] = key;
+  };
+  if (plain) {
+    group_floor(sh, key_of(best, 0xffffffffu), k);
+    const float least = value_of(sh.floor);
+    if (best >= least) {
+      if (edge_key && edge >= least) add(edge_key);
+      for (int c = 0; c < steps; ++c)
+        if (sh.top[c % kSlots][tid] >= least) keys_of_step(sp, j0, c, least, add);
     }
-    if (lane % GL == 0) sh.group[tid / GL] = gm;
-    if (tid == 0) sh.count = 0;
     __syncthreads();
-    if (wave == 0) {
-      const uint64_t v = sh.group[lane];
-      int rank = 0;
-      for (int i = 0; i < 64; ++i) {
-        const uint64_t o = sh.group[i];
-        rank += o > v || (o == v && i < lane) ? 1 : 0;
+    int n = sh.count;
+    if (n > kCap) {
+      uint64_t mine = edge_key;
+      for (int c = 0; c < steps; ++c)
+        keys_of_step(sp, j0, c, best, [&](uint64_t key) { mine = key > mine ? key : mine; });
+      __syncthreads();
+      group_floor(sh, mine, k);
+      const uint64_t floor = sh.floor;
+      if (mine >= floor) {
+        if (edge_key && edge_key >= floor) add(edge_key);
+        for (int c = 0; c < steps; ++c)
+          keys_of_step(sp, j0, c, floor ? value_of(floor) : -INFINITY, [&](uint64_t key) {
+            if (key >= floor) add(key);
+          });
       }
-      if (rank == k - 1) sh.floor = v;
+      __syncthreads();
+      n = sh.count;
     }
-    __syncthreads();
-    const uint64_t floor = sh.floor;
-    if (mine >= floor)
-      for (int64_t c = 0; c < steps; ++c)
-        keys_of_step(sp, j0, c, [&](uint64_t key) {
-          if (key >= floor) {
-            const int at = atomicAdd(&sh.count, 1);
-            if (at < kCap) sh.list[at] = key;
-          }
-        });
-    __syncthreads();
-    const int n = sh.count;
     if (n <= kCap) {
       rank_keys(sh.list, n, k, put);
       for (int i = n + tid; i < k; i += kNT) put(i, 0);  // a span of fewer than k elements
@@ -234,10 +276,10 @@ __device__ void top_keys(const Span<T>& sp, uint32_t j0, int k, int64_t best_ste
   if (one_by_one) {
     uint64_t last = ~0ull;
     for (int i = 0; i < k; ++i) {
-      uint64_t next = 0;
+      uint64_t next = edge_key < last ? edge_key : 0;
       if (last)
-        for (int64_t c = 0; c < steps; ++c)
-          keys_of_step(sp, j0, c, [&](uint64_t key) {
+        for (int c = 0; c < steps; ++c)
+          keys_of_step(sp, j0, c, -INFINITY, [&](uint64_t key) {
             if (key < last && key > next) next = key;
           });
 #pragma unroll
@@ -255,13 +297,6 @@ __device__ void top_keys(const Span<T>& sp, uint32_t j0, int k, int64_t best_ste
   }
 }
 
-// log p of a key's element: z - lse in the form that lp has.
-__device__ __forceinline__ float logp_of(uint64_t key, float m, float logl) {
-  const uint32_t o = (uint32_t)(key >> 32);
-  const float z = o == 0xffffffffu ? NAN : __uint_as_float((o >> 31) ? o & 0x7fffffffu : ~o);
-  return m == -INFINITY ? m : (z - m) - logl;
-}
-
 template <typename T>
 __global__ void __launch_bounds__(kNT, 4) token_logprobs_kernel(LpArgs g) {
   const TokenLogprobs& a = g.a;
@@ -272,21 +307,38 @@ __global__ void __launch_bounds__(kNT, 4) token_logprobs_kernel(LpArgs g) {
   const int64_t r = blockIdx.x / (unsigned)g.splits, j0 = split * g.chunk;
   const int64_t n = j0 + g.chunk < a.V ? g.chunk : a.V - j0;
   const T* z = (const T*)a.z + r * a.ld;
-  const Span<T> sp(z + j0, n);
-  const int64_t steps = sp.steps();
+  const Span<T> sp(z + j0, (int)n);
+  const int steps = sp.steps();
 
-  float m = kLowest, l = 0.f, rest = 0.f, dot = 0.f, best = -INFINITY;
-  int64_t best_step = 0;
+  float m = kLowest, l = 0.f, rest = 0.f, dot = 0.f;
+  // (a NaN stays one; -inf gives e = 0 and 0 to the sum of e d)
+  auto sum = [&](float x) __attribute__((always_inline)) {
+    const float d = __builtin_elementwise_maximum((x - m) * kLog2e, -200.f);
+    const float e = __builtin_amdgcn_exp2f(d);
+    l += e;
+    rest += __builtin_amdgcn_fractf(e);  // 0 for the elements at the maximum
+    dot += e * d;
+  };
+  const float edge = sp.edge >= 0 ? to_f(z[j0 + sp.edge]) : -INFINITY;
   uint4 cur[Span<T>::NV], nxt[Span<T>::NV];
   sp.load(0, cur);
-  for (int64_t c = 0; c < steps; ++c) {
+  if (a.top_k)
+    for (int i = 0; i < kSlots; ++i) sh.top[i][tid] = -INFINITY;
+  float best = edge == edge ? edge : -INFINITY;
+  m = fmaxf(m, best);
+  sum(edge);
+  for (int c = 0; c < steps; ++c) {
     if (c + 1 < steps) sp.load(c + 1, nxt);
     float x[kCh];
     Span<T>::floats(cur, x);
     float top = x[0];
 #pragma unroll
     for (int i = 1; i < kCh; ++i) top = fmaxf(top, x[i]);
-    if (top > best) { best = top; best_step = c; }
+    if (a.top_k) {
+      float* at = &sh.top[c % kSlots][tid];
+      *at = c < kSlots ? top : fmaxf(*at, top);
+      best = fmaxf(best, top);
+    }
     if (top > m) {
       const float d = fmaxf((m - top) * kLog2e, -200.f), f = __builtin_amdgcn_exp2f(d);
       dot = f * (dot + l * d);
@@ -295,14 +347,7 @@ __global__ void __launch_bounds__(kNT, 4) token_logprobs_kernel(LpArgs g) {
       m = top;
     }
 #pragma unroll
-    for (int i = 0; i < kCh; ++i) {
-      // (a NaN stays one; -inf gives e = 0 and 0 to the sum of e d)
-      const float d = __builtin_elementwise_maximum((x[i] - m) * kLog2e, -200.f);
-      const float e = __builtin_amdgcn_exp2f(d);
-      l += e;
-      rest += __builtin_amdgcn_fractf(e);  // 0 for the elements at the maximum
-      dot += e * d;
-    }
+    for (int i = 0; i < kCh; ++i) sum(x[i]);
 #pragma unroll
     for (int u = 0; u < Span<T>::NV; ++u) cur[u] = nxt[u];
   }
@@ -314,22 +359,24 @@ __global__ void __launch_bounds__(kNT, 4) token_logprobs_kernel(LpArgs g) {
   for (int w = 1; w < kNW; ++w) add_stats(s, wave_s[w]);
   const bool plain = s.dot == s.dot && s.rest == s.rest;
 
+  const int64_t at = r * g.splits + split;
+  float mm = 0.f, logl = 0.f;
   if (g.splits == 1) {
     const int64_t t = token_at(a, r);
-    float mm, logl;
     finish_row(a, r, t >= 0 && t < a.V ? to_f(z[t]) : 0.f, t, s, &mm, &logl);
-    if (a.top_k)
-      top_keys(sp, 0u, a.top_k, best_step, plain, sh, [&](int rank, uint64_t key) {
-        a.top_ids[r * a.top_k + rank] = (int32_t)index_of(key);
-        a.top_lp[r * a.top_k + rank] = logp_of(key, mm, logl);
-      });
-  } else {
-    const int64_t at = r * g.splits + split;
-    if (tid == 0) g.stats[at] = float4{s.m, s.ones, s.rest, s.dot};
-    if (a.top_k)
-      top_keys(sp, (uint32_t)j0, a.top_k, best_step, plain, sh,
-               [&](int rank, uint64_t key) { g.keys[at * a.top_k + rank] = key; });
+  } else if (tid == 0) {
+    g.stats[at] = float4{s.m, s.ones, s.rest, s.dot};
   }
+  if (a.top_k)
+    top_keys(sp, (uint32_t)j0, a.top_k, edge, best, plain, sh, [&](int rank, uint64_t key) {
+      const int64_t to = at * a.top_k + rank;
+      if (g.splits > 1) {
+        g.keys[to] = key;
+      } else {
+        a.top_ids[to] = (int32_t)index_of(key);
+        a.top_lp[to] = logp_of(key, mm, logl);
+      }
+    });
 }
 
 // One block per row: its splits' statistics in order, and the largest of
@@ -405,13 +452,13 @@ __global__ void __launch_bounds__(256) token_logprobs_grad(LpArgs g, const float
 LpArgs plan(const TokenLogprobs& a) {
   LpArgs g{};
   g.a = a;
-  // rows that fill the CUs take a block each; fewer are split, in parts of at
-  // least 4096 logits
+  // rows that fill the CUs take a block each; fewer are split, in equal parts
+  // of at least 4096 logits
   int64_t want = a.R > 0 && a.R < 512 ? (512 + a.R - 1) / a.R : 1;
-  const int64_t most = (a.V + 4095) / 4096;
+  const int64_t most = a.V / 4096 > 0 ? a.V / 4096 : 1;
   if (want > most) want = most;
   if (want > 64) want = 64;
-  g.chunk = ((a.V + want - 1) / want + 4095) / 4096 * 4096;
+  g.chunk = ((a.V + want - 1) / want + 63) / 64 * 64;
   g.splits = (int)((a.V + g.chunk - 1) / g.chunk);
   return g;
 }

@@ -2171,7 +2171,7 @@ static k::TokenLogprobs logprob_rows(const char* name, const TensorP& logits, co
   lead->pop_back();
   if (lead->empty()) *lead = {1};
   const int64_t V = logits->shape[logits->ndim - 1];
-  if (V < 1 || V > 0x7fffffffLL) fail("%s: %lld logits in a row", name, (long long)V);
+  if (V < 1 || V > k::kLogitsMax) fail("%s: %lld logits in a row", name, (long long)V);
   if (tokens->dtype != DType::I32 && tokens->dtype != DType::I64)
     fail("%s: tokens must be int32 or int64, got %s", name, dtype_name(tokens->dtype));
   k::TokenLogprobs a;
