@@ -128,9 +128,12 @@ struct L4Args {
   int nw;  // waves of a block
 };
 
-// Steps of 128 columns whose codes a wave has in flight (one where a step is
-// much work: the registers go to the tiles).
-template <int MT> struct InFlight { static constexpr int value = MT == 1 ? 4 : 1; };
+// What a wave keeps in flight: UN steps of 128 columns of codes, and the rows
+// of XB steps (two where they fit the registers: those of the next step are
+// loaded before this one is multiplied).
+template <typename T, int MT, int NT> struct InFlight {
+  static constexpr int UN = NT == 1 ? 4 : 2, XB = sizeof(T) == 2 && MT <= 2 ? 2 : 1;
+};
 
 // MT tiles of 16 rows of x by NT tiles of 16 columns of the output; the waves
 // of a block take 128-deep steps of K in turn.  G: columns of a scale.  XVEC:
@@ -139,14 +142,15 @@ template <typename T, int MT, int NT, int G, bool XVEC>
 __global__ void __launch_bounds__(MT == 1 ? 1024 : 512) linear_int4_mfma(L4Args g) {
   typedef In4<T> I;
   typedef typename I::vec V;
-  constexpr int NG = 128 / G, kUn = InFlight<MT>::value;
+  constexpr int NG = 128 / G, UN = InFlight<T, MT, NT>::UN, XB = InFlight<T, MT, NT>::XB, XW = sizeof(T) / 2;
+  static_assert(UN % XB == 0, "the rows' buffers follow the steps");
   extern __shared__ float red[];  // [nw][MT][NT][16][16]
   const LinearInt4& a = g.a;
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, q = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int steps = (int)g.steps, nw = g.nw, K = (int)a.K, groups = (K + G - 1) / G;
   const int64_t tiles = (a.N + 15) / 16, tile0 = (int64_t)blockIdx.x * NT, m0 = (int64_t)blockIdx.y * (16 * MT);
   const T* sc = (const T*)a.scales;
-  const int64_t groups = (a.K + G - 1) / G;
 
   V minus;  // -24: takes off what the codes are too large by
 #pragma unroll
@@ -165,9 +169,49 @@ __global__ void __launch_bounds__(MT == 1 ? 1024 : 512) linear_int4_mfma(L4Args 
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
     const int64_t t = tile0 + j < tiles ? tile0 + j : tiles - 1;
-    wp[j] = (const uint4*)a.packed + t * g.steps * 64 + lane;
+    wp[j] = (const uint4*)a.packed + t * steps * 64 + lane;
     col[j] = t * 16 + c < a.N ? t * 16 + c : a.N - 1;
   }
+
+  uint4 wv[UN][NT];
+  T sv[UN][NT][NG];
+  auto load_w = [&](int u, int st) __attribute__((always_inline)) {
+    st = st < steps ? st : steps - 1;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      wv[u][j] = wp[j][(int64_t)st * 64];
+#pragma unroll
+      for (int i = 0; i < NG; ++i) {
+        const int gr = st * NG + i < groups ? st * NG + i : groups - 1;
+        sv[u][j][i] = sc[(int64_t)gr * a.N + col[j]];
+      }
+    }
+  };
+  // columns that word t of a lane's codes belongs to
+  auto k_of = [&](int st, int t) __attribute__((always_inline)) {
+    return st * 128 + (G < 128 ? 32 * t + 8 * q : 32 * q + 8 * t);
+  };
+  uint4 xr[XB][4][MT][XW];
+  auto load_x = [&](int b, int st) __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const int k = k_of(st, t);
+#pragma unroll
+        for (int e = 0; e < XW; ++e) xr[b][t][i][e] = uint4{0, 0, 0, 0};
+        if constexpr (XVEC) {
+          if (row_ok[i] && k < K)
+#pragma unroll
+            for (int e = 0; e < XW; ++e) xr[b][t][i][e] = ((const uint4*)(x[i] + k))[e];
+        } else {
+          T v[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = row_ok[i] && k + e < K ? x[i][k + e] : (T)0.f;
+          __builtin_memcpy(xr[b][t][i], v, sizeof(v));
+        }
+      }
+  };
 
   f4 tot[MT][NT];
 #pragma unroll
@@ -175,110 +219,95 @@ __global__ void __launch_bounds__(MT == 1 ? 1024 : 512) linear_int4_mfma(L4Args 
 #pragma unroll
     for (int j = 0; j < NT; ++j) tot[i][j] = f4{0.f, 0.f, 0.f, 0.f};
 
-  for (int64_t s0 = w; s0 < g.steps; s0 += (int64_t)g.nw * kUn) {
-    uint4 wv[kUn][NT];
-    T sv[kUn][NT][NG];
+  auto multiply = [&](int u, int b) __attribute__((always_inline)) {
+    uint32_t word[NT][4];
 #pragma unroll
-    for (int u = 0; u < kUn; ++u) {
-      int64_t st = s0 + (int64_t)u * g.nw;
-      st = st < g.steps ? st : s0;
+    for (int j = 0; j < NT; ++j) {
+      word[j][0] = wv[u][j].x; word[j][1] = wv[u][j].y; word[j][2] = wv[u][j].z; word[j][3] = wv[u][j].w;
+      if constexpr (G < 128) {
+        // lane (c, q) holds columns 32 q + 8 t of word t: exchanged between
+        // the four lanes of a row so that word t holds 32 t + 8 q, and one
+        // product covers 32 columns in a row, of one scale
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        wv[u][j] = wp[j][st * 64];
+        for (int t = 0; t < 2; ++t) {
+          const auto r = __builtin_amdgcn_permlane32_swap(word[j][t], word[j][t + 2], false, false);
+          word[j][t] = r[0]; word[j][t + 2] = r[1];
+        }
 #pragma unroll
-        for (int i = 0; i < NG; ++i) {
-          const int64_t gr = st * NG + i < groups ? st * NG + i : groups - 1;
-          sv[u][j][i] = sc[gr * a.N + col[j]];
+        for (int t = 0; t < 4; t += 2) {
+          const auto r = __builtin_amdgcn_permlane16_swap(word[j][t], word[j][t + 1], false, false);
+          word[j][t] = r[0]; word[j][t + 1] = r[1];
         }
       }
     }
 #pragma unroll
-    for (int u = 0; u < kUn; ++u) {
-      const int64_t st = s0 + (int64_t)u * g.nw;
-      if (st >= g.steps) break;
-      uint32_t word[NT][4];
+    for (int gr = 0; gr < NG; ++gr) {
+      f4 acc[MT][NT], cor[MT];
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        word[j][0] = wv[u][j].x; word[j][1] = wv[u][j].y; word[j][2] = wv[u][j].z; word[j][3] = wv[u][j].w;
-        if constexpr (G < 128) {
-          // lane (c, q) holds columns 32 q + 8 t of word t: exchanged between
-          // the four lanes of a row so that word t holds 32 t + 8 q, and one
-          // product covers 32 columns in a row, of one scale
+      for (int i = 0; i < MT; ++i) {
+        cor[i] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            const auto r = __builtin_amdgcn_permlane32_swap(word[j][t], word[j][t + 2], false, false);
-            word[j][t] = r[0]; word[j][t + 2] = r[1];
-          }
-#pragma unroll
-          for (int t = 0; t < 4; t += 2) {
-            const auto r = __builtin_amdgcn_permlane16_swap(word[j][t], word[j][t + 1], false, false);
-            word[j][t] = r[0]; word[j][t + 1] = r[1];
-          }
-        }
+        for (int j = 0; j < NT; ++j) acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
       }
 #pragma unroll
-      for (int gr = 0; gr < NG; ++gr) {
-        f4 acc[MT][NT], cor[MT];
+      for (int t = gr * 4 / NG; t < (gr + 1) * 4 / NG; ++t) {
+        V wf[NT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) wf[j] = codes24<T>(word[j][t]);
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-          cor[i] = f4{0.f, 0.f, 0.f, 0.f};
+          if constexpr (I::P == 1) {
+            V xf;
+            __builtin_memcpy(&xf, xr[b][t][i], 16);
+            cor[i] = I::mfma(xf, minus, cor[i]);
 #pragma unroll
-          for (int j = 0; j < NT; ++j) acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
-        }
+            for (int j = 0; j < NT; ++j) acc[i][j] = I::mfma(xf, wf[j], acc[i][j]);
+          } else {
+            float f[8];
+            __builtin_memcpy(f, xr[b][t][i], 32);
 #pragma unroll
-        for (int t = gr * 4 / NG; t < (gr + 1) * 4 / NG; ++t) {
-          const int64_t k = st * 128 + (G < 128 ? 32 * t + 8 * q : 32 * q + 8 * t);
-          V wf[NT];
-#pragma unroll
-          for (int j = 0; j < NT; ++j) wf[j] = codes24<T>(word[j][t]);
-#pragma unroll
-          for (int i = 0; i < MT; ++i) {
-            T xr[8];
-            if constexpr (XVEC) {
-              constexpr int NV = sizeof(T) / 2;
-              uint4 raw[NV];
-              const bool ok = row_ok[i] && k < a.K;
-#pragma unroll
-              for (int e = 0; e < NV; ++e) raw[e] = ok ? ((const uint4*)(x[i] + k))[e] : uint4{0, 0, 0, 0};
-              __builtin_memcpy(xr, raw, sizeof(xr));
-            } else {
-#pragma unroll
-              for (int e = 0; e < 8; ++e) xr[e] = row_ok[i] && k + e < a.K ? x[i][k + e] : (T)0.f;
-            }
-            if constexpr (I::P == 1) {
+            for (int p = 0; p < 3; ++p) {
               V xf;
-              __builtin_memcpy(&xf, xr, 16);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                xf[e] = (__bf16)f[e];
+                f[e] -= (float)xf[e];
+              }
               cor[i] = I::mfma(xf, minus, cor[i]);
 #pragma unroll
               for (int j = 0; j < NT; ++j) acc[i][j] = I::mfma(xf, wf[j], acc[i][j]);
-            } else {
-              float f[8];
-#pragma unroll
-              for (int e = 0; e < 8; ++e) f[e] = to_f(xr[e]);
-#pragma unroll
-              for (int p = 0; p < 3; ++p) {
-                V xf;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                  xf[e] = (__bf16)f[e];
-                  f[e] -= (float)xf[e];
-                }
-                cor[i] = I::mfma(xf, minus, cor[i]);
-#pragma unroll
-                for (int j = 0; j < NT; ++j) acc[i][j] = I::mfma(xf, wf[j], acc[i][j]);
-              }
             }
           }
         }
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          const float s = to_f(sv[u][j][gr]);
-#pragma unroll
-          for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) tot[i][j][e] += s * (acc[i][j][e] + cor[i][e]);
-        }
       }
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const float s = to_f(sv[u][j][gr]);
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) tot[i][j][e] += s * (acc[i][j][e] + cor[i][e]);
+      }
+      // (the groups' products one after another: together their sums would
+      // not fit the registers)
+      if constexpr (NG > 1 && MT * NT > 1) __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+
+  if (w < steps) {
+#pragma unroll
+    for (int u = 0; u < UN; ++u) load_w(u, w + u * nw);
+    if constexpr (XB == 2) load_x(0, w);
+  }
+  for (int s0 = w; s0 < steps; s0 += nw * UN) {
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+      const int st = s0 + u * nw;
+      if (st >= steps) break;
+      if constexpr (XB == 1) load_x(0, st);
+      else if (st + nw < steps) load_x((u + 1) % 2, st + nw);
+      multiply(u, u % XB);
+      if (st + nw * UN < steps) load_w(u, st + nw * UN);
     }
   }
 
@@ -351,7 +380,8 @@ void dequantize_int4(DType dt, const uint8_t* packed, const void* scales, int64_
 
 void linear_int4(const LinearInt4& a, hipStream_t s) {
   if (a.M == 0) return;
-  if (a.M > kInt4Rows || (a.N + 15) / 16 > 0x7fffffffLL) fail("linear_int4: too many rows or columns");
+  if (a.M > kInt4Rows || a.K > 0x7fffff00LL || (a.N + 15) / 16 > 0x7fffffffLL)
+    fail("linear_int4: too many rows or columns");
   L4Args g;
   g.a = a;
   g.steps = (a.K + 127) / 128;
@@ -361,7 +391,8 @@ void linear_int4(const LinearInt4& a, hipStream_t s) {
   const int most = mt == 1 ? 16 : 8;
   g.nw = (int)(g.steps < most ? g.steps : most);
   AGPU_FLOAT_SWITCH(a.dt, {
-    if (mt == 1) launch_int4_g<T, 1, 1>(g, xvec, s);
+    if (mt == 1 && (a.N + 15) / 16 < 512) launch_int4_g<T, 1, 1>(g, xvec, s);
+    else if (mt == 1) launch_int4_g<T, 1, 2>(g, xvec, s);
     else if (mt == 2) launch_int4_g<T, 2, 2>(g, xvec, s);
     else launch_int4_g<T, 4, 2>(g, xvec, s);
   });
