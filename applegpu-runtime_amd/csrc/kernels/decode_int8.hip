@@ -44,16 +44,22 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 
-constexpr int kNW = 4;           // waves of a block
 constexpr int kStep = 32;        // keys of a wave's step
-constexpr int kIter = kNW * kStep;
+constexpr int kFew = 4;  // waves of a block of a split context
+// A block keeps its waves' sums in LDS.
+size_t lds_bytes(const DecodeInt8& a, int waves) {
+  const int64_t R = a.G * a.Tq;
+  return (size_t)(R < 16 ? R : 16) * (a.D + 4) * sizeof(float) * waves;
+}
+constexpr int kSplits = 1024;    // most parts of a context
 constexpr float kLift = 7.f;     // log2 of the weight at the reference maximum
 constexpr float kSlack = 8.f;    // log2 by which a weight may exceed that
 
 struct D8Args {
   DecodeInt8 a;
   int lg_block, splits, q_tiles;
-  int64_t chunk;  // keys of a split, a multiple of kIter
+  int nw;         // waves of a block: 4, 8 or 16 (D = 128: 8 at most)
+  int64_t chunk;  // keys of a split
   float* part;     // [units][splits][16 (D + 2)]: O, m, l of each query column
 };
 
@@ -79,6 +85,22 @@ __device__ __forceinline__ h8 codes8(uint32_t w0, uint32_t w1) {
   return o;
 }
 
+// 8 consecutive query values, raw.
+template <typename T>
+struct Raw8q {
+  uint4 v[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = ((const uint4*)p)[i];
+  }
+  __device__ __forceinline__ void floats(float (&x)[8]) const {
+    T e[8];
+    __builtin_memcpy(e, v, sizeof(e));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = to_f(e[i]);
+  }
+};
+
 // A wave's codes of one 32-key step.
 template <int D>
 struct Step {
@@ -89,33 +111,105 @@ struct Step {
   float ks[2], vs[2];
 };
 
-template <typename T, int D>
-__global__ void __launch_bounds__(64 * kNW) decode_int8_mfma(D8Args g) {
+template <typename T, int D, int NW>
+__global__ void __launch_bounds__(64 * NW) decode_int8_mfma(D8Args g) {
   constexpr bool F32 = sizeof(T) == 4;
   constexpr int NK = D / 32;     // MFMAs of a score tile
   constexpr int ND = D / 16;     // tiles of the output's D
   constexpr int LD = D + 4;      // padding of a query's row in LDS
-  __shared__ float sm_o[kNW][16][LD];
-  __shared__ float sm_m[kNW][16], sm_l[kNW][16];
+  constexpr int64_t kIter = NW * kStep;
+  extern __shared__ float sm_o[];  // [NW][rows of the tile][LD]
+  __shared__ float sm_m[NW][16], sm_l[NW][16];
   const DecodeInt8& a = g.a;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, q4 = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int split = (int)(blockIdx.x % (unsigned)g.splits);
-  const int64_t unit = blockIdx.x / (unsigned)g.splits;
-  const int qt = (int)(unit % g.q_tiles);
-  const int64_t bh = unit / g.q_tiles, h = bh % a.H, b = bh / a.H;
+  const uint32_t unit = blockIdx.x / (uint32_t)g.splits, split = blockIdx.x % (uint32_t)g.splits;
+  const uint32_t bh = unit / (uint32_t)g.q_tiles, qt = unit % (uint32_t)g.q_tiles;
+  const uint32_t b = bh / (uint32_t)a.H, h = bh % (uint32_t)a.H;
   const int R = (int)(a.G * a.Tq);
+  const int64_t j_lo = (int64_t)split * g.chunk;
+  const int8_t* K = a.k.codes + b * a.k.cs[0] + h * a.k.cs[1];
+  const int8_t* V = a.v.codes + b * a.v.cs[0] + h * a.v.cs[1];
+  const float* KS = a.k.scales + b * a.k.ss[0] + h * a.k.ss[1];
+  const float* VS = a.v.scales + b * a.v.ss[0] + h * a.v.ss[1];
+  // this lane's bytes of a row, and its rows of a step
+  const uint32_t k_at = (D == 32 ? 8 : 16) * q4, v_at = (D / 16) * n;
+  const uint32_t k_st = (uint32_t)a.k.cs[2], v_st = (uint32_t)a.v.cs[2];
+  uint32_t k_off[2], v_off[8];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) k_off[t] = (16 * t + n) * k_st + k_at;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v_off[e] = (16 * (e >> 2) + 4 * q4 + (e & 3)) * v_st + v_at;
+
+  auto load = [&](Step<D>& s, int64_t j0) __attribute__((always_inline)) {
+    const int8_t* kb = K + j0 * a.k.cs[2];
+    const int8_t* vb = V + j0 * a.v.cs[2];
+    // the last step of the cache reads its last row in place of those behind
+    const bool inside = j0 + kStep <= a.Tmax;
+    const uint32_t last = inside ? 0 : (uint32_t)(a.Tmax - 1 - j0);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      uint32_t off = k_off[t];
+      if (!inside) {
+        const uint32_t end = last * k_st + k_at;
+        off = off < end ? off : end;
+      }
+      const int8_t* p = kb + off;
+      if constexpr (D == 32) {
+        const uint2 x = *(const uint2*)p;
+        s.k[t][0] = x.x; s.k[t][1] = x.y;
+      } else {
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) {
+          const uint4 x = *(const uint4*)(p + 64 * c);
+          s.k[t][4 * c] = x.x; s.k[t][4 * c + 1] = x.y; s.k[t][4 * c + 2] = x.z; s.k[t][4 * c + 3] = x.w;
+        }
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      uint32_t off = v_off[e];
+      if (!inside) {
+        const uint32_t end = last * v_st + v_at;
+        off = off < end ? off : end;
+      }
+      const int8_t* p = vb + off;
+      if constexpr (D == 32) s.v[e][0] = *(const uint16_t*)p;
+      else if constexpr (D == 64) s.v[e][0] = *(const uint32_t*)p;
+      else {
+        const uint2 x = *(const uint2*)p;
+        s.v[e][0] = x.x; s.v[e][1] = x.y;
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int64_t row = j0 + 16 * t, blk = (row < a.Tmax ? row : a.Tmax - 1) >> g.lg_block;
+      s.ks[t] = KS[blk * a.k.ss[2]];
+      s.vs[t] = VS[blk * a.v.ss[2]];
+    }
+  };
+
+  // The loads that everything waits for go out first: the query row of this
+  // lane, r = (query head of the group, token), and the first step's rows (any
+  // row of the cache may be read before the length is known).
+  const int Tq = (int)a.Tq, r0 = (int)qt * 16, r = r0 + n < R ? r0 + n : R - 1;
+  const int g_q = Tq == 1 ? r : r / Tq, i_q = r - g_q * Tq;
+  const T* q = (const T*)a.q + b * a.q_sb + (h * a.G + g_q) * a.q_sh + i_q * a.q_st;
+  Raw8q<T> qr[NK];
+#pragma unroll
+  for (int t = 0; t < NK; ++t) qr[t].load(q + (D == 32 ? 8 * q4 : 64 * (t >> 1) + 16 * q4 + 8 * (t & 1)));
+  Step<D> one, two;
+  int64_t j0 = j_lo + w * kStep;
+  if (j0 < a.Tmax) load(one, j0);
   int64_t len = a.lens[b];
   len = len < 0 ? 0 : len > a.Tmax ? a.Tmax : len;
 
-  // the query rows of this tile, r = (query head of the group, token)
-  const int r0 = qt * 16, r1 = r0 + 15 < R ? r0 + 15 : R - 1, Tq = (int)a.Tq;
+  // the tile's rows r0 .. r1, and what they see
+  const int r1 = r0 + 15 < R ? r0 + 15 : R - 1;
   const bool one_head = r0 / Tq == r1 / Tq;
   const int64_t vis_lo = len - Tq + (one_head ? r0 % Tq : 0) + 1, vis_hi = len - Tq + (one_head ? r1 % Tq : Tq - 1) + 1;
-  const int r = r0 + n < R ? r0 + n : R - 1, i_q = r % Tq;
   const int64_t vis = r0 + n < R ? len - Tq + i_q + 1 : 0;
 
-  const int64_t j_lo = split * g.chunk;
   const int64_t j_hi = j_lo + g.chunk < vis_hi ? j_lo + g.chunk : vis_hi;
 
   // queries as MFMA operands: lane (n, q4) holds d = 64 c + 16 q4 + 8 x + e of
@@ -123,15 +217,13 @@ __global__ void __launch_bounds__(64 * kNW) decode_int8_mfma(D8Args g) {
   h8 qh[NK], ql[F32 ? NK : 1];
   float corr = 0.f, cq;
   {
-    const T* q = (const T*)a.q + b * a.q_sb + (h * a.G + r / Tq) * a.q_sh + i_q * a.q_st;
     float x[NK][8];
     uint32_t top = 0;
 #pragma unroll
     for (int t = 0; t < NK; ++t) {
-      const int d = D == 32 ? 8 * q4 : 64 * (t >> 1) + 16 * q4 + 8 * (t & 1);
+      qr[t].floats(x[t]);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        x[t][e] = to_f(q[d + e]);
         const uint32_t m = __float_as_uint(x[t][e]) & 0x7fffffffu;
         top = m > top ? m : top;
       }
@@ -164,53 +256,6 @@ __global__ void __launch_bounds__(64 * kNW) decode_int8_mfma(D8Args g) {
     cq = a.scale * 1.4426950408889634f * __uint_as_float((uint32_t)(ex - 7 + 127) << 23);
   }
 
-  const int8_t* K = a.k.codes + b * a.k.cs[0] + h * a.k.cs[1] + (D == 32 ? 8 : 16) * q4;
-  const int8_t* V = a.v.codes + b * a.v.cs[0] + h * a.v.cs[1] + (D / 16) * n;
-  const float* KS = a.k.scales + b * a.k.ss[0] + h * a.k.ss[1];
-  const float* VS = a.v.scales + b * a.v.ss[0] + h * a.v.ss[1];
-
-  auto load = [&](Step<D>& s, int64_t j0) __attribute__((always_inline)) {
-    const int64_t last = a.Tmax - 1;
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      int64_t row = j0 + 16 * t + n;
-      row = row < last ? row : last;
-      const int8_t* p = K + row * a.k.cs[2];
-      if constexpr (D == 32) {
-        const uint2 x = *(const uint2*)p;
-        s.k[t][0] = x.x; s.k[t][1] = x.y;
-      } else {
-#pragma unroll
-        for (int c = 0; c < D / 64; ++c) {
-          const uint4 x = *(const uint4*)(p + 64 * c);
-          s.k[t][4 * c] = x.x; s.k[t][4 * c + 1] = x.y; s.k[t][4 * c + 2] = x.z; s.k[t][4 * c + 3] = x.w;
-        }
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      int64_t row = j0 + 16 * (e >> 2) + 4 * q4 + (e & 3);
-      row = row < last ? row : last;
-      const int8_t* p = V + row * a.v.cs[2];
-      if constexpr (D == 32) s.v[e][0] = *(const uint16_t*)p;
-      else if constexpr (D == 64) s.v[e][0] = *(const uint32_t*)p;
-      else {
-        const uint2 x = *(const uint2*)p;
-        s.v[e][0] = x.x; s.v[e][1] = x.y;
-      }
-    }
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      // (a tile that no query sees may be past the cache, or of a block that
-      // holds nothing yet: its scales are not read)
-      const bool seen = j0 + 16 * t < j_hi;
-      const int64_t blk = seen ? (j0 + 16 * t) >> g.lg_block : 0;
-      const float ks = KS[blk * a.k.ss[2]], vs = VS[blk * a.v.ss[2]];
-      s.ks[t] = seen ? ks : 0.f;
-      s.vs[t] = seen ? vs : 0.f;
-    }
-  };
-
   f4 acc[ND];
 #pragma unroll
   for (int c = 0; c < ND; ++c) acc[c] = f4{0.f, 0.f, 0.f, 0.f};
@@ -218,11 +263,15 @@ __global__ void __launch_bounds__(64 * kNW) decode_int8_mfma(D8Args g) {
   int E = -126;          // O is kept in units of 2^E, at least the largest vs so far
   float vinv = 0x1p126f;
 
-  Step<D> cur, nxt;
-  int64_t j0 = j_lo + w * kStep;
-  if (j0 < j_hi) load(cur, j0);
-  for (; j0 < j_hi; j0 += kIter) {
-    if (j0 + kIter < j_hi) load(nxt, j0 + kIter);
+  auto attend = [&](const Step<D>& cur, int64_t j0) __attribute__((always_inline)) {
+    // (a tile that no query sees may be of a block that holds nothing yet)
+    float ks[2], vs[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const bool seen = j0 + 16 * t < j_hi;
+      ks[t] = seen ? cur.ks[t] : 0.f;
+      vs[t] = seen ? cur.vs[t] : 0.f;
+    }
     // scores of keys 16 t + 4 q4 + i for query n
     float s[8];
     float top = -INFINITY;
@@ -235,7 +284,7 @@ __global__ void __launch_bounds__(64 * kNW) decode_int8_mfma(D8Args g) {
         x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[c], x, 0, 0, 0);
         if constexpr (F32) x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[c], x, 0, 0, 0);
       }
-      const float f = cq * cur.ks[t];
+      const float f = cq * ks[t];
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[4 * t + i] = x[i] * f;
     }
@@ -257,7 +306,7 @@ __global__ void __launch_bounds__(64 * kNW) decode_int8_mfma(D8Args g) {
       for (int c = 0; c < ND; ++c) acc[c] *= f;
       m = M;
     }
-    const float v0 = fabsf(cur.vs[0]), v1 = fabsf(cur.vs[1]);
+    const float v0 = fabsf(vs[0]), v1 = fabsf(vs[1]);
     const float v_top = fmaxf(v0 < INFINITY ? v0 : 0.f, v1 < INFINITY ? v1 : 0.f);
     if (v_top * vinv > 1.f) {
       const int e1 = (int)(__float_as_uint(v_top) >> 23) - 126;
@@ -270,12 +319,17 @@ __global__ void __launch_bounds__(64 * kNW) decode_int8_mfma(D8Args g) {
     }
     const float ref = m == -INFINITY ? 0.f : m - kLift;
     float p[8];
+    const float vn[2] = {vs[0] * vinv, vs[1] * vinv};
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float x = __builtin_amdgcn_exp2f(s[e] - ref);
-      l += x;
+      p[e] = __builtin_amdgcn_exp2f(s[e] - ref);
+      l += p[e];
+      p[e] *= vn[e >> 2];
+    }
+    if (!(v0 < INFINITY && v1 < INFINITY)) {
       // a hidden key adds nothing, whatever its block's scale is
-      p[e] = s[e] == -INFINITY ? 0.f : x * (cur.vs[e >> 2] * vinv);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) p[e] = s[e] == -INFINITY ? 0.f : p[e];
     }
     h8 ph, pl;
 #pragma unroll
@@ -308,60 +362,97 @@ __global__ void __launch_bounds__(64 * kNW) decode_int8_mfma(D8Args g) {
         if constexpr (F32) o = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl, o, 0, 0, 0);
       }
     }
-    cur = nxt;
+  };
+
+  while (j0 < j_hi) {
+    if (j0 + kIter < j_hi) load(two, j0 + kIter);
+    attend(one, j0);
+    j0 += kIter;
+    if (j0 >= j_hi) break;
+    if (j0 + kIter < j_hi) load(one, j0 + kIter);
+    attend(two, j0);
+    j0 += kIter;
   }
 
   // the waves' states meet in LDS; lane (n, q4) holds d = (D/4) q4 + (D/16) i + c
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
-#pragma unroll
-  for (int c = 0; c < ND; ++c)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) sm_o[w][n][(D / 4) * q4 + (D / 16) * i + c] = ldexpf(acc[c][i], E);
-  if (q4 == 0) { sm_m[w][n] = m; sm_l[w][n] = l; }
-  __syncthreads();
   const int rows = r1 - r0 + 1;
-  for (int idx = tid; idx < rows * D; idx += 64 * kNW) {
+  if (n < rows) {
+    float* o = sm_o + (w * rows + n) * LD + (D / 4) * q4;
+#pragma unroll
+    for (int c = 0; c < ND; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[(D / 16) * i + c] = ldexpf(acc[c][i], E);
+    if (q4 == 0) { sm_m[w][n] = m; sm_l[w][n] = l; }
+  }
+  __syncthreads();
+  for (int idx = tid; idx < rows * D; idx += 64 * NW) {
     const int qr = idx / D, d = idx % D, rr = r0 + qr, iq = rr % Tq;
     float M = sm_m[0][qr];
 #pragma unroll
-    for (int x = 1; x < kNW; ++x) M = fmaxf(M, sm_m[x][qr]);
+    for (int x = 1; x < NW; ++x) M = fmaxf(M, sm_m[x][qr]);
     float L = 0.f, A = 0.f;
 #pragma unroll
-    for (int x = 0; x < kNW; ++x) {
+    for (int x = 0; x < NW; ++x) {
       const float mx = sm_m[x][qr], f = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - M);
       L += sm_l[x][qr] * f;
-      A += sm_o[x][qr][d] * f;
+      A += sm_o[(x * rows + qr) * LD + d] * f;
     }
     if (g.splits == 1) {
       T* o = (T*)a.o + b * a.o_sb + (h * a.G + rr / Tq) * a.o_sh + iq * a.o_st;
       o[d] = from_f<T>(len - Tq + iq + 1 > 0 ? A / L : 0.f);
     } else {
-      float* P = g.part + ((unit * g.splits + split) * 16 + qr) * (D + 2);
+      float* P = g.part + ((int64_t)blockIdx.x * 16 + qr) * (D + 2);
       P[d] = A;
       if (d == 0) { P[D] = M; P[D + 1] = L; }
     }
   }
 }
 
-// One block of D threads per query row: merges its splits.
+// One block per query row: merges its splits, parts of them by threads of
+// their own.
 template <typename T, int D>
-__global__ void __launch_bounds__(D < 64 ? 64 : D) decode_int8_merge(D8Args g) {
+__global__ void __launch_bounds__(256) decode_int8_merge(D8Args g) {
+  constexpr int NP = 256 / D;  // parts
+  __shared__ float f_of[kSplits], sum[NP][D], red[4], red_l[4];
   const DecodeInt8& a = g.a;
-  const int d = threadIdx.x, Tq = (int)a.Tq, R = (int)(a.G * a.Tq);
+  const int tid = threadIdx.x, d = tid % D, part = tid / D, Tq = (int)a.Tq, R = (int)(a.G * a.Tq);
   const int64_t row = blockIdx.x, bh = row / R, h = bh % a.H, b = bh / a.H;
   const int rr = (int)(row % R), iq = rr % Tq;
-  if (d >= D) return;
   const float* P = g.part + ((bh * g.q_tiles + rr / 16) * g.splits * 16 + rr % 16) * (D + 2);
-  const int64_t st = 16 * (D + 2);
-  float M = -INFINITY;
-  for (int s = 0; s < g.splits; ++s) M = fmaxf(M, P[s * st + D]);
-  float L = 0.f, A = 0.f;
-  for (int s = 0; s < g.splits; ++s) {
-    const float m = P[s * st + D], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
-    L += P[s * st + D + 1] * f;
-    A += P[s * st + d] * f;
+  constexpr int64_t st = 16 * (D + 2);
+  constexpr int MS = kSplits / 256;
+  float m[MS], l[MS], M = -INFINITY, L = 0.f;
+#pragma unroll
+  for (int i = 0; i < MS; ++i) {
+    const int s = tid + 256 * i;
+    m[i] = s < g.splits ? P[s * st + D] : -INFINITY;
+    l[i] = s < g.splits ? P[s * st + D + 1] : 0.f;
+    M = fmaxf(M, m[i]);
   }
+  M = wave_max(M);
+  if ((tid & 63) == 0) red[tid >> 6] = M;
+  __syncthreads();
+  M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+#pragma unroll
+  for (int i = 0; i < MS; ++i) {
+    const float f = m[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[i] - M);
+    if (tid + 256 * i < g.splits) f_of[tid + 256 * i] = f;
+    L += l[i] * f;
+  }
+  L = wave_sum(L);
+  if ((tid & 63) == 0) red_l[tid >> 6] = L;
+  __syncthreads();
+  float A = 0.f;
+#pragma unroll 4
+  for (int s = part; s < g.splits; s += NP) A += P[s * st + d] * f_of[s];
+  sum[part][d] = A;
+  __syncthreads();
+  if (part) return;
+#pragma unroll
+  for (int i = 1; i < NP; ++i) A += sum[i][d];
+  L = (red_l[0] + red_l[1]) + (red_l[2] + red_l[3]);
   int64_t len = a.lens[b];
   len = len < 0 ? 0 : len > a.Tmax ? a.Tmax : len;
   T* o = (T*)a.o + b * a.o_sb + (h * a.G + rr / Tq) * a.o_sh + iq * a.o_st;
@@ -373,22 +464,43 @@ D8Args plan(const DecodeInt8& a) {
   g.a = a;
   g.lg_block = a.block == 16 ? 4 : a.block == 32 ? 5 : a.block == 64 ? 6 : 7;
   g.q_tiles = (int)((a.G * a.Tq + 15) / 16);
-  const int64_t units = a.B * a.H * g.q_tiles, most = (a.Tmax + kIter - 1) / kIter;
-  int64_t want = units > 0 ? (1024 + units - 1) / units : 1;
-  if (want > most) want = most;
-  g.chunk = ((a.Tmax + want - 1) / want + kIter - 1) / kIter * kIter;
-  g.splits = (int)((a.Tmax + g.chunk - 1) / g.chunk);
+  // A context to a block, with the waves that fill the CUs (16 of them each);
+  // or split over blocks of 4 waves and merged by a second launch, which costs
+  // about as much as three steps of a wave, where that saves more steps than
+  // that: 12 heads, 2048 rows of 64: 12.1 us whole, 8.3 split; 160 heads: 14.3
+  // whole, 19.4 split.
+  const int64_t units = a.B * a.H * g.q_tiles;
+  g.nw = units <= 256 && a.D != 128 ? 16 : units <= 512 ? 8 : 4;
+  while (g.nw > kFew && (lds_bytes(a, g.nw) > (60 << 10) || a.Tmax <= g.nw / 2 * kStep)) g.nw /= 2;
+  const int64_t iters = (a.Tmax + g.nw * kStep - 1) / (g.nw * kStep);
+  const double per = (a.D == 128 ? 2.0 : 1.0) / 1e5;  // steps of a wave for a row of a unit, all CUs filled
+  g.splits = 1;
+  g.chunk = a.Tmax;
   g.part = nullptr;
+  if (units > 0 && units < kSplits && (double)iters > 3.0 + per * (double)a.Tmax * (double)units) {
+    g.nw = kFew;
+    const int64_t iter = kFew * kStep, most = (a.Tmax + iter - 1) / iter;
+    int64_t want = (kSplits + units - 1) / units;  // four blocks a CU
+    if (want > most) want = most;
+    g.chunk = ((a.Tmax + want - 1) / want + iter - 1) / iter * iter;
+    g.splits = (int)((a.Tmax + g.chunk - 1) / g.chunk);
+  }
   return g;
+}
+
+template <typename T, int D, int NW>
+void launch_nw(const D8Args& g, hipStream_t s) {
+  const dim3 grid((unsigned)(g.a.B * g.a.H * g.q_tiles * g.splits));
+  hipLaunchKernelGGL((decode_int8_mfma<T, D, NW>), grid, dim3(64 * NW), lds_bytes(g.a, NW), s, g);
 }
 
 template <typename T, int D>
 void launch(const D8Args& g, hipStream_t s) {
-  const int64_t units = g.a.B * g.a.H * g.q_tiles;
-  hipLaunchKernelGGL((decode_int8_mfma<T, D>), dim3((unsigned)(units * g.splits)), dim3(64 * kNW), 0, s, g);
+  if (g.nw == kFew) launch_nw<T, D, kFew>(g, s);
+  else if (g.nw == 8 || D == 128) launch_nw<T, D, 8>(g, s);
+  else launch_nw<T, D, D == 128 ? 8 : 16>(g, s);
   if (g.splits > 1)
-    hipLaunchKernelGGL((decode_int8_merge<T, D>), dim3((unsigned)(g.a.B * g.a.H * g.a.G * g.a.Tq)),
-                       dim3(D < 64 ? 64 : D), 0, s, g);
+    hipLaunchKernelGGL((decode_int8_merge<T, D>), dim3((unsigned)(g.a.B * g.a.H * g.a.G * g.a.Tq)), dim3(256), 0, s, g);
 }
 
 }  // namespace

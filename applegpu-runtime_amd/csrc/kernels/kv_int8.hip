@@ -28,7 +28,7 @@ namespace {
 struct KvArgs8 {
   KvInt8 a;
   int lg_block, lg_cpr;  // log2 of the block and of the 8-code chunks of a row
-  int64_t nbt, waves;    // blocks an append touches at most; B * H * nbt
+  uint32_t nbt, waves;   // blocks an append touches at most; B * H * nbt
 };
 
 __device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
@@ -40,21 +40,51 @@ __device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
   return v;
 }
 
+// 8 consecutive values, raw.
 template <typename T>
-__device__ __forceinline__ void load_row8(const T* p, float (&x)[8]) {
-  uint4 raw[sizeof(T) / 2];
+struct Raw8x {
+  uint4 v[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-  for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[i] = ((const uint4*)p)[i];
-  T e[8];
-  __builtin_memcpy(e, raw, sizeof(e));
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = ((const uint4*)p)[i];
+  }
+  __device__ __forceinline__ void floats(float (&x)[8]) const {
+    T e[8];
+    __builtin_memcpy(e, v, sizeof(e));
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = to_f(e[i]);
+    for (int i = 0; i < 8; ++i) x[i] = to_f(e[i]);
+  }
+};
+
+__device__ __forceinline__ uint32_t top_of(const float (&v)[8], uint32_t top) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t m = __float_as_uint(v[e]) & 0x7fffffffu;
+    top = m > top ? m : top;
+  }
+  return top;
 }
 
-// code of x for scale s (0 where the scale says nothing: 0, infinite or NaN)
-__device__ __forceinline__ int code_of(float x, float s, bool ok) {
-  const float r = ok ? rintf(x / s) : 0.f;
-  return (int)fminf(fmaxf(r, -127.f), 127.f);
+// clamp(rint(x / s), -127, 127) of 8 values; 0 where the scale says nothing
+// (0, infinite or NaN).  x / s is IEEE's; x times 1 / s is within 127 (2^-23 +
+// 2^-24) < 2.3e-5 of it, so only where that is nearer than 1e-4 to a half is
+// the division done (as 8 divisions a chunk the append of 8 x 20 x 509 rows
+// of 64 takes 13.7 us, bound by them).
+__device__ __forceinline__ void codes_of(const float (&v)[8], float s, float inv, bool ok, int (&c)[8]) {
+  float r[8];
+  bool near = !(inv < 1e30f);  // 1 / s overflows, or nearly
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float q = v[e] * inv;
+    r[e] = rintf(q);
+    near |= fabsf(fabsf(q - r[e]) - 0.5f) < 1e-4f;
+  }
+  if (near) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r[e] = rintf(v[e] / s);
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) c[e] = ok ? (int)fminf(fmaxf(r[e], -127.f), 127.f) : 0;
 }
 
 __device__ __forceinline__ void store_codes(int8_t* p, const int (&c)[8]) {
@@ -67,13 +97,16 @@ __device__ __forceinline__ void store_codes(int8_t* p, const int (&c)[8]) {
   *(uint2*)p = w;
 }
 
-template <typename T>
+// NC > 0: the new rows of a block are at most 64 NC chunks and stay in
+// registers between the search for the largest and the rounding; 0: any
+// number, read twice.
+template <typename T, int NC>
 __global__ void __launch_bounds__(256) kv_write_int8_kernel(KvArgs8 g) {
   const KvInt8& a = g.a;
   const int lane = threadIdx.x & 63, j = blockIdx.y;
-  const int64_t wave = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
   if (wave >= g.waves) return;
-  const int64_t nb = wave % g.nbt, bh = wave / g.nbt, h = bh % a.H, b = bh / a.H;
+  const uint32_t bh = wave / g.nbt, nb = wave % g.nbt, h = bh % (uint32_t)a.H, b = bh / (uint32_t)a.H;
   const int64_t p = (int64_t)a.pos[b] + a.pos_off;
   const int64_t first = p > 0 ? p : 0;  // first row written
   int64_t end = p + a.T;
@@ -85,18 +118,34 @@ __global__ void __launch_bounds__(256) kv_write_int8_kernel(KvArgs8 g) {
   const Int8Cache& c = a.c[j];
   int8_t* codes = c.codes + b * c.cs[0] + h * c.cs[1];
   float* scale = c.scales + b * c.ss[0] + h * c.ss[1] + n * c.ss[2];
-  const T* x = (const T*)a.x[j] + b * a.xs[j][0] + h * a.xs[j][1];
+  const T* x = (const T*)a.x[j] + b * a.xs[j][0] + h * a.xs[j][1] + (r0 - p) * a.xs[j][2];
+  int8_t* to = codes + r0 * c.cs[2];
   const int cpr = 1 << g.lg_cpr;
   const int chunks = (int)(r1 - r0) << g.lg_cpr;
 
   uint32_t top = 0;
-  for (int i = lane; i < chunks; i += 64) {
-    float v[8];
-    load_row8(x + (r0 + (i >> g.lg_cpr) - p) * a.xs[j][2] + (i & (cpr - 1)) * 8, v);
+  Raw8x<T> keep[NC ? NC : 1];
+  if constexpr (NC > 0) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t m = __float_as_uint(v[e]) & 0x7fffffffu;
-      top = m > top ? m : top;
+    for (int u = 0; u < NC; ++u) {
+      const int i = lane + 64 * u;
+#pragma unroll
+      for (int e = 0; e < (int)sizeof(T) / 2; ++e) keep[u].v[e] = uint4{0, 0, 0, 0};
+      if (i < chunks) keep[u].load(x + (i >> g.lg_cpr) * a.xs[j][2] + (i & (cpr - 1)) * 8);
+    }
+#pragma unroll
+    for (int u = 0; u < NC; ++u) {
+      float v[8];
+      keep[u].floats(v);
+      top = top_of(v, top);
+    }
+  } else {
+    for (int i = lane; i < chunks; i += 64) {
+      Raw8x<T> raw;
+      raw.load(x + (i >> g.lg_cpr) * a.xs[j][2] + (i & (cpr - 1)) * 8);
+      float v[8];
+      raw.floats(v);
+      top = top_of(v, top);
     }
   }
   uint32_t s_bits = __float_as_uint(__uint_as_float(wave_umax(top)) / 127.f) & 0x7fffffffu;
@@ -104,6 +153,7 @@ __global__ void __launch_bounds__(256) kv_write_int8_kernel(KvArgs8 g) {
   if (was > s_bits) s_bits = was;
   const float s = __uint_as_float(s_bits);
   const bool ok = s > 0.f && s < INFINITY;
+  const float inv = 1.f / s;
 
   if (s_bits != was) {  // rows before the append, if any, take the grown scale
     const int held = (int)(r0 - lo) << g.lg_cpr;
@@ -119,47 +169,54 @@ __global__ void __launch_bounds__(256) kv_write_int8_kernel(KvArgs8 g) {
       store_codes(q, cc);
     }
   }
-  for (int i = lane; i < chunks; i += 64) {
-    const int64_t r = r0 + (i >> g.lg_cpr);
-    const int d = (i & (cpr - 1)) * 8;
+  auto put = [&](int i, const Raw8x<T>& raw) {
     float v[8];
-    load_row8(x + (r - p) * a.xs[j][2] + d, v);
+    raw.floats(v);
     int cc[8];
+    codes_of(v, s, inv, ok, cc);
+    store_codes(to + (i >> g.lg_cpr) * c.cs[2] + (i & (cpr - 1)) * 8, cc);
+  };
+  if constexpr (NC > 0) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) cc[e] = code_of(v[e], s, ok);
-    store_codes(codes + r * c.cs[2] + d, cc);
+    for (int u = 0; u < NC; ++u)
+      if (lane + 64 * u < chunks) put(lane + 64 * u, keep[u]);
+  } else {
+    for (int i = lane; i < chunks; i += 64) {
+      Raw8x<T> raw;
+      raw.load(x + (i >> g.lg_cpr) * a.xs[j][2] + (i & (cpr - 1)) * 8);
+      put(i, raw);
+    }
   }
   if (lane == 0) *scale = s;
 }
 
+// A block per 2048 values of a (sequence, head): 8 a thread.
 template <typename T>
-__global__ void __launch_bounds__(256) kv_read_int8_kernel(KvArgs8 g, T* y0, T* y1, int64_t n) {
+__global__ void __launch_bounds__(256) kv_read_int8_kernel(KvArgs8 g, T* y0, T* y1, uint32_t per) {
   const KvInt8& a = g.a;
   const int j = blockIdx.y;
-  T* y = j ? y1 : y0;
+  const uint32_t bh = blockIdx.x / per, h = bh % (uint32_t)a.H, b = bh / (uint32_t)a.H;
+  const int64_t i = (int64_t)(blockIdx.x % per) * 256 + threadIdx.x, t = i >> g.lg_cpr;
+  if (t >= a.T) return;
+  const int d = (int)(i & ((1 << g.lg_cpr) - 1)) * 8;
   const Int8Cache& c = a.c[j];
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    const int64_t row = i >> g.lg_cpr;
-    const int d = (int)(i & ((1 << g.lg_cpr) - 1)) * 8;
-    const int64_t t = row % a.T, bh = row / a.T, h = bh % a.H, b = bh / a.H;
-    const int64_t r = (int64_t)a.pos[b] + t;
-    T e[8];
-    if (r >= 0 && r < a.Tmax) {
-      const uint2 w = *(const uint2*)(c.codes + b * c.cs[0] + h * c.cs[1] + r * c.cs[2] + d);
-      const float s = c.scales[b * c.ss[0] + h * c.ss[1] + (r >> g.lg_block) * c.ss[2]];
-      int8_t o[8];
-      __builtin_memcpy(o, &w, 8);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) e[k] = from_f<T>((float)o[k] * s);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) e[k] = from_f<T>(0.f);
-    }
-    uint4 raw[sizeof(T) / 2];
-    __builtin_memcpy(raw, e, sizeof(e));
-#pragma unroll
-    for (int k = 0; k < (int)sizeof(T) / 2; ++k) ((uint4*)(y + row * a.D + d))[k] = raw[k];
+  const int64_t r = (int64_t)a.pos[b] + t;
+  uint2 w{0, 0};
+  float s = 0.f;
+  if (r >= 0 && r < a.Tmax) {
+    w = *(const uint2*)(c.codes + b * c.cs[0] + h * c.cs[1] + r * c.cs[2] + d);
+    s = c.scales[b * c.ss[0] + h * c.ss[1] + (r >> g.lg_block) * c.ss[2]];
   }
+  int8_t o[8];
+  __builtin_memcpy(o, &w, 8);
+  T e[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) e[k] = from_f<T>((float)o[k] * s);
+  uint4 raw[sizeof(T) / 2];
+  __builtin_memcpy(raw, e, sizeof(e));
+  T* y = (j ? y1 : y0) + (bh * a.T + t) * a.D + d;
+#pragma unroll
+  for (int k = 0; k < (int)sizeof(T) / 2; ++k) ((uint4*)y)[k] = raw[k];
 }
 
 int lg2(int64_t v) {
@@ -168,13 +225,16 @@ int lg2(int64_t v) {
   return l;
 }
 
-KvArgs8 kv_args(const KvInt8& a) {
+// Fails where the grid would not hold `blocks` blocks.
+KvArgs8 kv_args(const char* name, const KvInt8& a, int64_t blocks) {
+  if (!kv_int8_supported(a.D, a.block)) fail("%s: head dim %lld or block %d not supported", name, (long long)a.D, a.block);
+  if (blocks > 0x7fffffffLL / 4) fail("%s: too many rows", name);
   KvArgs8 g;
   g.a = a;
   g.lg_block = lg2(a.block);
   g.lg_cpr = lg2(a.D / 8);
-  g.nbt = (a.T + a.block - 2) / a.block + 1;
-  g.waves = a.B * a.H * g.nbt;
+  g.nbt = (uint32_t)((a.T + a.block - 2) / a.block + 1);
+  g.waves = (uint32_t)(a.B * a.H * g.nbt);
   return g;
 }
 
@@ -185,24 +245,29 @@ bool kv_int8_supported(int64_t D, int64_t block) {
 }
 
 void kv_write_int8(const KvInt8& a, hipStream_t s) {
-  if (!kv_int8_supported(a.D, a.block)) fail("kv_write_int8: head dim %lld or block %d not supported", (long long)a.D, a.block);
   if (a.B * a.H * a.T == 0) return;
-  const KvArgs8 g = kv_args(a);
-  if ((g.waves + 3) / 4 > 0x7fffffffLL) fail("kv_write_int8: too many rows");
-  const dim3 grid((unsigned)((g.waves + 3) / 4), 2);
-  AGPU_FLOAT_SWITCH(a.dt, hipLaunchKernelGGL((kv_write_int8_kernel<T>), grid, dim3(256), 0, s, g));
+  const int64_t waves = a.B * a.H * ((a.T + a.block - 2) / a.block + 1);
+  const KvArgs8 g = kv_args("kv_write_int8", a, waves);
+  const dim3 grid((unsigned)((waves + 3) / 4), 2);
+  // 64-chunk parts of the new rows of a block
+  const int64_t parts = ((a.T < a.block ? a.T : a.block) * (a.D / 8) + 63) / 64;
+  AGPU_FLOAT_SWITCH(a.dt, {
+    if (parts <= 1) hipLaunchKernelGGL((kv_write_int8_kernel<T, 1>), grid, dim3(256), 0, s, g);
+    else if (parts <= 2) hipLaunchKernelGGL((kv_write_int8_kernel<T, 2>), grid, dim3(256), 0, s, g);
+    else if (parts <= 4) hipLaunchKernelGGL((kv_write_int8_kernel<T, 4>), grid, dim3(256), 0, s, g);
+    else if (parts <= 8) hipLaunchKernelGGL((kv_write_int8_kernel<T, 8>), grid, dim3(256), 0, s, g);
+    else hipLaunchKernelGGL((kv_write_int8_kernel<T, 0>), grid, dim3(256), 0, s, g);
+  });
   check_launch("kv_write_int8");
 }
 
 void kv_read_int8(const KvInt8& a, void* const y[2], hipStream_t s) {
-  if (!kv_int8_supported(a.D, a.block)) fail("kv_read_int8: head dim %lld or block %d not supported", (long long)a.D, a.block);
-  const int64_t n = a.B * a.H * a.T * (a.D / 8);
-  if (n == 0) return;
-  const KvArgs8 g = kv_args(a);
-  int64_t blocks = (n + 255) / 256;
-  if (blocks > 65536) blocks = 65536;
-  AGPU_FLOAT_SWITCH(a.dt, hipLaunchKernelGGL((kv_read_int8_kernel<T>), dim3((unsigned)blocks, 2), dim3(256), 0, s, g,
-                                             (T*)y[0], (T*)y[1], n));
+  if (a.B * a.H * a.T == 0) return;
+  const int64_t per = (a.T * (a.D / 8) + 255) / 256;
+  const KvArgs8 g = kv_args("kv_read_int8", a, a.B * a.H * per);
+  const dim3 grid((unsigned)(a.B * a.H * per), 2);
+  AGPU_FLOAT_SWITCH(a.dt, hipLaunchKernelGGL((kv_read_int8_kernel<T>), grid, dim3(256), 0, s, g, (T*)y[0], (T*)y[1],
+                                             (uint32_t)per));
   check_launch("kv_read_int8");
 }
 

@@ -55,21 +55,37 @@ __global__ void __launch_bounds__(256) int4_scales_kernel(const T* __restrict__ 
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256) dequantize_int4_kernel(const uint32_t* __restrict__ packed,
+// One lane per byte run: 32 codes of a row, of one scale.  A wave reads 1 KB in
+// a row and writes 64 bytes (16-bit types) of each of 16 rows four times over.
+// VEC: rows are aligned and whole runs of 8 values are one store.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) dequantize_int4_kernel(const uint4* __restrict__ packed,
                                                               const T* __restrict__ scales, int64_t N, int64_t K,
                                                               int64_t group, T* __restrict__ out, int64_t ld,
-                                                              int64_t words, int64_t steps) {
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < words; i += (int64_t)gridDim.x * 256) {
-    // words of a row of W in a row, so that the stores are contiguous
-    const int64_t wpr = steps * 16, n = i / wpr, kw = i % wpr, k0 = kw * 8;
-    if (k0 >= K) continue;
-    const int64_t step = kw >> 4;
-    const int run = (int)(n & 15) + 16 * (int)((kw >> 2) & 3), word = (int)(kw & 3);
-    const uint32_t v = packed[(((n >> 4) * steps + step) * 64 + run) * 4 + word];
+                                                              int64_t runs, int64_t steps) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < runs; i += (int64_t)gridDim.x * 256) {
+    const int run = (int)(i & 63);
+    const int64_t tile = i >> 6, n = tile / steps * 16 + (run & 15), k0 = tile % steps * 128 + (run >> 4) * 32;
+    if (n >= N || k0 >= K) continue;
+    const uint4 w = packed[i];
+    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
     const float s = to_f(scales[k0 / group * N + n]);
-    for (int e = 0; e < 8; ++e)
-      if (k0 + e < K) out[n * ld + k0 + e] = from_f<T>((float)((int)((v >> (4 * nibble_of(e))) & 15) - 8) * s);
+    T* o = out + n * ld + k0;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      T v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = from_f<T>((float)((int)((ws[t] >> (4 * nibble_of(e))) & 15) - 8) * s);
+      if (VEC && k0 + 8 * t + 8 <= K) {
+        uint4 raw[sizeof(T) / 2];
+        __builtin_memcpy(raw, v, sizeof(v));
+#pragma unroll
+        for (int e = 0; e < (int)sizeof(T) / 2; ++e) ((uint4*)(o + 8 * t))[e] = raw[e];
+      } else {
+        for (int e = 0; e < 8; ++e)
+          if (k0 + 8 * t + e < K) o[8 * t + e] = v[e];
+      }
+    }
   }
 }
 
@@ -131,8 +147,9 @@ struct L4Args {
 // What a wave keeps in flight: UN steps of 128 columns of codes, and the rows
 // of XB steps (two where they fit the registers: those of the next step are
 // loaded before this one is multiplied).
-template <typename T, int MT, int NT> struct InFlight {
-  static constexpr int UN = NT == 1 ? 4 : 2, XB = sizeof(T) == 2 && MT <= 2 ? 2 : 1;
+template <typename T, int MT, int NT, int G> struct InFlight {
+  static constexpr int UN = NT == 1 ? 4 : 2;
+  static constexpr int XB = sizeof(T) == 2 && MT <= 2 && !(MT == 1 && NT == 2 && G == 32) ? 2 : 1;
 };
 
 // MT tiles of 16 rows of x by NT tiles of 16 columns of the output; the waves
@@ -142,7 +159,7 @@ template <typename T, int MT, int NT, int G, bool XVEC>
 __global__ void __launch_bounds__(MT == 1 ? 1024 : 512) linear_int4_mfma(L4Args g) {
   typedef In4<T> I;
   typedef typename I::vec V;
-  constexpr int NG = 128 / G, UN = InFlight<T, MT, NT>::UN, XB = InFlight<T, MT, NT>::XB, XW = sizeof(T) / 2;
+  constexpr int NG = 128 / G, UN = InFlight<T, MT, NT, G>::UN, XB = InFlight<T, MT, NT, G>::XB, XW = sizeof(T) / 2;
   static_assert(UN % XB == 0, "the rows' buffers follow the steps");
   extern __shared__ float red[];  // [nw][MT][NT][16][16]
   const LinearInt4& a = g.a;
@@ -174,17 +191,14 @@ __global__ void __launch_bounds__(MT == 1 ? 1024 : 512) linear_int4_mfma(L4Args 
   }
 
   uint4 wv[UN][NT];
-  T sv[UN][NT][NG];
+  T sv[UN][NT];  // lane (c, q): the scale of column c for group q NG / 4 of the step
   auto load_w = [&](int u, int st) __attribute__((always_inline)) {
     st = st < steps ? st : steps - 1;
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       wv[u][j] = wp[j][(int64_t)st * 64];
-#pragma unroll
-      for (int i = 0; i < NG; ++i) {
-        const int gr = st * NG + i < groups ? st * NG + i : groups - 1;
-        sv[u][j][i] = sc[(int64_t)gr * a.N + col[j]];
-      }
+      const int gr = st * NG + q * NG / 4;
+      sv[u][j] = sc[(int64_t)(gr < groups ? gr : groups - 1) * a.N + col[j]];
     }
   };
   // columns that word t of a lane's codes belongs to
@@ -221,8 +235,26 @@ __global__ void __launch_bounds__(MT == 1 ? 1024 : 512) linear_int4_mfma(L4Args 
 
   auto multiply = [&](int u, int b) __attribute__((always_inline)) {
     uint32_t word[NT][4];
+    float sg[NT][NG];
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
+      // each group's scale to all lanes of its column
+      const uint32_t s1 = __float_as_uint(to_f(sv[u][j]));
+      if constexpr (NG == 1) {
+        sg[j][0] = __uint_as_float(s1);
+      } else {
+        const auto h = __builtin_amdgcn_permlane32_swap(s1, s1, false, false);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if constexpr (NG == 2) {
+            sg[j][i] = __uint_as_float(h[i]);
+          } else {
+            const auto r = __builtin_amdgcn_permlane16_swap(h[i], h[i], false, false);
+            sg[j][2 * i] = __uint_as_float(r[0]);
+            sg[j][2 * i + 1] = __uint_as_float(r[1]);
+          }
+        }
+      }
       word[j][0] = wv[u][j].x; word[j][1] = wv[u][j].y; word[j][2] = wv[u][j].z; word[j][3] = wv[u][j].w;
       if constexpr (G < 128) {
         // lane (c, q) holds columns 32 q + 8 t of word t: exchanged between
@@ -282,7 +314,7 @@ __global__ void __launch_bounds__(MT == 1 ? 1024 : 512) linear_int4_mfma(L4Args 
       }
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
-        const float s = to_f(sv[u][j][gr]);
+        const float s = sg[j][gr];
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -343,7 +375,8 @@ void launch_int4(const L4Args& g, bool xvec, hipStream_t s) {
 
 template <typename T, int MT, int NT>
 void launch_int4_g(const L4Args& g, bool xvec, hipStream_t s) {
-  if (g.a.group == 32) launch_int4<T, MT, NT, 32>(g, xvec, s);
+  // (64 rows' sums for groups of 32 fit the registers for one tile of columns)
+  if (g.a.group == 32) launch_int4<T, MT, MT == 4 ? 1 : NT, 32>(g, xvec, s);
   else if (g.a.group == 64) launch_int4<T, MT, NT, 64>(g, xvec, s);
   else launch_int4<T, MT, NT, 128>(g, xvec, s);
 }
@@ -371,10 +404,14 @@ void quantize_int4(DType dt, const void* w, int64_t sn, int64_t sk, int64_t N, i
 
 void dequantize_int4(DType dt, const uint8_t* packed, const void* scales, int64_t N, int64_t K, int64_t group,
                      void* out, int64_t ld, hipStream_t s) {
-  const int64_t steps = (K + 127) / 128, words = N * steps * 16;
-  AGPU_FLOAT_SWITCH(dt, hipLaunchKernelGGL((dequantize_int4_kernel<T>), dim3(grid_for(words)), dim3(256), 0, s,
-                                           (const uint32_t*)packed, (const T*)scales, N, K, group, (T*)out, ld, words,
-                                           steps));
+  const int64_t steps = (K + 127) / 128, runs = (N + 15) / 16 * steps * 64;
+  const bool vec = ((uintptr_t)out & 15) == 0 && ld * (int64_t)dtype_size(dt) % 16 == 0;
+  AGPU_FLOAT_SWITCH(dt, {
+    if (vec) hipLaunchKernelGGL((dequantize_int4_kernel<T, true>), dim3(grid_for(runs)), dim3(256), 0, s,
+                                (const uint4*)packed, (const T*)scales, N, K, group, (T*)out, ld, runs, steps);
+    else hipLaunchKernelGGL((dequantize_int4_kernel<T, false>), dim3(grid_for(runs)), dim3(256), 0, s,
+                            (const uint4*)packed, (const T*)scales, N, K, group, (T*)out, ld, runs, steps);
+  });
   check_launch("dequantize_int4");
 }
 
@@ -388,10 +425,14 @@ void linear_int4(const LinearInt4& a, hipStream_t s) {
   const int es = (int)dtype_size(a.dt);
   const bool xvec = a.K % 8 == 0 && ((uintptr_t)a.x & 15) == 0 && (a.M == 1 || a.x_sm * es % 16 == 0);
   const int mt = a.M <= 16 ? 1 : a.M <= 32 ? 2 : 4;
-  const int most = mt == 1 ? 16 : 8;
-  g.nw = (int)(g.steps < most ? g.steps : most);
+  const int64_t tiles = (a.N + 15) / 16;
+  const bool wide = mt > 1 || tiles >= 320;
+  const int64_t blocks = (tiles + wide) / (1 + wide), most = mt == 1 ? 16 : 8;
+  int64_t nw = 4096 / blocks;
+  nw = nw < 2 ? 2 : nw > most ? most : nw;
+  g.nw = (int)(g.steps < nw ? g.steps : nw);
   AGPU_FLOAT_SWITCH(a.dt, {
-    if (mt == 1 && (a.N + 15) / 16 < 512) launch_int4_g<T, 1, 1>(g, xvec, s);
+    if (mt == 1 && !wide) launch_int4_g<T, 1, 1>(g, xvec, s);
     else if (mt == 1) launch_int4_g<T, 1, 2>(g, xvec, s);
     else if (mt == 2) launch_int4_g<T, 2, 2>(g, xvec, s);
     else launch_int4_g<T, 4, 2>(g, xvec, s);

@@ -2031,6 +2031,8 @@ TensorP decode_attention_int8(const TensorP& q_in, const Int8KV& c, const Tensor
     fail("%s: q %s does not match a cache of %s (its heads must be a multiple of the cache's)", name,
          shape_str(q_in->dims()).c_str(), shape_str(c.kc->dims()).c_str());
   if (Tq > p.Tmax) fail("%s: %lld query rows exceed the cache length %lld", name, (long long)Tq, (long long)p.Tmax);
+  for (const k::Int8Cache& kv : p.c)  // a step's rows are at 32-bit offsets
+    if (kv.cs[2] < 0 || kv.cs[2] > ((int64_t)1 << 26)) fail("%s: cache rows are more than 2^26 bytes apart", name);
   if (!(scale > 0.f) || !std::isfinite(scale)) fail("%s: the scale must be positive and finite", name);
   TensorP lc = check_lens(name, "lens", lens, B);
   TensorP q = q_in;
