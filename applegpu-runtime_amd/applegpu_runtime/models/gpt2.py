@@ -67,7 +67,8 @@ def random_weights(cfg: dict, seed: int = 42, std: float = 0.02) -> dict:
 CONV1D = (".attn.c_attn.weight", ".attn.c_proj.weight", ".mlp.c_fc.weight", ".mlp.c_proj.weight")
 
 
-def load_model(np_weights: dict, cfg: dict, dtype: str = "float32", kmajor=None, packed=None, x3=None) -> dict:
+def load_model(np_weights: dict, cfg: dict, dtype: str = "float32", kmajor=None, packed=None, x3=None,
+               weight_bits: int = 16, group: int = 128) -> dict:
     """Upload numpy weights; returns the model dict the forward pass takes.
 
     kmajor (default: on for fp16/bf16) stores the Conv1D projection weights
@@ -83,8 +84,16 @@ def load_model(np_weights: dict, cfg: dict, dtype: str = "float32", kmajor=None,
     into bf16 hi/lo MFMA fragments (gpu.pack_weight_x3), which the fp32 GEMMs
     of the forward read instead of splitting the weights on every call; the
     forward then also passes the activations after each layer_norm and gelu
-    as packed rows (gpu.pack_rows_x3), written by their producers."""
+    as packed rows (gpu.pack_rows_x3), written by their producers.
+    weight_bits=4 (fp16/bf16 models) holds every projection weight in 4 bits
+    with a scale for each output and `group` inputs (gpu.quantize_int4) and
+    nothing else of it: an eighth to a quarter of the bytes that a decode step
+    reads; the embeddings and the tied head keep 16 bits."""
     gpu.init_backend()
+    if weight_bits not in (4, 16):
+        raise ValueError(f"weight_bits must be 4 or 16, got {weight_bits}")
+    if weight_bits == 4 and (dtype == "float32" or kmajor is False):
+        raise ValueError("4-bit weights need an fp16/bf16 model with k-major weights")
     if kmajor is None:
         kmajor = dtype != "float32"
     if packed is None:
@@ -106,6 +115,12 @@ def load_model(np_weights: dict, cfg: dict, dtype: str = "float32", kmajor=None,
             t.eval()
         w[k] = t
     pk = {}
+    if weight_bits == 4:
+        for k in [k for k in w if k.endswith(CONV1D)]:
+            t = w.pop(k)
+            p, scales = gpu.quantize_int4(t, group)
+            gpu.eval_many([p, scales])
+            pk[k] = (p, t.shape[0], "int4", scales, group)
     if packed:
         for k, t in w.items():
             if k.endswith(CONV1D) or k == "transformer.wte.weight":
@@ -175,12 +190,24 @@ def _mm(model: dict, x, name: str, rows: int = None):
     way the weight is stored; fp32 weights use their hi/lo packed copy, and
     16-bit ones their decode-packed copy for calls with at most 16 rows."""
     pk = model.get("packed", {}).get(name)
+    if pk is not None and pk[2] == "int4":
+        return gpu.linear_int4(x, pk[0], pk[3], group=pk[4])
     if pk is not None and (pk[2] == "x3" or (rows is not None and rows <= 16)):
         return gpu.matmul_packed(x, pk[0], pk[1])
     w = model["weights"][name]
     if name == "transformer.wte.weight":
         return x @ gpu.transpose(w)
     return x @ (gpu.transpose(w) if model.get("kmajor") else w)
+
+
+def _layer(model: dict, x, name: str, rows: int = None, act=None):
+    """act(x @ W + b) of the projection `name` (its weight and bias)."""
+    b = model["weights"][f"{name}.bias"]
+    pk = model.get("packed", {}).get(f"{name}.weight")
+    if pk is not None and pk[2] == "int4":   # bias and activation in its epilogue
+        return gpu.linear_int4(x, pk[0], pk[3], b, act, group=pk[4])
+    y = gpu.add_bias(_mm(model, x, f"{name}.weight", rows), b)
+    return gpu.gelu(y) if act == "gelu" else y
 
 
 def _mm_rows(model: dict, x, name: str, rows: int):
@@ -290,29 +317,56 @@ class KVCache:
     (python/applegpu_runtime/models/gpt2.py:122-126); here the cache is
     allocated once and written in place (`gpu.kv_write`), and every length
     the decode step needs lives in device memory, so one decode step can be
-    captured as a HIP graph and replayed for every generated token."""
+    captured as a HIP graph and replayed for every generated token.
 
-    def __init__(self, cfg: dict, batch: int, max_len: int, dtype: str = "float16"):
+    bits=8 holds the rows as int8 codes with a float32 scale for each head and
+    `block` rows (`gpu.kv_write_int8`; k_scale and v_scale beside k and v):
+    half the memory and, at long contexts, half the time of a 16-bit cache."""
+
+    def __init__(self, cfg: dict, batch: int, max_len: int, dtype: str = "float16", bits: int = 16, block: int = 16):
         gpu.init_backend()
         H, d = cfg["n_head"], cfg["n_embd"]
         if max_len > cfg["n_positions"]:
             raise ValueError(f"max_len {max_len} exceeds n_positions {cfg['n_positions']}")
+        if bits not in (8, 16):
+            raise ValueError(f"bits must be 8 or 16, got {bits}")
         shape = [batch, H, max_len, d // H]
-        self.batch, self.max_len, self.dtype = batch, max_len, dtype
-        self.k = [gpu.zeros(shape, dtype) for _ in range(cfg["n_layer"])]
-        self.v = [gpu.zeros(shape, dtype) for _ in range(cfg["n_layer"])]
+        self.batch, self.max_len, self.dtype, self.bits, self.block = batch, max_len, dtype, bits, block
+        held = "int8" if bits == 8 else dtype
+        self.k = [gpu.zeros(shape, held) for _ in range(cfg["n_layer"])]
+        self.v = [gpu.zeros(shape, held) for _ in range(cfg["n_layer"])]
+        self.k_scale = self.v_scale = None
+        if bits == 8:
+            shape = [batch, H, -(-max_len // block)]
+            self.k_scale = [gpu.zeros(shape) for _ in range(cfg["n_layer"])]
+            self.v_scale = [gpu.zeros(shape) for _ in range(cfg["n_layer"])]
         self.pos = gpu.from_numpy(np.zeros(batch, np.int32))
         self.one = gpu.from_numpy(np.ones(1, np.int32))
         self.length = 0   # host mirror of pos (all sequences advance together)
 
     def nbytes(self) -> int:
         n = 0
-        for t in self.k + self.v:
+        for t in self.k + self.v + (self.k_scale or []) + (self.v_scale or []):
             c = 1
             for s in t.shape:
                 c *= s
-            n += c * gpu.dtype_size(self.dtype)
+            n += c * gpu.dtype_size(t.dtype)
         return n
+
+    def write(self, i: int, k, v):
+        """Layer i's K and V rows [batch, n_head, T, d_head], at `pos`."""
+        if self.bits == 8:
+            gpu.kv_write_int8(self.k[i], self.k_scale[i], self.v[i], self.v_scale[i], k, v, self.pos, block=self.block)
+        else:
+            gpu.kv_write_pair(self.k[i], self.v[i], k, v, self.pos)
+
+    def attend(self, i: int, q, lens, k, v):
+        """Layer i's attention of one query row over the first lens[b] rows,
+        the last of them the given k and v, which the call appends."""
+        if self.bits == 8:
+            return gpu.decode_attention_int8(q, self.k[i], self.k_scale[i], self.v[i], self.v_scale[i], lens,
+                                             block=self.block, k_new=k, v_new=v)
+        return gpu.decode_attention(q, self.k[i], self.v[i], lens, k_new=k, v_new=v)
 
 
 def _block(model, i, x, B, T, attend):
@@ -327,8 +381,7 @@ def _block(model, i, x, B, T, attend):
     # layer-norm outputs stay anonymous temporaries: the graph can then fold
     # each layer_norm into the projection that consumes it
     R = B * T
-    qkv = gpu.add_bias(_mm(model, gpu.layer_norm(x, w[f"{p}.ln_1.weight"], w[f"{p}.ln_1.bias"]),
-                           f"{p}.attn.c_attn.weight", R), w[f"{p}.attn.c_attn.bias"])
+    qkv = _layer(model, gpu.layer_norm(x, w[f"{p}.ln_1.weight"], w[f"{p}.ln_1.bias"]), f"{p}.attn.c_attn", R)
 
     def heads(lo):
         part = gpu.slice(qkv, 1, lo, lo + d)
@@ -336,10 +389,9 @@ def _block(model, i, x, B, T, attend):
 
     a = attend(i, heads(0), heads(d), heads(2 * d))
     a = gpu.reshape(gpu.transpose_dims(a, 1, 2), [B * T, d])
-    x = x + gpu.add_bias(_mm(model, a, f"{p}.attn.c_proj.weight", R), w[f"{p}.attn.c_proj.bias"])
-    f = gpu.gelu(gpu.add_bias(_mm(model, gpu.layer_norm(x, w[f"{p}.ln_2.weight"], w[f"{p}.ln_2.bias"]),
-                                  f"{p}.mlp.c_fc.weight", R), w[f"{p}.mlp.c_fc.bias"]))
-    return x + gpu.add_bias(_mm(model, f, f"{p}.mlp.c_proj.weight", R), w[f"{p}.mlp.c_proj.bias"])
+    x = x + _layer(model, a, f"{p}.attn.c_proj", R)
+    f = _layer(model, gpu.layer_norm(x, w[f"{p}.ln_2.weight"], w[f"{p}.ln_2.bias"]), f"{p}.mlp.c_fc", R, "gelu")
+    return x + _layer(model, f, f"{p}.mlp.c_proj", R)
 
 
 def _head(model, x, rows):
@@ -379,7 +431,7 @@ def gpt2_prefill(model: dict, ids, cache: KVCache, positions=None):
     x = gpu.embedding(w["transformer.wte.weight"], idx) + gpu.embedding(w["transformer.wpe.weight"], positions)
 
     def attend(i, q, k, v):
-        gpu.kv_write_pair(cache.k[i], cache.v[i], k, v, cache.pos)
+        cache.write(i, k, v)
         return gpu.attention_causal(q, k, v)
 
     for i in range(cfg["n_layer"]):
@@ -409,13 +461,38 @@ def gpt2_decode_step(model: dict, tokens, cache: KVCache):
     lens = cache.pos + cache.one
 
     def attend(i, q, k, v):
-        # the attention kernel stores k, v as cache row pos (= lens - 1)
-        return gpu.decode_attention(q, cache.k[i], cache.v[i], lens, k_new=k, v_new=v)
+        # the attention stores k, v as cache row pos (= lens - 1)
+        return cache.attend(i, q, lens, k, v)
 
     for i in range(cfg["n_layer"]):
         x = _block(model, i, x, B, 1, attend)
     logits = _head(model, x, B)
     return logits, gpu.argmax(logits), lens
+
+
+def gpt2_score(model: dict, ids, top_k: int = 0):
+    """How likely each next token of a batch of texts [B, T] is: (logprobs,
+    entropy, lse), float32 [B, T] on the device, and with top_k also
+    (top_logprobs, top_ids) [B, T, top_k]; entry t is of token t + 1 given
+    those up to t (the last one's logprob, of no token, is 0).  Negative ids
+    are padding at the end of a text: they are read as token 0, which no
+    earlier position sees, and their log probabilities are 0."""
+    w = model["weights"]
+    ids = np.asarray(ids, dtype=np.int32)
+    if ids.ndim != 2 or ids.shape[1] < 1:
+        raise ValueError("ids must be [batch, length]")
+    B, T = ids.shape
+    if T > model["config"]["n_positions"]:
+        raise ValueError(f"length {T} exceeds n_positions {model['config']['n_positions']}")
+    idx = gpu.from_numpy(np.maximum(ids, 0).reshape(-1))
+    x = gpu.embedding(w["transformer.wte.weight"], idx) + \
+        gpu.embedding(w["transformer.wpe.weight"], gpu.from_numpy(np.tile(np.arange(T, dtype=np.int32), B)))
+    for i in range(model["config"]["n_layer"]):
+        x = _block(model, i, x, B, T, lambda i, q, k, v: gpu.attention_causal(q, k, v))
+    logits = _head(model, x, B * T)
+    nxt = np.full((B, T), -1, np.int32)
+    nxt[:, :-1] = ids[:, 1:]
+    return gpu.token_logprobs(gpu.reshape(logits, [B, T, logits.shape[-1]]), gpu.from_numpy(nxt), top_k=top_k)
 
 
 def generate_greedy(model: dict, prompt_ids, n_steps: int, cache: KVCache = None, capture: bool = True,
@@ -476,7 +553,8 @@ class Generation:
     """Greedy generation for B prompts of T ids as config C4 runs it: the
     prefill and one decode step are each captured once as a HIP graph
     (capture=True) over device-resident ids, positions, cache lengths and
-    tokens, so a generation is one prefill replay and `n_steps` decode
+    tokens (cache_bits=8 keeps the cache in 8 bits; logprobs=k also keeps the
+    log probability of each pick, the entropy and k alternatives), so a generation is one prefill replay and `n_steps` decode
     replays with no host work between them.  The picked tokens land in
     `out` [n_steps + 1, B] on the device.  With capture=False the same calls
     run op by op (the same kernels, launched one at a time).
@@ -487,13 +565,14 @@ class Generation:
     KV cache, python/applegpu_runtime/models/gpt2.py:84-178) for B sequences
     at once."""
 
-    def __init__(self, model: dict, prompt_ids, n_steps: int, capture: bool = True):
+    def __init__(self, model: dict, prompt_ids, n_steps: int, capture: bool = True, cache_bits: int = 16,
+                 logprobs: int = None):
         prompt = np.asarray(prompt_ids, dtype=np.int32)
         if prompt.ndim != 2:
             raise ValueError("prompt_ids must be [batch, length]")
         B, T = prompt.shape
         self.model, self.B, self.T, self.n_steps = model, B, T, n_steps
-        self.cache = KVCache(model["config"], B, T + n_steps, model.get("dtype", "float16"))
+        self.cache = KVCache(model["config"], B, T + n_steps, model.get("dtype", "float16"), bits=cache_bits)
         self.ids = gpu.from_numpy(prompt)
         self.positions = gpu.from_numpy(np.tile(np.arange(T, dtype=np.int32), B))
         self._zeros = gpu.from_numpy(np.zeros(B, np.int32))
@@ -501,20 +580,43 @@ class Generation:
         self.tokens = gpu.zeros([B], "int32")
         self.out = gpu.zeros([n_steps + 1, B], "int32")
         self._slots = [gpu.slice(self.out, 0, s, s + 1) for s in range(n_steps + 1)]
+        self.logprobs, self._picks, self._pick_slots = logprobs, [], []
+        if logprobs is not None:
+            # of each pick: log probability, entropy, and the alternatives
+            shapes = [([B], "float32"), ([B], "float32")]
+            if logprobs:
+                shapes += [([B, logprobs], "float32"), ([B, logprobs], "int32")]
+            self._picks = [gpu.zeros(s, d) for s, d in shapes]
+            self.pick_out = [gpu.zeros([n_steps + 1] + s, d) for s, d in shapes]
+            self._pick_slots = [[gpu.slice(t, 0, s, s + 1) for t in self.pick_out] for s in range(n_steps + 1)]
         self.graphs = None
         if capture:
             self.graphs = (gpu.capture(self._prefill), gpu.capture(self._step) if n_steps > 0 else None)
 
+    def _pick(self, logits, nxt):
+        """Keeps the picks, and what is asked for about them, of logits()
+        [B, vocab]."""
+        if self.logprobs is not None:
+            got = gpu.token_logprobs(logits(), nxt, top_k=self.logprobs)
+            for t, to in zip((got[0], got[1]) + got[3:], self._picks):
+                gpu.blit_copy(t, to)
+        gpu.blit_copy(nxt, self.tokens)
+
+    def _store(self, s: int):
+        gpu.blit_copy(self.tokens, self._slots[s])
+        for t, slot in zip(self._picks, self._pick_slots[s] if self._picks else []):
+            gpu.blit_copy(t, slot)
+
     def _prefill(self):
         gpu.blit_copy(self._zeros, self.cache.pos)
         logits, nxt = gpt2_prefill(self.model, self.ids, self.cache, positions=self.positions)
-        gpu.blit_copy(nxt, self.tokens)
+        self._pick(lambda: self.last_logits(logits), nxt)
         gpu.blit_copy(self._prompt_len, self.cache.pos)
         return logits
 
     def _step(self):
         logits, nxt, lens = gpt2_decode_step(self.model, self.tokens, self.cache)
-        gpu.blit_copy(nxt, self.tokens)
+        self._pick(lambda: logits, nxt)
         gpu.blit_copy(lens, self.cache.pos)
         return logits
 
@@ -527,7 +629,7 @@ class Generation:
         else:
             logits = self._prefill()
             logits.eval()
-        gpu.blit_copy(self.tokens, self._slots[0])
+        self._store(0)
         return logits
 
     def step(self, s: int):
@@ -541,7 +643,7 @@ class Generation:
         else:
             logits = self._step()
             logits.eval()
-        gpu.blit_copy(self.tokens, self._slots[s + 1])
+        self._store(s + 1)
         return logits
 
     def last_logits(self, prefill_logits):
@@ -564,6 +666,15 @@ class Generation:
                 kept.append(lg.to_numpy())
         toks = self.out.to_numpy().T.copy()
         return (toks, np.stack(kept)) if keep_logits else toks
+
+    def pick_logprobs(self):
+        """Of a generation with logprobs=k: numpy (log probabilities [B,
+        n_steps + 1] of the tokens that run returned, entropies of the
+        distributions they were picked from, and with k > 0 the most likely
+        tokens' log probabilities and ids, [B, n_steps + 1, k])."""
+        if self.logprobs is None:
+            raise ValueError("this generation keeps no log probabilities (logprobs=k)")
+        return tuple(np.swapaxes(t.to_numpy(), 0, 1).copy() for t in self.pick_out)
 
     def destroy(self):
         if self.graphs is not None:
