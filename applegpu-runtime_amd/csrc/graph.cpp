@@ -544,8 +544,36 @@ void eval_all(const std::vector<TensorP>& roots) {
   std::unordered_map<Tensor*, TensorP> pack_of;    // group final node or paired layer_norm -> pack_rows_x3 of it
   std::unordered_map<Tensor*, TensorP> stats_of;   // group final node -> row_stats_x3 of it
   std::unordered_map<Tensor*, TensorP> attn_pack;  // attention node -> pack_rows_x3 of its head-merged output
+  // linear_int4 nodes: the layer_norm that one reads (few rows) runs in its
+  // prologue, the add that alone reads one in its epilogue.
+  std::unordered_map<Tensor*, const Node*> int4_ln;   // linear_int4 node -> its absorbed layer_norm
+  std::unordered_map<Tensor*, Tensor*> int4_add;      // add -> the absorbed linear_int4 it completes
   for (auto& t : order) {
     Node* n = t->node.get();
+    if (n->code == OP_LINEAR_INT4) {
+      const TensorP& la = n->in[0];
+      if (la->pending() && la->node->code == OP_LAYER_NORM && la->ndim == 2 && la->node->in[1]->ndim == 1 &&
+          la->node->in[2]->ndim == 1 && ops::linear_int4_normalises(la->dtype, la->shape[0], la->shape[1]) &&
+          is_single_internal_use(la, uses)) {
+        int4_ln[t.get()] = la->node.get();
+        absorbed.insert(la.get());
+      }
+      continue;
+    }
+    if (n->code == OP_ADD) {
+      bool taken = false;
+      for (int side = 0; side < 2 && !taken; ++side) {
+        const TensorP& x = n->in[side];
+        const TensorP& other = n->in[1 - side];
+        if (!x->pending() || x->node->code != OP_LINEAR_INT4 || other.get() == x.get() || other->dims() != t->dims() ||
+            x->dims() != t->dims() || other->dtype != x->dtype || !is_single_internal_use(x, uses))
+          continue;
+        int4_add[t.get()] = x.get();
+        absorbed.insert(x.get());
+        taken = true;
+      }
+      if (taken) continue;
+    }
     if (n->code == OP_ADD_BIAS && t->ndim == 2) {
       const TensorP& x = n->in[0];
       if (x->pending() &&
@@ -734,7 +762,7 @@ void eval_all(const std::vector<TensorP>& roots) {
     auto fusable = [&](Tensor* t) {
       return chain_op(t->node->code) >= 0 && (t->dtype == DType::F32 || t->dtype == DType::F16 ||
                                               t->dtype == DType::BF16) &&
-             !absorbed.count(t) && !groups.count(t) && !emb_adds.count(t) && !post_ln.count(t);
+             !absorbed.count(t) && !groups.count(t) && !emb_adds.count(t) && !post_ln.count(t) && !int4_add.count(t);
     };
     std::unordered_set<Tensor*> taken;
     for (size_t i = 0; i < order.size(); ++i) {
@@ -942,6 +970,26 @@ void eval_all(const std::vector<TensorP>& roots) {
       }
       g_stats.fused_gemm_epilogues++;
       g_stats.launches_saved += (g.has_bias ? 1 : 0) + (g.act ? 1 : 0) + (g.residual ? 1 : 0) + (g.ln_gamma ? 1 : 0);
+    } else if (n->code == OP_LINEAR_INT4 || int4_add.count(t.get())) {
+      Tensor* lin = t.get();
+      ops::Int4More more;
+      if (n->code == OP_ADD) {
+        lin = int4_add[t.get()];
+        more.residual = n->in[0].get() == lin ? n->in[1] : n->in[0];
+        g_stats.launches_saved++;
+      }
+      const Node* ln = lin->node.get();
+      TensorP x = ln->in[0];
+      auto li = int4_ln.find(lin);
+      if (li != int4_ln.end()) {
+        x = li->second->in[0];
+        more.ln_gamma = li->second->in[1];
+        more.ln_beta = li->second->in[2];
+        more.ln_eps = li->second->f.empty() ? 1e-5f : (float)li->second->f[0];
+        g_stats.launches_saved++;
+      }
+      res = {ops::linear_int4(x, ln->in[1], ln->in[2], ln->in.size() == 4 ? ln->in[3] : nullptr, ln->iv[0],
+                              (int)ln->iv[1], &more)};
     } else if (n->code < 0) {
       fail("internal: multi-output selector reached without its producer");
     } else if (op_outputs(n->code) > 1) {

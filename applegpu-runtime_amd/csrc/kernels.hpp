@@ -547,8 +547,15 @@ struct LinearInt4 {
   const void* scales = nullptr;
   const void* bias = nullptr;
   int act = 0;
+  const void* residual = nullptr;  // [M, N] contiguous, added after the activation
+  // rows of x normalised first (gamma, beta [K]): layer_norm(x) W^T, where
+  // linear_int4_ln_ok
+  const void* ln_gamma = nullptr;
+  const void* ln_beta = nullptr;
+  float ln_eps = 1e-5f;
   void* out = nullptr;
 };
+bool linear_int4_ln_ok(const LinearInt4& a);
 void linear_int4(const LinearInt4& a, hipStream_t s);
 
 // ── log probabilities of given tokens ─────────────────────────────────────

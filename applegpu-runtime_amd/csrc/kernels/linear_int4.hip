@@ -152,17 +152,74 @@ template <typename T, int MT, int NT, int G> struct InFlight {
   static constexpr int XB = sizeof(T) == 2 && MT <= 2 && !(MT == 1 && NT == 2 && G == 32) ? 2 : 1;
 };
 
+constexpr int kLnK = 2048, kLnX = 14336;  // row and elements of x that the normalising form holds (LDS: 64 KB with the sums)
+
+// The rows of x normalised into LDS (row stride K + 8), a wave a row: the
+// mean, then the mean square of the differences, from registers, rounded to T
+// as layer_norm's own output is.
+template <typename T>
+__device__ __forceinline__ void normalise_rows(const LinearInt4& a, T* xs, int K, int w, int nw, int lane) {
+  const T* ga = (const T*)a.ln_gamma;
+  const T* be = (const T*)a.ln_beta;
+  for (int m = w; m < (int)a.M; m += nw) {
+    const T* x = (const T*)a.x + m * a.x_sm;
+    float v[kLnK / 512][8];
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < kLnK / 512; ++i) {
+      const int k = (lane + 64 * i) * 8;
+      T e[8];
+      uint4 raw{0, 0, 0, 0};
+      if (k < K) raw = *(const uint4*)(x + k);
+      __builtin_memcpy(e, &raw, 16);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[i][j] = to_f(e[j]);
+        sum += v[i][j];
+      }
+    }
+    const float mean = wave_sum(sum) / (float)K;
+    float var = 0.f;
+#pragma unroll
+    for (int i = 0; i < kLnK / 512; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float d = v[i][j] - mean;
+        var += (lane + 64 * i) * 8 < K ? d * d : 0.f;
+      }
+    const float inv = 1.f / sqrtf(wave_sum(var) / (float)K + a.ln_eps);
+#pragma unroll
+    for (int i = 0; i < kLnK / 512; ++i) {
+      const int k = (lane + 64 * i) * 8;
+      if (k < K) {
+        const uint4 gr = *(const uint4*)(ga + k), br = *(const uint4*)(be + k);
+        T ge[8], bb[8], o[8];
+        __builtin_memcpy(ge, &gr, 16);
+        __builtin_memcpy(bb, &br, 16);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[j] = from_f<T>(to_f(ge[j]) * (v[i][j] - mean) * inv + to_f(bb[j]));
+        uint4 raw;
+        __builtin_memcpy(&raw, o, 16);
+        *(uint4*)(xs + m * (K + 8) + k) = raw;
+      }
+    }
+  }
+}
+
 // MT tiles of 16 rows of x by NT tiles of 16 columns of the output; the waves
 // of a block take 128-deep steps of K in turn.  G: columns of a scale.  XVEC:
-// K and the rows of x are such that 8 columns are one aligned load.
-template <typename T, int MT, int NT, int G, bool XVEC>
+// K and the rows of x are such that 8 columns are one aligned load.  LN: the
+// rows are normalised into LDS first, while the first codes are on their way.
+template <typename T, int MT, int NT, int G, bool XVEC, bool LN>
 __global__ void __launch_bounds__(MT == 1 ? 1024 : 512) linear_int4_mfma(L4Args g) {
   typedef In4<T> I;
   typedef typename I::vec V;
   constexpr int NG = 128 / G, UN = InFlight<T, MT, NT, G>::UN, XB = InFlight<T, MT, NT, G>::XB, XW = sizeof(T) / 2;
   static_assert(UN % XB == 0, "the rows' buffers follow the steps");
-  extern __shared__ float red[];  // [nw][MT][NT][16][16]
+  static_assert(!LN || (XVEC && MT == 1 && sizeof(T) == 2), "few 16-bit rows of whole vectors");
+  extern __shared__ float red[];  // [nw][MT][NT][16][16], then the normalised rows
   const LinearInt4& a = g.a;
+  T* xs = (T*)(red + g.nw * MT * NT * 256);
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, q = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int steps = (int)g.steps, nw = g.nw, K = (int)a.K, groups = (K + G - 1) / G;
@@ -214,7 +271,9 @@ __global__ void __launch_bounds__(MT == 1 ? 1024 : 512) linear_int4_mfma(L4Args 
         const int k = k_of(st, t);
 #pragma unroll
         for (int e = 0; e < XW; ++e) xr[b][t][i][e] = uint4{0, 0, 0, 0};
-        if constexpr (XVEC) {
+        if constexpr (LN) {
+          if (row_ok[i] && k < K) xr[b][t][i][0] = *(const uint4*)(xs + c * (K + 8) + k);
+        } else if constexpr (XVEC) {
           if (row_ok[i] && k < K)
 #pragma unroll
             for (int e = 0; e < XW; ++e) xr[b][t][i][e] = ((const uint4*)(x[i] + k))[e];
@@ -329,8 +388,13 @@ __global__ void __launch_bounds__(MT == 1 ? 1024 : 512) linear_int4_mfma(L4Args 
   if (w < steps) {
 #pragma unroll
     for (int u = 0; u < UN; ++u) load_w(u, w + u * nw);
-    if constexpr (XB == 2) load_x(0, w);
   }
+  if constexpr (LN) {
+    normalise_rows<T>(a, xs, K, w, nw, lane);
+    __syncthreads();
+  }
+  if constexpr (XB == 2)
+    if (w < steps) load_x(0, w);
   for (int s0 = w; s0 < steps; s0 += nw * UN) {
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
@@ -360,7 +424,9 @@ __global__ void __launch_bounds__(MT == 1 ? 1024 : 512) linear_int4_mfma(L4Args 
     float v = 0.f;
     for (int i = 0; i < g.nw; ++i) v += red[i * MT * NT * 256 + at];
     if (a.bias) v += to_f(((const T*)a.bias)[n]);
-    ((T*)a.out)[m * a.N + n] = from_f<T>(act_of(v, a.act));
+    v = act_of(v, a.act);
+    if (a.residual) v += to_f(((const T*)a.residual)[m * a.N + n]);
+    ((T*)a.out)[m * a.N + n] = from_f<T>(v);
   }
 }
 
@@ -369,8 +435,15 @@ void launch_int4(const L4Args& g, bool xvec, hipStream_t s) {
   const int64_t tiles = (g.a.N + 15) / 16, bx = (tiles + NT - 1) / NT, by = (g.a.M + 16 * MT - 1) / (16 * MT);
   const dim3 grid((unsigned)bx, (unsigned)by);
   const size_t lds = (size_t)g.nw * MT * NT * 256 * sizeof(float);
-  if (xvec) hipLaunchKernelGGL((linear_int4_mfma<T, MT, NT, G, true>), grid, dim3(64 * g.nw), lds, s, g);
-  else hipLaunchKernelGGL((linear_int4_mfma<T, MT, NT, G, false>), grid, dim3(64 * g.nw), lds, s, g);
+  if constexpr (MT == 1 && sizeof(T) == 2) {
+    if (g.a.ln_gamma) {
+      hipLaunchKernelGGL((linear_int4_mfma<T, MT, NT, G, true, true>), grid, dim3(64 * g.nw),
+                         lds + (size_t)g.a.M * (g.a.K + 8) * sizeof(T), s, g);
+      return;
+    }
+  }
+  if (xvec) hipLaunchKernelGGL((linear_int4_mfma<T, MT, NT, G, true, false>), grid, dim3(64 * g.nw), lds, s, g);
+  else hipLaunchKernelGGL((linear_int4_mfma<T, MT, NT, G, false, false>), grid, dim3(64 * g.nw), lds, s, g);
 }
 
 template <typename T, int MT, int NT>
@@ -415,15 +488,24 @@ void dequantize_int4(DType dt, const uint8_t* packed, const void* scales, int64_
   check_launch("dequantize_int4");
 }
 
+static bool int4_rows_aligned(const LinearInt4& a) {
+  return a.K % 8 == 0 && ((uintptr_t)a.x & 15) == 0 && (a.M == 1 || a.x_sm * (int64_t)dtype_size(a.dt) % 16 == 0);
+}
+
+bool linear_int4_ln_ok(const LinearInt4& a) {
+  return a.dt != DType::F32 && a.M >= 1 && a.M <= 16 && a.K <= kLnK && a.M * a.K <= kLnX && int4_rows_aligned(a) &&
+         ((uintptr_t)a.ln_gamma & 15) == 0 && ((uintptr_t)a.ln_beta & 15) == 0;
+}
+
 void linear_int4(const LinearInt4& a, hipStream_t s) {
   if (a.M == 0) return;
+  if (a.ln_gamma && !linear_int4_ln_ok(a)) fail("linear_int4: these rows cannot be normalised in the product");
   if (a.M > kInt4Rows || a.K > 0x7fffff00LL || (a.N + 15) / 16 > 0x7fffffffLL)
     fail("linear_int4: too many rows or columns");
   L4Args g;
   g.a = a;
   g.steps = (a.K + 127) / 128;
-  const int es = (int)dtype_size(a.dt);
-  const bool xvec = a.K % 8 == 0 && ((uintptr_t)a.x & 15) == 0 && (a.M == 1 || a.x_sm * es % 16 == 0);
+  const bool xvec = int4_rows_aligned(a);
   const int mt = a.M <= 16 ? 1 : a.M <= 32 ? 2 : 4;
   const int64_t tiles = (a.N + 15) / 16;
   const bool wide = mt > 1 || tiles >= 320;

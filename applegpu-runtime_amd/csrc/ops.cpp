@@ -2117,9 +2117,17 @@ TensorP dequantize_int4(const TensorP& packed, const TensorP& scales, int64_t K,
   return out;
 }
 
-TensorP linear_int4(const TensorP& x, const TensorP& packed, const TensorP& scales, const TensorP& bias, int64_t group,
-                    int act) {
+bool linear_int4_normalises(DType dt, int64_t rows, int64_t in) {
+  k::LinearInt4 a;
+  a.dt = dt;
+  a.M = rows; a.K = a.x_sm = in;
+  return k::linear_int4_ln_ok(a);
+}
+
+TensorP linear_int4(const TensorP& x_in, const TensorP& packed, const TensorP& scales, const TensorP& bias,
+                    int64_t group, int act, const Int4More* more) {
   const char* name = "linear_int4";
+  TensorP x = x_in;
   check_dtype(name, kFloatOnly, x->dtype);
   if (x->ndim < 1) fail("%s requires at least 1D input", name);
   if (act < k::kActNone || act > k::kActGeluExact) fail("%s: unknown activation %d", name, act);
@@ -2146,6 +2154,8 @@ TensorP linear_int4(const TensorP& x, const TensorP& packed, const TensorP& scal
     Epilogue e;
     e.bias = bc;
     e.act = act;
+    if (more && more->residual) e.residual = reshape(contiguous(more->residual), {M, N});
+    if (more && more->ln_gamma) x = layer_norm(x, more->ln_gamma, more->ln_beta, more->ln_eps);
     return reshape(matmul(reshape(contiguous(x), {M, K}), view(w, {N, K}, {ld, 1}, 0), false, true, &e), od);
   }
   TensorP xc = contiguous(x);
@@ -2159,6 +2169,23 @@ TensorP linear_int4(const TensorP& x, const TensorP& packed, const TensorP& scal
   a.bias = bc ? bc->data() : nullptr;
   a.act = act;
   a.out = out->data();
+  TensorP keep[3];
+  if (more && more->residual) {
+    keep[0] = contiguous(more->residual);
+    a.residual = keep[0]->data();
+  }
+  if (more && more->ln_gamma) {
+    keep[1] = contiguous(more->ln_gamma);
+    keep[2] = contiguous(more->ln_beta);
+    a.ln_gamma = keep[1]->data();
+    a.ln_beta = keep[2]->data();
+    a.ln_eps = more->ln_eps;
+    if (!meta_mode() && !k::linear_int4_ln_ok(a)) {  // alignments that only the operands' addresses tell
+      xc = contiguous(layer_norm(x, more->ln_gamma, more->ln_beta, more->ln_eps));
+      a.x = xc->data();
+      a.ln_gamma = a.ln_beta = nullptr;
+    }
+  }
   LAUNCH k::linear_int4(a, rt().stream());
   return out;
 }

@@ -287,9 +287,18 @@ TensorP decode_attention_int8(const TensorP& q, const Int8KV& c, const TensorP& 
 // and its values again ([N, K], the scales' dtype).
 std::vector<TensorP> quantize_int4(const TensorP& w, int64_t group);
 TensorP dequantize_int4(const TensorP& packed, const TensorP& scales, int64_t K, int64_t group);
-// act(x W^T + bias) over the last dim of x; bias may be null.
+// act(x W^T + bias) over the last dim of x; bias may be null.  With `more`
+// (fused by the graph): residual, of the output's shape and dtype, is added,
+// and with ln_gamma and ln_beta ([in]) layer_norm(x) takes x's place.
+struct Int4More {
+  TensorP residual, ln_gamma, ln_beta;
+  float ln_eps = 1e-5f;
+};
 TensorP linear_int4(const TensorP& x, const TensorP& packed, const TensorP& scales, const TensorP& bias, int64_t group,
-                    int act);
+                    int act, const Int4More* more = nullptr);
+// Whether a layer_norm of `rows` rows of `in` 16-bit values is worth leaving
+// to the product that reads it.
+bool linear_int4_normalises(DType dt, int64_t rows, int64_t in);
 // {lp, entropy, lse} of logits [..., V] and int32/int64 tokens [...], fp32,
 // and with top_k > 0 also {top log probabilities, int32 indices} [..., top_k].
 std::vector<TensorP> token_logprobs(const TensorP& logits, const TensorP& tokens, int64_t top_k);

@@ -214,3 +214,65 @@ def test_refusals(gpu):
             call(**bad)
     with pytest.raises(ValueError, match="dequantize_int4"):
         gpu.dequantize_int4(packed, s, 300, 64)
+
+
+# ── norms and residuals of a graph ──────────────────────────────────────────
+def _norm(x, g, b):
+    m = x.mean(-1, keepdims=True)
+    return (x - m) / np.sqrt(((x - m) ** 2).mean(-1, keepdims=True) + 1e-5) * g + b
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16", "float32"])
+@pytest.mark.parametrize("M,N,K", [(1, 48, 128), (8, 5200, 1280), (16, 33, 896), (7, 40, 2048), (3, 17, 40), (2, 20, 33),
+                                   (16, 20, 1000), (17, 48, 128), (90, 48, 128)])
+@pytest.mark.parametrize("group", [32, 128])
+def test_layer_norm_and_residual_around(gpu, dtype, M, N, K, group):
+    """r + act(layer_norm(x) W^T + b): the norm's output is rounded once more
+    (half a step of each normalised value against |W|)."""
+    rng = np.random.default_rng(M + K)
+    w = _weights(rng, N, K, dtype)
+    codes, scales = O.quantize_int4(w, group, dtype)
+    wv = O.values_int4(codes, scales, group)
+    x, r, g, b, bias = (O.round_to(rng.standard_normal(s).astype(np.float32) + o, dtype)
+                        for s, o in (((M, K), 0.5), ((M, N), 0), ((K,), 1), ((K,), 0), ((N,), 0)))
+    d = [_dev(gpu, a, dtype) for a in (x, r, g, b, bias)]
+    packed, s = gpu.from_numpy(_pack(codes)), _dev(gpu, scales, dtype)
+    before = gpu.graph_stats()["launches_saved"]
+    y = d[1] + gpu.linear_int4(gpu.layer_norm(d[0], d[2], d[3]), packed, s, d[4], "gelu", group=group)
+    got = y.to_numpy().astype(np.float64)
+    saved = gpu.graph_stats()["launches_saved"] - before
+    assert saved == 1 + (dtype != "float32" and M <= 16 and K % 8 == 0 and M * K <= 14336)
+    n = _norm(x.astype(np.float64), g, b)
+    lin = O.linear(n, wv, bias)
+    want = r + O.linear(n, wv, bias, "gelu")
+    half = HALF_STEP[dtype]
+    step = np.repeat(scales.T.astype(np.float64), group, 1)[:, :K]
+    bar = 2.0 ** -24 * (16 * 24 + K / 32 + 32) * (np.abs(n) @ step.T) + (half + 2.0 ** -20) * (np.abs(n) @ np.abs(wv).T)
+    bar = bar + (half * (np.abs(n) @ np.abs(wv).T) if M > 64 else 0)
+    bar = 1.13 * bar + (half + 2.0 ** -20) * (np.abs(lin) + np.abs(want)) + 2.0 ** -20
+    assert (np.abs(got - want) <= bar).all(), (np.abs(got - want) / bar).max()
+
+
+def test_what_else_reads_a_norm_or_a_product_keeps_it(gpu):
+    rng = np.random.default_rng(1)
+    w = _weights(rng, 32, 64, "float16")
+    packed, s = gpu.quantize_int4(_dev(gpu, w, "float16"), 32)
+    x, g, b = (_dev(gpu, rng.standard_normal(sh).astype(np.float32), "float16") for sh in ((4, 64), (64,), (64,)))
+    n = gpu.layer_norm(x, g, b)
+    y = gpu.linear_int4(n, packed, s, group=32)
+    z = y + y                                   # the product twice
+    v = gpu.linear_int4(gpu.layer_norm(x, g, b), packed, s, group=32) + gpu.slice(_dev(gpu, np.ones((1, 32)), "float16"), 0, 0, 1)
+    np.testing.assert_allclose(v.to_numpy(), y.to_numpy() + np.float16(1), rtol=2e-3, atol=2e-3)
+    np.testing.assert_array_equal(z.to_numpy(), y.to_numpy() + y.to_numpy())
+    again = gpu.linear_int4(gpu.from_numpy(n.to_numpy()), packed, s, group=32).to_numpy()
+    np.testing.assert_array_equal(y.to_numpy(), again)
+    p, q = gpu.linear_int4(x, packed, s, group=32), gpu.linear_int4(x, packed, s, group=32)
+    t = p + q                                   # two products: one is the other's residual
+    np.testing.assert_allclose(t.to_numpy().astype(np.float64), 2 * gpu.linear_int4(x, packed, s, group=32).to_numpy(),
+                               rtol=2e-3, atol=2e-3)
+    # a view of a larger buffer as the norm's input, at an offset 16 bytes do not divide
+    big = _dev(gpu, rng.standard_normal((4, 67)).astype(np.float32), "float16")
+    part = gpu.slice(big, 1, 3, 67)
+    a = gpu.linear_int4(gpu.layer_norm(part, g, b), packed, s, group=32).to_numpy()
+    c = gpu.linear_int4(gpu.layer_norm(gpu.from_numpy(part.to_numpy()), g, b), packed, s, group=32).to_numpy()
+    np.testing.assert_allclose(a, c, rtol=2e-3, atol=2e-3)
