@@ -517,7 +517,14 @@ struct DecodeInt8 {
   void* o = nullptr; int64_t o_sb = 0, o_sh = 0, o_st = 0;
   const int32_t* lens = nullptr;
   float scale = 1.f;
+  // optional (decode_int8_appends): the step's own K and V rows [B, H, 1, D]
+  // (strides batch, head; 16-byte aligned), appended as row lens[b] - 1
+  const void* kn = nullptr; int64_t kn_sb = 0, kn_sh = 0;
+  const void* vn = nullptr; int64_t vn_sb = 0, vn_sh = 0;
 };
+// Whether the attention's own launch can append: one query row a sequence, a
+// cache head's query heads in one tile.
+bool decode_int8_appends(const DecodeInt8& a);
 size_t decode_int8_ws_bytes(const DecodeInt8& a);
 void decode_attention_int8(const DecodeInt8& a, void* ws, hipStream_t s);
 

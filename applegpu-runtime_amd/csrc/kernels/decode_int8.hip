@@ -32,7 +32,7 @@
 //    and within f16's normal range for 2^-21 of the maximum.
 // Work: waves of a block take 32-key steps in turn; a context is split over
 // blocks while these leave CUs idle, and the splits' (O, m, l) are merged.
-#include "device.hpp"
+#include "kv_int8.hpp"
 
 namespace agpu {
 namespace k {
@@ -111,7 +111,13 @@ struct Step {
   float ks[2], vs[2];
 };
 
-template <typename T, int D, int NW>
+// NEW: the step's own row is appended too.  The block of waves whose part of
+// the context holds it leaves its cache block to the end: two waves append to
+// K and V there (as kv_write_int8 does), before anything else, while the others
+// are at the rows before it, and after a barrier the block's rows are read
+// from the cache like any (8 x 20 heads over 640 rows of 64: 9.2 us without,
+// 11.6 so, 14.0 with a launch of its own for the append).
+template <typename T, int D, int NW, bool NEW>
 __global__ void __launch_bounds__(64 * NW) decode_int8_mfma(D8Args g) {
   constexpr bool F32 = sizeof(T) == 4;
   constexpr int NK = D / 32;     // MFMAs of a score tile
@@ -119,7 +125,7 @@ __global__ void __launch_bounds__(64 * NW) decode_int8_mfma(D8Args g) {
   constexpr int LD = D + 4;      // padding of a query's row in LDS
   constexpr int64_t kIter = NW * kStep;
   extern __shared__ float sm_o[];  // [NW][rows of the tile][LD]
-  __shared__ float sm_m[NW][16], sm_l[NW][16];
+  __shared__ float sm_m[NW][16], sm_l[NW][16], sm_new[2];
   const DecodeInt8& a = g.a;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, q4 = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -200,17 +206,41 @@ __global__ void __launch_bounds__(64 * NW) decode_int8_mfma(D8Args g) {
   for (int t = 0; t < NK; ++t) qr[t].load(q + (D == 32 ? 8 * q4 : 64 * (t >> 1) + 16 * q4 + 8 * (t & 1)));
   Step<D> one, two;
   int64_t j0 = j_lo + w * kStep;
-  if (j0 < a.Tmax) load(one, j0);
-  int64_t len = a.lens[b];
-  len = len < 0 ? 0 : len > a.Tmax ? a.Tmax : len;
+  const bool appends = NEW && w >= NW - 2;
+  if (!appends && j0 < a.Tmax) load(one, j0);
+  const int64_t asked = a.lens[b], len = asked < 0 ? 0 : asked > a.Tmax ? a.Tmax : asked;
 
   // the tile's rows r0 .. r1, and what they see
   const int r1 = r0 + 15 < R ? r0 + 15 : R - 1;
   const bool one_head = r0 / Tq == r1 / Tq;
-  const int64_t vis_lo = len - Tq + (one_head ? r0 % Tq : 0) + 1, vis_hi = len - Tq + (one_head ? r1 % Tq : Tq - 1) + 1;
-  const int64_t vis = r0 + n < R ? len - Tq + i_q + 1 : 0;
+  int64_t vis_lo = len - Tq + (one_head ? r0 % Tq : 0) + 1;
+  const int64_t vis_hi = len - Tq + (one_head ? r1 % Tq : Tq - 1) + 1;
+  int64_t vis = r0 + n < R ? len - Tq + i_q + 1 : 0;
 
-  const int64_t j_hi = j_lo + g.chunk < vis_hi ? j_lo + g.chunk : vis_hi;
+  int64_t j_hi = j_lo + g.chunk < vis_hi ? j_lo + g.chunk : vis_hi;
+
+  // the rows of the cache block that the step's row joins, if it is of this part
+  int64_t tail = -1;
+  if constexpr (NEW) {
+    const int64_t at = asked - 1;  // (a length outside 1 .. Tmax names no row)
+    if (at >= 0 && at < a.Tmax && at >= j_lo && at < j_lo + g.chunk) {
+      tail = (at >> g.lg_block) << g.lg_block;
+      j_hi = vis_lo = tail;
+      vis = vis < tail ? vis : tail;
+    }
+    if (appends) {
+      if (tail >= 0) {
+        const bool v = w == NW - 2;
+        const Int8Cache& c = v ? a.v : a.k;
+        const T* x = v ? (const T*)a.vn + b * a.vn_sb + h * a.vn_sh : (const T*)a.kn + b * a.kn_sb + h * a.kn_sh;
+        const float s = kv8::append_rows<T, 1>(x, 0, c.codes + b * c.cs[0] + h * c.cs[1], c.cs[2],
+                                               c.scales + b * c.ss[0] + h * c.ss[1] + (tail >> g.lg_block) * c.ss[2],
+                                               tail, len - 1, len, D == 32 ? 2 : D == 64 ? 3 : 4, lane);
+        if (lane == 0) sm_new[v] = s;
+      }
+      if (j0 < j_hi) load(one, j0);
+    }
+  }
 
   // queries as MFMA operands: lane (n, q4) holds d = 64 c + 16 q4 + 8 x + e of
   // row n (D = 32: d = 8 q4 + e), scaled to [128, 256) at the row's largest
@@ -374,6 +404,24 @@ __global__ void __launch_bounds__(64 * NW) decode_int8_mfma(D8Args g) {
     j0 += kIter;
   }
 
+  if constexpr (NEW) {
+    if (tail >= 0) {
+      __threadfence_block();  // what the two waves stored, for the others
+      __syncthreads();
+      j_hi = len;
+      vis = r0 + n < R ? len : 0;
+      for (j0 = tail + w * kStep; j0 < j_hi; j0 += kIter) {
+        load(one, j0);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {  // (the scales may be in the scalar cache as they were)
+          one.ks[t] = sm_new[0];
+          one.vs[t] = sm_new[1];
+        }
+        attend(one, j0);
+      }
+    }
+  }
+
   // the waves' states meet in LDS; lane (n, q4) holds d = (D/4) q4 + (D/16) i + c
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
@@ -491,7 +539,8 @@ D8Args plan(const DecodeInt8& a) {
 template <typename T, int D, int NW>
 void launch_nw(const D8Args& g, hipStream_t s) {
   const dim3 grid((unsigned)(g.a.B * g.a.H * g.q_tiles * g.splits));
-  hipLaunchKernelGGL((decode_int8_mfma<T, D, NW>), grid, dim3(64 * NW), lds_bytes(g.a, NW), s, g);
+  if (g.a.kn) hipLaunchKernelGGL((decode_int8_mfma<T, D, NW, true>), grid, dim3(64 * NW), lds_bytes(g.a, NW), s, g);
+  else hipLaunchKernelGGL((decode_int8_mfma<T, D, NW, false>), grid, dim3(64 * NW), lds_bytes(g.a, NW), s, g);
 }
 
 template <typename T, int D>
@@ -504,6 +553,8 @@ void launch(const D8Args& g, hipStream_t s) {
 }
 
 }  // namespace
+
+bool decode_int8_appends(const DecodeInt8& a) { return a.Tq == 1 && a.G <= 16; }
 
 size_t decode_int8_ws_bytes(const DecodeInt8& a) {
   const D8Args g = plan(a);
@@ -518,6 +569,7 @@ void decode_attention_int8(const DecodeInt8& a, void* ws, hipStream_t s) {
   D8Args g = plan(a);
   if (a.G * a.Tq > 0x7fffffffLL / 2 || a.B * a.H * a.G * a.Tq > 0x7fffffffLL || a.B * a.H * g.q_tiles * g.splits > 0x7fffffffLL)
     fail("decode_attention_int8: too many query rows");
+  if (a.kn && (!a.vn || !decode_int8_appends(a))) fail("decode_attention_int8: cannot append in this launch");
   if (g.splits > 1 && !ws) fail("decode_attention_int8: workspace missing");
   g.part = (float*)ws;
   AGPU_FLOAT_SWITCH(a.dt, {

@@ -17,7 +17,7 @@
 //
 // One wave per (sequence, head, touched block); all traffic is the new rows,
 // their codes and, for the first block, the codes before them.
-#include "device.hpp"
+#include "kv_int8.hpp"
 
 namespace agpu {
 namespace k {
@@ -31,75 +31,6 @@ struct KvArgs8 {
   uint32_t nbt, waves;   // blocks an append touches at most; B * H * nbt
 };
 
-__device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) {
-    const uint32_t o = (uint32_t)__shfl_xor((int)v, m, 64);
-    v = o > v ? o : v;
-  }
-  return v;
-}
-
-// 8 consecutive values, raw.
-template <typename T>
-struct Raw8x {
-  uint4 v[sizeof(T) / 2];
-  __device__ __forceinline__ void load(const T* p) {
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = ((const uint4*)p)[i];
-  }
-  __device__ __forceinline__ void floats(float (&x)[8]) const {
-    T e[8];
-    __builtin_memcpy(e, v, sizeof(e));
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = to_f(e[i]);
-  }
-};
-
-__device__ __forceinline__ uint32_t top_of(const float (&v)[8], uint32_t top) {
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const uint32_t m = __float_as_uint(v[e]) & 0x7fffffffu;
-    top = m > top ? m : top;
-  }
-  return top;
-}
-
-// clamp(rint(x / s), -127, 127) of 8 values; 0 where the scale says nothing
-// (0, infinite or NaN).  x / s is IEEE's; x times 1 / s is within 127 (2^-23 +
-// 2^-24) < 2.3e-5 of it, so only where that is nearer than 1e-4 to a half is
-// the division done (as 8 divisions a chunk the append of 8 x 20 x 509 rows
-// of 64 takes 13.7 us, bound by them).
-__device__ __forceinline__ void codes_of(const float (&v)[8], float s, float inv, bool ok, int (&c)[8]) {
-  float r[8];
-  bool near = !(inv < 1e30f);  // 1 / s overflows, or nearly
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float q = v[e] * inv;
-    r[e] = rintf(q);
-    near |= fabsf(fabsf(q - r[e]) - 0.5f) < 1e-4f;
-  }
-  if (near) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) r[e] = rintf(v[e] / s);
-  }
-#pragma unroll
-  for (int e = 0; e < 8; ++e) c[e] = ok ? (int)fminf(fmaxf(r[e], -127.f), 127.f) : 0;
-}
-
-__device__ __forceinline__ void store_codes(int8_t* p, const int (&c)[8]) {
-  uint2 w{0, 0};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    w.x |= (uint32_t)(c[i] & 255) << (8 * i);
-    w.y |= (uint32_t)(c[4 + i] & 255) << (8 * i);
-  }
-  *(uint2*)p = w;
-}
-
-// NC > 0: the new rows of a block are at most 64 NC chunks and stay in
-// registers between the search for the largest and the rounding; 0: any
-// number, read twice.
 template <typename T, int NC>
 __global__ void __launch_bounds__(256) kv_write_int8_kernel(KvArgs8 g) {
   const KvInt8& a = g.a;
@@ -119,75 +50,7 @@ __global__ void __launch_bounds__(256) kv_write_int8_kernel(KvArgs8 g) {
   int8_t* codes = c.codes + b * c.cs[0] + h * c.cs[1];
   float* scale = c.scales + b * c.ss[0] + h * c.ss[1] + n * c.ss[2];
   const T* x = (const T*)a.x[j] + b * a.xs[j][0] + h * a.xs[j][1] + (r0 - p) * a.xs[j][2];
-  int8_t* to = codes + r0 * c.cs[2];
-  const int cpr = 1 << g.lg_cpr;
-  const int chunks = (int)(r1 - r0) << g.lg_cpr;
-
-  uint32_t top = 0;
-  Raw8x<T> keep[NC ? NC : 1];
-  if constexpr (NC > 0) {
-#pragma unroll
-    for (int u = 0; u < NC; ++u) {
-      const int i = lane + 64 * u;
-#pragma unroll
-      for (int e = 0; e < (int)sizeof(T) / 2; ++e) keep[u].v[e] = uint4{0, 0, 0, 0};
-      if (i < chunks) keep[u].load(x + (i >> g.lg_cpr) * a.xs[j][2] + (i & (cpr - 1)) * 8);
-    }
-#pragma unroll
-    for (int u = 0; u < NC; ++u) {
-      float v[8];
-      keep[u].floats(v);
-      top = top_of(v, top);
-    }
-  } else {
-    for (int i = lane; i < chunks; i += 64) {
-      Raw8x<T> raw;
-      raw.load(x + (i >> g.lg_cpr) * a.xs[j][2] + (i & (cpr - 1)) * 8);
-      float v[8];
-      raw.floats(v);
-      top = top_of(v, top);
-    }
-  }
-  uint32_t s_bits = __float_as_uint(__uint_as_float(wave_umax(top)) / 127.f) & 0x7fffffffu;
-  const uint32_t was = r0 > lo ? __float_as_uint(*scale) & 0x7fffffffu : 0u;
-  if (was > s_bits) s_bits = was;
-  const float s = __uint_as_float(s_bits);
-  const bool ok = s > 0.f && s < INFINITY;
-  const float inv = 1.f / s;
-
-  if (s_bits != was) {  // rows before the append, if any, take the grown scale
-    const int held = (int)(r0 - lo) << g.lg_cpr;
-    const float rate = ok ? __uint_as_float(was) / s : 0.f;
-    for (int i = lane; i < held; i += 64) {
-      int8_t* q = codes + (lo + (i >> g.lg_cpr)) * c.cs[2] + (i & (cpr - 1)) * 8;
-      const uint2 w = *(const uint2*)q;
-      int8_t o[8];
-      __builtin_memcpy(o, &w, 8);
-      int cc[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) cc[e] = (int)rintf((float)o[e] * rate);
-      store_codes(q, cc);
-    }
-  }
-  auto put = [&](int i, const Raw8x<T>& raw) {
-    float v[8];
-    raw.floats(v);
-    int cc[8];
-    codes_of(v, s, inv, ok, cc);
-    store_codes(to + (i >> g.lg_cpr) * c.cs[2] + (i & (cpr - 1)) * 8, cc);
-  };
-  if constexpr (NC > 0) {
-#pragma unroll
-    for (int u = 0; u < NC; ++u)
-      if (lane + 64 * u < chunks) put(lane + 64 * u, keep[u]);
-  } else {
-    for (int i = lane; i < chunks; i += 64) {
-      Raw8x<T> raw;
-      raw.load(x + (i >> g.lg_cpr) * a.xs[j][2] + (i & (cpr - 1)) * 8);
-      put(i, raw);
-    }
-  }
-  if (lane == 0) *scale = s;
+  kv8::append_rows<T, NC>(x, a.xs[j][2], codes, c.cs[2], scale, lo, r0, r1, g.lg_cpr, lane);
 }
 
 // A block per 2048 values of a (sequence, head): 8 a thread.

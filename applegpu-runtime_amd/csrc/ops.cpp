@@ -1981,27 +1981,31 @@ static TensorP int8_rows(const char* name, const TensorP& rows, const k::KvInt8&
   return ok ? rows : materialize(rows);
 }
 
-static void append_int8(const char* name, k::KvInt8 a, const Int8KV& c, const TensorP& k_rows, const TensorP& v_rows,
-                        const TensorP& pos, int pos_off) {
+// The append of rows at row pos[b] + pos_off, checked; r keeps the operands.
+static k::KvInt8 append_int8(const char* name, k::KvInt8 a, const Int8KV& c, const TensorP& k_rows,
+                             const TensorP& v_rows, const TensorP& pos, int pos_off, TensorP (&r)[3]) {
   if (c.kc->data() && c.kc->data() == c.vc->data()) fail("%s: K and V need codes of their own", name);
   if (c.ks->data() && c.ks->data() == c.vs->data()) fail("%s: K and V need scales of their own", name);
   a.dt = k_rows->dtype;
   a.T = k_rows->ndim == 4 ? k_rows->shape[2] : 0;
-  TensorP r[2] = {int8_rows(name, k_rows, a, a.dt), int8_rows(name, v_rows, a, a.dt)};
+  r[0] = int8_rows(name, k_rows, a, a.dt);
+  r[1] = int8_rows(name, v_rows, a, a.dt);
   if (r[1]->shape[2] != a.T) fail("%s: the K and V rows differ in number", name);
   if (a.T > a.Tmax) fail("%s: %lld rows exceed the cache length %lld", name, (long long)a.T, (long long)a.Tmax);
-  TensorP pc = check_lens(name, "positions", pos, a.B);
+  r[2] = check_lens(name, "positions", pos, a.B);
   for (int j = 0; j < 2; ++j) {
     a.x[j] = r[j]->data();
     for (int i = 0; i < 3; ++i) a.xs[j][i] = r[j]->strides[i];
   }
-  a.pos = (const int32_t*)pc->data();
+  a.pos = (const int32_t*)r[2]->data();
   a.pos_off = pos_off;
-  LAUNCH k::kv_write_int8(a, rt().stream());
+  return a;
 }
 
 void kv_write_int8(const Int8KV& c, const TensorP& k_rows, const TensorP& v_rows, const TensorP& pos) {
-  append_int8("kv_write_int8", int8_pair("kv_write_int8", c), c, k_rows, v_rows, pos, 0);
+  TensorP r[3];
+  const k::KvInt8 a = append_int8("kv_write_int8", int8_pair("kv_write_int8", c), c, k_rows, v_rows, pos, 0, r);
+  LAUNCH k::kv_write_int8(a, rt().stream());
 }
 
 std::vector<TensorP> kv_read_int8(const Int8KV& c, const TensorP& pos, int64_t T, DType dt) {
@@ -2047,7 +2051,6 @@ TensorP decode_attention_int8(const TensorP& q_in, const Int8KV& c, const Tensor
     if (Tq != 1) fail("%s: appending new rows needs one query row per sequence, got %lld", name, (long long)Tq);
     if (k_new->dtype != q->dtype) fail("%s: new rows must share q's dtype", name);
     if (k_new->ndim == 4 && k_new->shape[2] != 1) fail("%s: new rows must hold one token", name);
-    append_int8(name, p, c, k_new, v_new, lc, -1);
   }
   k::DecodeInt8 a;
   a.dt = q->dtype;
@@ -2057,6 +2060,16 @@ TensorP decode_attention_int8(const TensorP& q_in, const Int8KV& c, const Tensor
   a.k = p.c[0]; a.v = p.c[1];
   a.lens = (const int32_t*)lc->data();
   a.scale = scale;
+  TensorP r[3];
+  if (k_new) {
+    const k::KvInt8 w = append_int8(name, p, c, k_new, v_new, lc, -1, r);
+    if (k::decode_int8_appends(a)) {
+      a.kn = w.x[0]; a.kn_sb = w.xs[0][0]; a.kn_sh = w.xs[0][1];
+      a.vn = w.x[1]; a.vn_sb = w.xs[1][0]; a.vn_sh = w.xs[1][1];
+    } else {
+      LAUNCH k::kv_write_int8(w, rt().stream());
+    }
+  }
   // physical [B, Tq, Hq, D], logical [B, Hq, Tq, D]
   TensorP base = alloc_out(q->dtype, {B, Tq, Hq, D});
   TensorP out = make_meta(q->dtype, q->dims());
