@@ -540,12 +540,12 @@ int64_t int4_bytes(int64_t N, int64_t K);
 // scale rounded half to even, within -7 .. 7; w [N, K] read through strides.
 void quantize_int4(DType dt, const void* w, int64_t sn, int64_t sk, int64_t N, int64_t K, int64_t group,
                    uint8_t* packed, void* scales, hipStream_t s);
-// out [N, K] = the values, of the scales' dtype, row stride ld.
+// out [N, ld] = the values, of the scales' dtype, and zeros from column K on
+// (ld at most K rounded up to 128).
 void dequantize_int4(DType dt, const uint8_t* packed, const void* scales, int64_t N, int64_t K, int64_t group,
                      void* out, int64_t ld, hipStream_t s);
-// out [M, N] = act(x [M, K] W^T + bias) for M up to kInt4Rows; x rows
-// contiguous along K.
-constexpr int64_t kInt4Rows = 64;
+// out [M, N] = act(x [M, K] W^T + bias); x rows contiguous along K, and for
+// M > 1 16-byte aligned with K a multiple of 8.
 struct LinearInt4 {
   DType dt = DType::F16;
   int64_t M = 0, N = 0, K = 0, group = 128;
@@ -562,6 +562,8 @@ struct LinearInt4 {
   float ln_eps = 1e-5f;
   void* out = nullptr;
 };
+// out [M, ld] = x [M, K] (row stride sm) with zeros behind its rows.
+void pad_rows(DType dt, const void* x, int64_t sm, int64_t M, int64_t K, void* out, int64_t ld, hipStream_t s);
 bool linear_int4_ln_ok(const LinearInt4& a);
 void linear_int4(const LinearInt4& a, hipStream_t s);
 

@@ -57,7 +57,8 @@ __global__ void __launch_bounds__(256) int4_scales_kernel(const T* __restrict__ 
 
 // One lane per byte run: 32 codes of a row, of one scale.  A wave reads 1 KB in
 // a row and writes 64 bytes (16-bit types) of each of 16 rows four times over.
-// VEC: rows are aligned and whole runs of 8 values are one store.
+// VEC: rows are aligned and whole runs of 8 values are one store.  Columns K ..
+// ld - 1 become 0.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) dequantize_int4_kernel(const uint4* __restrict__ packed,
                                                               const T* __restrict__ scales, int64_t N, int64_t K,
@@ -66,24 +67,24 @@ __global__ void __launch_bounds__(256) dequantize_int4_kernel(const uint4* __res
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < runs; i += (int64_t)gridDim.x * 256) {
     const int run = (int)(i & 63);
     const int64_t tile = i >> 6, n = tile / steps * 16 + (run & 15), k0 = tile % steps * 128 + (run >> 4) * 32;
-    if (n >= N || k0 >= K) continue;
-    const uint4 w = packed[i];
+    if (n >= N || k0 >= ld) continue;
+    const uint4 w = packed[i];  // (padding has code 0)
     const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-    const float s = to_f(scales[k0 / group * N + n]);
+    const float s = k0 < K ? to_f(scales[k0 / group * N + n]) : 0.f;
     T* o = out + n * ld + k0;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       T v[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = from_f<T>((float)((int)((ws[t] >> (4 * nibble_of(e))) & 15) - 8) * s);
-      if (VEC && k0 + 8 * t + 8 <= K) {
+      if (VEC && k0 + 8 * t + 8 <= ld) {
         uint4 raw[sizeof(T) / 2];
         __builtin_memcpy(raw, v, sizeof(v));
 #pragma unroll
         for (int e = 0; e < (int)sizeof(T) / 2; ++e) ((uint4*)(o + 8 * t))[e] = raw[e];
       } else {
         for (int e = 0; e < 8; ++e)
-          if (k0 + 8 * t + e < K) o[8 * t + e] = v[e];
+          if (k0 + 8 * t + e < ld) o[8 * t + e] = v[e];
       }
     }
   }
@@ -136,6 +137,14 @@ __device__ __forceinline__ typename In4<T>::vec codes24(uint32_t w) {
   typename In4<T>::vec o;
   __builtin_memcpy(&o, r, 16);
   return o;
+}
+
+// Rows of x [M, K] with zeros behind them, [M, ld].
+template <typename T>
+__global__ void __launch_bounds__(256) pad_rows_kernel(const T* __restrict__ x, int64_t sm, int64_t K,
+                                                       T* __restrict__ out, int64_t ld) {
+  const int64_t m = blockIdx.x;
+  for (int64_t k = threadIdx.x; k < ld; k += 256) out[m * ld + k] = k < K ? x[m * sm + k] : (T)0.f;
 }
 
 struct L4Args {
@@ -442,8 +451,13 @@ void launch_int4(const L4Args& g, bool xvec, hipStream_t s) {
       return;
     }
   }
-  if (xvec) hipLaunchKernelGGL((linear_int4_mfma<T, MT, NT, G, true, false>), grid, dim3(64 * g.nw), lds, s, g);
-  else hipLaunchKernelGGL((linear_int4_mfma<T, MT, NT, G, false, false>), grid, dim3(64 * g.nw), lds, s, g);
+  if constexpr (MT == 1) {
+    if (!xvec) {
+      hipLaunchKernelGGL((linear_int4_mfma<T, MT, NT, G, false, false>), grid, dim3(64 * g.nw), lds, s, g);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((linear_int4_mfma<T, MT, NT, G, true, false>), grid, dim3(64 * g.nw), lds, s, g);
 }
 
 template <typename T, int MT, int NT>
@@ -488,6 +502,14 @@ void dequantize_int4(DType dt, const uint8_t* packed, const void* scales, int64_
   check_launch("dequantize_int4");
 }
 
+void pad_rows(DType dt, const void* x, int64_t sm, int64_t M, int64_t K, void* out, int64_t ld, hipStream_t s) {
+  if (M == 0) return;
+  if (M > 0x7fffffffLL) fail("pad_rows: too many rows");
+  AGPU_FLOAT_SWITCH(dt, hipLaunchKernelGGL((pad_rows_kernel<T>), dim3((unsigned)M), dim3(256), 0, s, (const T*)x, sm, K,
+                                           (T*)out, ld));
+  check_launch("pad_rows");
+}
+
 static bool int4_rows_aligned(const LinearInt4& a) {
   return a.K % 8 == 0 && ((uintptr_t)a.x & 15) == 0 && (a.M == 1 || a.x_sm * (int64_t)dtype_size(a.dt) % 16 == 0);
 }
@@ -500,16 +522,19 @@ bool linear_int4_ln_ok(const LinearInt4& a) {
 void linear_int4(const LinearInt4& a, hipStream_t s) {
   if (a.M == 0) return;
   if (a.ln_gamma && !linear_int4_ln_ok(a)) fail("linear_int4: these rows cannot be normalised in the product");
-  if (a.M > kInt4Rows || a.K > 0x7fffff00LL || (a.N + 15) / 16 > 0x7fffffffLL)
+  if (a.K > 0x7fffff00LL || (a.N + 15) / 16 > 0x7fffffffLL)
     fail("linear_int4: too many rows or columns");
   L4Args g;
   g.a = a;
   g.steps = (a.K + 127) / 128;
   const bool xvec = int4_rows_aligned(a);
+  if (!xvec && a.M > 1) fail("linear_int4: rows are not aligned");
   const int mt = a.M <= 16 ? 1 : a.M <= 32 ? 2 : 4;
   const int64_t tiles = (a.N + 15) / 16;
   const bool wide = mt > 1 || tiles >= 320;
-  const int64_t blocks = (tiles + wide) / (1 + wide), most = mt == 1 ? 16 : 8;
+  const int64_t rows = (a.M + 16 * mt - 1) / (16 * mt);
+  if (rows > 65535) fail("linear_int4: too many rows");
+  const int64_t blocks = (tiles + wide) / (1 + wide) * rows, most = mt == 1 ? 16 : 8;
   int64_t nw = 4096 / blocks;
   nw = nw < 2 ? 2 : nw > most ? most : nw;
   g.nw = (int)(g.steps < nw ? g.steps : nw);

@@ -5,7 +5,7 @@ as code + 16 in the matrix units and 24 of them is subtracted again, so that a
 group of at most 128 terms loses at most 16 roundings of sums of 24 |x| s; the
 groups, waves and the bias are added in float32, at most K / 32 + 32 of them:
 2^-24 (16 * 24 + K / 32 + 32) sum |x| s.  float32 activations are split into
-three 8-bit parts (2^-24 relative).  16-bit weights of prompts (more than 64
+three 8-bit parts (2^-24 relative).  16-bit weights of prompts (more than 256
 rows) are rounded to the type once: half a step of sum |x| |w|.  gelu has a
 slope of at most 1.13.  The output is rounded once."""
 import numpy as np
@@ -90,7 +90,7 @@ def _check(gpu, rng, dtype, M, N, K, group, act=None, bias=True, lead=None):
     step = np.repeat(scales.T.astype(np.float64), group, 1)[:, :K]
     ax = np.abs(x).astype(np.float64)
     bar = 2.0 ** -24 * (16 * 24 + K / 32 + 32) * (ax @ step.T) + 2.0 ** -22 * (np.abs(b) if bias else 0)
-    if dtype != "float32" and M > 64:
+    if dtype != "float32" and M > 256:
         bar += HALF_STEP[dtype] * (ax @ np.abs(wv).T)
     bar = 1.13 * bar + (HALF_STEP[dtype] + 2.0 ** -20) * np.abs(want) + (2.0 ** -25 if dtype == "float16" else 0)
     assert np.isfinite(got).all()
@@ -99,7 +99,7 @@ def _check(gpu, rng, dtype, M, N, K, group, act=None, bias=True, lead=None):
 
 
 @pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
-@pytest.mark.parametrize("M", [1, 2, 15, 16, 17, 33, 64, 65, 130])
+@pytest.mark.parametrize("M", [1, 2, 15, 16, 17, 33, 64, 65, 130, 256, 257, 400])
 @pytest.mark.parametrize("N,K,group", [(48, 256, 128), (33, 321, 32), (17, 64, 64)])
 def test_rows_and_odd_sizes(gpu, dtype, M, N, K, group):
     _check(gpu, np.random.default_rng(M * N), dtype, M, N, K, group)
@@ -115,7 +115,7 @@ def test_sizes(gpu, dtype, M, N, K):
 
 @pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
 @pytest.mark.parametrize("act", [None, "relu", "gelu", "gelu_exact"])
-@pytest.mark.parametrize("M", [1, 20, 100])
+@pytest.mark.parametrize("M", [1, 20, 100, 300])
 def test_epilogues(gpu, dtype, act, M):
     _check(gpu, np.random.default_rng(7), dtype, M, 70, 300, 64, act, bias=act != "relu")
 
@@ -139,7 +139,7 @@ def test_leading_dims_and_views(gpu):
 
 
 @pytest.mark.parametrize("dtype", ["float16", "bfloat16", "float32"])
-@pytest.mark.parametrize("M", [1, 16, 80])
+@pytest.mark.parametrize("M", [1, 16, 80, 280])
 def test_magnitudes_and_infinities_in_rows(gpu, dtype, M):
     """Rows of unlike size; an infinity or NaN in one row stays in that row."""
     rng = np.random.default_rng(M)
@@ -162,7 +162,7 @@ def test_magnitudes_and_infinities_in_rows(gpu, dtype, M):
     ax = np.abs(np.where(np.isfinite(x), x, 0)).astype(np.float64)
     step = np.repeat(scales.T.astype(np.float64), group, 1)[:, :K]
     bar = 2.0 ** -24 * (16 * 24 + K / 32 + 32) * (ax @ step.T) + (HALF_STEP[dtype] + 2.0 ** -20) * np.abs(want)
-    bar = bar + (HALF_STEP[dtype] * (ax @ np.abs(wv).T) if M > 64 else 0) + (2.0 ** -25 if dtype == "float16" else 0)
+    bar = bar + (HALF_STEP[dtype] * (ax @ np.abs(wv).T) if M > 256 else 0) + (2.0 ** -25 if dtype == "float16" else 0)
     assert (np.abs(y - want) <= bar)[good].all()
 
 
@@ -172,7 +172,7 @@ def test_captured_and_replayed(gpu):
     packed, s = gpu.quantize_int4(_dev(gpu, w, "float16"), 64)
     gpu.eval_many([packed, s])
     graphs = []
-    for M in (4, 100):
+    for M in (4, 100, 300):
         x = gpu.zeros([M, 256], "float16")
         graphs.append((x, gpu.capture(lambda x=x: gpu.linear_int4(x, packed, s, group=64))))
     for _ in range(4):
@@ -224,7 +224,7 @@ def _norm(x, g, b):
 
 @pytest.mark.parametrize("dtype", ["float16", "bfloat16", "float32"])
 @pytest.mark.parametrize("M,N,K", [(1, 48, 128), (8, 5200, 1280), (16, 33, 896), (7, 40, 2048), (3, 17, 40), (2, 20, 33),
-                                   (16, 20, 1000), (17, 48, 128), (90, 48, 128)])
+                                   (16, 20, 1000), (17, 48, 128), (90, 48, 128), (300, 48, 130)])
 @pytest.mark.parametrize("group", [32, 128])
 def test_layer_norm_and_residual_around(gpu, dtype, M, N, K, group):
     """r + act(layer_norm(x) W^T + b): the norm's output is rounded once more
@@ -248,7 +248,7 @@ def test_layer_norm_and_residual_around(gpu, dtype, M, N, K, group):
     half = HALF_STEP[dtype]
     step = np.repeat(scales.T.astype(np.float64), group, 1)[:, :K]
     bar = 2.0 ** -24 * (16 * 24 + K / 32 + 32) * (np.abs(n) @ step.T) + (half + 2.0 ** -20) * (np.abs(n) @ np.abs(wv).T)
-    bar = bar + (half * (np.abs(n) @ np.abs(wv).T) if M > 64 else 0)
+    bar = bar + (half * (np.abs(n) @ np.abs(wv).T) if M > 256 else 0)
     bar = 1.13 * bar + (half + 2.0 ** -20) * (np.abs(lin) + np.abs(want)) + 2.0 ** -20
     assert (np.abs(got - want) <= bar).all(), (np.abs(got - want) / bar).max()
 
