@@ -163,7 +163,14 @@ def test_magnitudes_and_infinities_in_rows(gpu, dtype, M):
     step = np.repeat(scales.T.astype(np.float64), group, 1)[:, :K]
     bar = 2.0 ** -24 * (16 * 24 + K / 32 + 32) * (ax @ step.T) + (HALF_STEP[dtype] + 2.0 ** -20) * np.abs(want)
     bar = bar + (HALF_STEP[dtype] * (ax @ np.abs(wv).T) if M > 256 else 0) + (2.0 ** -25 if dtype == "float16" else 0)
-    assert (np.abs(y - want) <= bar)[good].all()
+    # The largest rows pass float16's range: 65520 is halfway to the step after the largest value, so an exact
+    # value further from it than the bar above has to be an infinity of its sign, or has to be finite.
+    top = 65520.0 if dtype == "float16" else np.inf
+    inf = np.isinf(y)
+    assert (np.sign(y) == np.sign(want))[good & inf.any(1)][inf[good & inf.any(1)]].all()
+    assert (np.abs(want) + bar >= top)[inf & good[:, None]].all()
+    assert inf[(np.abs(want) - bar > top) & good[:, None]].all()
+    assert (np.abs(y - want) <= bar)[good[:, None] & ~inf].all()
 
 
 def test_captured_and_replayed(gpu):
