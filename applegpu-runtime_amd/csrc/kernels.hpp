@@ -566,6 +566,13 @@ struct LinearInt4 {
 void pad_rows(DType dt, const void* x, int64_t sm, int64_t M, int64_t K, void* out, int64_t ld, hipStream_t s);
 bool linear_int4_ln_ok(const LinearInt4& a);
 void linear_int4(const LinearInt4& a, hipStream_t s);
+// The same for many 16-bit rows, with the weights rounded to dt (no ln_gamma,
+// K a multiple of 8).
+void linear_int4_rows(const LinearInt4& a, int cus, hipStream_t s);
+// What a product of these sizes takes: linear_int4, linear_int4_rows, or a GEMM
+// over dequantize_int4's values.
+enum class Int4Way { Few, Rows, Values };
+Int4Way linear_int4_way(const LinearInt4& a, int cus);
 
 // ── log probabilities of given tokens ─────────────────────────────────────
 // For each row of logits [R, V] (row stride ld): lp[r] = log p(token r) (0

@@ -2157,10 +2157,12 @@ TensorP linear_int4(const TensorP& x_in, const TensorP& packed, const TensorP& s
   }
   std::vector<int64_t> od = x->dims();
   od.back() = N;
-  // Past these rows the product is what counts.  MI355X, f16, 1280 x 3840:
-  // 256 rows 19 us against 29, 384 rows 32 against 27; bf16, 8192 x 8192: 192
-  // rows 110 against 114, 256 rows 131 against 112.
-  if (M > (N * K <= (int64_t)1 << 24 ? 256 : 192) && !meta_mode()) {
+  k::LinearInt4 a;
+  a.dt = x->dtype;
+  a.M = M; a.N = N; a.K = K; a.group = group;
+  const k::Int4Way way = meta_mode() ? k::Int4Way::Few : k::linear_int4_way(a, rt().info().cu_count);
+  if (way != k::Int4Way::Few && more && more->ln_gamma) x = layer_norm(x, more->ln_gamma, more->ln_beta, more->ln_eps);
+  if (way == k::Int4Way::Values) {
     // The weights become values of x's dtype once (rounded to it) and the GEMM
     // multiplies them, over rows of whole 64-column steps.
     const int64_t ld = (K + 63) / 64 * 64;
@@ -2170,7 +2172,6 @@ TensorP linear_int4(const TensorP& x_in, const TensorP& packed, const TensorP& s
     e.bias = bc;
     e.act = act;
     if (more && more->residual) e.residual = reshape(contiguous(more->residual), {M, N});
-    if (more && more->ln_gamma) x = layer_norm(x, more->ln_gamma, more->ln_beta, more->ln_eps);
     TensorP rows = reshape(contiguous(x), {M, K});
     if (ld != K) {
       TensorP wide = rt().alloc(x->dtype, {M, ld});
@@ -2181,9 +2182,6 @@ TensorP linear_int4(const TensorP& x_in, const TensorP& packed, const TensorP& s
   }
   TensorP xc = contiguous(x);
   TensorP out = alloc_out(x->dtype, od);
-  k::LinearInt4 a;
-  a.dt = x->dtype;
-  a.M = M; a.N = N; a.K = K; a.group = group;
   const int64_t k8 = (K + 7) / 8 * 8;
   if (M > 1 && !meta_mode() && (k8 != K || ((uintptr_t)xc->data() & 15))) {
     // Several rows are made rows of whole, aligned vectors (the columns behind
@@ -2206,7 +2204,7 @@ TensorP linear_int4(const TensorP& x_in, const TensorP& packed, const TensorP& s
     keep[0] = contiguous(more->residual);
     a.residual = keep[0]->data();
   }
-  if (more && more->ln_gamma) {
+  if (way == k::Int4Way::Few && more && more->ln_gamma) {
     keep[1] = contiguous(more->ln_gamma);
     keep[2] = contiguous(more->ln_beta);
     a.ln_gamma = keep[1]->data();
@@ -2217,6 +2215,10 @@ TensorP linear_int4(const TensorP& x_in, const TensorP& packed, const TensorP& s
       a.x = xc->data();
       a.ln_gamma = a.ln_beta = nullptr;
     }
+  }
+  if (way == k::Int4Way::Rows) {
+    k::linear_int4_rows(a, rt().info().cu_count, rt().stream());
+    return out;
   }
   LAUNCH k::linear_int4(a, rt().stream());
   return out;

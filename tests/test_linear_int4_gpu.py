@@ -5,8 +5,9 @@ as code + 16 in the matrix units and 24 of them is subtracted again, so that a
 group of at most 128 terms loses at most 16 roundings of sums of 24 |x| s; the
 groups, waves and the bias are added in float32, at most K / 32 + 32 of them:
 2^-24 (16 * 24 + K / 32 + 32) sum |x| s.  float32 activations are split into
-three 8-bit parts (2^-24 relative).  16-bit weights of prompts (more than 256
-rows) are rounded to the type once: half a step of sum |x| |w|.  gelu has a
+three 8-bit parts (2^-24 relative).  16-bit weights of many rows (more than 256
+in the narrow matrices here, fewer in wide ones) may be rounded to the type
+once: half a step of sum |x| |w|.  gelu has a
 slope of at most 1.13.  The output is rounded once."""
 import numpy as np
 import pytest
@@ -191,6 +192,102 @@ def test_captured_and_replayed(gpu):
                                           gpu.linear_int4(gpu.from_numpy(a), packed, s, group=64).to_numpy())
     for _, g in graphs:
         g.destroy()
+
+
+# ── many 16-bit rows ────────────────────────────────────────────────────────
+# Sizes that take row tiles of 64, 96, 128 and 160 (256 compute units), last
+# columns and rows that fill no tile, K that fills no stage of 64, and rows that
+# are padded to whole vectors first.
+MANY = [(520, 999, 200, 32), (1100, 2001, 72, 64), (1540, 2001, 136, 128), (1900, 2200, 64, 32), (257, 8200, 131, 64),
+        (40, 21000, 64, 128)]
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("M,N,K,group", MANY)
+def test_many_rows(gpu, dtype, M, N, K, group):
+    """The weights are rounded to the type (half a step of sum |x| |w|, or 2^-25
+    of sum |x| where float16 values are subnormal), the exact products added in float32, at most K + 2 of them, the bias and the
+    residual among them, and the output is rounded once."""
+    rng = np.random.default_rng(M + N)
+    w = _weights(rng, N, K, dtype)
+    codes, scales = O.quantize_int4(w, group, dtype)
+    x = O.round_to(rng.standard_normal((M, K)).astype(np.float32), dtype)
+    b = O.round_to(rng.standard_normal(N).astype(np.float32), dtype)
+    r = O.round_to(rng.standard_normal((M, N)).astype(np.float32), dtype)
+    wv = O.values_int4(codes, scales, group)
+    want = O.linear(x, wv, b)
+    size = np.abs(x).astype(np.float64) @ np.abs(wv).T
+    tiny = 2.0 ** -25 * np.abs(x).astype(np.float64).sum(1, keepdims=True) if dtype == "float16" else 0
+    bar = (HALF_STEP[dtype] + 2.0 ** -24 * (K + 2)) * 1.01 * size + tiny + 2.0 ** -24 * (K + 2) * (np.abs(b) + np.abs(r))
+    bar = bar + HALF_STEP[dtype] * 1.01 * (np.abs(want) + bar) + (2.0 ** -24 if dtype == "float16" else 0)
+    packed, s, xt, bt = gpu.from_numpy(_pack(codes)), _dev(gpu, scales, dtype), _dev(gpu, x, dtype), _dev(gpu, b, dtype)
+    got = gpu.linear_int4(xt, packed, s, bt, group=group).to_numpy().astype(np.float64)
+    assert (np.abs(got - want) <= bar).all(), (np.abs(got - want) - bar).max()
+    for act in ("relu", "gelu"):
+        got = gpu.linear_int4(xt, packed, s, bt, act, group=group).to_numpy().astype(np.float64)
+        assert (np.abs(got - O.linear(x, wv, b, act)) <= 1.13 * bar + 2.0 ** -20).all()
+    y = gpu.linear_int4(xt, packed, s, bt, group=group) + _dev(gpu, r, dtype)
+    both = want + r
+    # (the sum may be rounded before the residual is added)
+    bar = bar + HALF_STEP[dtype] * 1.01 * (np.abs(both) + np.abs(want) + bar)
+    assert (np.abs(y.to_numpy().astype(np.float64) - both) <= bar).all()
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("M,N,K,group", MANY)
+def test_many_rows_pick_single_weights(gpu, dtype, M, N, K, group):
+    """Rows with a single 1 give the dequantised weights themselves, to the bit:
+    every code meets its own column and scale."""
+    rng = np.random.default_rng(M)
+    w = _weights(rng, N, K, dtype)
+    packed, s = gpu.quantize_int4(_dev(gpu, w, dtype), group)
+    back = gpu.dequantize_int4(packed, s, K, group).to_numpy().astype(np.float32)
+    at = np.arange(M) % K
+    x = np.zeros((M, K), np.float32)
+    x[np.arange(M), at] = 1
+    got = gpu.linear_int4(_dev(gpu, x, dtype), packed, s, group=group).to_numpy().astype(np.float32)
+    np.testing.assert_array_equal(got, back[:, at].T)
+
+
+def test_many_rows_keep_infinities_to_themselves(gpu):
+    rng = np.random.default_rng(9)
+    M, N, K = 1100, 2001, 200
+    packed, s = gpu.quantize_int4(_dev(gpu, _weights(rng, N, K, "float16"), "float16"), 64)
+    x = rng.standard_normal((M, K)).astype(np.float16)
+    good = gpu.linear_int4(gpu.from_numpy(x), packed, s, group=64).to_numpy()
+    rows = [0, 95, 96, 640, M - 1]
+    x[rows, [0, 199, 63, 64, 130]] = [np.inf, np.nan, -np.inf, np.nan, np.inf]
+    got = gpu.linear_int4(gpu.from_numpy(x), packed, s, group=64).to_numpy()
+    keep = np.ones(M, bool)
+    keep[rows] = False
+    np.testing.assert_array_equal(got[keep], good[keep])
+    assert not np.isfinite(got[rows][:, np.arange(N) != N // 2]).all(1).any()
+
+
+def test_many_rows_of_views_captured_and_replayed(gpu):
+    """Scales and rows that begin inside other tensors, also at odd halves of a
+    word; replays with eager work between them."""
+    rng = np.random.default_rng(4)
+    M, N, K, group = 600, 2001, 160, 32
+    w = _weights(rng, N, K, "float16")
+    packed, s = gpu.quantize_int4(_dev(gpu, w, "float16"), group)
+    want_of = lambda a: gpu.linear_int4(gpu.from_numpy(a), packed, s, group=group).to_numpy()
+    flat = gpu.from_numpy(np.concatenate([np.full(1, 7, np.float16), s.to_numpy().ravel()]))
+    inside = gpu.reshape(gpu.slice(flat, 0, 1, 1 + s.shape[0] * N), [s.shape[0], N])
+    x = gpu.zeros([M + 1, K], "float16")
+    y = gpu.zeros([M, K + 8], "float16")
+    for t in (x, y, inside):
+        t.eval()
+    graph = gpu.capture(lambda: (gpu.linear_int4(gpu.slice(x, 0, 1, M + 1), packed, inside, group=group),
+                                 gpu.linear_int4(gpu.slice(y, 1, 0, K), packed, s, group=group)))
+    for _ in range(4):
+        a, b = rng.standard_normal((M + 1, K)).astype(np.float16), rng.standard_normal((M, K + 8)).astype(np.float16)
+        x.write(a)
+        y.write(b)
+        graph.replay()
+        for got, rows in zip(graph.outputs, (a[1:], b[:, :K])):
+            np.testing.assert_array_equal(got.to_numpy(), want_of(np.ascontiguousarray(rows)))
+    graph.destroy()
 
 
 def test_empty_rows(gpu):
