@@ -516,7 +516,10 @@ D8Args plan(const DecodeInt8& a) {
   // or split over blocks of 4 waves and merged by a second launch, which costs
   // about as much as three steps of a wave, where that saves more steps than
   // that: 12 heads, 2048 rows of 64: 12.1 us whole, 8.3 split; 160 heads: 14.3
-  // whole, 19.4 split.
+  // whole, 19.4 split.  (Merged by a unit's last block in the same launch: 20
+  // heads, 8192 rows of 64 14.5 us against 13.4; 32 heads of 4 queries, 32768
+  // rows of 128 60 against 55: the blocks' wait for their stores and the count
+  // cost more than the launch.)
   const int64_t units = a.B * a.H * g.q_tiles;
   g.nw = units <= 256 && a.D != 128 ? 16 : units <= 512 ? 8 : 4;
   while (g.nw > kFew && (lds_bytes(a, g.nw) > (60 << 10) || a.Tmax <= g.nw / 2 * kStep)) g.nw /= 2;

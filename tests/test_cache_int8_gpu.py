@@ -118,6 +118,28 @@ def test_infinities_zeros_and_tiny_values(gpu):
 
 
 # ── attention ───────────────────────────────────────────────────────────────
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+def test_append_halves_and_every_size_bit_exact(gpu, dtype):
+    """Values that lie at or next to the middle of two codes, of every size
+    down to the smallest, and scales that are subnormal themselves."""
+    rng = np.random.default_rng(8)
+    B, H, T, D, block = 1, 64, 32, 64, 16
+    lo, hi = {"float32": (-149, 127), "float16": (-24, 15), "bfloat16": (-133, 127)}[dtype]
+    size = np.ldexp(1.0, np.linspace(lo, hi, H).round().astype(int))[None, :, None, None]
+    x = (rng.integers(-126, 127, (B, H, T, D)) + 0.5) / 127.0
+    x = x * (1 + rng.choice([0, 1, -1], x.shape) * 2.0 ** -23)
+    x[:, :, ::block, 0] = 1.0
+    x = O.round_to((x * size).astype(np.float32), dtype)
+    codes, scales = np.zeros((B, H, T, D), np.int8), np.zeros((B, H, T // block), np.float32)
+    dev = _upload(gpu, codes, scales, codes.copy(), scales.copy())
+    r = _dev(gpu, x, dtype)
+    np.testing.assert_array_equal(r.to_numpy().astype(np.float32), x)
+    gpu.kv_write_int8(*dev, r, r, gpu.from_numpy(np.zeros(1, np.int32)), block=block)
+    O.append_int8(codes, scales, x, [0], block)
+    for t, want in zip(dev, (codes, scales, codes, scales)):
+        np.testing.assert_array_equal(t.to_numpy(), want)
+
+
 def _bar(q, k, v, scale, dtype, n):
     vmax = np.abs(v).max()
     d = (q.shape[-1] + 16) * 2.0 ** -24 * scale * np.abs(q).max() * np.abs(k).sum(-1).max()
