@@ -252,6 +252,25 @@ int32_t applegpu_kv_write_pair(uint64_t k_cache_id, uint64_t v_cache_id, uint64_
 int32_t applegpu_kv_write_int8(uint64_t k_codes_id, uint64_t k_scales_id, uint64_t v_codes_id, uint64_t v_scales_id,
                                uint64_t k_rows_id, uint64_t v_rows_id, uint64_t pos_id, int64_t block);
 
+/* Lazy ops (applegpu_graph_op) for weights in 4 bits and for log
+ * probabilities; inputs, then int parameters.
+ *   "quantize_int4" (w [N, K]; group 32, 64 or 128): packed codes uint8
+ *     [ceil(N / 16), ceil(K / 128), 64, 16] and scales [ceil(K / group), N] of
+ *     w's dtype, scale = the group's largest magnitude / 7, codes within
+ *     -7 .. 7.  Byte run l of a tile of 16 rows by 128 columns holds row l %
+ *     16's codes from column 32 (l / 16) on, eight to each 4 bytes, as code +
+ *     8, nibble j (lowest first) code 2 j for j < 4 and 2 (j - 4) + 1 for the
+ *     others.
+ *   "dequantize_int4" (packed, scales; K, group): the values [N, K].
+ *   "linear_int4" (x [..., K], packed, scales[, bias [N]]; group, activation
+ *     0 none, 1 relu, 2 gelu with tanh, 3 gelu with erf): [..., N].
+ *   "token_logprobs" (logits [..., V], tokens [...] int32 or int64; top_k 0 ..
+ *     32): log probability of each token, entropy and log sum of exponentials,
+ *     float32 [...], and with top_k > 0 the top_k largest log probabilities and
+ *     their int32 indices, [..., top_k].
+ *   "token_logprobs_backward" (grad_logprobs, logits, tokens, entropy, lse[,
+ *     grad_entropy]): the gradient of the logits in their dtype. */
+
 int32_t applegpu_capture_begin(void);
 int64_t applegpu_capture_end(void);
 int32_t applegpu_capture_abort(void);
