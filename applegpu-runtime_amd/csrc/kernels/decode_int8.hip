@@ -32,6 +32,11 @@
 //    and within f16's normal range for 2^-21 of the maximum.
 // Work: waves of a block take 32-key steps in turn; a context is split over
 // blocks while these leave CUs idle, and the splits' (O, m, l) are merged.
+// Bound by the read of the codes where contexts are long: 4 x 8 heads of 4
+// queries over up to 32768 rows of 128, 218 MB in 45.7 us (4.8 TB/s) and 5 for
+// the merge; 16 x 20 heads over 8192 rows of 64 73 us, against 131 for a 16-bit
+// cache.  Short contexts are bound by one chain of loads, products and
+// exponentials: 12 heads over 100 rows 5 us.
 #include "kv_int8.hpp"
 
 namespace agpu {

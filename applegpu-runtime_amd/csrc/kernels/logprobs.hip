@@ -12,7 +12,11 @@
 // Both directions are bound by the read (and write) of the logits: one pass,
 // each thread with a running maximum that moves its sums, 16 elements a step
 // as 16-byte loads whose next ones are in flight.  Few rows are split over
-// blocks, whose states a second launch merges.
+// blocks, whose states a second launch merges.  Measured: 2047 x 50257 fp32
+// with 20 alternatives 85 us (4.84 TB/s), in bf16 67 us (bound by its
+// instructions, an exponential and some eight others a value); 8 rows in f16
+// 8 us and 6 for the merge; the gradient in bf16 88 us (4.6 TB/s, read and
+// written).
 #include "device.hpp"
 
 namespace agpu {
