@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(256) dequantize_int4_kernel(const uint4* __res
 }
 
 __device__ __forceinline__ float act_of(float v, int act) {
-  if (act == kActRelu) return v > 0.f ? v : (v != v ? v : 0.f);
+  if (act == kActRelu) return fmaxf(v, 0.f);  // (0 for NaN, as relu gives elsewhere)
   if (act == kActGelu) return gelu_tanh(v);
   if (act == kActGeluExact) return 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
   return v;

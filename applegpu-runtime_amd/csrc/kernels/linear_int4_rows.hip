@@ -8,7 +8,9 @@
 //    bytes a copy instruction).
 //  - The codes go the same way, a wavefront's own 1 KB a stage: 16 bytes, one
 //    row's 32 codes of one scale, to the lane that multiplies them.  They
-//    become values of x's type in registers, code * scale rounded once as
+//    become values of x's type in registers, code * scale rounded once (half a
+//    step of the type, what weights held in it would have lost, and far below
+//    the codes' own rounding; unrounded they would take two products each) as
 //    dequantize_int4 rounds it, while the MFMAs before run: no value of W
 //    passes LDS or memory, and each is made once a block.
 //  - A ring of S stages: a wavefront waits for its copies of the next stage
@@ -92,7 +94,7 @@ struct L4RArgs {
 
 template <int ACT>
 __device__ __forceinline__ float act_of(float v) {
-  if constexpr (ACT == kActRelu) return v > 0.f ? v : (v != v ? v : 0.f);
+  if constexpr (ACT == kActRelu) return fmaxf(v, 0.f);  // (0 for NaN, as relu gives elsewhere)
   else if constexpr (ACT == kActGelu) return gelu_tanh(v);
   else if constexpr (ACT == kActGeluExact) return 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
   else return v;
@@ -344,6 +346,13 @@ int pick_tm(int64_t M, int64_t N, int cus, int64_t* cost) {
 
 }  // namespace
 
+// The rows of a block lie within the 2 GiB that a buffer resource spans, and so
+// do its codes and all scales (K after the rows are padded to whole vectors).
+static bool rows_fit(const LinearInt4& a) {
+  const int64_t K = (a.K + 7) / 8 * 8;
+  return K < (1 << 21) && (K + a.group - 1) / a.group * a.N < (1 << 30) && row_tiles(a.M, a.N, 2) < (1LL << 31);
+}
+
 // Which kernels a product of these sizes takes, by what they measured (us):
 // few rows straight from the codes (few), these tiles (rows), or the weights
 // made values in memory for the framework's GEMM (values).
@@ -375,17 +384,14 @@ Int4Way linear_int4_way(const LinearInt4& a, int cus) {
   // (a GEMM splits a long K over the chip where there are few tiles, and has
   // larger tiles where there are many rows)
   const bool few_tiles = row_tiles(a.M, a.N, 2) < cus / 2 && a.K > 4096;
-  if (few_tiles || a.M > (a.dt == DType::F16 ? 4096 : 2048) || a.K >= (1 << 21)) return Int4Way::Values;
+  if (few_tiles || a.M > (a.dt == DType::F16 ? 4096 : 2048) || !rows_fit(a)) return Int4Way::Values;
   return Int4Way::Rows;
 }
 
 void linear_int4_rows(const LinearInt4& a, int cus, hipStream_t s) {
   if (a.M == 0) return;
-  // the rows of a block lie within the 2 GiB that a buffer resource spans, and
-  // so do its codes and all scales
-  const int64_t groups = (a.K + a.group - 1) / a.group;
   if (a.dt == DType::F32 || a.ln_gamma || a.K % 8 || a.x_sm % 8 || ((uintptr_t)a.x & 15) || a.x_sm < a.K ||
-      a.x_sm >= (1 << 21) || groups * a.N >= (1 << 30) || row_tiles(a.M, a.N, 2) >= (1LL << 31))
+      a.x_sm >= (1 << 21) || !rows_fit(a))
     fail("linear_int4: these rows do not fit the tiles");
   L4RArgs g{};
   g.p.A = a.x; g.p.a_sm = a.x_sm;
@@ -397,7 +403,7 @@ void linear_int4_rows(const LinearInt4& a, int cus, hipStream_t s) {
   g.packed = a.packed;
   g.scales = a.scales;
   g.steps = (int)((a.K + 127) / 128);
-  g.groups = (int)groups;
+  g.groups = (int)((a.K + a.group - 1) / a.group);
   g.group_log2 = a.group == 32 ? 5 : a.group == 64 ? 6 : 7;
   int64_t cost = 0;
   const int tm = pick_tm(a.M, a.N, cus, &cost);

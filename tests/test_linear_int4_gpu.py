@@ -121,6 +121,21 @@ def test_epilogues(gpu, dtype, act, M):
     _check(gpu, np.random.default_rng(7), dtype, M, 70, 300, 64, act, bias=act != "relu")
 
 
+@pytest.mark.parametrize("dtype,M,N,K", [("float16", 1, 70, 300), ("bfloat16", 40, 70, 300), ("float16", 600, 999, 64),
+                                         ("float32", 3, 70, 300), ("float32", 300, 70, 300), ("bfloat16", 2100, 999, 64)])
+def test_relu_of_nan_and_infinities_is_the_frameworks(gpu, dtype, M, N, K):
+    """The same, whatever kernels the number of rows takes: relu(NaN) = 0."""
+    rng = np.random.default_rng(2)
+    packed, s = gpu.quantize_int4(_dev(gpu, _weights(rng, N, K, dtype), dtype), 64)
+    x = rng.standard_normal((M, K)).astype(np.float32)
+    x[0, 5], x[M - 1, 0] = np.nan, np.inf
+    x = _dev(gpu, x, dtype)
+    y = gpu.linear_int4(x, packed, s, None, "relu", group=64).to_numpy().astype(np.float32)
+    want = gpu.relu(gpu.linear_int4(x, packed, s, group=64)).to_numpy().astype(np.float32)
+    np.testing.assert_array_equal(y, want)
+    assert (y[0] == 0).all() and not np.isnan(y).any()
+
+
 def test_leading_dims_and_views(gpu):
     rng = np.random.default_rng(11)
     _check(gpu, rng, "float16", 6, 40, 96, 32, lead=[2, 3])
@@ -197,9 +212,10 @@ def test_captured_and_replayed(gpu):
 # ── many 16-bit rows ────────────────────────────────────────────────────────
 # Sizes that take row tiles of 64, 96, 128 and 160 (256 compute units), last
 # columns and rows that fill no tile, K that fills no stage of 64, and rows that
-# are padded to whole vectors first.
+# are padded to whole vectors first; then sizes for which the weights become
+# values in memory (a long K with few tiles, and very many rows).
 MANY = [(520, 999, 200, 32), (1100, 2001, 72, 64), (1540, 2001, 136, 128), (1900, 2200, 64, 32), (257, 8200, 131, 64),
-        (40, 21000, 64, 128)]
+        (40, 21000, 64, 128), (700, 1024, 4130, 128), (4200, 200, 72, 32)]
 
 
 @pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
@@ -288,6 +304,30 @@ def test_many_rows_of_views_captured_and_replayed(gpu):
         for got, rows in zip(graph.outputs, (a[1:], b[:, :K])):
             np.testing.assert_array_equal(got.to_numpy(), want_of(np.ascontiguousarray(rows)))
     graph.destroy()
+
+
+@pytest.mark.parametrize("dtype,M,N,K", [("float32", 300, 96, 250), ("float16", 4200, 200, 72), ("bfloat16", 600, 999, 67)])
+def test_two_graphs_with_workspaces_replayed_in_turn(gpu, dtype, M, N, K):
+    rng = np.random.default_rng(5)
+    made = []
+    for seed in (0, 1):
+        packed, s = gpu.quantize_int4(_dev(gpu, _weights(rng, N, K, dtype), dtype), 32)
+        x = gpu.zeros([M, K], dtype)
+        for t in (packed, s, x):
+            t.eval()
+        made.append((x, packed, s, gpu.capture(lambda x=x, p=packed, s=s: gpu.linear_int4(x, p, s, None, "gelu", group=32))))
+    for _ in range(3):
+        new = []
+        for x, _, _, _ in made:
+            new.append(_dev(gpu, rng.standard_normal((M, K)), dtype))
+            gpu.blit_copy(new[-1], x)
+        for x, _, _, g in made:
+            g.replay()
+        for (x, packed, s, g), a in zip(made, new):
+            want = gpu.linear_int4(a, packed, s, None, "gelu", group=32).to_numpy()
+            np.testing.assert_array_equal(g.outputs.to_numpy(), want)
+    for *_, g in made:
+        g.destroy()
 
 
 def test_empty_rows(gpu):
