@@ -254,11 +254,20 @@ __global__ void __launch_bounds__(256) linear_int4_rows(L4RArgs g) {
   struct V { T e[8]; };
   const int64_t col = n0 + w * 32 + (lane % 4) * 8;
   const bool full = col + 8 <= p.N;
+  // (without the empty asm the compiler gives both branches one access of 2
+  // bytes and splits the 16 for it)
+  auto load8 = [&](V& v, const T* from) __attribute__((always_inline)) {
+    if (full) {
+      __builtin_memcpy(&v, from, 16);
+      asm volatile("" ::: "memory");
+    } else {
+      for (int e = 0; e < 8; ++e) v.e[e] = col + e < p.N ? from[e] : (T)0.f;
+    }
+  };
   float bs[8] = {};
   if (bias) {
     V b;
-    if (full) __builtin_memcpy(&b, bias + col, 16);
-    else for (int e = 0; e < 8; ++e) b.e[e] = col + e < p.N ? bias[col + e] : (T)0.f;
+    load8(b, bias + col);
 #pragma unroll
     for (int e = 0; e < 8; ++e) bs[e] = to_f(b.e[e]);
   }
@@ -283,8 +292,7 @@ __global__ void __launch_bounds__(256) linear_int4_rows(L4RArgs g) {
       const T* res = R + row * p.r_sm + col;
       V x, o;
       if (R) {
-        if (full) __builtin_memcpy(&x, res, 16);
-        else for (int e = 0; e < 8; ++e) x.e[e] = col + e < p.N ? res[e] : (T)0.f;
+        load8(x, res);
       } else {
         x = V{};
       }
@@ -292,6 +300,7 @@ __global__ void __launch_bounds__(256) linear_int4_rows(L4RArgs g) {
       for (int e = 0; e < 8; ++e) o.e[e] = from_f<T>(act_of<ACT>(v[e] + bs[e]) + to_f(x.e[e]));
       if (full) {
         __builtin_memcpy(out, &o, 16);
+        asm volatile("" ::: "memory");
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
