@@ -19,15 +19,17 @@
 //    codes that begin at column 32 (l / 32); x is read in the same order of k.
 //  - The epilogue goes through LDS, 16 bytes a lane, in loops that stay rolled
 //    and for one activation: its instructions come from memory once a launch
-//    and compute unit.  (Unrolled, with all activations: 35 us instead of 24 at
-//    1111 x 1280 x 3840.)
+//    and compute unit.  (Unrolled, with all activations: 37 us at 1111 x 1280 x
+//    3840.)
 //
-// f16, 1111 x 1280 x 3840, group 128: 23.6 us (463 TFLOP/s), against 33 for
+// f16, 1111 x 1280 x 3840, group 128: 22.9 us (477 TFLOP/s), against 33 for
 // values written out and multiplied and 21.5 for a library's product of values.
 // One block on a compute unit takes 0.5 (TM = 2) to 0.8 us (TM = 5) a stage, of
 // which its MFMAs are 0.1 to 0.3: four wavefronts that wait for LDS reads and
 // make 2 x 16 values of W a lane (in f16 four instructions a pair, in bf16
-// seven) do not fill it, two or three blocks do.
+// seven) do not fill it, two or three blocks do.  (Eight, half of them for
+// half of each stage's k: 85 us for 95 at 300 x 8192 x 8192, but 25.2 for 24.2
+// here and 74 for 62 at 4096 rows.)
 #include "gemm_kernels.hpp"
 
 namespace agpu {
@@ -337,11 +339,11 @@ int64_t row_tiles(int64_t M, int64_t N, int tm) { return (M + 32 * tm - 1) / (32
 
 // A stage's time on the compute unit with the most blocks grows as blocks x (2
 // TM + 3).  f16, us with TM = 2 / 3 / 4 / 5 (the rule's choice in brackets):
-//   512 x 1280 x 3840    [14.9]  16.9   17.9   20.7
-//   1111 x 1280 x 3840   28.2    24.2   25.4  [23.6]
-//   2000 x 5120 x 1280   57.9   [51.3]  55.1   62.4
-//   300 x 8192 x 8192    112    [95.6]  97.7   104   (bf16)
-//   4096 x 1280 x 3840   70.5    68.0  [63.4]  64.1
+//   512 x 1280 x 3840    [14.6]  16.3   17.4   20.1
+//   1111 x 1280 x 3840   27.0    24.1   25.8  [23.0]
+//   2000 x 5120 x 1280   56.7   [51.6]  53.8   62.3
+//   300 x 8192 x 8192    115    [93.8]  95.5   104   (bf16)
+//   4096 x 1280 x 3840   71.9    65.1  [62.2]  64.8
 int pick_tm(int64_t M, int64_t N, int cus, int64_t* cost) {
   int best = 0;
   for (int tm = 2; tm <= 5; ++tm) {
@@ -367,10 +369,10 @@ static bool rows_fit(const LinearInt4& a) {
 // made values in memory for the framework's GEMM (values).
 //   M x K x N              few    rows   values
 //   128 x 1280 x 3840      10.7   13.1
-//   192 x 1280 x 3840      18.3   13.8
-//   256 x 1280 x 1280      9.6    13.0
-//   320 x 1280 x 3840             14.3   27.5
-//   32 x 768 x 50257       22.2   13.1
+//   192 x 1280 x 3840      18.3   13.4
+//   256 x 1280 x 1280      9.7    13.0
+//   320 x 1280 x 3840             14.0   27.5
+//   32 x 768 x 50257       22.2   13.0
 //   64 x 8192 x 8192       39.3   74.5          (bf16)
 //   256 x 8192 x 8192      112    81.6          (bf16)
 //   640 x 8192 x 1024             58.9   44.8
