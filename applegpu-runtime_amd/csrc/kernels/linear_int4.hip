@@ -107,7 +107,9 @@ __device__ __forceinline__ float act_of(float v, int act) {
 //    and an or, and the 24 too many come off through one more product, of the
 //    rows with a constant -24, which all tiles of columns share.  The products
 //    and their difference are exact up to the fp32 sums, and a group's scale is
-//    multiplied once, on its sum.
+//    multiplied once, on its sum.  Where the difference is not a number (an
+//    infinite x, or one next to fp32's largest) the sum is taken again from the
+//    values, behind a test of 0 to 0.3 us.
 //  - The waves of a block split K and add their sums through LDS.
 // Two tiles of columns a wave (NT = 2) share the rows' loads where they leave
 // enough blocks, and fewer waves a block where there are many (us, one row):
@@ -232,6 +234,29 @@ __device__ __forceinline__ void normalise_rows(const LinearInt4& a, T* xs, int K
       }
     }
   }
+}
+
+// A wave's share (steps w, w + nw, ..) of sum_k x[k] (code scale)[k] of one
+// output, from the column's codes of its tile and its scales (N apart).
+template <typename T, int G>
+__device__ __forceinline__ float sum_of_values(const uint32_t* codes, const T* scales, const T* x, int64_t N,
+                                                         int K, int w, int nw) {
+  float v = 0.f;
+#pragma unroll 1
+  for (int k0 = 128 * w; k0 < K; k0 += 128 * nw) {
+#pragma unroll 1
+    for (int k = k0; k < k0 + 128 && k < K; k += 8) {
+      const uint32_t word = codes[(int64_t)(k / 128) * 256 + (k % 128) / 32 * 64 + (k % 32) / 8];
+      const float s = to_f(scales[k / G * N]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float xe = k + e < K ? to_f(x[k + e]) : 0.f;
+        if (k + e < K) v = fmaf(xe, (float)((int)((word >> (4 * nibble_of(e))) & 15) - 8) * s, v);
+      }
+      if (v != v) return v;
+    }
+  }
+  return v;
 }
 
 // MT tiles of 16 rows of x by NT tiles of 16 columns of the output; the waves
@@ -437,12 +462,31 @@ __global__ void __launch_bounds__(MT == 1 ? 1024 : 512) linear_int4_mfma(L4Args 
 
   // lane (c, q) holds rows 4 q + e, column c of each tile; the waves' sums
   // are added in wave order
+  bool past = false;
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) red[((w * MT + i) * NT + j) * 256 + (4 * q + e) * 16 + c] = tot[i][j][e];
+      for (int e = 0; e < 4; ++e) {
+        red[((w * MT + i) * NT + j) * 256 + (4 * q + e) * 16 + c] = tot[i][j][e];
+        past |= !(fabsf(tot[i][j][e]) < INFINITY);
+      }
+  if (past) {
+    // An infinity, and an x past 2^112, are infinities of both signs in the two
+    // products and NaN in their sum (so is the first part of an fp32 x that
+    // rounds up to 2^128): this lane's sums that are not finite are taken again
+    // from the weights' values, and are then what the products give.
+#pragma unroll 1
+    for (int at = 0; at < MT * NT * 4; ++at) {
+      const int e = at & 3, j = (at >> 2) % NT, i = (at >> 2) / NT;
+      float* sum = red + ((w * MT + i) * NT + j) * 256 + (4 * q + e) * 16 + c;
+      const int64_t m = m0 + 16 * i + 4 * q + e, n = (tile0 + j) * 16 + c;
+      if (fabsf(*sum) < INFINITY || m >= a.M || n >= a.N) continue;
+      const T* xm = LN ? xs + m * (K + 8) : (const T*)a.x + m * a.x_sm;
+      *sum = sum_of_values<T, G>((const uint32_t*)a.packed + (tile0 + j) * steps * 256 + c * 4, sc + n, xm, a.N, K, w, nw);
+    }
+  }
   __syncthreads();
   for (int idx = tid; idx < MT * NT * 256; idx += 64 * g.nw) {
     const int cc = idx & 15, j = (idx >> 4) % NT, mm = idx / (16 * NT);

@@ -420,3 +420,71 @@ def test_what_else_reads_a_norm_or_a_product_keeps_it(gpu):
     a = gpu.linear_int4(gpu.layer_norm(part, g, b), packed, s, group=32).to_numpy()
     c = gpu.linear_int4(gpu.layer_norm(gpu.from_numpy(part.to_numpy()), g, b), packed, s, group=32).to_numpy()
     np.testing.assert_allclose(a, c, rtol=2e-3, atol=2e-3)
+
+
+# ── infinities and values next to the type's largest ────────────────────────
+def _huge_rows(rng, M, K, dtype):
+    """Rows with one or two values that are infinite or next to the largest of
+    the type, ordinary ones between them."""
+    x = rng.standard_normal((M, K)).astype(np.float32)
+    huge = {"float16": [6e4, 65504.0], "bfloat16": [2e37, 3.3e38], "float32": [2e37, np.finfo(np.float32).max]}[dtype]
+    for m in range(0, M, 2 if M > 1 else 1):
+        v = ([np.inf, -np.inf] + huge + [-huge[0], -huge[1]])[(m // 2 + K) % 6]
+        x[m, rng.integers(0, K)] = v
+        if m % 5 == 3:
+            x[m, rng.integers(0, K)] = np.inf
+    return O.round_to(x, dtype)
+
+
+@pytest.mark.parametrize("dtype,M,N,K,group", [
+    (t, *size) for t in ("float16", "bfloat16", "float32")
+    for size in ((1, 70, 33, 32), (1, 70, 64, 64), (1, 70, 300, 128), (2, 70, 300, 64), (16, 5200, 256, 32),
+                 (17, 70, 300, 64), (40, 70, 136, 32), (130, 70, 300, 128))] + [
+    ("float16", 300, 70, 300, 64), ("bfloat16", 300, 70, 300, 64), ("float16", 600, 999, 64, 32),
+    ("bfloat16", 600, 999, 64, 64), ("float16", 4200, 60, 72, 32), ("bfloat16", 2100, 999, 64, 128)])
+def test_infinities_and_largest_values_are_the_products(gpu, dtype, M, N, K, group):
+    """sum x code scale, whatever kernels the number of rows takes: an infinity
+    gives infinities of the weights' signs (NaN where a weight is 0), and a
+    large x what it is worth.  Sums of such rows are added value by value: K
+    roundings, and those of the waves and the bias."""
+    rng = np.random.default_rng(M + N + K)
+    w = O.round_to(rng.standard_normal((N, K)).astype(np.float32) * 0.02, dtype)
+    codes, scales = O.quantize_int4(w, group, dtype)
+    wv = O.values_int4(codes, scales, group)
+    x = _huge_rows(rng, M, K, dtype)
+    packed, s, xt = gpu.from_numpy(_pack(codes)), _dev(gpu, scales, dtype), _dev(gpu, x, dtype)
+    rows = np.r_[0:min(M, 60), max(0, M - 8):M]
+    with np.errstate(invalid="ignore"):
+        want = np.stack([(x[m].astype(np.float64) * wv).sum(1) for m in rows])
+    ax = np.abs(np.where(np.isfinite(x), x, 0)).astype(np.float64)[rows]
+    step = np.repeat(scales.T.astype(np.float64), group, 1)[:, :K]
+    bar = 2.0 ** -24 * (16 * 24 + K + 34) * (ax @ step.T)
+    if dtype != "float32":
+        bar = bar + HALF_STEP[dtype] * 1.01 * (ax @ np.abs(wv).T) + (2.0 ** -25 * ax.sum(1, keepdims=True) if dtype == "float16" else 0)
+    finite = np.isfinite(want)
+    bar = bar + HALF_STEP[dtype] * 1.01 * (np.abs(np.where(finite, want, 0)) + bar) + 2.0 ** -25
+    assert finite.any() or M == 1
+    for act in (None, "relu"):
+        got = gpu.linear_int4(xt, packed, s, None, act, group=group).to_numpy().astype(np.float64)[rows]
+        exact = want if act is None else np.where(want > 0, want, 0)   # (relu(NaN) = 0 here)
+        keep = np.isfinite(exact)
+        np.testing.assert_array_equal(np.isnan(got), np.isnan(exact))
+        np.testing.assert_array_equal(got[np.isinf(exact)], exact[np.isinf(exact)])
+        assert (np.abs(got[keep] - exact[keep]) <= bar[keep]).all()
+
+
+def test_normalised_rows_of_large_gain(gpu):
+    """The same where the rows come out of the layer_norm in the launch."""
+    rng = np.random.default_rng(3)
+    M, N, K, group = 4, 48, 128, 64
+    w = O.round_to(rng.standard_normal((N, K)).astype(np.float32) * 0.02, "bfloat16")
+    codes, scales = O.quantize_int4(w, group, "bfloat16")
+    wv = O.values_int4(codes, scales, group)
+    x = O.round_to(rng.standard_normal((M, K)).astype(np.float32), "bfloat16")
+    g, b = np.full(K, O.round_to(np.float32(4e37), "bfloat16")), np.zeros(K, np.float32)
+    y = gpu.linear_int4(gpu.layer_norm(*(_dev(gpu, a, "bfloat16") for a in (x, g, b))), gpu.from_numpy(_pack(codes)),
+                        _dev(gpu, scales, "bfloat16"), group=group).to_numpy().astype(np.float64)
+    n = _norm(x.astype(np.float64), g.astype(np.float64), b)
+    want = n @ wv.T
+    bar = (2.0 ** -8 + 2.0 ** -18) * (np.abs(n) @ np.abs(wv).T) + 2.0 ** -8 * np.abs(want)
+    assert (np.abs(y - want) <= bar).all()
