@@ -662,8 +662,9 @@ def dequantize_int4(packed, scales, in_features, group=128):
 def linear_int4(x, packed, scales, bias=None, activation=None, group=128):
     """y = act(x @ W^T + bias) with the 4-bit weights of quantize_int4(W,
     group): x [..., in] of the scales' dtype, any number of rows, summed in
-    float32.  Decode steps and prompts take the same call; for many rows the
-    weights are first rounded to x's dtype, as dequantize_int4 returns them."""
+    float32.  Decode steps and prompts take the same call; for many 16-bit rows
+    the weights are first rounded to x's dtype, as dequantize_int4 returns
+    them.  float32 rows keep their 24 bits however many they are."""
     if activation not in _ACTS:
         raise ValueError(f"linear_int4: unknown activation {activation!r}")
     ins = [_t(x), _t(packed), _t(scales)] + ([_t(bias)] if bias is not None else [])

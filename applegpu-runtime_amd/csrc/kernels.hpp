@@ -569,8 +569,8 @@ void linear_int4(const LinearInt4& a, hipStream_t s);
 // The same for many 16-bit rows, with the weights rounded to dt (no ln_gamma,
 // K a multiple of 8).
 void linear_int4_rows(const LinearInt4& a, int cus, hipStream_t s);
-// What a product of these sizes takes: linear_int4, linear_int4_rows, or a GEMM
-// over dequantize_int4's values.
+// What a product of these sizes takes: linear_int4, or for many 16-bit rows
+// linear_int4_rows or a GEMM over dequantize_int4's values.
 enum class Int4Way { Few, Rows, Values };
 Int4Way linear_int4_way(const LinearInt4& a, int cus);
 

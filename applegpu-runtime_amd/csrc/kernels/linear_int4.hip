@@ -587,6 +587,19 @@ void linear_int4(const LinearInt4& a, hipStream_t s) {
   if (a.ln_gamma && !linear_int4_ln_ok(a)) fail("linear_int4: these rows cannot be normalised in the product");
   if (a.K > 0x7fffff00LL || (a.N + 15) / 16 > 0x7fffffffLL)
     fail("linear_int4: too many rows or columns");
+  constexpr int64_t kMost = 65535 * 64;  // rows of a grid
+  if (a.M > kMost) {
+    const int64_t es = (int64_t)dtype_size(a.dt);
+    for (int64_t m = 0; m < a.M; m += kMost) {
+      LinearInt4 part = a;
+      part.M = a.M - m < kMost ? a.M - m : kMost;
+      part.x = (const char*)a.x + m * a.x_sm * es;
+      part.out = (char*)a.out + m * a.N * es;
+      if (a.residual) part.residual = (const char*)a.residual + m * a.N * es;
+      linear_int4(part, s);
+    }
+    return;
+  }
   L4Args g;
   g.a = a;
   g.steps = (a.K + 127) / 128;
@@ -598,7 +611,6 @@ void linear_int4(const LinearInt4& a, hipStream_t s) {
   const int64_t tiles = (a.N + 15) / 16;
   const bool wide = mt > 1 || tiles >= 320;
   const int64_t rows = (a.M + 16 * mt - 1) / (16 * mt);
-  if (rows > 65535) fail("linear_int4: too many rows");
   const int64_t blocks = (tiles + wide) / (1 + wide) * rows, most = mt == 1 ? 16 : 8;
   int64_t nw = 4096 / blocks;
   nw = nw < 2 ? 2 : nw > most ? most : nw;

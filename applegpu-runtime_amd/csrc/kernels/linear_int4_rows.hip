@@ -382,11 +382,13 @@ static bool rows_fit(const LinearInt4& a) {
 //   4000 x 8192 x 8192            605    474    (bf16)
 // The few-row kernel takes 4 us + K / 233 for each round of 256 blocks of 32
 // (16: groups of 32) columns x 64 rows (K / 333 for 32 rows), the tiles 4 us +
-// K (2.4 + cost) / 1430.  fp32 rows (three products a code there, one split in
-// two for values): 256 rows, 192 for matrices past 2^24 weights.
+// K (2.4 + cost) / 1430.  fp32 rows stay there however many they are: three
+// products a code keep the 24 bits of x, where values in memory and the split
+// fp32 GEMM (two bf16 parts an operand, infinities NaN) are 1.0 to 2.2 times as
+// fast (1111 x 1280 x 3840 136 against 91 us, 4096 x 8192 x 8192 4.4 against
+// 2.0 ms) and the native fp32 GEMM is slower (236 us, 4.5 ms).
 Int4Way linear_int4_way(const LinearInt4& a, int cus) {
-  if (a.M <= 16) return Int4Way::Few;
-  if (a.dt == DType::F32) return a.M > (a.N * a.K <= (int64_t)1 << 24 ? 256 : 192) ? Int4Way::Values : Int4Way::Few;
+  if (a.M <= 16 || a.dt == DType::F32) return Int4Way::Few;
   const int64_t columns = a.group == 32 && a.M > 32 ? 16 : 32, rows = a.M > 32 ? 64 : 32;
   const int64_t blocks = (a.N + columns - 1) / columns * ((a.M + rows - 1) / rows);
   int64_t cost = 0;

@@ -488,3 +488,42 @@ def test_normalised_rows_of_large_gain(gpu):
     want = n @ wv.T
     bar = (2.0 ** -8 + 2.0 ** -18) * (np.abs(n) @ np.abs(wv).T) + 2.0 ** -8 * np.abs(want)
     assert (np.abs(y - want) <= bar).all()
+
+
+# ── many float32 rows ───────────────────────────────────────────────────────
+@pytest.mark.parametrize("M", [16, 200, 300, 1000])
+def test_float32_rows_keep_their_bits_whatever_their_number(gpu, M):
+    """Rows of a single value v: v code scale, whose sums of v (code + 24) and
+    -24 v (at most 31 |v| and 24 |v|, three parts each) and their difference
+    round by at most 2^-24 (31 * 3 + 24 * 3 + 7) |v| before the scale, and the
+    scale's product and the waves' sums by 3 steps of the result."""
+    rng = np.random.default_rng(M)
+    N, K, group = 300, 512, 64
+    w = rng.standard_normal((N, K)).astype(np.float32)
+    codes, scales = O.quantize_int4(w, group)
+    x = np.zeros((M, K), np.float32)
+    at = rng.integers(0, K, M)
+    v = rng.standard_normal(M).astype(np.float32)
+    x[np.arange(M), at] = v
+    got = gpu.linear_int4(gpu.from_numpy(x), gpu.from_numpy(_pack(codes)), gpu.from_numpy(scales), group=group).to_numpy()
+    want = v[:, None].astype(np.float64) * O.values_int4(codes, scales, group)[:, at].T
+    bar = 2.0 ** -24 * (172 * np.abs(v)[:, None] * scales[at // group] + 3 * np.abs(want))
+    assert (np.abs(got - want) <= bar).all(), (np.abs(got - want) / bar).max()
+
+
+@pytest.mark.parametrize("M,N,K,group", [(300, 70, 300, 64), (1000, 999, 64, 32), (4200, 60, 72, 128)])
+def test_float32_infinities_of_many_rows(gpu, M, N, K, group):
+    test_infinities_and_largest_values_are_the_products(gpu, "float32", M, N, K, group)
+
+
+def test_float32_rows_of_more_than_one_grid(gpu):
+    rng = np.random.default_rng(0)
+    M, N, K = 65535 * 64 + 70, 16, 8
+    packed, s = gpu.quantize_int4(gpu.from_numpy(_weights(rng, N, K, "float32")), 32)
+    x = rng.standard_normal((M, K)).astype(np.float32)
+    r = np.arange(M * N, dtype=np.float32).reshape(M, N) % 7
+    got = (gpu.from_numpy(r) + gpu.linear_int4(gpu.from_numpy(x), packed, s, None, "relu", group=32)).to_numpy()
+    for lo in (0, 65535 * 64 - 70, M - 70):
+        part = gpu.linear_int4(gpu.from_numpy(x[lo:lo + 70]), packed, s, None, "relu", group=32).to_numpy()
+        want = r[lo:lo + 70] + part.astype(np.float64)
+        assert (np.abs(got[lo:lo + 70] - want) <= 2.0 ** -23 * np.abs(want)).all()
