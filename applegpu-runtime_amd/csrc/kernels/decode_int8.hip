@@ -319,7 +319,9 @@ __global__ void __launch_bounds__(64 * NW) decode_int8_mfma(D8Args g) {
         x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[c], x, 0, 0, 0);
         if constexpr (F32) x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[c], x, 0, 0, 0);
       }
-      const float f = cq * ks[t];
+      // (a scale that is not finite as NaN: a sum of codes of 0 is not always 0
+      // with -1152 sum q in it)
+      const float f = cq * fmaf(ks[t], 0.f, ks[t]);
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[4 * t + i] = x[i] * f;
     }

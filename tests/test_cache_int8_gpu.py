@@ -367,6 +367,41 @@ def test_cache_past_two_to_the_31(gpu):
     assert np.abs(out[0, 0, 0] - want).max() <= np.abs(v).max() * (2 * d + 2.0 ** -20)
 
 
+# ── blocks that are not finite ──────────────────────────────────────────────
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16", "float32"])
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
+def test_appended_infinities_reach_every_query_that_sees_them(gpu, dtype, D, bad):
+    """A block given an infinity or NaN as a key or as a value makes the
+    queries that see it NaN, in every head, and no others."""
+    rng = np.random.default_rng(D)
+    B, H, T, block = 3, 64, 40, 16
+    for which in (0, 1):
+        dev = _upload(gpu, *(a for _ in range(2) for a in (np.zeros((B, H, T, D), np.int8), np.zeros((B, H, 3), np.float32))))
+        x = [rng.standard_normal((B, H, 33, D)).astype(np.float32) for _ in range(2)]
+        x[which][:, :, 20, 3] = bad
+        gpu.kv_write_int8(*dev, *(_dev(gpu, a, dtype) for a in x), gpu.from_numpy(np.zeros(B, np.int32)), block=block)
+        q = _dev(gpu, rng.standard_normal((B, H, 2, D)).astype(np.float32), dtype)
+        out = gpu.decode_attention_int8(q, *dev, gpu.from_numpy(np.array([33, 17, 16], np.int32)), block=block).to_numpy()
+        np.testing.assert_array_equal(np.isnan(out.astype(np.float32)).all(-1), [[[True, True]] * H, [[False, True]] * H, [[False, False]] * H])
+        np.testing.assert_array_equal(np.isnan(out.astype(np.float32)).any(-1), np.isnan(out.astype(np.float32)).all(-1))
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16", "float32"])
+@pytest.mark.parametrize("which", [0, 1])
+def test_an_infinity_appended_in_the_launch(gpu, dtype, which):
+    rng = np.random.default_rng(5)
+    B, H, T, D, block = 2, 64, 40, 64, 16
+    kc, ks = _cache(rng, B, H, T, D, block)
+    vc, vs = _cache(rng, B, H, T, D, block)
+    new = [rng.standard_normal((B, H, 1, D)).astype(np.float32) for _ in range(2)]
+    new[which][1, :, 0, 7] = np.inf
+    out = gpu.decode_attention_int8(_dev(gpu, rng.standard_normal((B, H, 1, D)).astype(np.float32), dtype),
+                                    *_upload(gpu, kc, ks, vc, vs), gpu.from_numpy(np.array([36, 36], np.int32)),
+                                    block=block, k_new=_dev(gpu, new[0], dtype), v_new=_dev(gpu, new[1], dtype)).to_numpy()
+    assert np.isfinite(out[0].astype(np.float32)).all() and np.isnan(out[1].astype(np.float32)).all()
+
+
 # ── refusals ────────────────────────────────────────────────────────────────
 def test_refusals(gpu):
     def cache(B=2, H=2, T=32, D=64, n=2):
