@@ -26,10 +26,13 @@
 //    is read 4 bytes of 8 keys a lane (D = 64) and its bytes interleaved by
 //    v_perm, which the conversion needs anyway.
 //  - Weights are rounded to f16 (2^-11 relative, against 2^-8 .. 2^-11 of the
-//    output's own rounding), hi + lo for fp32 outputs; they are kept within
-//    2^15 of a reference maximum that moves only when a score exceeds it by
-//    2^8, so that the exchange between lanes that a new maximum needs is rare,
-//    and within f16's normal range for 2^-21 of the maximum.
+//    output's own rounding), hi + lo for fp32 outputs.  The sum of weights and
+//    that of weights times vs have a reference each, a power of two that moves
+//    only when the query's own weight, or its weight times vs, exceeds it by
+//    2^8: the exchange between lanes that this needs is rare, both stay within
+//    2^15 of the reference, a weight times vs is in f16's normal range down to
+//    2^-21 of the largest, and blocks that a query does not see or gives no
+//    weight move nothing of it, whatever their scales.
 // Work: waves of a block take 32-key steps in turn; a context is split over
 // blocks while these leave CUs idle, and the splits' (O, m, l) are merged.
 // Bound by the read of the codes where contexts are long: 4 x 8 heads of 4
@@ -59,11 +62,12 @@ size_t lds_bytes(const DecodeInt8& a, int waves) {
 constexpr int kSplits = 1024;    // most parts of a context
 constexpr float kLift = 7.f;     // log2 of the weight at the reference maximum
 constexpr float kSlack = 8.f;    // log2 by which a weight may exceed that
+constexpr int kFar = 1000;       // log2 of what is nothing beside anything in fp32
 
 struct D8Args {
   DecodeInt8 a;
   int lg_block, splits, q_tiles;
-  int nw;         // waves of a block: 4, 8 or 16 (D = 128: 8 at most)
+  int nw;         // waves of a block: 4, 8 or 16
   int64_t chunk;  // keys of a split
   float* part;     // [units][splits][16 (D + 2)]: O, m, l of each query column
 };
@@ -89,6 +93,13 @@ __device__ __forceinline__ h8 codes8(uint32_t w0, uint32_t w1) {
   __builtin_memcpy(&o, r, 16);
   return o;
 }
+
+// A whole number of any size as a power of two for ldexp.
+__device__ __forceinline__ int power(float x) { return (int)fminf(fmaxf(x, (float)-kFar), (float)kFar); }
+// 2^(m - M) of two such, 0 for no weight.
+__device__ __forceinline__ float weight(float m, float M) { return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M); }
+// x = [1/2, 1) 2^exponent(x).
+__device__ __forceinline__ int exponent(float x) { return x != 0.f ? __builtin_amdgcn_frexp_expf(x) : -kFar; }
 
 // 8 consecutive query values, raw.
 template <typename T>
@@ -120,8 +131,8 @@ struct Step {
 // the context holds it leaves its cache block to the end: two waves append to
 // K and V there (as kv_write_int8 does), before anything else, while the others
 // are at the rows before it, and after a barrier the block's rows are read
-// from the cache like any (8 x 20 heads over 640 rows of 64: 9.2 us without,
-// 11.6 so, 14.0 with a launch of its own for the append).
+// from the cache like any (8 x 20 heads over 640 rows of 64: 7.6 us without,
+// 10.1 so).
 template <typename T, int D, int NW, bool NEW>
 __global__ void __launch_bounds__(64 * NW) decode_int8_mfma(D8Args g) {
   constexpr bool F32 = sizeof(T) == 4;
@@ -220,7 +231,7 @@ __global__ void __launch_bounds__(64 * NW) decode_int8_mfma(D8Args g) {
   const bool one_head = r0 / Tq == r1 / Tq;
   int64_t vis_lo = len - Tq + (one_head ? r0 % Tq : 0) + 1;
   const int64_t vis_hi = len - Tq + (one_head ? r1 % Tq : Tq - 1) + 1;
-  int64_t vis = r0 + n < R ? len - Tq + i_q + 1 : 0;
+  int vis = r0 + n < R && len - Tq + i_q + 1 > 0 ? (int)(len - Tq + i_q + 1) : 0;  // (a length fits 32 bits)
 
   int64_t j_hi = j_lo + g.chunk < vis_hi ? j_lo + g.chunk : vis_hi;
 
@@ -231,7 +242,7 @@ __global__ void __launch_bounds__(64 * NW) decode_int8_mfma(D8Args g) {
     if (at >= 0 && at < a.Tmax && at >= j_lo && at < j_lo + g.chunk) {
       tail = (at >> g.lg_block) << g.lg_block;
       j_hi = vis_lo = tail;
-      vis = vis < tail ? vis : tail;
+      vis = vis < tail ? vis : (int)tail;
     }
     if (appends) {
       if (tail >= 0) {
@@ -294,9 +305,10 @@ __global__ void __launch_bounds__(64 * NW) decode_int8_mfma(D8Args g) {
   f4 acc[ND];
 #pragma unroll
   for (int c = 0; c < ND; ++c) acc[c] = f4{0.f, 0.f, 0.f, 0.f};
+  // Of this lane's query, in whole powers of two: m, what its weights in l are
+  // relative to, and m - d, what its weights times vs in acc are relative to.
   float m = -INFINITY, l = 0.f;
-  int E = -126;          // O is kept in units of 2^E, at least the largest vs so far
-  float vinv = 0x1p126f;
+  int d = kFar;
 
   auto attend = [&](const Step<D>& cur, int64_t j0) __attribute__((always_inline)) {
     // (a tile that no query sees may be of a block that holds nothing yet)
@@ -309,7 +321,6 @@ __global__ void __launch_bounds__(64 * NW) decode_int8_mfma(D8Args g) {
     }
     // scores of keys 16 t + 4 q4 + i for query n
     float s[8];
-    float top = -INFINITY;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       f4 x = f4{corr, corr, corr, corr};
@@ -326,47 +337,44 @@ __global__ void __launch_bounds__(64 * NW) decode_int8_mfma(D8Args g) {
       for (int i = 0; i < 4; ++i) s[4 * t + i] = x[i] * f;
     }
     if (j0 + kStep > vis_lo) {
-      const int left = (int)(vis - j0 < 64 ? vis - j0 : 64);  // this query's keys of the step
+      const int left = vis - (int)j0;  // this query's keys from the step's first on
 #pragma unroll
       for (int e = 0; e < 8; ++e)
         if (16 * (e >> 2) + 4 * q4 + (e & 3) >= left) s[e] = -INFINITY;
     }
+    const float t0 = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), t1 = fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7]));
+    float top = fmaxf(t0, t1), top_v = fmaxf(t0 + (float)exponent(vs[0]), t1 + (float)exponent(vs[1]));
+    if (__any(top > m + kSlack || top_v > m + (kSlack - (float)d))) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) top = fmaxf(top, s[e]);
-    if (__any(top > m + kSlack)) {
-      top = fmaxf(top, __shfl_xor(top, 16, 64));
-      top = fmaxf(top, __shfl_xor(top, 32, 64));
-      const float M = fmaxf(m, top);
-      const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
-      l *= f;
+      for (int x = 16; x <= 32; x <<= 1) {
+        top = fmaxf(top, __shfl_xor(top, x, 64));
+        top_v = fmaxf(top_v, __shfl_xor(top_v, x, 64));
+      }
+      const float mv = m - (float)d;
+      const float M = top > m + kSlack ? ceilf(top) : m, Mv = top_v > mv + kSlack ? ceilf(top_v) : mv;
+      l = ldexpf(l, power(m - M));
+      const float f = ldexpf(1.f, power(mv - Mv));
 #pragma unroll
       for (int c = 0; c < ND; ++c) acc[c] *= f;
       m = M;
-    }
-    const float v0 = fabsf(vs[0]), v1 = fabsf(vs[1]);
-    const float v_top = fmaxf(v0 < INFINITY ? v0 : 0.f, v1 < INFINITY ? v1 : 0.f);
-    if (v_top * vinv > 1.f) {
-      const int e1 = (int)(__float_as_uint(v_top) >> 23) - 126;
-#pragma unroll
-      for (int c = 0; c < ND; ++c)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[c][i] = ldexpf(acc[c][i], E - e1);
-      E = e1;
-      vinv = ldexpf(1.f, -E);
+      d = power(M - Mv);
     }
     const float ref = m == -INFINITY ? 0.f : m - kLift;
     float p[8];
-    const float vn[2] = {vs[0] * vinv, vs[1] * vinv};
+    // (a weight that a factor past 2^126 would save is 0 in fp32)
+    float vn[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) vn[t] = __builtin_amdgcn_fmed3f(ldexpf(vs[t], d), -0x1p126f, 0x1p126f);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       p[e] = __builtin_amdgcn_exp2f(s[e] - ref);
       l += p[e];
       p[e] *= vn[e >> 2];
     }
-    if (!(v0 < INFINITY && v1 < INFINITY)) {
+    if (!(fabsf(vs[0]) < INFINITY && fabsf(vs[1]) < INFINITY)) {
       // a hidden key adds nothing, whatever its block's scale is
 #pragma unroll
-      for (int e = 0; e < 8; ++e) p[e] = s[e] == -INFINITY ? 0.f : p[e];
+      for (int e = 0; e < 8; ++e) p[e] = s[e] == -INFINITY ? 0.f : fabsf(vs[e >> 2]) < INFINITY ? p[e] : NAN;
     }
     h8 ph, pl;
 #pragma unroll
@@ -416,7 +424,7 @@ __global__ void __launch_bounds__(64 * NW) decode_int8_mfma(D8Args g) {
       __threadfence_block();  // what the two waves stored, for the others
       __syncthreads();
       j_hi = len;
-      vis = r0 + n < R ? len : 0;
+      vis = r0 + n < R ? (int)len : 0;
       for (j0 = tail + w * kStep; j0 < j_hi; j0 += kIter) {
         load(one, j0);
 #pragma unroll
@@ -432,13 +440,15 @@ __global__ void __launch_bounds__(64 * NW) decode_int8_mfma(D8Args g) {
   // the waves' states meet in LDS; lane (n, q4) holds d = (D/4) q4 + (D/16) i + c
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
+  // (each as its own weighted mean, which no sum of large values overflows)
   const int rows = r1 - r0 + 1;
   if (n < rows) {
     float* o = sm_o + (w * rows + n) * LD + (D / 4) * q4;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
     for (int c = 0; c < ND; ++c)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[(D / 16) * i + c] = ldexpf(acc[c][i], E);
+      for (int i = 0; i < 4; ++i) o[(D / 16) * i + c] = ldexpf(acc[c][i] * inv, -d);
     if (q4 == 0) { sm_m[w][n] = m; sm_l[w][n] = l; }
   }
   __syncthreads();
@@ -447,16 +457,18 @@ __global__ void __launch_bounds__(64 * NW) decode_int8_mfma(D8Args g) {
     float M = sm_m[0][qr];
 #pragma unroll
     for (int x = 1; x < NW; ++x) M = fmaxf(M, sm_m[x][qr]);
-    float L = 0.f, A = 0.f;
+    float L = 0.f, A = 0.f, f[NW];
 #pragma unroll
     for (int x = 0; x < NW; ++x) {
-      const float mx = sm_m[x][qr], f = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - M);
-      L += sm_l[x][qr] * f;
-      A += sm_o[(x * rows + qr) * LD + d] * f;
+      f[x] = sm_l[x][qr] * weight(sm_m[x][qr], M);
+      L += f[x];
     }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+    for (int x = 0; x < NW; ++x) A += sm_o[(x * rows + qr) * LD + d] * (f[x] * inv);
     if (g.splits == 1) {
       T* o = (T*)a.o + b * a.o_sb + (h * a.G + rr / Tq) * a.o_sh + iq * a.o_st;
-      o[d] = from_f<T>(len - Tq + iq + 1 > 0 ? A / L : 0.f);
+      o[d] = from_f<T>(len - Tq + iq + 1 > 0 ? A : 0.f);
     } else {
       float* P = g.part + ((int64_t)blockIdx.x * 16 + qr) * (D + 2);
       P[d] = A;
@@ -492,26 +504,27 @@ __global__ void __launch_bounds__(256) decode_int8_merge(D8Args g) {
   M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
 #pragma unroll
   for (int i = 0; i < MS; ++i) {
-    const float f = m[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[i] - M);
+    const float f = l[i] * weight(m[i], M);
     if (tid + 256 * i < g.splits) f_of[tid + 256 * i] = f;
-    L += l[i] * f;
+    L += f;
   }
   L = wave_sum(L);
   if ((tid & 63) == 0) red_l[tid >> 6] = L;
   __syncthreads();
+  L = (red_l[0] + red_l[1]) + (red_l[2] + red_l[3]);
+  const float inv = L == 0.f ? 0.f : 1.f / L;
   float A = 0.f;
 #pragma unroll 4
-  for (int s = part; s < g.splits; s += NP) A += P[s * st + d] * f_of[s];
+  for (int s = part; s < g.splits; s += NP) A += P[s * st + d] * (f_of[s] * inv);
   sum[part][d] = A;
   __syncthreads();
   if (part) return;
 #pragma unroll
   for (int i = 1; i < NP; ++i) A += sum[i][d];
-  L = (red_l[0] + red_l[1]) + (red_l[2] + red_l[3]);
   int64_t len = a.lens[b];
   len = len < 0 ? 0 : len > a.Tmax ? a.Tmax : len;
   T* o = (T*)a.o + b * a.o_sb + (h * a.G + rr / Tq) * a.o_sh + iq * a.o_st;
-  o[d] = from_f<T>(len - Tq + iq + 1 > 0 ? A / L : 0.f);
+  o[d] = from_f<T>(len - Tq + iq + 1 > 0 ? A : 0.f);
 }
 
 D8Args plan(const DecodeInt8& a) {
@@ -519,23 +532,35 @@ D8Args plan(const DecodeInt8& a) {
   g.a = a;
   g.lg_block = a.block == 16 ? 4 : a.block == 32 ? 5 : a.block == 64 ? 6 : 7;
   g.q_tiles = (int)((a.G * a.Tq + 15) / 16);
-  // A context to a block, with the waves that fill the CUs (16 of them each);
-  // or split over blocks of 4 waves and merged by a second launch, which costs
-  // about as much as three steps of a wave, where that saves more steps than
-  // that: 12 heads, 2048 rows of 64: 12.1 us whole, 8.3 split; 160 heads: 14.3
-  // whole, 19.4 split.  (Merged by a unit's last block in the same launch: 20
-  // heads, 8192 rows of 64 14.5 us against 13.4; 32 heads of 4 queries, 32768
-  // rows of 128 60 against 55: the blocks' wait for their stores and the count
-  // cost more than the launch.)
+  // A context to a block, with the waves that fill the CUs; or split over blocks
+  // of 4 waves and merged by a second launch, which costs about as much as three
+  // steps of a wave, where that saves more steps than that.  16 waves to a block
+  // where few contexts are long, 8 where they are short or many, or where 16
+  // would spill more than a few registers (D = 64 in fp32, or with an append:
+  // 160 heads, 4096 rows 32 us).  f16, D = 64, us:
+  //   heads, rows     16 waves   8 waves   split
+  //   12, 600             8.6       7.2      8.5
+  //   12, 1536           11.5      10.9      9.0
+  //   64, 1536           11.4      11.1     11.2
+  //   160, 640            9.2       7.6     12.4
+  //   160, 2048          14.4      14.3     18.0
+  //   160, 8192          33.7      39.8     37.4
+  // (Merged by a unit's last block in the same launch: 20 heads, 8192 rows of 64
+  // 14.5 us against 13.4; 32 heads of 4 queries, 32768 rows of 128 60 against
+  // 55: the blocks' wait for their stores and the count cost more than the
+  // launch.)
   const int64_t units = a.B * a.H * g.q_tiles;
-  g.nw = units <= 256 && a.D != 128 ? 16 : units <= 512 ? 8 : 4;
+  const bool few = units <= 256 && a.D != 128, brief = few && a.Tmax <= 2048;
+  const bool fits = a.D == 32 || (a.dt != DType::F32 && !a.kn);
+  g.nw = few && !brief && fits ? 16 : units <= 512 ? 8 : 4;
   while (g.nw > kFew && (lds_bytes(a, g.nw) > (60 << 10) || a.Tmax <= g.nw / 2 * kStep)) g.nw /= 2;
   const int64_t iters = (a.Tmax + g.nw * kStep - 1) / (g.nw * kStep);
-  const double per = (a.D == 128 ? 2.0 : 1.0) / 1e5;  // steps of a wave for a row of a unit, all CUs filled
+  // steps of a wave for the merge, and for a row of a unit with all CUs filled
+  const double merge = brief ? 3.7 : 3.0, per = (brief ? 2.3 : a.D == 128 ? 2.0 : 1.0) / 1e5;
   g.splits = 1;
   g.chunk = a.Tmax;
   g.part = nullptr;
-  if (units > 0 && units < kSplits && (double)iters > 3.0 + per * (double)a.Tmax * (double)units) {
+  if (units > 0 && units < kSplits && (double)iters > merge + per * (double)a.Tmax * (double)units) {
     g.nw = kFew;
     const int64_t iter = kFew * kStep, most = (a.Tmax + iter - 1) / iter;
     int64_t want = (kSplits + units - 1) / units;  // four blocks a CU
@@ -548,16 +573,19 @@ D8Args plan(const DecodeInt8& a) {
 
 template <typename T, int D, int NW>
 void launch_nw(const D8Args& g, hipStream_t s) {
+  constexpr bool kAppends = NW < 16 || D == 32;
   const dim3 grid((unsigned)(g.a.B * g.a.H * g.q_tiles * g.splits));
-  if (g.a.kn) hipLaunchKernelGGL((decode_int8_mfma<T, D, NW, true>), grid, dim3(64 * NW), lds_bytes(g.a, NW), s, g);
-  else hipLaunchKernelGGL((decode_int8_mfma<T, D, NW, false>), grid, dim3(64 * NW), lds_bytes(g.a, NW), s, g);
+  if (!g.a.kn) hipLaunchKernelGGL((decode_int8_mfma<T, D, NW, false>), grid, dim3(64 * NW), lds_bytes(g.a, NW), s, g);
+  else if constexpr (kAppends)
+    hipLaunchKernelGGL((decode_int8_mfma<T, D, NW, true>), grid, dim3(64 * NW), lds_bytes(g.a, NW), s, g);
 }
 
 template <typename T, int D>
 void launch(const D8Args& g, hipStream_t s) {
+  constexpr bool kWide = D == 32 || (D == 64 && sizeof(T) == 2);
   if (g.nw == kFew) launch_nw<T, D, kFew>(g, s);
-  else if (g.nw == 8 || D == 128) launch_nw<T, D, 8>(g, s);
-  else launch_nw<T, D, D == 128 ? 8 : 16>(g, s);
+  else if (g.nw == 8) launch_nw<T, D, 8>(g, s);
+  else if constexpr (kWide) launch_nw<T, D, 16>(g, s);
   if (g.splits > 1)
     hipLaunchKernelGGL((decode_int8_merge<T, D>), dim3((unsigned)(g.a.B * g.a.H * g.a.G * g.a.Tq)), dim3(256), 0, s, g);
 }

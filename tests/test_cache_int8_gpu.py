@@ -402,6 +402,126 @@ def test_an_infinity_appended_in_the_launch(gpu, dtype, which):
     assert np.isfinite(out[0].astype(np.float32)).all() and np.isnan(out[1].astype(np.float32)).all()
 
 
+# ── blocks of unlike scale ──────────────────────────────────────────────────
+RATIOS = [(t, k) for t, ks in (("float16", (0, 12, 24)), ("bfloat16", (0, 24, 40, 100)), ("float32", (0, 12, 24, 60, 100)))
+          for k in ks]
+
+
+@pytest.mark.parametrize("dtype,k", RATIOS)
+@pytest.mark.parametrize("T,block,at", [(32, 16, 0), (32, 16, 1), (300, 32, 3), (300, 16, 18), (3000, 64, 0), (3000, 128, 20)])
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_a_scale_without_weight_moves_nothing(gpu, dtype, k, T, block, at, D):
+    """All weight on the rows of one block, equal keys of which the output is
+    the plain mean; the values of the others, 2^k as large, have weights below
+    2^-200.  n equal weights kept to w, and n + 16 roundings of the sums."""
+    rng = np.random.default_rng(T + k)
+    H, nb = 3, -(-T // block)
+    q = O.round_to(rng.choice([-1.0, 1.0], (1, H, 1, D)).astype(np.float32) * 2, dtype)
+    kc = np.zeros((1, H, T, D), np.int8)
+    rows = slice(at * block, min((at + 1) * block, T))
+    kc[:, :, rows] = (np.sign(q) * 100).astype(np.int8)
+    ks = np.full((1, H, nb), 240 * np.log(2) * D ** 0.5 / (200 * D), np.float32)    # a score of 240 ln 2
+    vc = rng.integers(-127, 128, (1, H, T, D)).astype(np.int8)
+    vs = np.full((1, H, nb), 1e-5 * 2.0 ** k, np.float32)
+    vs[:, :, at] = 1e-5
+    out = gpu.decode_attention_int8(_dev(gpu, q, dtype), *_upload(gpu, kc, ks, vc, vs),
+                                    gpu.from_numpy(np.array([T], np.int32)), block=block).to_numpy().astype(np.float64)
+    v = O.values_int8(vc, vs, block)[:, :, rows].astype(np.float64)
+    want, n = v.mean(2, keepdims=True), v.shape[2]
+    w = 2.0 ** -11 if dtype != "float32" else 2.0 ** -22
+    bar = (w + (n + 16) * 2.0 ** -24) * np.abs(v).mean(2, keepdims=True) + HALF_STEP[dtype] * np.abs(want)
+    assert (np.abs(out - want) <= bar + 2.0 ** -25 * (dtype == "float16")).all(), np.abs(out - want).max()
+
+
+@pytest.mark.parametrize("dtype,k", RATIOS)
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_a_scale_that_a_query_does_not_see_moves_nothing_of_it(gpu, dtype, k, D):
+    """Three queries of a chunk, the last two of which see one and two rows of
+    a block 2^k as large: each is as exact as the rows it sees."""
+    rng = np.random.default_rng(k)
+    H, T, block = 3, 32, 16
+    kc, ks = _cache(rng, 1, H, T, D, block)
+    vc, _ = _cache(rng, 1, H, T, D, block)
+    vs = np.full((1, H, 2), 1e-5, np.float32)
+    vs[:, :, 1] *= np.float32(2.0 ** k)
+    q = O.round_to(rng.standard_normal((1, H, 3, D)).astype(np.float32), dtype)
+    out = gpu.decode_attention_int8(_dev(gpu, q, dtype), *_upload(gpu, kc, ks, vc, vs),
+                                    gpu.from_numpy(np.array([18], np.int32)), block=block).to_numpy()
+    kv, v = O.values_int8(kc, ks, block), O.values_int8(vc, vs, block)
+    want = O.decode_attention(q, kv, v, [18])
+    for i in range(3):
+        bar = _bar(q, kv, v[:, :, :16 + i], D ** -0.5, dtype, T)
+        _check(out[:, :, i], want[:, :, i], (bar[0] + 2.0 ** -25 * (dtype == "float16"), bar[1]))
+
+
+@pytest.mark.parametrize("dtype,k", [("float16", 20), ("bfloat16", 60), ("float32", 60), ("float32", 100)])
+@pytest.mark.parametrize("T,block", [(48, 16), (3000, 64)])
+def test_a_small_weight_on_large_values_counts(gpu, dtype, k, T, block):
+    """Rows whose weights are 2^-k of the others' and whose values are 2^k of
+    theirs: sum P_j |v_j| of both parts, each kept to its own error."""
+    rng = np.random.default_rng(k)
+    H, D, nb = 2, 64, -(-T // block)
+    q = O.round_to(rng.choice([-1.0, 1.0], (1, H, 1, D)).astype(np.float32) * 2, dtype)
+    kc = np.zeros((1, H, T, D), np.int8)
+    kc[:, :, block:2 * block] = (np.sign(q) * 100).astype(np.int8)
+    ks = np.full((1, H, nb), k * np.log(2) * D ** 0.5 / (200 * D), np.float32)
+    vc = rng.integers(-127, 128, (1, H, T, D)).astype(np.int8)
+    vs = np.full((1, H, nb), 1e-5 * 2.0 ** k, np.float32)
+    vs[:, :, 1] = 1e-5
+    out = gpu.decode_attention_int8(_dev(gpu, q, dtype), *_upload(gpu, kc, ks, vc, vs),
+                                    gpu.from_numpy(np.array([T], np.int32)), block=block).to_numpy().astype(np.float64)
+    kv, v = O.values_int8(kc, ks, block), O.values_int8(vc, vs, block)
+    want, size = O.decode_attention(q, kv, v, [T]), O.decode_attention(q, kv, np.abs(v), [T])
+    d = (D + 16) * 2.0 ** -24 * k * np.log(2)
+    w = 2.0 ** -11 if dtype != "float32" else 2.0 ** -22
+    bar = (2 * d + w + (T + 16) * 2.0 ** -24) * size + HALF_STEP[dtype] * np.abs(want)
+    assert (np.abs(out - want) <= bar + 2.0 ** -25 * (dtype == "float16")).all(), (np.abs(out - want) / bar).max()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("T,B,size", [(100, 1, 2e38), (600, 8, 2e38), (3000, 1, 2e38), (3000, 40, 1e35), (100, 1, 1e-36),
+                                      (3000, 1, 1e-36), (100, 1, 2e-41)])
+def test_values_next_to_the_largest_and_smallest(gpu, dtype, T, B, size):
+    """A mean of values is as large as they are, however many they are."""
+    rng = np.random.default_rng(T)
+    H, D, block = 2, 64, 16
+    kc, ks = _cache(rng, B, H, T, D, block)
+    vc, vs = _cache(rng, B, H, T, D, block)
+    vc[..., ::2] = np.abs(vc[..., ::2])     # half of the columns do not cancel
+    vs[:] = np.float32(size / 127)
+    q = O.round_to(rng.standard_normal((B, H, 1, D)).astype(np.float32), dtype)
+    out = gpu.decode_attention_int8(_dev(gpu, q, dtype), *_upload(gpu, kc, ks, vc, vs),
+                                    gpu.from_numpy(np.full(B, T, np.int32)), block=block).to_numpy()
+    kv, v = O.values_int8(kc, ks, block), O.values_int8(vc, vs, block)
+    bar = _bar(q, kv, v, D ** -0.5, dtype, T)
+    _check(out, O.decode_attention(q, kv, v, [T] * B),
+           (bar[0] + 2.0 ** (-133 if dtype == "bfloat16" else -148), bar[1]))
+
+
+@pytest.mark.parametrize("dtype,D", [("float16", 64), ("float32", 64), ("bfloat16", 32), ("float32", 32)])
+def test_many_heads_over_long_rows(gpu, dtype, D):
+    """160 contexts past 2048 rows, whole in blocks of 16 or 8 waves, the last
+    of them appended in the launch too."""
+    rng = np.random.default_rng(D)
+    B, H, Tmax, block = 8, 20, 2200, 32
+    lens = [Tmax, 2049, 1, 0, 2100, 513, 2176, 2177]
+    dev, q, want, bar = _attend(gpu, rng, dtype, D, block, Tmax, 1, 1, lens, H=H)
+    new = [O.round_to(rng.standard_normal((B, H, 1, D)).astype(np.float32), dtype) for _ in range(2)]
+    held = [t.to_numpy() for t in dev]
+    for codes, scales, x in ((held[0], held[1], new[0]), (held[2], held[3], new[1])):
+        O.append_int8(codes, scales, x, np.array(lens) - 1, block)
+    out = gpu.decode_attention_int8(_dev(gpu, q, dtype), *dev, gpu.from_numpy(np.array(lens, np.int32)), block=block,
+                                    k_new=_dev(gpu, new[0], dtype), v_new=_dev(gpu, new[1], dtype)).to_numpy()
+    for t, a in zip(dev, held):
+        np.testing.assert_array_equal(t.to_numpy(), a)
+    for b, n in enumerate(lens):
+        if n == 0:
+            assert (out[b] == 0).all()
+            continue
+        k, v = (O.values_int8(held[i][b:b + 1, :, :n], held[i + 1][b:b + 1, :, :-(-n // block)], block) for i in (0, 2))
+        _check(out[b:b + 1], O.decode_attention(q[b:b + 1], k, v, [n]), _bar(q[b:b + 1], k, v, D ** -0.5, dtype, Tmax))
+
+
 # ── refusals ────────────────────────────────────────────────────────────────
 def test_refusals(gpu):
     def cache(B=2, H=2, T=32, D=64, n=2):
