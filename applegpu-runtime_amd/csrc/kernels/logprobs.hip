@@ -15,7 +15,7 @@
 // blocks, whose states a second launch merges.  Measured: 2047 x 50257 fp32
 // with 20 alternatives 85 us (4.84 TB/s), in bf16 67 us (bound by its
 // instructions, an exponential and some eight others a value); 8 rows in f16
-// 8 us and 6 for the merge; the gradient in bf16 88 us (4.6 TB/s, read and
+// 8 us and 6 for the merge; the gradient in bf16 89 us (4.6 TB/s, read and
 // written).
 #include "device.hpp"
 
@@ -409,48 +409,103 @@ __global__ void __launch_bounds__(256) token_logprobs_merge(LpArgs g) {
   });
 }
 
-// 16 logits a thread; VEC: the rows of z and dz are aligned alike.
+constexpr float kSure = 0.75f;  // (at most one element of a row is past it)
+
+// A row to g.splits blocks, 16-byte vectors (VEC: the rows of z and dz are
+// aligned alike) to threads in turn.
+//
+// 1 - p_t and log p + H lose their digits where one element has nearly all of
+// the probability, since lse is known to half its last place only.  So the
+// others' probabilities are summed on the way, and the block that meets an
+// element past kSure adds those of the row's other blocks: with T = sum p_i /
+// p_j, p = 1 / (1 + T), 1 - p = T p and log p = -log1p(T).  2047 x 50257 bf16
+// 89 us with no such row, 102 with half, 125 with all of them.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) token_logprobs_grad(LpArgs g, const float* __restrict__ g_lp,
                                                            const float* __restrict__ g_h, T* __restrict__ dz) {
   const TokenLogprobs& a = g.a;
-  constexpr int VE = 16 / (int)sizeof(T);
-  const int64_t r = blockIdx.x, t = token_at(a, r);
+  constexpr int VE = VEC ? 16 / (int)sizeof(T) : 1;
+  const uint32_t gy = (uint32_t)g.splits, part_of = blockIdx.x % gy;
+  const int64_t r = blockIdx.x / gy, t = token_at(a, r);
   const T* z = (const T*)a.z + r * a.ld;
   T* out = dz + r * a.V;
   const float lse = a.lse[r];
   const bool none = lse == -INFINITY;
   const float gl = t >= 0 && t < a.V ? g_lp[r] : 0.f, gh = g_h ? g_h[r] : 0.f, H = g_h ? a.entropy[r] : 0.f;
   const float c0 = gl + gh * H, c1 = gh * kLn2;
-  // -p (g_lp + g_H (log p + H)), + g_lp at the token
-  auto grad = [&](float x, int64_t j) __attribute__((always_inline)) {
-    const float d = __builtin_elementwise_maximum((x - lse) * kLog2e, -200.f);
-    const float v = -__builtin_amdgcn_exp2f(d) * (c0 + c1 * d);
-    return none ? 0.f : j == t ? v + gl : v;
+  const int mis = VEC ? (int)(((uintptr_t)z & 15) / sizeof(T)) : 0;
+  const int V = (int)a.V, vecs = (V + mis + VE - 1) / VE, tid = (int)threadIdx.x;
+  auto prob = [&](float x) __attribute__((always_inline)) {
+    return __builtin_amdgcn_exp2f(__builtin_elementwise_maximum((x - lse) * kLog2e, -200.f));
   };
-  if constexpr (VEC) {
-    const int mis = (int)(((uintptr_t)z & 15) / sizeof(T));
-    const int64_t vecs = (a.V + mis + VE - 1) / VE;
-    for (int64_t v = (int64_t)blockIdx.y * 256 + threadIdx.x; v < vecs; v += (int64_t)gridDim.y * 256) {
-      const int64_t j = v * VE - mis;
-      if (j >= 0 && j + VE <= a.V) {
-        const uint4 raw = *(const uint4*)(z + j);
-        T e[VE];
-        __builtin_memcpy(e, &raw, 16);
+  // f(x, j) of vector v's elements in the row
+  auto each = [&](int v, auto&& f) __attribute__((always_inline)) {
+    const int j = v * VE - mis;
+    if (VEC && j >= 0 && j + VE <= V) {
+      const uint4 raw = *(const uint4*)(z + j);
+      T e[VE];
+      __builtin_memcpy(e, &raw, sizeof(e));
 #pragma unroll
-        for (int i = 0; i < VE; ++i) e[i] = from_f<T>(grad(to_f(e[i]), j + i));
-        uint4 o;
-        __builtin_memcpy(&o, e, 16);
-        *(uint4*)(out + j) = o;
-      } else {
-        for (int i = 0; i < VE; ++i)
-          if (j + i >= 0 && j + i < a.V) out[j + i] = from_f<T>(grad(to_f(z[j + i]), j + i));
-      }
+      for (int i = 0; i < VE; ++i) f(to_f(e[i]), j + i);
+    } else {
+      for (int i = 0; i < VE; ++i)
+        if (j + i >= 0 && j + i < V) f(to_f(z[j + i]), j + i);
     }
-  } else {
-    for (int64_t j = (int64_t)blockIdx.y * 256 + threadIdx.x; j < a.V; j += (int64_t)gridDim.y * 256)
-      out[j] = from_f<T>(grad(to_f(z[j]), j));
+  };
+  float sum = 0.f;
+  int at = -1;
+  for (int v = (int)part_of * 256 + tid; v < vecs; v += (int)gy * 256) {
+    float top = 0.f, part = 0.f;
+    // -p (g_lp + g_H (log p + H)), + g_lp at the token
+    auto grad = [&](float x, int j) __attribute__((always_inline)) {
+      const float d = __builtin_elementwise_maximum((x - lse) * kLog2e, -200.f);
+      const float p = __builtin_amdgcn_exp2f(d), w = -p * (c0 + c1 * d);
+      top = fmaxf(top, p);
+      part += p;
+      return none ? 0.f : j == t ? w + gl : w;
+    };
+    const int j = v * VE - mis;
+    if (VEC && j >= 0 && j + VE <= V) {
+      const uint4 raw = *(const uint4*)(z + j);
+      T e[VE];
+      __builtin_memcpy(e, &raw, sizeof(e));
+#pragma unroll
+      for (int i = 0; i < VE; ++i) e[i] = from_f<T>(grad(to_f(e[i]), j + i));
+      uint4 o;
+      __builtin_memcpy(&o, e, sizeof(e));
+      *(uint4*)(out + j) = o;
+    } else {
+      for (int i = 0; i < VE; ++i)
+        if (j + i >= 0 && j + i < V) out[j + i] = from_f<T>(grad(to_f(z[j + i]), j + i));
+    }
+    if (top > kSure) {
+      part = 0.f;
+      each(v, [&](float x, int i) {
+        const float p = prob(x);
+        if (p > kSure) at = i;
+        else part += p;
+      });
+    }
+    sum += part;
   }
+
+  __shared__ int sure[4];
+  __shared__ float parts[4];
+  const int lane = tid & 63, wave = tid >> 6;
+  const uint64_t who = __ballot(at >= 0);
+  if (lane == (who ? __ffsll((long long)who) - 1 : 0)) sure[wave] = at;
+  __syncthreads();
+  const int j = max(max(sure[0], sure[1]), max(sure[2], sure[3]));
+  if (j < 0) return;
+  for (int v = tid; v < vecs; v += 256)
+    if ((uint32_t)v / 256 % gy != part_of) each(v, [&](float x, int) { sum += prob(x); });
+  sum = wave_sum(sum);
+  if (lane == 0) parts[wave] = sum;
+  __syncthreads();  // (and the stores to dz before the last one)
+  if (tid) return;
+  sum = ((parts[0] + parts[1]) + (parts[2] + parts[3])) / prob(to_f(z[j]));
+  const float p = 1.f / (1.f + sum);
+  out[j] = from_f<T>((j == t ? gl * (sum * p) : -gl * p) - gh * p * (H - log1pf(sum)));
 }
 
 LpArgs plan(const TokenLogprobs& a) {
@@ -497,10 +552,14 @@ void token_logprobs_backward(const TokenLogprobs& a, const float* g_lp, const fl
   g.a = a;
   const int64_t es = (int64_t)dtype_size(a.dt);
   const bool vec = ((uintptr_t)a.z & 15) == ((uintptr_t)dz & 15) && (a.ld - a.V) * es % 16 == 0;
-  const int64_t per = 256 * 16 / es * 2;
-  int64_t by = (a.V + per - 1) / per;
-  if (by > 65535) by = 65535;
-  const dim3 grid((unsigned)a.R, (unsigned)by);
+  // blocks of a row, one after another: what an element past kSure has its
+  // block read again is in the caches then, and writes are in a row (2047 x
+  // 50257 fp32 150 us; a part of every row first 177)
+  const int64_t per = 256 * 16 / es * 2, most = a.R < (1 << 23) ? (1 << 23) / a.R : 1;
+  int64_t parts = (a.V + per - 1) / per;
+  if (parts > most) parts = most;
+  g.splits = (int)parts;
+  const dim3 grid((unsigned)(a.R * parts));
   AGPU_FLOAT_SWITCH(a.dt, {
     if (vec) hipLaunchKernelGGL((token_logprobs_grad<T, true>), grid, dim3(256), 0, s, g, g_lp, g_H, (T*)dz);
     else hipLaunchKernelGGL((token_logprobs_grad<T, false>), grid, dim3(256), 0, s, g, g_lp, g_H, (T*)dz);

@@ -178,6 +178,58 @@ def test_gradients_vs_formula(gpu, dtype, R, V, entropy):
     assert (np.abs(got - want) <= bar).all(), np.abs(got - want).max()
 
 
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("V,off", [(2, 0), (40, 0), (1000, 0), (1000, 1), (1000, 1024), (50257, 0), (50257, -64)])
+@pytest.mark.parametrize("view", [False, True])
+def test_gradients_of_nearly_certain_rows_keep_their_digits(gpu, dtype, V, off, view):
+    """One word with all but e^-8 .. e^-80 of the probability, and 3/4 and
+    about; T = sum exp(z_i - z_j) of the others to 2^-21 (2 + |z_i - z_j|)
+    relative gives 1 - p = T / (1 + T) and log p = -log1p(T) as well, whatever
+    is added to the row; the entropy is given to 2^-17."""
+    rng = np.random.default_rng(V)
+    R = 12
+    z = O.round_to(rng.standard_normal((R, V)).astype(np.float32), dtype)
+    at = rng.integers(0, V, R)
+    at[:3] = 0, V - 1, V // 2
+    lift = np.array([8, 12, 16, 20, 24, 32, 80, 0.5, 1, 1.5, 2, 4], np.float32)
+    z[np.arange(R), at] = lift + np.log(np.float32(V)) + 1
+    z = O.round_to(z + off, dtype).astype(np.float64)
+    tokens = np.where(np.arange(R) % 4 == 3, (at + 1) % V, at).astype(np.int32)
+    tokens[5] = -100
+    zj = z[np.arange(R), at][:, None]
+    e = np.exp(z - zj)
+    e[np.arange(R), at] = 0
+    T = e.sum(1, keepdims=True)
+    e[np.arange(R), at] = 1
+    p, logp = e / (1 + T), (z - zj) - np.log1p(T)
+    H = -(p * logp).sum(1, keepdims=True)
+    g, gh = rng.standard_normal((2, R)).astype(np.float32)
+    lse = (zj + np.log1p(T)).astype(np.float32)
+    one = np.arange(V) == tokens[:, None]
+    rest = np.where(one & (np.arange(V) == at[:, None]), T / (1 + T), one - p) * (tokens >= 0)[:, None]
+    want = g[:, None] * rest - gh[:, None] * p * (logp + H)
+    zt = _dev(gpu, z, dtype)
+    if view:    # rows that begin anywhere
+        zt = gpu.slice(_dev(gpu, np.pad(z, ((0, 0), (3, 6))), dtype), 1, 3, 3 + V)
+    d = gpu.token_logprobs_backward(gpu.from_numpy(g), gpu.from_numpy(gh), zt, gpu.from_numpy(tokens),
+                                    gpu.from_numpy(H[:, 0].astype(np.float32)), gpu.from_numpy(lse[:, 0]))
+    got = d.to_numpy().astype(np.float64)
+    rate = 2.0 ** -21 * (2 + np.where(p > 0, zj - z, 0) + np.abs(lse))
+    size = np.abs(g)[:, None] * (1 + 2 * one) * p + np.abs(gh)[:, None] * p * (1 + np.abs(logp) + H)
+    bar = rate * size
+    # the certain element, and the token among the others
+    sure = (np.arange(V) == at[:, None]) & (p > 0.75)
+    far = np.where(p > 0, zj - z, 0).max(1, keepdims=True)
+    tight = 2.0 ** -21 * (2 + far) * (np.abs(g)[:, None] * np.where(one, T, p) + np.abs(gh)[:, None] * p * (np.abs(logp) + H)) \
+        + 2.0 ** -17 * np.abs(gh)[:, None] * p * H
+    bar = np.where(sure, tight, bar + 2.0 ** -22 * np.abs(g)[:, None] * one)
+    # (a p below float32's normal range may be taken as 0: an error of at most 2^-126 in it, times the gradients' factor,
+    # and of V of them in T)
+    bar = bar + 2.0 ** -126 * (np.abs(g)[:, None] + np.abs(gh)[:, None] * (1 + np.abs(logp) + H)) * np.where(sure, V, 1)
+    bar = bar + HALF_STEP[dtype] * np.abs(want) + {"float16": 2.0 ** -25, "bfloat16": 2.0 ** -133, "float32": 2.0 ** -149}[dtype]
+    assert (np.abs(got - want) <= bar).all(), (np.abs(got - want) / bar).max()
+
+
 def test_gradients_vs_differences(gpu):
     """Differences of the device's own outputs along a direction: the step is
     1/64, so a third derivative of at most 8 |direction|^3 adds 2^-12, and the
