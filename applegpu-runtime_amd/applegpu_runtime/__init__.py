@@ -745,7 +745,8 @@ def kv_write_int8(k_codes, k_scales, v_codes, v_scales, k_rows, v_rows, pos, blo
     magnitude / 127.  The rows that the first touched block holds before
     pos[b] keep their values, to half a step of its scale where that grows.  A
     block given an infinity or NaN reads as NaN.  Rows that would land outside
-    the cache are not written."""
+    the cache are not written.  Reads and attentions that were asked for before
+    see the cache as it was, also where they are evaluated later."""
     ids = [_t(t)._id for t in (k_codes, k_scales, v_codes, v_scales, k_rows, v_rows, pos)]
     if lib.applegpu_kv_write_int8(*ids, int(block)) != 0:
         raise ValueError(ffi_error())
@@ -753,7 +754,8 @@ def kv_write_int8(k_codes, k_scales, v_codes, v_scales, k_rows, v_rows, pos, blo
 
 def kv_read_int8(k_codes, k_scales, v_codes, v_scales, pos, rows, block=16, dtype="float32"):
     """(K, V) rows pos[b] .. pos[b] + rows of an 8-bit cache as values,
-    [B, H, rows, D] each; zeros for rows outside the cache."""
+    [B, H, rows, D] each; zeros for rows outside the cache.  They are the rows
+    that the cache holds at the call (kv_write_int8)."""
     return _op(b"kv_read_int8", [_t(k_codes), _t(k_scales), _t(v_codes), _t(v_scales), _t(pos)],
                i=(int(rows), int(block), DTYPE_CODES[canon_dtype(dtype)]), nout=2)
 
@@ -765,7 +767,8 @@ def decode_attention_int8(q, k_codes, k_scales, v_codes, v_scales, lens, block=1
     sees none gets zeros.  The softmax scale is 1 / sqrt(D) by default.
 
     k_new, v_new ([B, H, 1, D], Tq = 1): the step's own K and V rows, appended
-    as row lens[b] - 1 when the result is evaluated, before it attends."""
+    as row lens[b] - 1 when the result is evaluated, before it attends, and at
+    the latest when something else is asked of the cache."""
     ins = [_t(q), _t(k_codes), _t(k_scales), _t(v_codes), _t(v_scales), _t(lens)]
     if k_new is not None or v_new is not None:
         ins += [_t(k_new), _t(v_new)]

@@ -299,8 +299,10 @@ int32_t applegpu_kv_write_int8(uint64_t k_codes_id, uint64_t k_scales_id, uint64
                                uint64_t k_rows_id, uint64_t v_rows_id, uint64_t pos_id, int64_t block) {
   return guarded<int32_t>(kFfi, -1, [&]() -> int32_t {
     TensorP kr = kv_operand(k_rows_id), vr = kv_operand(v_rows_id), pos = kv_operand(pos_id);
-    ops::kv_write_int8({kv_cache_operand(k_codes_id), kv_cache_operand(k_scales_id), kv_cache_operand(v_codes_id),
-                        kv_cache_operand(v_scales_id), block}, kr, vr, pos);
+    const ops::Int8KV c{kv_cache_operand(k_codes_id), kv_cache_operand(k_scales_id), kv_cache_operand(v_codes_id),
+                        kv_cache_operand(v_scales_id), block};
+    eval_cache_uses({c.kc, c.ks, c.vc, c.vs}, false);
+    ops::kv_write_int8(c, kr, vr, pos);
     return 0;
   });
 }

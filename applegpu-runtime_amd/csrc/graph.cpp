@@ -344,6 +344,40 @@ std::vector<TensorP> run_op(int code, const std::vector<TensorP>& in, const std:
 }
 
 // ── lazy recording ─────────────────────────────────────────────────────────
+// Outputs of the recorded reads of, and attentions over, K/V caches in 8 bits.
+// Those caches are written in place, so what was recorded before a write runs
+// before it (an attention that appends its step's row writes too).
+struct CacheUse {
+  std::weak_ptr<Tensor> out;
+  bool appends;
+};
+static std::vector<CacheUse> g_cache_uses;
+
+// The node that makes t: a selector's producer.
+static const Node* producer(const Tensor& t) {
+  const Node* n = t.node.get();
+  return n->code < 0 ? n->in[0]->node.get() : n;
+}
+
+void eval_cache_uses(const std::vector<TensorP>& cache, bool appends_only) {
+  std::vector<TensorP> before;
+  size_t kept = 0;
+  for (const CacheUse& use : g_cache_uses) {
+    TensorP t = use.out.lock();
+    if (!t || !t->pending()) continue;
+    g_cache_uses[kept++] = use;
+    if (appends_only && !use.appends) continue;
+    const Node* n = producer(*t);
+    const size_t first = n->code == OP_KV_READ_INT8 ? 0 : 1;
+    bool same = false;
+    for (size_t i = first; i < first + 4; ++i)
+      for (const TensorP& c : cache) same = same || !n->in[i]->buf || !c->buf || n->in[i]->buf == c->buf;
+    if (same) before.push_back(t);
+  }
+  g_cache_uses.resize(kept);
+  eval_all(before);
+}
+
 std::vector<TensorP> record_op(int code, const std::vector<TensorP>& in, const std::vector<double>& f,
                                const std::vector<int64_t>& iv) {
   if (code == OP_SGD_MATMUL || code == OP_SGD_SUM_ROWS || code == OP_LINEAR_BACKWARD_SGD ||
@@ -354,6 +388,11 @@ std::vector<TensorP> record_op(int code, const std::vector<TensorP>& in, const s
   {
     MetaScope ms;
     metas = run_op(code, in, f, iv);
+  }
+  const bool uses_cache = code == OP_KV_READ_INT8 || code == OP_DECODE_ATTENTION_INT8, appends = uses_cache && in.size() == 8;
+  if (uses_cache) {
+    const size_t first = code == OP_KV_READ_INT8 ? 0 : 1;
+    eval_cache_uses({in.begin() + first, in.begin() + first + 4}, !appends);
   }
   auto node = std::make_shared<Node>();
   node->code = code;
@@ -385,6 +424,8 @@ std::vector<TensorP> record_op(int code, const std::vector<TensorP>& in, const s
       node->selectors.push_back(t);
     }
   }
+  if (uses_cache)
+    for (auto& t : outs) g_cache_uses.push_back({t, appends});
   return outs;
 }
 

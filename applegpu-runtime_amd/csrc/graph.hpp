@@ -47,6 +47,10 @@ std::vector<TensorP> run_op(int code, const std::vector<TensorP>& in, const std:
 std::vector<TensorP> record_op(int code, const std::vector<TensorP>& in, const std::vector<double>& f,
                                const std::vector<int64_t>& iv);
 
+// Runs what was recorded and reads a K/V cache in 8 bits (codes and scales),
+// or with appends_only what also writes it.
+void eval_cache_uses(const std::vector<TensorP>& cache, bool appends_only);
+
 // Materialise a pending tensor (no-op when it already has storage).
 void eval(const TensorP& t);
 // Materialise several pending tensors with one fusion plan over all their

@@ -247,7 +247,9 @@ int32_t applegpu_kv_write_pair(uint64_t k_cache_id, uint64_t v_cache_id, uint64_
  * v_codes, v_scales, pos; ints rows, block, dtype code: the rows' values) and
  * "decode_attention_int8" (q [B, Hq, Tq, D] with Hq a multiple of H, k_codes,
  * k_scales, v_codes, v_scales, lens[, k_new, v_new]; int block; optional
- * float scale), which attends and appends as "decode_attention" does.
+ * float scale), which attends and appends as "decode_attention" does.  What was
+ * recorded on a cache before it is written, here or by an append that is
+ * recorded, is evaluated first, and an append before the next use is recorded.
  * Returns 0, or -1 with the error set. */
 int32_t applegpu_kv_write_int8(uint64_t k_codes_id, uint64_t k_scales_id, uint64_t v_codes_id, uint64_t v_scales_id,
                                uint64_t k_rows_id, uint64_t v_rows_id, uint64_t pos_id, int64_t block);

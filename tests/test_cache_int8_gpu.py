@@ -522,6 +522,61 @@ def test_many_heads_over_long_rows(gpu, dtype, D):
         _check(out[b:b + 1], O.decode_attention(q[b:b + 1], k, v, [n]), _bar(q[b:b + 1], k, v, D ** -0.5, dtype, Tmax))
 
 
+# ── what was asked for before a write ───────────────────────────────────────
+def _small(gpu, rng):
+    return _upload(gpu, *(x for _ in range(2) for x in _cache(rng, 1, 2, 40, 64, 16)))
+
+
+def test_reads_asked_for_before_a_write_see_what_was_there(gpu):
+    rng = np.random.default_rng(3)
+    dev = _small(gpu, rng)
+    part = [gpu.slice(t, 1, 0, 1) for t in dev]
+    rows = [gpu.from_numpy(rng.standard_normal((1, 2, 8, 64)).astype(np.float32)) for _ in range(2)]
+    q, lens = gpu.from_numpy(rng.standard_normal((1, 2, 1, 64)).astype(np.float32)), gpu.from_numpy(np.array([40], np.int32))
+    zero, ten = (gpu.from_numpy(np.array([n], np.int32)) for n in (0, 10))
+    was = [t.to_numpy() for t in gpu.kv_read_int8(*dev, zero, 40)] + [gpu.decode_attention_int8(q, *dev, lens).to_numpy()]
+    read, view, seen = (gpu.kv_read_int8(*dev, zero, 40), gpu.kv_read_int8(*part, zero, 40),
+                        gpu.decode_attention_int8(q, *dev, lens) + q)
+    gpu.kv_write_int8(*dev, *rows, ten)
+    for a, b in zip(read, was):
+        np.testing.assert_array_equal(a.to_numpy(), b)
+    for a, b in zip(view, was):
+        np.testing.assert_array_equal(a.to_numpy(), b[:, :1])
+    np.testing.assert_array_equal(seen.to_numpy(), was[2] + q.to_numpy())
+    assert (gpu.kv_read_int8(*dev, zero, 40)[0].to_numpy() != was[0]).any()
+    # rows that are made of a read of the cache they are written to
+    want = [t.to_numpy() for t in gpu.kv_read_int8(*dev, ten, 8)]
+    gpu.kv_write_int8(*dev, *(t + t for t in gpu.kv_read_int8(*dev, ten, 8)), zero)
+    for a, b in zip(gpu.kv_read_int8(*dev, zero, 8), want):
+        assert np.abs(a.to_numpy() - 2 * b).max() <= np.abs(2 * b).max() / 254 * 1.001
+
+
+def test_appends_and_reads_keep_the_order_they_were_asked_for(gpu):
+    rng = np.random.default_rng(4)
+    q, *new = (rng.standard_normal((1, 2, 1, 64)).astype(np.float32) * s for s in (1, 1, 1, 9, 9))
+    q, *new = (gpu.from_numpy(a) for a in (q, *new))
+    lens = [gpu.from_numpy(np.array([n], np.int32)) for n in (20, 21)]
+    zero = gpu.from_numpy(np.zeros(1, np.int32))
+    one, two = _small(gpu, np.random.default_rng(5)), _small(gpu, np.random.default_rng(5))
+
+    def steps(dev, now):
+        out = list(gpu.kv_read_int8(*dev, zero, 40))
+        now(out)
+        for i in (0, 1):
+            out.append(gpu.decode_attention_int8(q, *dev, lens[i], k_new=new[2 * i], v_new=new[2 * i + 1]))
+            now(out)
+            out += gpu.kv_read_int8(*dev, zero, 40)
+            now(out)
+        return out
+
+    want = [t.to_numpy() for t in steps(one, lambda out: gpu.eval_many(out))]
+    got = steps(two, lambda out: None)
+    for a, b in zip(reversed(got), reversed(want)):     # the last first
+        np.testing.assert_array_equal(a.to_numpy(), b)
+    for a, b in zip(one, two):
+        np.testing.assert_array_equal(a.to_numpy(), b.to_numpy())
+
+
 # ── refusals ────────────────────────────────────────────────────────────────
 def test_refusals(gpu):
     def cache(B=2, H=2, T=32, D=64, n=2):
