@@ -764,7 +764,9 @@ def decode_attention_int8(q, k_codes, k_scales, v_codes, v_scales, lens, block=1
     """decode_attention over a cache held in 8 bits (kv_write_int8): q [B, Hq,
     Tq, D], the caches' H heads each serving Hq / H query heads in a row; query
     row i of sequence b sees cache rows j <= lens[b] - Tq + i, and a row that
-    sees none gets zeros.  The softmax scale is 1 / sqrt(D) by default.
+    sees none gets zeros.  The softmax scale is 1 / sqrt(D) by default.  Sums
+    are float32's; the weights are rounded to float16 for 16-bit queries, and
+    kept to 2^-22 for float32 ones.
 
     k_new, v_new ([B, H, 1, D], Tq = 1): the step's own K and V rows, appended
     as row lens[b] - 1 when the result is evaluated, before it attends, and at

@@ -87,8 +87,9 @@ def load_model(np_weights: dict, cfg: dict, dtype: str = "float32", kmajor=None,
     as packed rows (gpu.pack_rows_x3), written by their producers.
     weight_bits=4 (fp16/bf16 models) holds every projection weight in 4 bits
     with a scale for each output and `group` inputs (gpu.quantize_int4) and
-    nothing else of it: an eighth to a quarter of the bytes that a decode step
-    reads; the embeddings and the tied head keep 16 bits."""
+    nothing else of it: 0.26 to 0.28 of the projections' bytes; the embeddings
+    and the tied head keep 16 bits.  At GPT-2's sizes a step is bound by its
+    launches, and takes 1.05 to 1.06 times as long."""
     gpu.init_backend()
     if weight_bits not in (4, 16):
         raise ValueError(f"weight_bits must be 4 or 16, got {weight_bits}")
@@ -321,7 +322,10 @@ class KVCache:
 
     bits=8 holds the rows as int8 codes with a float32 scale for each head and
     `block` rows (`gpu.kv_write_int8`; k_scale and v_scale beside k and v):
-    half the memory and, at long contexts, half the time of a 16-bit cache."""
+    half the memory.  A step of GPT-2 large at 512 to 640 positions takes 0.93
+    times as long as with a 16-bit cache for one sequence, 1.06 for eight;
+    contexts past GPT-2's own positions take half the time (70 us against 131
+    for 16 x 20 heads over 8192 rows)."""
 
     def __init__(self, cfg: dict, batch: int, max_len: int, dtype: str = "float16", bits: int = 16, block: int = 16):
         gpu.init_backend()

@@ -37,7 +37,7 @@
 // blocks while these leave CUs idle, and the splits' (O, m, l) are merged.
 // Bound by the read of the codes where contexts are long: 4 x 8 heads of 4
 // queries over up to 32768 rows of 128, 218 MB in 45.7 us (4.8 TB/s) and 5 for
-// the merge; 16 x 20 heads over 8192 rows of 64 73 us, against 131 for a 16-bit
+// the merge; 16 x 20 heads over 8192 rows of 64 70 us, against 131 for a 16-bit
 // cache.  Short contexts are bound by one chain of loads, products and
 // exponentials: 12 heads over 100 rows 5 us.
 #include "kv_int8.hpp"
@@ -131,8 +131,8 @@ struct Step {
 // the context holds it leaves its cache block to the end: two waves append to
 // K and V there (as kv_write_int8 does), before anything else, while the others
 // are at the rows before it, and after a barrier the block's rows are read
-// from the cache like any (8 x 20 heads over 640 rows of 64: 7.6 us without,
-// 10.1 so).
+// from the cache like any (8 x 20 heads over 640 rows of 64: 7.5 us without,
+// 9.9 so, 11.4 with a launch of its own for the append).
 template <typename T, int D, int NW, bool NEW>
 __global__ void __launch_bounds__(64 * NW) decode_int8_mfma(D8Args g) {
   constexpr bool F32 = sizeof(T) == 4;

@@ -99,7 +99,7 @@ __device__ __forceinline__ float act_of(float v, int act) {
 
 // ── few rows: codes straight into the matrix units ─────────────────────────
 // Bound by the codes, N K / 2 bytes, and for small matrices by latency: 16 x
-// 8192 x 8192 (bf16, groups of 64) 13.5 us, 2.6 TB/s of codes and scales; 1 x
+// 8192 x 8192 (bf16, groups of 64) 14.5 us, 2.5 TB/s of codes and scales; 1 x
 // 1280 x 5120 (f16) 4.5 us.
 //  - A wave instruction reads 1 KB of codes in a row and each byte is read
 //    once; UN steps of them are under way before the first is multiplied.
