@@ -578,6 +578,7 @@ void launch_nw(const D8Args& g, hipStream_t s) {
   if (!g.a.kn) hipLaunchKernelGGL((decode_int8_mfma<T, D, NW, false>), grid, dim3(64 * NW), lds_bytes(g.a, NW), s, g);
   else if constexpr (kAppends)
     hipLaunchKernelGGL((decode_int8_mfma<T, D, NW, true>), grid, dim3(64 * NW), lds_bytes(g.a, NW), s, g);
+  else fail("decode_attention_int8: no append in blocks of %d waves", NW);
 }
 
 template <typename T, int D>
@@ -586,6 +587,7 @@ void launch(const D8Args& g, hipStream_t s) {
   if (g.nw == kFew) launch_nw<T, D, kFew>(g, s);
   else if (g.nw == 8) launch_nw<T, D, 8>(g, s);
   else if constexpr (kWide) launch_nw<T, D, 16>(g, s);
+  else fail("decode_attention_int8: no blocks of %d waves", g.nw);
   if (g.splits > 1)
     hipLaunchKernelGGL((decode_int8_merge<T, D>), dim3((unsigned)(g.a.B * g.a.H * g.a.G * g.a.Tq)), dim3(256), 0, s, g);
 }
