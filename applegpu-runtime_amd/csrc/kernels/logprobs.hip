@@ -15,7 +15,7 @@
 // blocks, whose states a second launch merges.  Measured: 2047 x 50257 fp32
 // with 20 alternatives 85 us (4.84 TB/s), in bf16 67 us (bound by its
 // instructions, an exponential and some eight others a value); 8 rows in f16
-// 8 us and 6 for the merge; the gradient in bf16 89 us (4.6 TB/s, read and
+// 8 us and 6 for the merge; the gradient in bf16 86 us (4.8 TB/s, read and
 // written).
 #include "device.hpp"
 
@@ -411,15 +411,43 @@ __global__ void __launch_bounds__(256) token_logprobs_merge(LpArgs g) {
 
 constexpr float kSure = 0.75f;  // (at most one element of a row is past it)
 
+// This thread's share (of 256) of the sum of f(z_i) over the row but for z_j,
+// by 16-byte vectors at 16-byte boundaries.
+template <typename T, typename F>
+__device__ __forceinline__ float sum_of_others(const T* z, int V, int j, F&& f) {
+  constexpr int VE = 16 / (int)sizeof(T), U = 4;
+  const int tid = (int)threadIdx.x, mis = (int)(((uintptr_t)z & 15) / sizeof(T));
+  const int head = mis ? (VE - mis < V ? VE - mis : V) : 0, vecs = (V - head) / VE;
+  float sum = 0.f;
+  if (tid < head && tid != j) sum += f(to_f(z[tid]));
+  for (int i = head + vecs * VE + tid; i < V; i += 256) sum += i != j ? f(to_f(z[i])) : 0.f;
+  const T* at = z + head;
+  for (int v = tid; v < vecs; v += 256 * U) {
+    uint4 raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) raw[u] = *(const uint4*)(at + (int64_t)(v + 256 * u < vecs ? v + 256 * u : v) * VE);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (v + 256 * u >= vecs) break;
+      T e[VE];
+      __builtin_memcpy(e, &raw[u], 16);
+#pragma unroll
+      for (int i = 0; i < VE; ++i) sum += head + (v + 256 * u) * VE + i != j ? f(to_f(e[i])) : 0.f;
+    }
+  }
+  return sum;
+}
+
 // A row to g.splits blocks, 16-byte vectors (VEC: the rows of z and dz are
 // aligned alike) to threads in turn.
 //
 // 1 - p_t and log p + H lose their digits where one element has nearly all of
 // the probability, since lse is known to half its last place only.  So the
-// others' probabilities are summed on the way, and the block that meets an
-// element past kSure adds those of the row's other blocks: with T = sum p_i /
-// p_j, p = 1 / (1 + T), 1 - p = T p and log p = -log1p(T).  2047 x 50257 bf16
-// 89 us with no such row, 102 with half, 125 with all of them.
+// others' probabilities are summed, on the way where the row has one block, else
+// by the block that meets an element past kSure in a second read: with T = sum
+// p_i / p_j, p = 1 / (1 + T), 1 - p = T p and log p = -log1p(T).  2047 x 50257
+// bf16 86 us with no such row, 102 with half, 121 with all of them; 8 rows 5.0
+// and 11.4.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) token_logprobs_grad(LpArgs g, const float* __restrict__ g_lp,
                                                            const float* __restrict__ g_h, T* __restrict__ dz) {
@@ -497,8 +525,7 @@ __global__ void __launch_bounds__(256) token_logprobs_grad(LpArgs g, const float
   __syncthreads();
   const int j = max(max(sure[0], sure[1]), max(sure[2], sure[3]));
   if (j < 0) return;
-  for (int v = tid; v < vecs; v += 256)
-    if ((uint32_t)v / 256 % gy != part_of) each(v, [&](float x, int) { sum += prob(x); });
+  if (gy > 1) sum = sum_of_others(z, V, j, prob);
   sum = wave_sum(sum);
   if (lane == 0) parts[wave] = sum;
   __syncthreads();  // (and the stores to dz before the last one)

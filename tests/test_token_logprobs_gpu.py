@@ -179,7 +179,8 @@ def test_gradients_vs_formula(gpu, dtype, R, V, entropy):
 
 
 @pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
-@pytest.mark.parametrize("V,off", [(2, 0), (40, 0), (1000, 0), (1000, 1), (1000, 1024), (50257, 0), (50257, -64)])
+@pytest.mark.parametrize("V,off", [(2, 0), (40, 0), (1000, 0), (1000, 1), (1000, 1024), (50257, 0), (50257, -64),
+                                   (130001, 0)])
 @pytest.mark.parametrize("view", [False, True])
 def test_gradients_of_nearly_certain_rows_keep_their_digits(gpu, dtype, V, off, view):
     """One word with all but e^-8 .. e^-80 of the probability, and 3/4 and
