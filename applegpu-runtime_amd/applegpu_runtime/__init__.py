@@ -692,6 +692,59 @@ def token_logprobs_backward(grad_logprobs, grad_entropy, logits, tokens, entropy
     return _op(b"token_logprobs_backward", ins + ([_t(grad_entropy)] if grad_entropy is not None else []))
 
 
+def linear_cross_entropy(x, weight, targets):
+    """Softmax cross entropy of the logits x @ weight^T over a vocabulary,
+    which are not kept: for x [..., K], weight [V, K] of one float dtype and
+    targets [...] (int32 or int64), (loss, lse), float32 [...], where lse = log
+    sum exp(logits) and loss = lse - logits[target].  A target outside [0, V)
+    (padding) has loss 0.  A nearly certain word's loss keeps its digits.  A
+    row with a logit of NaN or +inf gives NaN, and so does a float32 row whose
+    x is not finite.
+
+    Products are summed in float32; float32 operands count with 22 bits of
+    each value, by magnitudes of at least 2^-27 of the operand's largest."""
+    return _op(b"linear_cross_entropy", [_t(x), _t(weight), _t(targets)], nout=2)
+
+
+def linear_cross_entropy_backward(grad_loss, x, weight, targets, loss, lse, grad_lse=None):
+    """(dx, dweight), in the operands' dtype, of linear_cross_entropy from the
+    gradients of its loss and lse (float32 [...]; grad_lse may be None) and the
+    loss and lse it returned.  The logits are formed again, in pieces of the
+    vocabulary; their gradient is rounded to 16 bits before its products for
+    16-bit operands.  Rows whose target is outside [0, V) get lse's part only;
+    one without any weight gets zeros whatever its logits are."""
+    ins = [_t(grad_loss), _t(x), _t(weight), _t(targets), _t(loss), _t(lse)]
+    return _op(b"linear_cross_entropy_backward", ins + ([_t(grad_lse)] if grad_lse is not None else []), nout=2)
+
+
+def orthogonalize(g, steps=5, eps=1e-7):
+    """The matrices of g [..., m, n] with their singular values taken towards 1
+    by Newton-Schulz products: X = g / (|g|_F + eps), then `steps` times
+    A = X X^T, X = 3.4445 X + (-4.7750 A + 2.0315 A A) X.  Products are of 11
+    bits of each value for 16-bit matrices, of 22 for float32 ones, with
+    float32 sums; X itself is kept in float32.  A matrix of zeros stays one."""
+    return _op(b"orthogonalize", [_t(g)], f=(float(eps),), i=(int(steps),))
+
+
+def muon_step_(weights, momenta, grads, lr=0.02, beta=0.95, weight_decay=0.0, nesterov=True, steps=5, eps=1e-7):
+    """An optimiser's step with orthogonalised updates, in place, at once, on a
+    matrix [m, n] or a list of matrices of one shape: momentum = beta momentum +
+    grad, U = grad + beta momentum (or the momentum, without nesterov), weight =
+    (1 - lr weight_decay) weight - lr sqrt(max(1, m / n)) orthogonalize(U).
+    Weights and gradients have one float dtype, momenta are float32; all are
+    stored apart.  What was asked of them before the step sees them as they
+    were, also where it is evaluated later."""
+    def ids(t):
+        t = [_t(x)._id for x in (t if isinstance(t, (list, tuple)) else [t])]
+        return len(t), (c_uint64 * len(t))(*t)
+    (n, w), (nm, m), (ng, g) = ids(weights), ids(momenta), ids(grads)
+    if not n == nm == ng:
+        raise ValueError(f"muon_step: {n} weights, {nm} momenta and {ng} gradients")
+    if lib.applegpu_muon_step(w, m, g, n, float(lr), float(beta), float(weight_decay), int(bool(nesterov)), int(steps),
+                              float(eps)) != 0:
+        raise ValueError(ffi_error())
+
+
 def blit_copy(src, dst):
     """dst = src on the device, at once; dst may be a view (a slice of a
     larger tensor, any strides), which is then written in place."""

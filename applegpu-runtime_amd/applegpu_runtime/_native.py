@@ -106,6 +106,8 @@ _SIGS = {
     "applegpu_kv_write": (c_int32, [c_uint64, c_uint64, c_uint64]),
     "applegpu_kv_write_pair": (c_int32, [c_uint64, c_uint64, c_uint64, c_uint64, c_uint64]),
     "applegpu_kv_write_int8": (c_int32, [c_uint64] * 7 + [c_int64]),
+    "applegpu_muon_step": (c_int32, [POINTER(c_uint64)] * 3 + [c_uint32, c_double, c_double, c_double, c_int32, c_int64,
+                                                             c_double]),
     "applegpu_capture_begin": (c_int32, []),
     "applegpu_capture_end": (c_int64, []),
     "applegpu_capture_abort": (c_int32, []),

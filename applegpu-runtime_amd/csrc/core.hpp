@@ -200,6 +200,7 @@ class Runtime {
   size_t memory_usage();
   uint64_t find_by_data_ptr(const void* p);
   void replace(uint64_t id, TensorP t);
+  std::vector<TensorP> pending();        // the registered tensors that wait for their ops
 
   std::recursive_mutex& big_lock() { return big_; }
 

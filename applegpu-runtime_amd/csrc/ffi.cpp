@@ -268,6 +268,13 @@ static TensorP kv_operand(uint64_t id) {
   return t;
 }
 
+static TensorP in_place_operand(const char* name, uint64_t id) {
+  TensorP t = kv_operand(id);
+  if (!t->buf) fail("%s: an operand that is written has no storage", name);
+  if (t->extent_bytes() + (size_t)t->offset > t->buf->requested) fail("%s: a view that is written is out of bounds", name);
+  return t;
+}
+
 static TensorP kv_cache_operand(uint64_t id) {
   TensorP c = kv_operand(id);
   if (!c->buf) fail("kv_write: cache has no storage");
@@ -303,6 +310,28 @@ int32_t applegpu_kv_write_int8(uint64_t k_codes_id, uint64_t k_scales_id, uint64
                         kv_cache_operand(v_scales_id), block};
     eval_cache_uses({c.kc, c.ks, c.vc, c.vs}, false);
     ops::kv_write_int8(c, kr, vr, pos);
+    return 0;
+  });
+}
+
+int32_t applegpu_muon_step(const uint64_t* weight_ids, const uint64_t* momentum_ids, const uint64_t* grad_ids, uint32_t n,
+                           double lr, double beta, double weight_decay, int32_t nesterov, int64_t steps, double eps) {
+  return guarded<int32_t>(kFfi, -1, [&]() -> int32_t {
+    if (n > 0 && (!weight_ids || !momentum_ids || !grad_ids)) fail("muon_step: null id array");
+    std::vector<TensorP> w, m, g, written;
+    for (uint32_t i = 0; i < n; ++i) {
+      g.push_back(kv_operand(grad_ids[i]));
+      w.push_back(in_place_operand("muon_step", weight_ids[i]));
+      m.push_back(in_place_operand("muon_step", momentum_ids[i]));
+      written.push_back(w.back());
+      written.push_back(m.back());
+    }
+    eval_uses(written);
+    ops::MuonStep o;
+    o.lr = lr; o.beta = beta; o.decay = weight_decay; o.eps = eps;
+    o.nesterov = nesterov != 0;
+    o.steps = steps;
+    ops::muon_step_(w, m, g, o);
     return 0;
   });
 }

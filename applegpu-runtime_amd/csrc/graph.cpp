@@ -38,6 +38,7 @@ enum Op : int {
   OP_LINEAR_RELU_MSE_BACKWARD_SGD, OP_ATTENTION_BACKWARD, OP_LAYER_NORM_STATS,
   OP_KV_READ_INT8, OP_DECODE_ATTENTION_INT8, OP_QUANTIZE_INT4, OP_DEQUANTIZE_INT4, OP_LINEAR_INT4,
   OP_TOKEN_LOGPROBS, OP_TOKEN_LOGPROBS_BACKWARD,
+  OP_LINEAR_CROSS_ENTROPY, OP_LINEAR_CROSS_ENTROPY_BACKWARD, OP_ORTHOGONALIZE,
   OP_COUNT
 };
 
@@ -62,6 +63,7 @@ static const char* kNames[OP_COUNT] = {
     "linear_relu_mse_backward_sgd_", "attention_backward", "layer_norm_stats",
     "kv_read_int8", "decode_attention_int8", "quantize_int4", "dequantize_int4", "linear_int4",
     "token_logprobs", "token_logprobs_backward",
+    "linear_cross_entropy", "linear_cross_entropy_backward", "orthogonalize",
 };
 
 int op_code(const char* name) {
@@ -82,7 +84,8 @@ const char* op_name(int code) { return code >= 0 && code < OP_COUNT ? kNames[cod
 int op_outputs(int code) {
   if (code == OP_LAYER_NORM_GRADS || code == OP_ATTENTION_BACKWARD || code == OP_LAYER_NORM_STATS) return 3;
   if (code == OP_TOKEN_LOGPROBS) return 3;  // 5 with alternatives
-  return code == OP_QUANTIZE_PER_ROW || code == OP_MSE_LOSS_GRAD || code == OP_KV_READ_INT8 || code == OP_QUANTIZE_INT4
+  return code == OP_QUANTIZE_PER_ROW || code == OP_MSE_LOSS_GRAD || code == OP_KV_READ_INT8 || code == OP_QUANTIZE_INT4 ||
+                 code == OP_LINEAR_CROSS_ENTROPY || code == OP_LINEAR_CROSS_ENTROPY_BACKWARD
              ? 2 : 1;
 }
 
@@ -270,6 +273,15 @@ std::vector<TensorP> run_op(int code, const std::vector<TensorP>& in, const std:
       // (grad_logprobs, logits, tokens, entropy, lse[, grad_entropy])
       if (in.size() != 6) need(in, 5, code);
       return {token_logprobs_backward(in[0], in.size() == 6 ? in[5] : nullptr, in[1], in[2], in[3], in[4])};
+    case OP_LINEAR_CROSS_ENTROPY: need(in, 3, code); return linear_cross_entropy(in[0], in[1], in[2]);
+    case OP_LINEAR_CROSS_ENTROPY_BACKWARD:
+      // (grad_loss, x, weight, targets, loss, lse[, grad_lse])
+      if (in.size() != 7) need(in, 6, code);
+      return linear_cross_entropy_backward(in[0], in.size() == 7 ? in[6] : nullptr, in[1], in[2], in[3], in[4], in[5]);
+    case OP_ORTHOGONALIZE:
+      // (g); iv: steps; f: eps
+      need(in, 1, code);
+      return {orthogonalize(in[0], iv.empty() ? 5 : iv[0], f.empty() ? 1e-7f : (float)f[0])};
     case OP_PACK_WEIGHT: need(in, 1, code); return {pack_weight(in[0])};
     case OP_PACK_WEIGHT_X3: need(in, 1, code); return {pack_weight_x3(in[0])};
     case OP_MATMUL_PACKED: need(in, 2, code); return {matmul_packed(in[0], in[1], ip(iv, 0, code))};
@@ -376,6 +388,37 @@ void eval_cache_uses(const std::vector<TensorP>& cache, bool appends_only) {
   }
   g_cache_uses.resize(kept);
   eval_all(before);
+}
+
+void eval_uses(const std::vector<TensorP>& written) {
+  std::unordered_set<const Buffer*> bufs;
+  for (const TensorP& t : written) bufs.insert(t->buf.get());
+  std::unordered_map<const Node*, bool> seen;  // whether a node's values come from one of them
+  std::vector<TensorP> roots;
+  for (const TensorP& t : Runtime::get().pending()) {
+    // a walk without recursion: a recorded chain can be long
+    std::vector<std::pair<const Node*, size_t>> todo{{t->node.get(), 0}};
+    while (!todo.empty()) {
+      const Node* n = todo.back().first;
+      if (todo.back().second == 0) seen.emplace(n, false);
+      if (todo.back().second == n->in.size()) {
+        todo.pop_back();
+        if (!todo.empty() && seen[n]) seen[todo.back().first] = true;
+        continue;
+      }
+      const TensorP& x = n->in[todo.back().second++];
+      if (!x) continue;
+      if (!x->pending()) {
+        if (bufs.count(x->buf.get())) seen[n] = true;
+      } else {
+        auto it = seen.find(x->node.get());
+        if (it == seen.end()) todo.push_back({x->node.get(), 0});
+        else if (it->second) seen[n] = true;
+      }
+    }
+    if (seen[t->node.get()]) roots.push_back(t);
+  }
+  if (!roots.empty()) eval_all(roots);
 }
 
 std::vector<TensorP> record_op(int code, const std::vector<TensorP>& in, const std::vector<double>& f,

@@ -51,6 +51,10 @@ std::vector<TensorP> record_op(int code, const std::vector<TensorP>& in, const s
 // or with appends_only what also writes it.
 void eval_cache_uses(const std::vector<TensorP>& cache, bool appends_only);
 
+// Runs what was recorded and reads the storage of one of these tensors, which
+// are about to be written in place.
+void eval_uses(const std::vector<TensorP>& written);
+
 // Materialise a pending tensor (no-op when it already has storage).
 void eval(const TensorP& t);
 // Materialise several pending tensors with one fusion plan over all their

@@ -597,6 +597,53 @@ void token_logprobs(const TokenLogprobs& a, void* ws, hipStream_t s);
 // p from the logits and lse; g_H may be null.  dz contiguous [R, V].
 void token_logprobs_backward(const TokenLogprobs& a, const float* g_lp, const float* g_H, void* dz, hipStream_t s);
 
+// ── cross entropy of a linear layer over a vocabulary ─────────────────────
+// z = x w^T for x [R, K] (row stride ldx) and w [V, K] (ldw): lse[r] = log sum
+// exp z[r], loss[r] = lse[r] - z[r][t_r], 0 where t_r is outside [0, V).
+struct LinearCE {
+  DType dt = DType::F32;
+  int64_t R = 0, K = 0, V = 0;
+  const void* x = nullptr; int64_t ldx = 0;
+  const void* w = nullptr; int64_t ldw = 0;
+  DType idx_dt = DType::I32;
+  const void* targets = nullptr;
+  float* loss = nullptr; float* lse = nullptr;  // outputs; inputs of the gradient
+  const float* g_loss = nullptr; const float* g_lse = nullptr;  // g_lse may be null
+  void* dx = nullptr; void* dw = nullptr;       // contiguous, of dtype dt
+};
+constexpr int64_t kLinearCEFeatures = (int64_t)1 << 19;  // K
+constexpr int64_t kLinearCEWords = (int64_t)1 << 30;     // V
+size_t linear_ce_ws_bytes(const LinearCE& a, int cus);
+void linear_ce(const LinearCE& a, void* ws, int cus, hipStream_t s);
+// d = g_loss (p - [v = t]) + g_lse p with p = exp(z - lse); dx = d w, dw = d^T x.
+size_t linear_ce_backward_ws_bytes(const LinearCE& a, int cus);
+void linear_ce_backward(const LinearCE& a, void* ws, int cus, hipStream_t s);
+
+// ── orthogonalised updates ────────────────────────────────────────────────
+// Newton-Schulz on `count` matrices [m, n] at once: X = U / (|U|_F + eps),
+// then `steps` times A = X X^T (of the shorter side), X = a X + (b A + c A A) X
+// with (a, b, c) = (3.4445, -4.7750, 2.0315).  Without momentum U = in and out
+// = X.  With it, in place: mom = beta mom + in, U = in + beta mom (nesterov) or
+// mom, out = keep out - rate X.  Matrix i is at ptr[i], or with `apart` > 0 at
+// ptr[0] plus i * apart values.
+constexpr int kOrthoMats = 32;
+struct Mats {
+  void* p[kOrthoMats] = {};
+  int64_t apart = 0;
+};
+struct Orthogonalize {
+  DType dt = DType::F32;
+  int64_t count = 0, m = 0, n = 0;
+  int steps = 5;
+  float eps = 1e-7f;
+  Mats in, out, mom;  // mom: fp32
+  bool momentum = false, nesterov = true;
+  float beta = 0.f, keep = 1.f, rate = 1.f;
+};
+constexpr int64_t kOrthoSide = (int64_t)1 << 19;  // m, n
+size_t orthogonalize_ws_bytes(const Orthogonalize& a, int cus);
+void orthogonalize(const Orthogonalize& a, void* ws, int cus, hipStream_t s);
+
 // o = x elementwise with dtype conversion, o written through the strides of
 // `so` (shape and destination strides) and x read through `sx`.
 void copy_strided(DType in, DType out, const void* x, const ND& sx, void* o, const ND& so, hipStream_t s);

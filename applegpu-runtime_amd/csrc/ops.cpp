@@ -15,6 +15,7 @@
 #include "ops.hpp"
 #include "graph.hpp"
 
+#include <algorithm>
 #include <cmath>
 
 namespace agpu {
@@ -2304,6 +2305,192 @@ TensorP token_logprobs_backward(const TensorP& g_lp, const TensorP& g_H, const T
   TensorP out = alloc_out(logits->dtype, logits->dims());
   LAUNCH k::token_logprobs_backward(a, gl, gh, out->data(), rt().stream());
   return out;
+}
+
+// ── cross entropy of a linear layer over a vocabulary ──────────────────────
+// The checked operands: rows with a unit stride along their features.
+static k::LinearCE ce_operands(const char* name, const TensorP& x, const TensorP& w, const TensorP& targets,
+                               TensorP (&keep)[3], std::vector<int64_t>* lead) {
+  check_dtype(name, kFloatOnly, x->dtype);
+  if (w->dtype != x->dtype) fail("Dtype mismatch: %s vs %s", dtype_name(x->dtype), dtype_name(w->dtype));
+  if (x->ndim < 1 || w->ndim != 2 || w->shape[1] != x->shape[x->ndim - 1])
+    fail("%s: x %s does not match weight %s ([..., in] and [words, in])", name, shape_str(x->dims()).c_str(),
+         shape_str(w->dims()).c_str());
+  if (targets->dtype != DType::I32 && targets->dtype != DType::I64)
+    fail("%s: targets must be int32 or int64, got %s", name, dtype_name(targets->dtype));
+  k::LinearCE a;
+  a.dt = x->dtype;
+  a.V = w->shape[0];
+  a.K = w->shape[1];
+  if (a.V < 1 || a.V > k::kLinearCEWords) fail("%s: %lld words", name, (long long)a.V);
+  if (a.K < 1 || a.K >= k::kLinearCEFeatures) fail("%s: %lld features", name, (long long)a.K);
+  *lead = x->dims();
+  lead->pop_back();
+  if (lead->empty()) *lead = {1};
+  a.R = x->numel() / a.K;
+  if (targets->numel() != a.R || (x->ndim > 1 && targets->dims() != *lead))
+    fail("%s: targets %s do not match x %s", name, shape_str(targets->dims()).c_str(), shape_str(x->dims()).c_str());
+  auto rows = [&](const TensorP& t, TensorP* kept, int64_t* ld) {
+    int64_t r;
+    *kept = t;
+    if (!as_rows(*t, &r, ld)) {
+      *kept = contiguous(t);
+      *ld = a.K;
+    }
+    return (const void*)(*kept)->data();
+  };
+  a.x = rows(x, &keep[0], &a.ldx);
+  a.w = rows(w, &keep[1], &a.ldw);
+  keep[2] = contiguous(targets);
+  a.idx_dt = targets->dtype;
+  a.targets = keep[2]->data();
+  return a;
+}
+
+std::vector<TensorP> linear_cross_entropy(const TensorP& x, const TensorP& weight, const TensorP& targets) {
+  TensorP keep[3];
+  std::vector<int64_t> lead;
+  k::LinearCE a = ce_operands("linear_cross_entropy", x, weight, targets, keep, &lead);
+  TensorP loss = alloc_out(DType::F32, lead), lse = alloc_out(DType::F32, lead);
+  if (a.R == 0 || meta_mode()) return {loss, lse};
+  a.loss = (float*)loss->data();
+  a.lse = (float*)lse->data();
+  const int cus = rt().info().cu_count;
+  BufferP ws = scratch(k::linear_ce_ws_bytes(a, cus));
+  k::linear_ce(a, ws->ptr, cus, rt().stream());
+  return {loss, lse};
+}
+
+std::vector<TensorP> linear_cross_entropy_backward(const TensorP& g_loss, const TensorP& g_lse, const TensorP& x,
+                                                   const TensorP& weight, const TensorP& targets, const TensorP& loss,
+                                                   const TensorP& lse) {
+  const char* name = "linear_cross_entropy_backward";
+  TensorP keep[3];
+  std::vector<int64_t> lead;
+  k::LinearCE a = ce_operands(name, x, weight, targets, keep, &lead);
+  std::vector<TensorP> rows;
+  auto row = [&](const char* what, const TensorP& t) -> float* {
+    if (t->dtype != DType::F32 || t->numel() != a.R)
+      fail("%s: %s must be float32 with one value a row (%lld), got %s %s", name, what, (long long)a.R,
+           dtype_name(t->dtype), shape_str(t->dims()).c_str());
+    rows.push_back(contiguous(t));
+    return (float*)rows.back()->data();
+  };
+  a.g_loss = row("grad_loss", g_loss);
+  a.g_lse = g_lse ? row("grad_lse", g_lse) : nullptr;
+  a.loss = row("loss", loss);
+  a.lse = row("lse", lse);
+  if (a.R == 0) return {alloc_out(x->dtype, x->dims()), full(x->dtype, weight->dims(), 0.f)};
+  TensorP dx = alloc_out(x->dtype, x->dims()), dw = alloc_out(x->dtype, weight->dims());
+  if (meta_mode()) return {dx, dw};
+  a.dx = dx->data();
+  a.dw = dw->data();
+  const int cus = rt().info().cu_count;
+  BufferP ws = scratch(k::linear_ce_backward_ws_bytes(a, cus));
+  k::linear_ce_backward(a, ws->ptr, cus, rt().stream());
+  return {dx, dw};
+}
+
+// ── orthogonalised updates ─────────────────────────────────────────────────
+static void check_ortho(const char* name, int64_t m, int64_t n, int64_t steps, double eps) {
+  if (steps < 1 || steps > 100) fail("%s: %lld steps (1 to 100)", name, (long long)steps);
+  if (!(eps >= 0.0) || std::isinf(eps)) fail("%s: eps must be a number that is not negative", name);
+  if (m >= k::kOrthoSide || n >= k::kOrthoSide) fail("%s: matrices of %lld x %lld", name, (long long)m, (long long)n);
+}
+// Matrices at once: as many as 4 GB of workspace hold, one at least.
+static int64_t ortho_group(k::Orthogonalize a, int64_t most) {
+  a.count = 1;
+  const size_t each = k::orthogonalize_ws_bytes(a, rt().info().cu_count);
+  return std::max<int64_t>(1, std::min<int64_t>({most, (int64_t)(((size_t)4 << 30) / each), 65535}));
+}
+
+TensorP orthogonalize(const TensorP& g, int64_t steps, float eps) {
+  const char* name = "orthogonalize";
+  check_dtype(name, kFloatOnly, g->dtype);
+  if (g->ndim < 2) fail("%s requires at least 2D input, got %s", name, shape_str(g->dims()).c_str());
+  k::Orthogonalize a;
+  a.dt = g->dtype;
+  a.m = g->shape[g->ndim - 2];
+  a.n = g->shape[g->ndim - 1];
+  check_ortho(name, a.m, a.n, steps, eps);
+  TensorP c = contiguous(g), out = alloc_out(g->dtype, g->dims());
+  if (meta_mode() || g->numel() == 0) return out;
+  a.steps = (int)steps;
+  a.eps = eps;
+  a.in.apart = a.out.apart = a.m * a.n;
+  const int64_t all = g->numel() / a.in.apart, each = ortho_group(a, all);
+  a.count = each;
+  BufferP ws = scratch(k::orthogonalize_ws_bytes(a, rt().info().cu_count));
+  for (int64_t i = 0; i < all; i += each) {
+    a.count = std::min(each, all - i);
+    const size_t at = (size_t)(i * a.in.apart) * dtype_size(g->dtype);
+    a.in.p[0] = c->data() + at;
+    a.out.p[0] = out->data() + at;
+    k::orthogonalize(a, ws->ptr, rt().info().cu_count, rt().stream());
+  }
+  return out;
+}
+
+void muon_step_(const std::vector<TensorP>& w, const std::vector<TensorP>& mom, const std::vector<TensorP>& grad,
+                const MuonStep& o) {
+  const char* name = "muon_step";
+  if (w.size() != mom.size() || w.size() != grad.size())
+    fail("%s: %zu weights, %zu momenta and %zu gradients", name, w.size(), mom.size(), grad.size());
+  if (w.empty()) return;
+  for (double v : {o.lr, o.beta, o.decay})
+    if (!std::isfinite(v)) fail("%s: lr, beta and weight_decay must be finite", name);
+  k::Orthogonalize a;
+  a.dt = w[0]->dtype;
+  check_dtype(name, kFloatOnly, a.dt);
+  struct Span { const char *lo, *hi; bool written; };
+  std::vector<Span> spans;
+  std::vector<TensorP> gc;
+  for (size_t i = 0; i < w.size(); ++i) {
+    if (w[i]->ndim != 2 || w[i]->dims() != w[0]->dims() || mom[i]->dims() != w[0]->dims() ||
+        grad[i]->dims() != w[0]->dims())
+      fail("%s: weight %s, momentum %s and gradient %s must be matrices of one shape, %s", name,
+           shape_str(w[i]->dims()).c_str(), shape_str(mom[i]->dims()).c_str(), shape_str(grad[i]->dims()).c_str(),
+           shape_str(w[0]->dims()).c_str());
+    if (w[i]->dtype != a.dt || grad[i]->dtype != a.dt)
+      fail("Dtype mismatch: %s vs %s", dtype_name(a.dt), dtype_name(w[i]->dtype != a.dt ? w[i]->dtype : grad[i]->dtype));
+    if (mom[i]->dtype != DType::F32) fail("%s: the momentum must be float32, got %s", name, dtype_name(mom[i]->dtype));
+    if (!w[i]->is_contiguous() || !mom[i]->is_contiguous())
+      fail("%s: weights and momenta are written in place and must be contiguous", name);
+    gc.push_back(contiguous(grad[i]));
+    for (const TensorP& t : {w[i], mom[i]}) spans.push_back({t->data(), t->data() + t->nbytes(), true});
+    if (gc.back() == grad[i]) spans.push_back({grad[i]->data(), grad[i]->data() + grad[i]->nbytes(), false});
+  }
+  a.m = w[0]->shape[0];
+  a.n = w[0]->shape[1];
+  check_ortho(name, a.m, a.n, o.steps, o.eps);
+  if (w[0]->numel() == 0) return;
+  // what is written may be neither written twice nor read as a gradient
+  std::sort(spans.begin(), spans.end(), [](const Span& x, const Span& y) { return x.lo < y.lo; });
+  const char *end = nullptr, *written_end = nullptr;
+  for (const Span& s : spans) {
+    if (s.lo < written_end || (s.written && s.lo < end)) fail("%s: weights, momenta and gradients share storage", name);
+    end = std::max(end, s.hi);
+    if (s.written) written_end = std::max(written_end, s.hi);
+  }
+  a.steps = (int)o.steps;
+  a.eps = (float)o.eps;
+  a.momentum = true;
+  a.nesterov = o.nesterov;
+  a.beta = (float)o.beta;
+  a.keep = (float)(1.0 - o.lr * o.decay);
+  a.rate = (float)(o.lr * std::sqrt(std::max(1.0, (double)a.m / (double)a.n)));
+  const int64_t all = (int64_t)w.size(), each = ortho_group(a, std::min<int64_t>(all, k::kOrthoMats));
+  a.count = each;
+  BufferP ws = scratch(k::orthogonalize_ws_bytes(a, rt().info().cu_count));
+  for (int64_t i = 0; i < all; i += each) {
+    a.count = std::min(each, all - i);
+    for (int64_t j = 0; j < a.count; ++j) {
+      a.in.p[j] = gc[i + j]->data();
+      a.out.p[j] = w[i + j]->data();
+      a.mom.p[j] = mom[i + j]->data();
+    }
+    k::orthogonalize(a, ws->ptr, rt().info().cu_count, rt().stream());
+  }
 }
 
 }  // namespace ops

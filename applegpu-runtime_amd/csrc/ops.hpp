@@ -306,5 +306,26 @@ std::vector<TensorP> token_logprobs(const TensorP& logits, const TensorP& tokens
 TensorP token_logprobs_backward(const TensorP& g_lp, const TensorP& g_H, const TensorP& logits, const TensorP& tokens,
                                 const TensorP& entropy, const TensorP& lse);
 
+// ── training ───────────────────────────────────────────────────────────────
+// {loss, lse}, fp32 [...], of logits x weight^T for x [..., K], weight [V, K]
+// and int32/int64 targets [...]; the logits are not kept.
+std::vector<TensorP> linear_cross_entropy(const TensorP& x, const TensorP& weight, const TensorP& targets);
+// {dx, dweight} of the loss and lse (g_lse may be null).
+std::vector<TensorP> linear_cross_entropy_backward(const TensorP& g_loss, const TensorP& g_lse, const TensorP& x,
+                                                   const TensorP& weight, const TensorP& targets, const TensorP& loss,
+                                                   const TensorP& lse);
+// The matrices of g [..., m, n] orthogonalised by Newton-Schulz products.
+TensorP orthogonalize(const TensorP& g, int64_t steps, float eps);
+// In place: mom = beta mom + grad, then w = (1 - lr decay) w - lr sqrt(max(1,
+// m / n)) orthogonalize(U), U = grad + beta mom (nesterov) or mom, for matrices
+// [m, n] of one shape; mom fp32.
+struct MuonStep {
+  double lr = 0.02, beta = 0.95, decay = 0.0, eps = 1e-7;
+  bool nesterov = true;
+  int64_t steps = 5;
+};
+void muon_step_(const std::vector<TensorP>& w, const std::vector<TensorP>& mom, const std::vector<TensorP>& grad,
+                const MuonStep& o);
+
 }  // namespace ops
 }  // namespace agpu

@@ -496,6 +496,14 @@ void Runtime::replace(uint64_t id, TensorP t) {
   tensors_[id] = std::move(t);
 }
 
+std::vector<TensorP> Runtime::pending() {
+  std::lock_guard<std::mutex> g(reg_mu_);
+  std::vector<TensorP> r;
+  for (const auto& e : tensors_)
+    if (e.second->pending()) r.push_back(e.second);
+  return r;
+}
+
 bool Runtime::erase(uint64_t id) {
   TensorP keep;  // destroyed outside the registry lock
   std::lock_guard<std::mutex> g(reg_mu_);

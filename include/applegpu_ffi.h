@@ -273,6 +273,26 @@ int32_t applegpu_kv_write_int8(uint64_t k_codes_id, uint64_t k_scales_id, uint64
  *   "token_logprobs_backward" (grad_logprobs, logits, tokens, entropy, lse[,
  *     grad_entropy]): the gradient of the logits in their dtype. */
 
+/* Lazy ops (applegpu_graph_op) for training a language model; inputs, then
+ * parameters.
+ *   "linear_cross_entropy" (x [..., K], weight [V, K], targets [...] int32 or
+ *     int64): loss and lse, float32 [...], of the logits x weight^T, which are
+ *     not kept; a target outside [0, V) has loss 0.
+ *   "linear_cross_entropy_backward" (grad_loss, x, weight, targets, loss, lse[,
+ *     grad_lse]): the gradients of x and weight in their dtype.
+ *   "orthogonalize" (g [..., m, n]; int steps, default 5; float eps, default
+ *     1e-7): X = g / (|g| + eps), then steps times A = X X^T,
+ *     X = a X + (b A + c A A) X, (a, b, c) = (3.4445, -4.7750, 2.0315). */
+
+/* In place, for n matrices of one shape [rows, cols] (weights and gradients of
+ * one float dtype, momenta float32, all stored apart): momentum = beta momentum
+ * + grad, U = grad + beta momentum (nesterov) or momentum, weight = (1 - lr
+ * weight_decay) weight - lr sqrt(max(1, rows / cols)) orthogonalize(U).  What
+ * was recorded on the weights or momenta is evaluated first.  Returns 0, or -1
+ * with the error set. */
+int32_t applegpu_muon_step(const uint64_t* weight_ids, const uint64_t* momentum_ids, const uint64_t* grad_ids, uint32_t n,
+                           double lr, double beta, double weight_decay, int32_t nesterov, int64_t steps, double eps);
+
 int32_t applegpu_capture_begin(void);
 int64_t applegpu_capture_end(void);
 int32_t applegpu_capture_abort(void);
