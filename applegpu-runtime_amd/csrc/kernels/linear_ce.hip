@@ -34,10 +34,12 @@ constexpr float kInf = __builtin_inff();
 
 __device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 
-// A maximum and the sum of exponentials below it; no term: {-inf, 0}.
+// A sum of exponentials as {c, s}: s 2^c, c the largest exponent; no term:
+// {-inf, 0}.  An exponent is z log2(e) - c in one fused operation, whatever c
+// was rounded to.
 __device__ __forceinline__ float2 join(float2 a, float2 b) {
   const float m = fmaxf(a.x, b.x), ref = m == -kInf ? 0.f : m;
-  return make_float2(m, a.y * exp_fast(a.x - ref) + b.y * exp_fast(b.x - ref));
+  return make_float2(m, a.y * __builtin_amdgcn_exp2f(a.x - ref) + b.y * __builtin_amdgcn_exp2f(b.x - ref));
 }
 
 // ── powers of two that bring values into fp16's range ─────────────────────
@@ -130,18 +132,18 @@ __device__ __forceinline__ int64_t target_of(const void* t, bool wide, int64_t r
   return v >= 0 && v < V ? v : -1;
 }
 
-// Of each row of the tile: {maximum, sum of exponentials} of the logits but
-// the target's, and the target's logit.
+// Of each row of the tile: the sum of exponentials of the logits but the
+// target's, and the target's logit.
 struct EpiLoss {
   float2* part;  // [tiles_n][R]
   float* zt;
   const void* targets;
   bool wide;
   const float2 *px, *pw;  // fp32: the operands' powers
+  // the accumulators' first registers take a row's {c, s}
   template <class TL>
-  __device__ void store(const Args& p, const Place& c, typename TL::T* lds, typename TL::Acc& acc) const {
+  __device__ __forceinline__ void form(const Args& p, const Place& c, typename TL::Acc& acc) const {
     constexpr int TM = TL::TM, TN = TL::TN;
-    float2* pair = (float2*)lds;  // [BM][WN]
     float ux = 1.f, uw = 1.f;
     if constexpr (TL::PL == 2) { ux = px->y; uw = pw->y; }
     const int64_t cols = c.n0 + c.wn * 32 * TN;
@@ -183,14 +185,23 @@ struct EpiLoss {
 #pragma unroll
       for (int e = 1; e < TN * 16; ++e) m = fmaxf(m, z[e]);
       m = fmaxf(m, __shfl_xor(m, 32));
-      // (a NaN is no maximum but makes the sum NaN)
+      // (a NaN is no maximum but makes the sum NaN, and so does +inf)
+      m = m > -kInf ? m * kLog2e : -kInf;
       const float ref = m > -kInf ? m : 0.f;
       float s = 0.f;
 #pragma unroll
-      for (int e = 0; e < TN * 16; ++e) s += exp_fast(z[e] - ref);
+      for (int e = 0; e < TN * 16; ++e) s += __builtin_amdgcn_exp2f(fmaf(z[e], kLog2e, -ref));
       s += __shfl_xor(s, 32);
-      if (hi == 0) pair[TL::row_of(c, i) * TL::WN + c.wn] = make_float2(m > -kInf ? m : -kInf, s);
+      acc[i][0][0] = m;
+      acc[i][0][1] = s;
     }
+  }
+  template <class TL>
+  __device__ __forceinline__ void store(const Args& p, const Place& c, typename TL::T* lds, typename TL::Acc& acc) const {
+    float2* pair = (float2*)(lds + TL::STAGE);  // [BM][WN]
+#pragma unroll
+    for (int i = 0; i < TL::TM; ++i)
+      if (c.lane < 32) pair[TL::row_of(c, i) * TL::WN + c.wn] = make_float2(acc[i][0][0], acc[i][0][1]);
     __syncthreads();
     for (int r = threadIdx.x; r < TL::BM; r += 64 * TL::NW) {
       if (c.m0 + r >= p.M) break;
@@ -218,19 +229,20 @@ __global__ void __launch_bounds__(256) loss_kernel(const float2* part, int64_t p
     if (y < h) red[threadIdx.x] = a = join(a, red[threadIdx.x + h * rx]);
   }
   if (y != 0 || row >= R) return;
+  constexpr float kLn2 = 0.69314718055994531f;
   float out = 0.f, sum;
   if (target_of(targets, wide, row, V) < 0) {
-    sum = a.x + logf(a.y);
+    sum = (a.x + log2f(a.y)) * kLn2;
   } else {
     // log(exp z_t + the others), from the larger of the two
-    const float z = zt[row];
-    if (z >= a.x) {
-      out = log1pf(a.y * expf(a.x - z));
+    const float z = zt[row], q = z * kLog2e;
+    if (q >= a.x) {
+      out = log1pf(a.y * exp2f(fmaf(-z, kLog2e, a.x)));
       sum = z + out;
     } else {
-      const float others = logf(a.y + expf(z - a.x));
-      out = (a.x - z) + others;
-      sum = a.x + others;
+      const float others = log2f(a.y + exp2f(fmaf(z, kLog2e, -a.x)));
+      out = (fmaf(-z, kLog2e, a.x) + others) * kLn2;
+      sum = (a.x + others) * kLn2;
     }
   }
   loss[row] = out;
@@ -239,7 +251,8 @@ __global__ void __launch_bounds__(256) loss_kernel(const float2* part, int64_t p
 
 // ── backward ──────────────────────────────────────────────────────────────
 // d of the tile's logits, times the power of the rows' gradients; zeros behind
-// the words up to the row's end.
+// the words up to the row's end.  Formed where the accumulators are, from the
+// few rows that a lane has.
 template <typename T>
 struct EpiGrad {
   T* d;
@@ -250,31 +263,72 @@ struct EpiGrad {
   const float *loss, *lse, *g, *h;
   const float2 *px, *pw, *pg;
   template <class TL>
-  __device__ void store(const Args& p, const Place& c, typename TL::T* lds, typename TL::Acc& acc) const {
-    constexpr int PL = TL::PL;
+  __device__ __forceinline__ void form(const Args& p, const Place& c, typename TL::Acc& acc) const {
+    constexpr int PL = TL::PL, TM = TL::TM, TN = TL::TN;
     float ux = 1.f, uw = 1.f, up = 1.f;
     if constexpr (PL == 2) { ux = px->y; uw = pw->y; }
     if (pg) up = pg->x;
+    const int64_t cols = c.n0 + c.wn * 32 * TN;
+    const bool ragged = cols + 32 * TN > p.N;
+    const int hi = c.lane >> 5;
+    float l[TM], all[TM], gr[TM], hr[TM];
+    int rel[TM];
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      const int64_t row = c.m0 + TL::row_of(c, i), at = row < p.M ? row : p.M - 1;
+      const int64_t t = row < p.M ? target_of(targets, wide, at, V) : -1, far = t - v0 - cols;
+      gr[i] = t >= 0 ? g[at] : 0.f;
+      hr[i] = h ? h[at] : 0.f;
+      all[i] = (gr[i] + hr[i]) * up;
+      l[i] = lse[at];
+      rel[i] = t >= 0 && far >= 0 && far < 32 * TN && ((far >> 2) & 1) == hi ? (int)far - 4 * hi : -1;
+    }
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      // a row without weight has no gradient, whatever its logits are
+      const bool none = gr[i] == 0.f && hr[i] == 0.f;
+      float zt = 0.f;
+      if (rel[i] >= 0) {
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (rel[i] == j * 32 + 8 * (e >> 2) + (e & 3)) zt = acc[i][j][e];
+        if constexpr (PL == 2) zt = zt * ux * uw;
+      }
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float z = acc[i][j][e];
+          if constexpr (PL == 2) z = z * ux * uw;
+          acc[i][j][e] = none ? 0.f : exp_fast(z - l[i]) * all[i];
+        }
+      // p - 1 of the target from its loss, which keeps the digits of 1 - p
+      if (rel[i] >= 0 && !none) {
+        const float dt = (gr[i] * expm1f(-loss[c.m0 + TL::row_of(c, i)]) + hr[i] * exp_fast(zt - l[i])) * up;
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (rel[i] == j * 32 + 8 * (e >> 2) + (e & 3)) acc[i][j][e] = dt;
+      }
+      if (ragged) {
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (c.n0 + TL::col_of(c, j, e) >= p.N) acc[i][j][e] = 0.f;
+      }
+    }
+  }
+  template <class TL>
+  __device__ __forceinline__ void store(const Args& p, const Place& c, typename TL::T* lds, typename TL::Acc& acc) const {
+    constexpr int PL = TL::PL;
     TL::template runs<false>(
         c, lds, acc, false,
-        [&](int64_t row, int64_t col, float (&z)[8]) {
-          if (row >= p.M || col * PL >= ldd) return;
-          const int64_t t = target_of(targets, wide, row, V) - v0;  // (below 0: none here)
-          const bool there = target_of(targets, wide, row, V) >= 0;
-          const float gr = there ? g[row] : 0.f, hr = h ? h[row] : 0.f, all = gr + hr, l = lse[row];
-          float v[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            float q = z[e];
-            if constexpr (PL == 2) q = q * ux * uw;
-            const float pr = exp_fast(q - l);
-            float dv = pr * all;
-            // p - 1 of the target from its loss, which keeps the digits of 1 - p
-            if (there && col + e == t) dv = gr * expm1f(-loss[row]) + hr * pr;
-            // a row without weight has no gradient, whatever its logits are
-            v[e] = col + e < p.N && (gr != 0.f || hr != 0.f) ? dv * up : 0.f;
-          }
-          put_planes<T, PL>(d + row * ldd, col, v);
+        [&](int64_t row, int64_t col, float (&v)[8]) {
+          if (row < p.M && col * PL < ldd) put_planes<T, PL, true>(d + row * ldd, col, v);
         },
         [](int64_t, int64_t, float (&)[8]) {});
   }
@@ -288,7 +342,9 @@ struct EpiOut {
   bool more;     // parts are added to what is there
   const float2 *pa, *pb;
   template <class TL>
-  __device__ void store(const Args& p, const Place& c, typename TL::T* lds, typename TL::Acc& acc) const {
+  __device__ __forceinline__ void form(const Args&, const Place&, typename TL::Acc&) const {}
+  template <class TL>
+  __device__ __forceinline__ void store(const Args& p, const Place& c, typename TL::T* lds, typename TL::Acc& acc) const {
     const float ua = pa ? pa->y : 1.f, ub = pb ? pb->y : 1.f;
     float* sums = part ? part + (int64_t)c.split * p.M * p.N : nullptr;
     TL::template runs<false>(
@@ -299,25 +355,28 @@ struct EpiOut {
           const int n = p.N - col < 8 ? (int)(p.N - col) : 8;
           if (sums) {
             if (n == 8) {
-              float t[8] = {};
+              struct F4 { float e[4]; } t[2] = {};
               if (more) __builtin_memcpy(t, sums + at, 32);
 #pragma unroll
-              for (int e = 0; e < 8; ++e) t[e] += v[e];
-              __builtin_memcpy(sums + at, t, 32);
+              for (int e = 0; e < 8; ++e) t[e >> 2].e[e & 3] += v[e];
+              put_past(sums + at, t[0]);
+              put_past(sums + at + 4, t[1]);
             } else {
               for (int e = 0; e < 8; ++e)
                 if (e < n) sums[at + e] = v[e] + (more ? sums[at + e] : 0.f);
             }
             return;
           }
-          struct V { TO e[8]; } o;
+          constexpr int W = 16 / sizeof(TO);  // a store
+          struct V { TO e[W]; } o[8 / W];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) o.e[e] = from_f<TO>(v[e] * ua * ub);
+          for (int e = 0; e < 8; ++e) o[e / W].e[e % W] = from_f<TO>(v[e] * ua * ub);
           if (n == 8) {
-            __builtin_memcpy(out + at, &o, sizeof(o));
+#pragma unroll
+            for (int q = 0; q < 8 / W; ++q) put_past(out + at + q * W, o[q]);
           } else {
             for (int e = 0; e < 8; ++e)
-              if (e < n) out[at + e] = o.e[e];
+              if (e < n) out[at + e] = o[e / W].e[e % W];
           }
         },
         [](int64_t, int64_t, float (&)[8]) {});
@@ -435,8 +494,27 @@ size_t forward(const LinearCE& a, void* wsp, int cus, hipStream_t s) {
   return ws.used;
 }
 
-// Values of d that are held at once: 2^28 (512 MB of 16 bits).
-constexpr int64_t kHeld = (int64_t)1 << 28;
+// Values of d that are held at once: 2^29 (1 GB of 16 bits).
+constexpr int64_t kHeld = (int64_t)1 << 29;
+
+// Parts of dx's sum over the words, with the blocks of dw beside them: the
+// least of what a compute unit has to do, in stages of 64 k (a block's start
+// and end count as 4, half of a last block's length as waiting, a part's
+// writing and reading back by its bytes).
+int dx_parts(int64_t xtiles, int64_t stages, int64_t wtiles, int64_t wstages, int64_t values, int slots) {
+  int best = 1;
+  double least = 1e300;
+  for (int s = 1; s <= 64 && s * 4 <= std::max<int64_t>(stages, 4); ++s) {
+    const double len = (double)ceil_div(stages, s) + 4, last = std::min<double>(len, (double)wstages + 4);
+    const double work = ((double)xtiles * s * len + (double)wtiles * ((double)wstages + 4)) / slots;
+    const double t = std::max(work, len) + 0.5 * last + (s > 1 ? s * (double)values * 8 / 8e6 : 0);
+    if (t < least) {
+      least = t;
+      best = s;
+    }
+  }
+  return best;
+}
 
 template <typename TI, typename T, int PL>
 size_t backward(const LinearCE& a, void* wsp, int cus, hipStream_t s) {
@@ -447,16 +525,16 @@ size_t backward(const LinearCE& a, void* wsp, int cus, hipStream_t s) {
   // pieces of the vocabulary, whole tiles of it
   const int64_t most = std::min<int64_t>(std::max<int64_t>(kHeld / PL / a.R / 256 * 256, 256), 1 << 19);
   const int64_t pieces = ceil_div(a.V, most), each = ceil_div(ceil_div(a.V, pieces), 256) * 256;
-  const int64_t ldd = std::min(each, (a.V + 31) / 32 * 32) * PL;
+  const int64_t len = std::min(each, a.V), ldd = (len + 31) / 32 * 32 * PL;
   T* d = ws.take<T>((size_t)(a.R * ldd));
   constexpr bool scaled = !std::is_same<T, bf16_t>::value;
   float2* pg = scaled ? ws.take<float2>(1) : nullptr;
-  // dx: parts over a piece's words
-  const int64_t len = std::min(each, a.V), stages = ceil_div(len, 64 / PL);
-  const int xtile = pick(a.R, a.K, std::max<int64_t>(stages / 16, 1), cus);
-  const int64_t xtiles = ceil_div(a.R, xtile == kBig ? 256 : xtile == kMid ? 128 : 32) * ceil_div(a.K, bn_of(xtile));
-  const int64_t slots = cus * (xtile == kBig ? 1 : 2);
-  const int splits = (int)std::max<int64_t>(1, std::min<int64_t>(slots / xtiles, stages / 4));
+  // both products of a piece in one launch: large tiles where they fill the
+  // chip at one block a compute unit
+  const bool big = a.R > 32 && ceil_div(len, 256) * ceil_div(a.K, 256) >= cus / 2;
+  const int64_t b = big ? 256 : 128, xb = a.R <= 32 ? 32 : b;
+  const int splits = dx_parts(ceil_div(a.R, xb) * ceil_div(a.K, b), ceil_div(len, 64 / PL),
+                              ceil_div(len, b) * ceil_div(a.K, b), ceil_div(a.R, 64 / PL), a.R * a.K, big ? cus : 2 * cus);
   const bool parted = splits > 1 || pieces > 1;
   float* part = parted ? ws.take<float>((size_t)(splits * a.R * a.K)) : nullptr;
   if (!wsp) return ws.used;
@@ -473,15 +551,20 @@ size_t backward(const LinearCE& a, void* wsp, int cus, hipStream_t s) {
     run<T, PL, false, false>(pick(a.R, n, 1, cus), p,
                              EpiGrad<T>{d, ldd, v0, a.V, a.targets, wide, a.loss, a.lse, a.g_loss, a.g_lse, x.power,
                                         w.power, pg}, s, what);
-    p = Args();
-    p.a = dp; p.b = wp;
-    p.M = a.R; p.N = a.K; p.K = n; p.splits = splits;
-    run<T, PL, false, true>(xtile, p, EpiOut<TI>{(TI*)a.dx, part, v0 > 0, pg, w.power}, s, what);
-    p = Args();
-    p.a = dp; p.b = x.o;
-    p.M = n; p.N = a.K; p.K = a.R;
-    run<T, PL, true, true>(pick(n, a.K, 1, cus), p, EpiOut<TI>{(TI*)a.dw + v0 * a.K, nullptr, false, pg, x.power}, s,
-                           what);
+    Args px, pw;
+    px.a = pw.a = dp;
+    px.b = wp;
+    px.M = a.R; px.N = a.K; px.K = n; px.splits = splits;
+    pw.b = x.o;
+    pw.M = n; pw.N = a.K; pw.K = a.R;
+    const EpiOut<TI> ex{(TI*)a.dx, part, v0 > 0, pg, w.power}, ew{(TI*)a.dw + v0 * a.K, nullptr, false, pg, x.power};
+    typedef Tile<T, 2, 2, 2, 2, PL, true, true> WMid;
+    if (big)
+      launch_pair<Tile<T, 4, 2, 2, 4, PL, false, true>, Tile<T, 4, 2, 2, 4, PL, true, true>>(px, ex, pw, ew, s, what);
+    else if (a.R > 32)
+      launch_pair<Tile<T, 2, 2, 2, 2, PL, false, true>, WMid>(px, ex, pw, ew, s, what);
+    else
+      launch_pair<Tile<T, 1, 1, 1, 4, PL, false, true>, WMid>(px, ex, pw, ew, s, what);
   }
   if (parted) {
     const int64_t n = a.R * a.K;

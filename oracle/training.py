@@ -65,17 +65,19 @@ def planes(a, n, unit=2.0 ** 14):
 
 def orthogonalize(g, steps=5, eps=1e-7, halves=0):
     """[..., m, n] by Newton-Schulz products in float64.  With halves = 1 or 2
-    the factors of every product are rounded as the device holds them (that
-    many float16 planes), for a measure of what these roundings alone do; with
-    2, products are summed in float32 too."""
+    (or one for each step) the factors of every product are rounded as the
+    device holds them (that many float16 planes), for a measure of what these
+    roundings alone do; with 2, products are summed in float32 too."""
     a, b, c = COEFFS
     g = np.asarray(g, F64)
 
+    per_step = list(halves) if isinstance(halves, (list, tuple)) else [halves] * steps
+
     def hold(x):
-        return planes(x, halves) if halves else x
+        return planes(x, n) if n else x
 
     def mul(x, y):
-        if halves == 2:   # high x high + high x low + low x high, float32 sums
+        if n == 2:   # high x high + high x low + low x high, float32 sums
             (xh, yh) = (planes(x, 1), planes(y, 1))
             (xl, yl) = (x - xh, y - yh)
             x32 = np.concatenate([xh, xh, xl], -1).astype(F32)
@@ -86,13 +88,13 @@ def orthogonalize(g, steps=5, eps=1e-7, halves=0):
     norm = np.sqrt((g * g).sum((-2, -1), keepdims=True)) + eps
     x = g / np.where(norm > 0, norm, 1.0)
     tall = g.shape[-2] > g.shape[-1]
-    for _ in range(steps):
+    for n in per_step:
         xr = hold(x)
         xt = np.swapaxes(xr, -1, -2)
         A = hold(mul(xt, xr) if tall else mul(xr, xt))
         B = hold(b * A + c * mul(A, A))
         x = a * x + (mul(xr, B) if tall else mul(B, xr))
-        if halves:
+        if n:
             x = x.astype(F32).astype(F64)
     return x
 

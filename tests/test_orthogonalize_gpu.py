@@ -2,7 +2,9 @@
 float64.
 
 Bars.  What the device rounds is known: the factors of every product, to one
-float16 plane (16-bit matrices) or two (float32), and the sums to float32.  The
+float16 plane (bfloat16, and float16 before the last three steps) or two
+(float32, float16's last three steps and all of its small matrices'), and the
+sums to float32.  The
 oracle makes the same roundings on the same matrix, and what they do to it,
 d = oracle with roundings - oracle without, measures the conditioning of this
 matrix; the device's roundings fall elsewhere (sums differ in their last
@@ -41,7 +43,10 @@ def _gradient(shape, dtype, seed=0, size=1e-3):
 def _bars(g, dtype, **kw):
     """(result, bar of the Frobenius norm, bar of a value) of each matrix."""
     want = O.orthogonalize(g, **kw)
-    d = O.orthogonalize(g, halves=2 if dtype == "float32" else 1, **kw) - want
+    steps = kw.get("steps", 5)
+    halves = {"float32": [2] * steps, "bfloat16": [1] * steps,
+              "float16": [2 if i + 3 >= steps or min(g.shape[-2:]) <= 256 else 1 for i in range(steps)]}[dtype]
+    d = O.orthogonalize(g, halves=halves, **kw) - want
     side = np.sqrt(min(g.shape[-2:]))
     sums = 15 * 2.0 ** -22 * side
     norm = 2 * np.sqrt((d * d).sum((-2, -1))) + sums * np.sqrt((want * want).sum((-2, -1)) / side)
