@@ -328,7 +328,7 @@ struct EpiGrad {
     TL::template runs<false>(
         c, lds, acc, false,
         [&](int64_t row, int64_t col, float (&v)[8]) {
-          if (row < p.M && col * PL < ldd) put_planes<T, PL, true>(d + row * ldd, col, v);
+          if (row < p.M && col * PL < ldd) put_planes<T, PL>(d + row * ldd, col, v);
         },
         [](int64_t, int64_t, float (&)[8]) {});
   }

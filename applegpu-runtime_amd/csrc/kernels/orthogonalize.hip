@@ -14,9 +14,11 @@
 // bits), see planes_of.  All entries are at most about
 // 1.3 in magnitude (singular values stay below 1.2), so X, A and B are held
 // times 2^14, where fp16 keeps 11 bits of everything down to 2^-28.  X itself
-// stays in fp32 beside its planes: a X is what carries the small singular
-// values, multiplied by 3.4 in each step, and would carry a rounding of X
-// along; what fp16 loses of X inside B X is B's small share of that direction.
+// keeps more beside its planes, 22 bits for 16-bit matrices and fp32 for fp32
+// ones: a X is what carries the small singular values, multiplied by 3.4 in
+// each step, and would carry a rounding of X along (256 x 512 of rank 8 and 3 %
+// noise: relative error 9.5e-3 with X in 11 bits, 3.8e-4 in 22); what fp16 loses
+// of X inside B X is B's small share of that direction.
 #include "tile16.hpp"
 
 namespace agpu {
@@ -34,38 +36,74 @@ __device__ __forceinline__ T* mat(const Mats& t, int64_t i) {
   return t.apart ? (T*)t.p[0] + i * t.apart : (T*)t.p[i];
 }
 
-constexpr int kNormParts = 128;  // blocks a matrix for its norm
-
-// Of matrix blockIdx.y: the squares' sum in kNormParts parts, and with
-// momentum the new momentum and U (fp32, contiguous).
-template <typename TI, bool MOM>
-__global__ void __launch_bounds__(256) norm_kernel(Mats in, Mats mom, float beta, bool nesterov, int64_t n,
-                                                   double* part, float* u) {
-  __shared__ double red[4];
-  const int64_t i = blockIdx.y;
-  const TI* g = mat<TI>(in, i);
-  float* b = MOM ? mat<float>(mom, i) : nullptr;
-  double sum = 0.0;
-  auto one = [&](int64_t j, float gv) {
-    float v = gv;
-    if constexpr (MOM) {
-      const float mv = beta * b[j] + gv;
-      b[j] = mv;
-      v = nesterov ? gv + beta * mv : mv;
-      u[i * n + j] = v;
-    }
-    sum += (double)v * (double)v;
-  };
-  struct alignas(4 * sizeof(TI)) V { TI e[4]; };
-  if (n % 4 == 0 && ((uintptr_t)g % sizeof(V)) == 0) {
-#pragma unroll 2
-    for (int64_t j = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; j < n; j += (int64_t)kNormParts * 1024) {
-      const V v = *(const V*)(g + j);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) one(j + e, to_f(v.e[e]));
+// 8 values or the first n of them, at any alignment.
+template <typename E>
+struct Run { E e[8]; };
+template <typename E>
+__device__ __forceinline__ Run<E> get_run(const E* at, int n) {
+  Run<E> r{};
+  if (n >= 8) __builtin_memcpy(&r, at, sizeof(r));
+  else
+    for (int e = 0; e < 8; ++e)
+      if (e < n) r.e[e] = at[e];
+  return r;
+}
+template <typename E>
+__device__ __forceinline__ void put_run(E* at, const Run<E>& r, int n) {
+  if (n >= 8) {
+    struct Half { E e[4]; } h[2];
+    __builtin_memcpy(h, &r, sizeof(r));
+    if constexpr (sizeof(E) == 4) {
+      put_past(at, h[0]);
+      put_past(at + 4, h[1]);
+    } else {
+      put_past(at, r);
     }
   } else {
-    for (int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x; j < n; j += (int64_t)kNormParts * 256) one(j, to_f(g[j]));
+    for (int e = 0; e < 8; ++e)
+      if (e < n) at[e] = r.e[e];
+  }
+}
+
+constexpr int kNormParts = 128;  // blocks a matrix for its norm
+
+// Of matrix blockIdx.y: the sum of U's squares in kNormParts parts, and with
+// momentum the new momentum.  Four runs' loads are under way at a time.
+template <typename TI, bool MOM>
+__global__ void __launch_bounds__(256) norm_kernel(Mats in, Mats mom, float beta, bool nesterov, int64_t n, double* part) {
+  __shared__ double red[4];
+  const int64_t i = blockIdx.y;
+  const TI* __restrict__ g = mat<TI>(in, i);
+  float* __restrict__ b = MOM ? mat<float>(mom, i) : nullptr;
+  constexpr int kAtOnce = 4;
+  double sum = 0.0;
+  const int64_t apart = (int64_t)kNormParts * 256 * 8;
+  for (int64_t j0 = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; j0 < n; j0 += apart * kAtOnce) {
+    Run<TI> gv[kAtOnce];
+    Run<float> bv[kAtOnce];
+#pragma unroll
+    for (int q = 0; q < kAtOnce; ++q) {
+      const int64_t j = j0 + q * apart, left = n - j;
+      const int m = left < 0 ? 0 : left < 8 ? (int)left : 8;
+      gv[q] = get_run(g + j, m);
+      if constexpr (MOM) bv[q] = get_run(b + j, m);
+    }
+#pragma unroll
+    for (int q = 0; q < kAtOnce; ++q) {
+      const int64_t j = j0 + q * apart, left = n - j;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float v = to_f(gv[q].e[e]);
+        if constexpr (MOM) {
+          const float m = beta * bv[q].e[e] + v;
+          bv[q].e[e] = m;
+          v = nesterov ? v + beta * m : m;
+        }
+        sum += (double)v * (double)v;  // (nothing where nothing was read)
+      }
+      if constexpr (MOM)
+        if (left > 0) put_run(b + j, bv[q], left < 8 ? (int)left : 8);
+    }
   }
 #pragma unroll
   for (int m = 32; m >= 1; m >>= 1) sum += __shfl_xor(sum, m);
@@ -74,14 +112,22 @@ __global__ void __launch_bounds__(256) norm_kernel(Mats in, Mats mom, float beta
   if (threadIdx.x == 0) part[i * kNormParts + blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-// X = U / (|U| + eps) in units of 2^-14: fp32 [m, n] and planes with rows of
-// ld values.  TI: what U is held as (the matrices, or fp32 at u).
-template <typename TI, int PL>
-__global__ void __launch_bounds__(256) start_kernel(Mats in, const float* u, int64_t m, int64_t n, const double* part,
-                                                    float eps, float* x, half_t* planes, int64_t ld) {
+// What X keeps beside the planes of a step's factor, in units of 2^-14: fp32
+// (F32), or with one plane the low half, rows as long as the plane's.
+struct Kept {
+  float* x = nullptr;     // [count][m][n]
+  half_t* low = nullptr;  // [count][m][ld]
+};
+
+// X = U / (|U| + eps) and its planes, rows of ld values.
+template <typename TI, bool MOM, int PL>
+__global__ void __launch_bounds__(256) start_kernel(Mats in, Mats mom, float beta, bool nesterov, int64_t m, int64_t n,
+                                                   const double* part, float eps, Kept keep, half_t* planes, int64_t ld) {
+  constexpr bool F32 = sizeof(TI) == 4;
   __shared__ double red[2];
   const int64_t i = blockIdx.y;
-  const TI* g = u ? (const TI*)(u + i * m * n) : mat<TI>(in, i);
+  const TI* __restrict__ g = mat<TI>(in, i);
+  const float* __restrict__ b = MOM ? mat<float>(mom, i) : nullptr;
   if (threadIdx.x < kNormParts) {
     double s = part[i * kNormParts + threadIdx.x];
 #pragma unroll
@@ -91,16 +137,47 @@ __global__ void __launch_bounds__(256) start_kernel(Mats in, const float* u, int
   __syncthreads();
   const float norm = (float)sqrt(red[0] + red[1]) + eps;
   const float by = norm > 0.f || norm != norm ? norm : 1.f;  // a matrix of zeros stays one
-  const int64_t chunks = ld / (8 * PL), total = m * chunks;
-  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (int64_t)gridDim.x * 256) {
-    const int64_t r = t / chunks, c = (t - r * chunks) * 8;
-    float v[8];
+  const int chunks = (int)(ld / (8 * PL));
+  constexpr int kAtOnce = 2;
+  const int64_t total = m * chunks, apart = (int64_t)gridDim.x * 256;
+  for (int64_t t0 = (int64_t)blockIdx.x * 256 + threadIdx.x; t0 < total; t0 += apart * kAtOnce) {
+    Run<TI> gv[kAtOnce];
+    Run<float> bv[kAtOnce];
+    int64_t row[kAtOnce];
+    int col[kAtOnce], len[kAtOnce];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = c + e < n ? to_f(g[r * n + c + e]) / by * kUnit : 0.f;
+    for (int q = 0; q < kAtOnce; ++q) {
+      const int64_t t = t0 + q * apart;
+      row[q] = t < total ? t / chunks : -1;
+      col[q] = (int)(t - row[q] * chunks) * 8;
+      const int64_t left = n - col[q];
+      len[q] = row[q] < 0 || left < 0 ? 0 : left < 8 ? (int)left : 8;
+      gv[q] = get_run(g + row[q] * n + col[q], len[q]);
+      if constexpr (MOM) bv[q] = get_run(b + row[q] * n + col[q], len[q]);
+    }
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (c + e < n) x[(i * m + r) * n + c + e] = v[e];
-    put_planes<half_t, PL>(planes + (i * m + r) * ld, c, v);
+    for (int q = 0; q < kAtOnce; ++q) {
+      if (row[q] < 0) continue;
+      const int64_t r = i * m + row[q];
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float u = to_f(gv[q].e[e]);
+        if constexpr (MOM) u = nesterov ? u + beta * bv[q].e[e] : bv[q].e[e];
+        v[e] = u / by * kUnit;
+      }
+      put_planes<half_t, PL>(planes + r * ld, col[q], v);
+      if constexpr (F32) {
+        Run<float> x;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x.e[e] = v[e];
+        put_run(keep.x + r * n + col[q], x, len[q]);
+      } else if constexpr (PL == 1) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] -= (float)(half_t)v[e];
+        put_planes<half_t, 1>(keep.low + r * ld, col[q], v);
+      }
+    }
   }
 }
 
@@ -150,42 +227,25 @@ struct EpiGram {
   }
 };
 
-// 8 values or the first n of them, at any alignment.
-template <typename E>
-struct Run { E e[8]; };
-template <typename E>
-__device__ __forceinline__ Run<E> get_run(const E* at, int n) {
-  Run<E> r{};
-  if (n >= 8) __builtin_memcpy(&r, at, sizeof(r));
-  else
-    for (int e = 0; e < 8; ++e)
-      if (e < n) r.e[e] = at[e];
-  return r;
-}
-template <typename E>
-__device__ __forceinline__ void put_run(E* at, const Run<E>& r, int n) {
-  if (n >= 8) __builtin_memcpy(at, &r, sizeof(r));
-  else
-    for (int e = 0; e < 8; ++e)
-      if (e < n) at[e] = r.e[e];
-}
-
-// X = a X + B X, in fp32 and as the next step's NEXT planes; after the last
-// step (NEXT = 0) the result instead.  Tiles within the columns of a matrix
-// whose rows stay aligned read X and the weights where the accumulators are,
-// eight loads under way at a time; others run by run (a load and its use after
-// one another: 18 us more a tile of 256 x 256).
-template <typename TO, int NEXT>
+// X = a X + B X, as the next step's NEXT planes and what is kept beside them;
+// after the last step (NEXT = 0) the result instead.  X is read where the
+// accumulators are, eight loads under way at a time (a load and its use after
+// one another, run by run, took 18 us more a tile of 256 x 256); fp32 X and
+// the weights run by run where a tile reaches past the columns or their rows
+// are not aligned.
+template <typename TO, bool F32, int NEXT>
 struct EpiUpdate {
-  float* x;        // [count][m][n]
-  half_t* planes;  // rows ld apart
+  const half_t* from;  // the step's planes, rows ld apart
   int64_t ld;
+  Kept keep;
+  half_t* planes;      // the next step's, rows ld_next apart
+  int64_t ld_next;
   Mats out;
-  bool step;       // out = keep out - rate X
-  float keep, rate;
+  bool step;           // out = keep out - rate X
+  float hold, rate;
   __device__ __forceinline__ float result(float v, float was) const {
     const float s = v * kPerUnit;
-    return step ? keep * was - rate * s : s;
+    return step ? hold * was - rate * s : s;
   }
   template <class TL>
   __device__ __forceinline__ bool near(const Args& p, const Place& c) const {
@@ -194,61 +254,89 @@ struct EpiUpdate {
   }
   template <class TL>
   __device__ __forceinline__ void form(const Args& p, const Place& c, typename TL::Acc& acc) const {
-    const float* xb = x + (int64_t)c.batch * p.M * p.N;
-    const TO* o = NEXT ? nullptr : mat<TO>(out, c.batch);
-    if (near<TL>(p, c)) {
-      const typename TL::template Places<float> xs(c, xb, p.N, p.M);
-      const typename TL::template Places<TO> os(c, NEXT ? (const TO*)xb : o, p.N, p.M);
-      TL::fours(acc, [&](int i, int j, int g, float (&v)[4]) {
-        float t[4];
-        xs.load(i, j, g, t);
-        if (NEXT == 0 && step) {
-          float w[4];
-          os.load(i, j, g, w);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = result(kA * t[e] + v[e] * kPerUnit, w[e]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            v[e] = kA * t[e] + v[e] * kPerUnit;
-            if constexpr (NEXT == 0) v[e] = result(v[e], 0.f);
-          }
-        }
-      });
+    constexpr int PL = TL::PL;
+    if constexpr (F32) {
+      if (!near<TL>(p, c)) return;
     }
+    const bool weights = NEXT == 0 && step && near<TL>(p, c);
+    const int64_t b = c.batch;
+    const TO* o = NEXT ? nullptr : mat<TO>(out, b);
+    const typename TL::template Places<float> xs(c, F32 ? keep.x + b * p.M * p.N : nullptr, p.N, F32 ? p.M : c.m0);
+    const typename TL::template Places<half_t, PL> hs(c, from + b * p.M * ld, ld, p.M);
+    const typename TL::template Places<half_t> ls(c, PL == 1 && !F32 ? keep.low + b * p.M * ld : from, ld, p.M);
+    const typename TL::template Places<TO> os(c, NEXT ? (const TO*)from : o, p.N, weights ? p.M : c.m0);
+    TL::fours(acc, [&](int i, int j, int g, float (&v)[4]) {
+      float t[4];
+      if constexpr (F32) {
+        xs.load(i, j, g, t);
+      } else {
+        float l[4];
+        hs.load(i, j, g, t);
+        if constexpr (PL == 2) hs.load(i, j, g, l, 1);
+        else ls.load(i, j, g, l);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t[e] += l[e];
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = kA * t[e] + v[e] * kPerUnit;
+      if constexpr (NEXT == 0) {
+        if (weights) {
+          os.load(i, j, g, t);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = result(v[e], t[e]);
+        } else if (!step) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = result(v[e], 0.f);
+        }
+      }
+    });
   }
   template <class TL>
   __device__ __forceinline__ void store(const Args& p, const Place& c, typename TL::T* lds, typename TL::Acc& acc) const {
-    float* xb = x + (int64_t)c.batch * p.M * p.N;
+    float* xb = F32 ? keep.x + (int64_t)c.batch * p.M * p.N : nullptr;
     TO* o = NEXT ? nullptr : mat<TO>(out, c.batch);
-    const bool near = this->near<TL>(p, c);
+    const bool close = near<TL>(p, c), ragged = c.n0 + TL::BN > p.N;
     TL::template runs<false>(
         c, lds, acc, false,
         [&](int64_t row, int64_t col, float (&v)[8]) {
-          if (row >= p.M || (col >= p.N && col * NEXT >= ld * (NEXT != 0))) return;
-          const int n = p.N - col < 8 ? (int)(p.N - col) : 8;  // (none behind the columns, where planes hold zeros)
+          if (row >= p.M || (col >= p.N && (NEXT == 0 || col * NEXT >= ld_next))) return;
+          // (none behind the columns, where planes hold zeros)
+          const int n = p.N - col < 8 ? (int)(p.N - col) : 8;
           const int64_t at = row * p.N + col;
-          if (near) {
-            if constexpr (NEXT != 0) {
-              float4* to = (float4*)(xb + at);
-              to[0] = make_float4(v[0], v[1], v[2], v[3]);
-              to[1] = make_float4(v[4], v[5], v[6], v[7]);
-            }
-          } else {
-            Run<float> t = get_run(xb + at, n);
-            Run<TO> w{};
-            if (NEXT == 0 && step) w = get_run(o + at, n);
+          if constexpr (F32) {
+            if (!close) {
+              const Run<float> t = get_run(xb + at, n);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              v[e] = e < n ? kA * t.e[e] + v[e] * kPerUnit : 0.f;
-              t.e[e] = v[e];
-              if constexpr (NEXT == 0) v[e] = result(v[e], to_f(w.e[e]));
+              for (int e = 0; e < 8; ++e) v[e] = kA * t.e[e] + v[e] * kPerUnit;
+              if constexpr (NEXT == 0)
+                if (!step)
+#pragma unroll
+                  for (int e = 0; e < 8; ++e) v[e] = result(v[e], 0.f);
             }
-            if constexpr (NEXT != 0) put_run(xb + at, t, n);
           }
           if constexpr (NEXT != 0) {
-            put_planes<half_t, NEXT>(planes + ((int64_t)c.batch * p.M + row) * ld, col, v);
+            if (ragged) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) v[e] = e < n ? v[e] : 0.f;
+            }
+            const int64_t r = (int64_t)c.batch * p.M + row;
+            put_planes<half_t, NEXT>(planes + r * ld_next, col, v);
+            if constexpr (F32) {
+              Run<float> x;
+#pragma unroll
+              for (int e = 0; e < 8; ++e) x.e[e] = v[e];
+              put_run(xb + at, x, n);
+            } else if constexpr (NEXT == 1) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) v[e] -= (float)(half_t)v[e];
+              put_planes<half_t, 1>(keep.low + r * ld_next, col, v);
+            }
           } else {
+            if (step && !close) {
+              const Run<TO> w = get_run(o + at, n);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) v[e] = result(v[e], to_f(w.e[e]));
+            }
             Run<TO> q;
 #pragma unroll
             for (int e = 0; e < 8; ++e) q.e[e] = from_f<TO>(v[e]);
@@ -259,20 +347,29 @@ struct EpiUpdate {
   }
 };
 
-// Square tiles of 256 (8 wavefronts), 128 or 64 (4).
+// Square tiles of 256 (one block a compute unit), 128 (both 8 wavefronts) or 64
+// (4).  Large ones where they fill whole rounds of the chip, else the next size
+// that makes enough blocks.  Gram, poly and update in us, 256 / 128 / 64:
+//   2 x 4096 x 4096 fp32      526/419/572  520/393/575  635/692/889  (272 and 512 tiles of 256)
+//   12 x 768 x 2304           56/28/30     32/13/14     83/66/74
+//   12 x 768 x 768            28/12/13     33/14/14     41/25/28
+//   1280 x 1280               36/14/9.5    42/15/10     50/20/16
+//   200 x 400                 22/9/6       18/7.5/5.4   20/8.4/5.5
 enum { kBig, kMid, kSmall };
 int pick(int64_t M, int64_t N, int64_t count, bool sym, int cus) {
   auto tiles = [&](int64_t b) {
     const int64_t m = ceil_div(M, b), n = ceil_div(N, b);
     return (sym ? m * (m + 1) / 2 : m * n) * count;
   };
-  return tiles(256) * 4 >= 3 * cus ? kBig : tiles(128) * 4 >= 3 * cus ? kMid : kSmall;
+  const int64_t big = tiles(256);
+  if (big * 10 >= ceil_div(big, cus) * cus * 9) return kBig;
+  return tiles(128) * 8 >= 5 * cus ? kMid : kSmall;
 }
 
 template <int PL, bool AC, bool BC, bool SYM, class Epi>
 void run(int tile, const Args& p, const Epi& e, hipStream_t s, const char* what) {
   if (tile == kBig) launch<Tile<half_t, 4, 2, 2, 4, PL, AC, BC, SYM>>(p, e, s, what);
-  else if (tile == kMid) launch<Tile<half_t, 2, 2, 2, 2, PL, AC, BC, SYM>>(p, e, s, what);
+  else if (tile == kMid) launch<Tile<half_t, 2, 1, 2, 4, PL, AC, BC, SYM>>(p, e, s, what);
   else launch<Tile<half_t, 1, 1, 2, 2, PL, AC, BC, SYM>>(p, e, s, what);
 }
 
@@ -282,8 +379,8 @@ void run(int tile, const Args& p, const Epi& e, hipStream_t s, const char* what)
 // with one plane throughout, 1.2e-4 with two in the last three steps, 1e-6 with
 // two throughout.  Against the rounding of the result itself, 1.7e-3 in bf16,
 // 2.1e-4 in fp16 and 3e-8 in fp32, that is one plane, two in the last three
-// steps, and two.  Small matrices take two in fp16 throughout: their error is
-// larger (64 x 128: 2.5e-4) and their time is the launches'.
+// steps, and two.  Matrices of a short side take two in fp16 throughout: their
+// error is larger (64 x 128: 2.5e-4) and their time is the launches'.
 int planes_of(const Orthogonalize& a, int step) {
   if (a.dt == DType::F32) return 2;
   if (a.dt == DType::BF16) return 1;
@@ -293,7 +390,7 @@ int64_t row_of(int64_t n, int planes) { return (n + 31) / 32 * 32 * planes; }
 
 struct Space {
   double* part;
-  float* x;
+  Kept keep;
   half_t *planes[2], *a, *b;
   size_t bytes;
 };
@@ -308,7 +405,8 @@ Space space(const Orthogonalize& a, char* base) {
   const int pl = planes_of(a, a.steps - 1);  // the most of all steps
   const int64_t side = std::min(a.m, a.n);
   w.part = (double*)take((size_t)a.count * kNormParts * 8);
-  w.x = (float*)take((size_t)(a.count * a.m * a.n) * 4);
+  if (a.dt == DType::F32) w.keep.x = (float*)take((size_t)(a.count * a.m * a.n) * 4);
+  else if (planes_of(a, 0) == 1) w.keep.low = (half_t*)take((size_t)(a.count * a.m * row_of(a.n, 1)) * 2);
   for (auto& q : w.planes) q = (half_t*)take((size_t)(a.count * a.m * row_of(a.n, pl)) * 2);
   w.a = (half_t*)take((size_t)(a.count * side * row_of(side, pl)) * 2);
   w.b = (half_t*)take((size_t)(a.count * side * row_of(side, pl)) * 2);
@@ -316,31 +414,25 @@ Space space(const Orthogonalize& a, char* base) {
   return w;
 }
 
-template <typename TI>
+template <typename TI, bool MOM>
 void start(const Orthogonalize& a, const Space& w, hipStream_t s, const char* what) {
-  const int64_t n = a.m * a.n;
-  const dim3 parts(kNormParts, (unsigned)a.count);
-  if (a.momentum)
-    hipLaunchKernelGGL((norm_kernel<TI, true>), parts, dim3(256), 0, s, a.in, a.mom, a.beta, a.nesterov, n, w.part, w.x);
-  else
-    hipLaunchKernelGGL((norm_kernel<TI, false>), parts, dim3(256), 0, s, a.in, a.mom, a.beta, a.nesterov, n, w.part,
-                       (float*)nullptr);
+  hipLaunchKernelGGL((norm_kernel<TI, MOM>), dim3(kNormParts, (unsigned)a.count), dim3(256), 0, s, a.in, a.mom, a.beta,
+                     a.nesterov, a.m * a.n, w.part);
   check_launch(what);
   const int pl = planes_of(a, 0);
   const int64_t ld = row_of(a.n, pl);
-  const dim3 grid((unsigned)std::min<int64_t>(blocks_for(a.m * (ld / (8 * pl)), 256), 1024), (unsigned)a.count);
-  // (U and X share their place: a value is read before it is written, by the
-  // same thread)
-  auto go = [&](auto kernel, const float* u) {
-    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a.in, u, a.m, a.n, w.part, a.eps, w.x, w.planes[0], ld);
+  const dim3 grid((unsigned)std::min<int64_t>(blocks_for(a.m * (ld / (8 * pl)), 512), 512), (unsigned)a.count);
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a.in, a.mom, a.beta, a.nesterov, a.m, a.n, w.part, a.eps, w.keep,
+                       w.planes[0], ld);
   };
-  if (a.momentum) pl == 1 ? go(start_kernel<float, 1>, w.x) : go(start_kernel<float, 2>, w.x);
-  else pl == 1 ? go(start_kernel<TI, 1>, nullptr) : go(start_kernel<TI, 2>, nullptr);
+  if constexpr (sizeof(TI) == 4) go(start_kernel<TI, MOM, 2>);
+  else pl == 1 ? go(start_kernel<TI, MOM, 1>) : go(start_kernel<TI, MOM, 2>);
   check_launch(what);
 }
 
 // Step i on PL planes, the next on NEXT (0: none follows).
-template <typename TO, int PL, int NEXT>
+template <typename TO, bool F32, int PL, int NEXT>
 void step(const Orthogonalize& a, const Space& w, int i, int cus, hipStream_t s, const char* what) {
   const int64_t m = a.m, n = a.n, side = std::min(m, n), ld = row_of(n, PL), lda = row_of(side, PL);
   const bool tall = m > n;
@@ -361,29 +453,240 @@ void step(const Orthogonalize& a, const Space& w, int i, int cus, hipStream_t s,
   p.N = n;
   p.a = tall ? xo : bo;
   p.b = tall ? bo : xo;
-  const EpiUpdate<TO, NEXT> eu{w.x, w.planes[(i + 1) & 1], row_of(n, NEXT), a.out, a.momentum, a.keep, a.rate};
+  const EpiUpdate<TO, F32, NEXT> eu{w.planes[i & 1], ld, w.keep, w.planes[(i + 1) & 1], row_of(n, NEXT), a.out,
+                                    a.momentum, a.keep, a.rate};
   if (tall) run<PL, false, false, false>(upd, p, eu, s, what);
   else run<PL, false, true, false>(upd, p, eu, s, what);
 }
 
+// ── small matrices: everything in one block ───────────────────────────────
+// A matrix of at most kSmallValues values (sides rounded up to 32), the shorter
+// side at most 128, stays in one block's LDS and registers from its norm to its
+// result: one launch where the products of a step would be three of 4.5 us each
+// (128 x 64 fp32, five steps: 73 us, so 17).  X and the Gram matrix (then the
+// polynomial in its place) are two fp16 planes each; a wavefront holds two 32 x
+// 32 tiles of X in fp32.
+constexpr int kSmallValues = 16384, kSmallWaves = 8;
+
+// Rows of a plane in LDS, 8 values apart from being multiples of 32: a
+// fragment's 16 rows lie in different banks.
+struct Flat {
+  half_t *high, *low;
+  int ld;
+};
+typedef typename Mfma<half_t>::vec H8;
+template <bool COLS>
+__device__ __forceinline__ H8 flat_read(const half_t* plane, int ld, int blk, int kk, int lane) {
+  if constexpr (COLS) {
+    const int i = lane & 15, k = kk * 16 + 8 * (lane >> 5) + (i >> 2);
+    const half_t* at = plane + k * ld + blk * 32 + (lane & 16) + 4 * (i & 3);
+    union {
+      i16x4 h[2];
+      H8 v;
+    } u;
+    u.h[0] = read_transposed((lds_i16x4)at);
+    u.h[1] = read_transposed((lds_i16x4)(at + 4 * ld));
+    return u.v;
+  } else {
+    return *(const H8*)(plane + (blk * 32 + (lane & 31)) * ld + kk * 16 + 8 * (lane >> 5));
+  }
+}
+// Tile (ra, rb) of the product over k: rows of a, columns of b.
+template <bool AC, bool BC>
+__device__ __forceinline__ f32x16 flat_product(const Flat& a, int ra, const Flat& b, int rb, int k, int lane) {
+  f32x16 high, cross;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) high[e] = cross[e] = 0.f;
+  for (int kk = 0; kk < k / 16; ++kk) {
+    const H8 ah = flat_read<AC>(a.high, a.ld, ra, kk, lane), al = flat_read<AC>(a.low, a.ld, ra, kk, lane);
+    const H8 bh = flat_read<BC>(b.high, b.ld, rb, kk, lane), bl = flat_read<BC>(b.low, b.ld, rb, kk, lane);
+    high = Mfma<half_t>::run(bh, ah, high);
+    cross = Mfma<half_t>::run(bl, ah, cross);
+    cross = Mfma<half_t>::run(bh, al, cross);
+  }
+#pragma unroll
+  for (int e = 0; e < 16; ++e) high[e] += cross[e];
+  return high;
+}
+// 4 values of a row as planes.
+__device__ __forceinline__ void flat_put(const Flat& f, int row, int col, const float (&v)[4]) {
+  typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+  h4 h, l;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    h[e] = (_Float16)v[e];
+    l[e] = (_Float16)(fabsf((float)h[e]) < INFINITY ? v[e] - (float)h[e] : 0.f);
+  }
+  *(h4*)(f.high + row * f.ld + col) = h;
+  *(h4*)(f.low + row * f.ld + col) = l;
+}
+__device__ __forceinline__ void flat_get(const Flat& f, int row, int col, float (&v)[4]) {
+  typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+  const h4 h = *(const h4*)(f.high + row * f.ld + col), l = *(const h4*)(f.low + row * f.ld + col);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = (float)h[e] + (float)l[e];
+}
+
+template <typename TI, bool MOM, bool TALL>
+__global__ void __launch_bounds__(64 * kSmallWaves, 2) small_kernel(Orthogonalize a) {
+  __shared__ __attribute__((aligned(16))) half_t lds[69632];  // 2 x 128 x 136 of X and of A
+  __shared__ double red[kSmallWaves];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int m = (int)a.m, n = (int)a.n, mp = (m + 31) & ~31, np = (n + 31) & ~31, side = TALL ? np : mp;
+  const Flat x{lds, lds + mp * (np + 8), np + 8};
+  const Flat g{lds + 2 * mp * (np + 8), lds + 2 * mp * (np + 8) + side * (side + 8), side + 8};
+  const TI* in = mat<TI>(a.in, blockIdx.x);
+  const int xt = np / 32, xtiles = mp / 32 * xt, gt = side / 32;
+  // this lane's places of tile t (of `wide` tiles a row): row, and column of 4
+  // values for each i
+  auto row_at = [&](int t, int wide) { return t / wide * 32 + (lane & 31); };
+  auto col_at = [&](int t, int wide, int i) { return t % wide * 32 + 8 * i + 4 * (lane >> 5); };
+  float v[2][16];
+  double sum = 0.0;
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const int t = wave + kSmallWaves * q;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      v[q][e] = 0.f;
+      const int r = row_at(t, xt), c = col_at(t, xt, e >> 2) + (e & 3);
+      if (t < xtiles && r < m && c < n) {
+        float u = to_f(in[r * n + c]);
+        if constexpr (MOM) {
+          float* b = mat<float>(a.mom, blockIdx.x) + r * n + c;
+          const float mv = a.beta * *b + u;
+          *b = mv;
+          u = a.nesterov ? u + a.beta * mv : mv;
+        }
+        v[q][e] = u;
+        sum += (double)u * (double)u;
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 32; k >= 1; k >>= 1) sum += __shfl_xor(sum, k);
+  if (lane == 0) red[wave] = sum;
+  __syncthreads();
+  sum = 0.0;
+#pragma unroll
+  for (int w = 0; w < kSmallWaves; ++w) sum += red[w];
+  const float norm = (float)sqrt(sum) + a.eps;
+  const float by = norm > 0.f || norm != norm ? norm : 1.f;  // a matrix of zeros stays one
+#pragma unroll
+  for (int q = 0; q < 2; ++q)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) v[q][e] = v[q][e] / by * kUnit;
+  auto put = [&](const Flat& f, const float (&w)[16], int t, int wide) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float p[4] = {w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
+      flat_put(f, row_at(t, wide), col_at(t, wide, i), p);
+    }
+  };
+#pragma unroll
+  for (int q = 0; q < 2; ++q)
+    if (wave + kSmallWaves * q < xtiles) put(x, v[q], wave + kSmallWaves * q, xt);
+  __syncthreads();
+  for (int s = 0; s < a.steps; ++s) {
+    float w[2][16];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int t = wave + kSmallWaves * q;
+      if (t >= gt * gt) break;
+      const f32x16 p = flat_product<TALL, TALL>(x, t / gt, x, t % gt, TALL ? mp : np, lane);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) w[q][e] = p[e] * kPerUnit;
+      put(g, w[q], t, gt);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int t = wave + kSmallWaves * q;
+      if (t >= gt * gt) break;
+      const f32x16 p = flat_product<false, false>(g, t / gt, g, t % gt, side, lane);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float was[4];
+        flat_get(g, row_at(t, gt), col_at(t, gt, i), was);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[q][4 * i + e] = kB * was[e] + kC * (p[4 * i + e] * kPerUnit);
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+      if (wave + kSmallWaves * q < gt * gt) put(g, w[q], wave + kSmallWaves * q, gt);
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int t = wave + kSmallWaves * q;
+      if (t >= xtiles) break;
+      const f32x16 p = TALL ? flat_product<false, false>(x, t / xt, g, t % xt, side, lane)
+                            : flat_product<false, true>(g, t / xt, x, t % xt, side, lane);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) v[q][e] = kA * v[q][e] + p[e] * kPerUnit;
+    }
+    if (s + 1 == a.steps) break;
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+      if (wave + kSmallWaves * q < xtiles) put(x, v[q], wave + kSmallWaves * q, xt);
+    __syncthreads();
+  }
+  TI* out = mat<TI>(a.out, blockIdx.x);
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const int t = wave + kSmallWaves * q;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int r = row_at(t, xt), c = col_at(t, xt, e >> 2) + (e & 3);
+      if (t < xtiles && r < m && c < n) {
+        const float o = v[q][e] * kPerUnit;
+        out[r * n + c] = from_f<TI>(MOM ? a.keep * to_f(out[r * n + c]) - a.rate * o : o);
+      }
+    }
+  }
+}
+
+bool small_ok(const Orthogonalize& a) {
+  const int64_t mp = (a.m + 31) / 32 * 32, np = (a.n + 31) / 32 * 32;
+  return mp * np <= kSmallValues && std::min(mp, np) <= 128;
+}
+
+template <typename TI>
+void small(const Orthogonalize& a, hipStream_t s, const char* what) {
+  const dim3 grid((unsigned)a.count), block(64 * kSmallWaves);
+  const bool tall = a.m > a.n;
+  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, s, a); };
+  if (a.momentum) tall ? go(small_kernel<TI, true, true>) : go(small_kernel<TI, true, false>);
+  else tall ? go(small_kernel<TI, false, true>) : go(small_kernel<TI, false, false>);
+  check_launch(what);
+}
+
 }  // namespace
 
-size_t orthogonalize_ws_bytes(const Orthogonalize& a, int) { return space(a, nullptr).bytes; }
+size_t orthogonalize_ws_bytes(const Orthogonalize& a) { return small_ok(a) ? 0 : space(a, nullptr).bytes; }
 
 void orthogonalize(const Orthogonalize& a, void* ws, int cus, hipStream_t s) {
   const char* what = a.momentum ? "muon_step" : "orthogonalize";
-  const Space w = space(a, (char*)ws);
-  AGPU_FLOAT_SWITCH(a.dt, start<T>(a, w, s, what));
-  for (int i = 0; i + 1 < a.steps; ++i) {
-    // (the type of a result matters to the last step alone)
-    const int pl = planes_of(a, i), next = planes_of(a, i + 1);
-    if (pl == 2) step<float, 2, 2>(a, w, i, cus, s, what);
-    else if (next == 2) step<float, 1, 2>(a, w, i, cus, s, what);
-    else step<float, 1, 1>(a, w, i, cus, s, what);
+  if (small_ok(a)) {
+    AGPU_FLOAT_SWITCH(a.dt, small<T>(a, s, what));
+    return;
   }
-  if (a.dt == DType::F32) step<float, 2, 0>(a, w, a.steps - 1, cus, s, what);
-  else if (a.dt == DType::F16) step<half_t, 2, 0>(a, w, a.steps - 1, cus, s, what);
-  else step<bf16_t, 1, 0>(a, w, a.steps - 1, cus, s, what);
+  const Space w = space(a, (char*)ws);
+  AGPU_FLOAT_SWITCH(a.dt, if (a.momentum) start<T, true>(a, w, s, what); else start<T, false>(a, w, s, what));
+  const bool f32 = a.dt == DType::F32;
+  for (int i = 0; i + 1 < a.steps; ++i) {
+    // (the type of a 16-bit result matters to the last step alone)
+    const int pl = planes_of(a, i), next = planes_of(a, i + 1);
+    if (f32) step<float, true, 2, 2>(a, w, i, cus, s, what);
+    else if (pl == 2) step<half_t, false, 2, 2>(a, w, i, cus, s, what);
+    else if (next == 2) step<half_t, false, 1, 2>(a, w, i, cus, s, what);
+    else step<half_t, false, 1, 1>(a, w, i, cus, s, what);
+  }
+  if (f32) step<float, true, 2, 0>(a, w, a.steps - 1, cus, s, what);
+  else if (a.dt == DType::F16) step<half_t, false, 2, 0>(a, w, a.steps - 1, cus, s, what);
+  else step<bf16_t, false, 1, 0>(a, w, a.steps - 1, cus, s, what);
 }
 
 }  // namespace k

@@ -2400,7 +2400,7 @@ static void check_ortho(const char* name, int64_t m, int64_t n, int64_t steps, d
 // Matrices at once: as many as 4 GB of workspace hold, one at least.
 static int64_t ortho_group(k::Orthogonalize a, int64_t most) {
   a.count = 1;
-  const size_t each = k::orthogonalize_ws_bytes(a, rt().info().cu_count);
+  const size_t each = std::max<size_t>(k::orthogonalize_ws_bytes(a), 1);
   return std::max<int64_t>(1, std::min<int64_t>({most, (int64_t)(((size_t)4 << 30) / each), 65535}));
 }
 
@@ -2420,13 +2420,15 @@ TensorP orthogonalize(const TensorP& g, int64_t steps, float eps) {
   a.in.apart = a.out.apart = a.m * a.n;
   const int64_t all = g->numel() / a.in.apart, each = ortho_group(a, all);
   a.count = each;
-  BufferP ws = scratch(k::orthogonalize_ws_bytes(a, rt().info().cu_count));
+  const size_t wsb = k::orthogonalize_ws_bytes(a);
+  BufferP ws;
+  if (wsb) ws = scratch(wsb);
   for (int64_t i = 0; i < all; i += each) {
     a.count = std::min(each, all - i);
     const size_t at = (size_t)(i * a.in.apart) * dtype_size(g->dtype);
     a.in.p[0] = c->data() + at;
     a.out.p[0] = out->data() + at;
-    k::orthogonalize(a, ws->ptr, rt().info().cu_count, rt().stream());
+    k::orthogonalize(a, ws ? ws->ptr : nullptr, rt().info().cu_count, rt().stream());
   }
   return out;
 }
@@ -2481,7 +2483,9 @@ void muon_step_(const std::vector<TensorP>& w, const std::vector<TensorP>& mom, 
   a.rate = (float)(o.lr * std::sqrt(std::max(1.0, (double)a.m / (double)a.n)));
   const int64_t all = (int64_t)w.size(), each = ortho_group(a, std::min<int64_t>(all, k::kOrthoMats));
   a.count = each;
-  BufferP ws = scratch(k::orthogonalize_ws_bytes(a, rt().info().cu_count));
+  const size_t wsb = k::orthogonalize_ws_bytes(a);
+  BufferP ws;
+  if (wsb) ws = scratch(wsb);
   for (int64_t i = 0; i < all; i += each) {
     a.count = std::min(each, all - i);
     for (int64_t j = 0; j < a.count; ++j) {
@@ -2489,7 +2493,7 @@ void muon_step_(const std::vector<TensorP>& w, const std::vector<TensorP>& mom, 
       a.out.p[j] = w[i + j]->data();
       a.mom.p[j] = mom[i + j]->data();
     }
-    k::orthogonalize(a, ws->ptr, rt().info().cu_count, rt().stream());
+    k::orthogonalize(a, ws ? ws->ptr : nullptr, rt().info().cu_count, rt().stream());
   }
 }
 

@@ -3,8 +3,8 @@ float64.
 
 Bars.  What the device rounds is known: the factors of every product, to one
 float16 plane (bfloat16, and float16 before the last three steps) or two
-(float32, float16's last three steps and all of its small matrices'), and the
-sums to float32.  The
+(float32, float16's last three steps, float16 of a short side and all small
+matrices), and the sums to float32.  The
 oracle makes the same roundings on the same matrix, and what they do to it,
 d = oracle with roundings - oracle without, measures the conditioning of this
 matrix; the device's roundings fall elsewhere (sums differ in their last
@@ -23,7 +23,7 @@ pytestmark = pytest.mark.gpu
 DTYPES = ["float32", "float16", "bfloat16"]
 HALF_STEP = {"float32": 2.0 ** -24, "float16": 2.0 ** -11, "bfloat16": 2.0 ** -8}
 SHAPES = [(1, 1), (1, 5), (7, 3), (33, 65), (64, 128), (128, 64), (130, 257), (200, 40), (3, 70, 70),
-          (32, 257, 300), (32, 300, 257), (64, 257, 260), (64, 260, 257), (2, 3, 16, 24)]
+          (32, 257, 300), (32, 300, 257), (64, 257, 260), (64, 260, 257), (2, 3, 16, 24), (10, 128), (1, 512), (512, 20), (128, 128), (100, 160), (129, 33)]
 
 
 def _dev(gpu, a, dtype="float32"):
@@ -43,9 +43,10 @@ def _gradient(shape, dtype, seed=0, size=1e-3):
 def _bars(g, dtype, **kw):
     """(result, bar of the Frobenius norm, bar of a value) of each matrix."""
     want = O.orthogonalize(g, **kw)
-    steps = kw.get("steps", 5)
-    halves = {"float32": [2] * steps, "bfloat16": [1] * steps,
-              "float16": [2 if i + 3 >= steps or min(g.shape[-2:]) <= 256 else 1 for i in range(steps)]}[dtype]
+    steps, (m, n) = kw.get("steps", 5), g.shape[-2:]
+    small = min(m, n) <= 128 and -(-m // 32) * -(-n // 32) <= 16
+    halves = {"float32": [2] * steps, "bfloat16": [2 if small else 1] * steps,
+              "float16": [2 if i + 3 >= steps or min(m, n) <= 256 else 1 for i in range(steps)]}[dtype]
     d = O.orthogonalize(g, halves=halves, **kw) - want
     side = np.sqrt(min(g.shape[-2:]))
     sums = 15 * 2.0 ** -22 * side
