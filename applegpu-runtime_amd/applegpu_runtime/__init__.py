@@ -698,8 +698,8 @@ def linear_cross_entropy(x, weight, targets):
     targets [...] (int32 or int64), (loss, lse), float32 [...], where lse = log
     sum exp(logits) and loss = lse - logits[target].  A target outside [0, V)
     (padding) has loss 0.  A nearly certain word's loss keeps its digits.  A
-    row with a logit of NaN or +inf gives NaN, and so does a float32 row whose
-    x is not finite.
+    row with a logit of NaN or +inf gives NaN, and so does a float32 x or weight
+    that is not finite.
 
     Products are summed in float32; float32 operands count with 22 bits of
     each value, by magnitudes of at least 2^-27 of the operand's largest."""

@@ -68,61 +68,78 @@ __device__ __forceinline__ float block_max(float v, float* red) {
 }
 
 constexpr int kParts = 512;  // blocks of the largest magnitude's first pass
-// part[b] = the largest finite magnitude of every kParts-th run of x [rows, n].
-__global__ void __launch_bounds__(256) most_kernel(const float* x, int64_t rows, int64_t n, int64_t ld, float* part) {
+struct Rows32 {
+  const float* x;
+  int64_t rows, n, ld;
+};
+// part[y][b] = the largest finite magnitude of every kParts-th run of operand y.
+__global__ void __launch_bounds__(256) most_kernel(Rows32 x0, Rows32 x1, float* part) {
   __shared__ float red[4];
+  const Rows32 o = blockIdx.y ? x1 : x0;
   float m = 0.f;
-  if (ld == n && n % 4 == 0 && ((uintptr_t)x & 15) == 0) {
-    const int64_t q = rows * n / 4;
+  if (o.ld == o.n && o.n % 4 == 0 && ((uintptr_t)o.x & 15) == 0) {
+    const int64_t q = o.rows * o.n / 4;
 #pragma unroll 4
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < q; i += (int64_t)gridDim.x * 256) {
-      const float4 v = ((const float4*)x)[i];
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < q; i += (int64_t)kParts * 256) {
+      const float4 v = ((const float4*)o.x)[i];
       m = fmaxf(fmaxf(m, fmaxf(finite_abs(v.x), finite_abs(v.y))), fmaxf(finite_abs(v.z), finite_abs(v.w)));
     }
   } else {
-    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x)
-      for (int64_t i = threadIdx.x; i < n; i += 256) m = fmaxf(m, finite_abs(x[r * ld + i]));
+    for (int64_t r = blockIdx.x; r < o.rows; r += kParts)
+      for (int64_t i = threadIdx.x; i < o.n; i += 256) m = fmaxf(m, finite_abs(o.x[r * o.ld + i]));
   }
   m = block_max(m, red);
-  if (threadIdx.x == 0) part[blockIdx.x] = m;
+  if (threadIdx.x == 0) part[blockIdx.y * kParts + blockIdx.x] = m;
 }
-// The power of the largest |g| + |h|.
-__global__ void __launch_bounds__(1024) grad_power_kernel(const float* g, const float* h, int64_t R, float2* power) {
-  __shared__ float red[16];
-  float m = 0.f;
-  for (int64_t i = threadIdx.x; i < R; i += 1024) m = fmaxf(m, finite_abs(g[i]) + (h ? finite_abs(h[i]) : 0.f));
-  m = block_max(m, red);
-  if (threadIdx.x == 0) *power = power_for(m);
+// The power of kParts parts, for a block of 256.
+__device__ __forceinline__ float2 power_of_parts(const float* part, float* red) {
+  static_assert(kParts == 512, "two parts a thread");
+  return power_for(block_max(fmaxf(part[threadIdx.x], part[threadIdx.x + 256]), red));
 }
-
 // Rows [rows, n] as 16-bit rows of ld values, zeros behind n: fp32 as planes of
-// x times its power of two (from part), 16-bit values as they are.
+// x times its power of two (from part; and the other operand's power, where it
+// is asked for), 16-bit values as they are.
 template <typename TI, typename T, int PL>
 __global__ void __launch_bounds__(256) pack_kernel(const TI* x, int64_t rows, int64_t n, int64_t ldi, const float* part,
-                                                   float2* power, T* out, int64_t ld) {
+                                                   float2* power, const float* other_part, float2* other_power, T* out,
+                                                   int64_t ld) {
   __shared__ float red[4];
   float s = 1.f;
   if constexpr (PL == 2) {
-    const float2 pw = power_for(block_max(fmaxf(part[threadIdx.x], part[threadIdx.x + 256]), red));
+    const float2 pw = power_of_parts(part, red);
     s = pw.x;
     if (blockIdx.x == 0 && threadIdx.x == 0) *power = pw;
-  }
-  const int64_t chunks = ld / (8 * PL), total = rows * chunks;
-  const bool whole = ldi % 8 == 0 && ((uintptr_t)x & 15) == 0;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / chunks, c = (i - r * chunks) * 8;
-    float v[8];
-    const TI* at = x + r * ldi + c;
-    if (whole && c + 8 <= n) {
-      struct alignas(16) V { TI e[8]; };
-      const V t = *(const V*)at;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = to_f(t.e[e]) * s;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = c + e < n ? to_f(at[e]) * s : 0.f;
+    if (other_power && blockIdx.x == 0) {
+      const float2 o = power_of_parts(other_part, red);
+      if (threadIdx.x == 0) *other_power = o;
     }
-    put_planes<T, PL>(out + r * ld, c, v);
+  }
+  const int chunks = (int)(ld / (8 * PL));
+  const int64_t total = rows * chunks, apart = (int64_t)gridDim.x * 256;
+  struct V { TI e[8]; };
+  for (int64_t i0 = (int64_t)blockIdx.x * 256 + threadIdx.x; i0 < total; i0 += 2 * apart) {
+    V t[2] = {};
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int64_t i = i0 + q * apart;
+      if (i >= total) continue;
+      const int64_t r = i / chunks, c = (i - r * chunks) * 8;
+      const TI* at = x + r * ldi + c;
+      if (c + 8 <= n) __builtin_memcpy(&t[q], at, sizeof(V));  // (at any alignment)
+      else
+        for (int e = 0; e < 8; ++e)
+          if (c + e < n) t[q].e[e] = at[e];
+    }
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int64_t i = i0 + q * apart;
+      if (i >= total) continue;
+      const int64_t r = i / chunks, c = (i - r * chunks) * 8;
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = to_f(t[q].e[e]) * s;
+      put_planes<T, PL>(out + r * ld, c, v);
+    }
   }
 }
 
@@ -198,7 +215,7 @@ struct EpiLoss {
   }
   template <class TL>
   __device__ __forceinline__ void store(const Args& p, const Place& c, typename TL::T* lds, typename TL::Acc& acc) const {
-    float2* pair = (float2*)(lds + TL::STAGE);  // [BM][WN]
+    float2* pair = (float2*)lds;  // [BM][WN]
 #pragma unroll
     for (int i = 0; i < TL::TM; ++i)
       if (c.lane < 32) pair[TL::row_of(c, i) * TL::WN + c.wn] = make_float2(acc[i][0][0], acc[i][0][1]);
@@ -250,9 +267,43 @@ __global__ void __launch_bounds__(256) loss_kernel(const float2* part, int64_t p
 }
 
 // ── backward ──────────────────────────────────────────────────────────────
-// d of the tile's logits, times the power of the rows' gradients; zeros behind
-// the words up to the row's end.  Formed where the accumulators are, from the
-// few rows that a lane has.
+// What a row of d is made of: {lse, weight of p, d of the target in 16 bits,
+// what that rounding lost}.  The first two of d hold the power of the largest
+// |g| + |h| (not for bf16, whose range needs none).  A row's largest part is its
+// target's, alone in its size, so its rounding would be dx's: dx gets back what
+// it lost times the target's weights (fp16, 30 rows: error of dx 3.3e-4, so
+// 2.2e-4; of dw, where a word's rows have errors of their own, 3e-4).  Every
+// block finds the power from all rows.
+template <typename T, int PL>
+__global__ void __launch_bounds__(1024) rows_kernel(const float* g, const float* h, const float* loss, const float* lse,
+                                                    const void* targets, bool wide, int64_t R, int64_t V, float2* power,
+                                                    float4* rows) {
+  __shared__ float red[16];
+  float up = 1.f;
+  if constexpr (!std::is_same<T, bf16_t>::value) {
+    float m = 0.f;
+    for (int64_t i = threadIdx.x; i < R; i += 1024) m = fmaxf(m, finite_abs(g[i]) + (h ? finite_abs(h[i]) : 0.f));
+    const float2 pw = power_for(block_max(m, red));
+    if (blockIdx.x == 0 && threadIdx.x == 0) *power = pw;
+    up = pw.x;
+  }
+  const int64_t r = (int64_t)blockIdx.x * 1024 + threadIdx.x;
+  if (r >= R) return;
+  const bool there = target_of(targets, wide, r, V) >= 0;
+  const float gr = there ? g[r] : 0.f, hr = h ? h[r] : 0.f;
+  // p - 1 of the target from its loss, which keeps the digits of 1 - p
+  const float dt = there ? gr * expm1f(-loss[r]) + hr * expf(-loss[r]) : 0.f;
+  float held = dt * up, lost = 0.f;
+  if constexpr (PL == 1) {
+    held = to_f(from_f<T>(dt * up));
+    lost = (dt * up - held) / up;
+    if (!(fabsf(lost) < kInf)) lost = 0.f;
+  }
+  rows[r] = make_float4(lse[r], (gr + hr) * up, held, lost);
+}
+
+// d of the tile's logits; zeros behind the words up to the row's end.  Formed
+// where the accumulators are, from the few rows that a lane has.
 template <typename T>
 struct EpiGrad {
   T* d;
@@ -260,58 +311,42 @@ struct EpiGrad {
   int64_t v0, V;  // the piece's first word; all words
   const void* targets;
   bool wide;
-  const float *loss, *lse, *g, *h;
-  const float2 *px, *pw, *pg;
+  const float4* rows;
+  const float2 *px, *pw;
   template <class TL>
   __device__ __forceinline__ void form(const Args& p, const Place& c, typename TL::Acc& acc) const {
     constexpr int PL = TL::PL, TM = TL::TM, TN = TL::TN;
-    float ux = 1.f, uw = 1.f, up = 1.f;
+    float ux = 1.f, uw = 1.f;
     if constexpr (PL == 2) { ux = px->y; uw = pw->y; }
-    if (pg) up = pg->x;
     const int64_t cols = c.n0 + c.wn * 32 * TN;
     const bool ragged = cols + 32 * TN > p.N;
     const int hi = c.lane >> 5;
-    float l[TM], all[TM], gr[TM], hr[TM];
+    float4 of[TM];
     int rel[TM];
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
       const int64_t row = c.m0 + TL::row_of(c, i), at = row < p.M ? row : p.M - 1;
       const int64_t t = row < p.M ? target_of(targets, wide, at, V) : -1, far = t - v0 - cols;
-      gr[i] = t >= 0 ? g[at] : 0.f;
-      hr[i] = h ? h[at] : 0.f;
-      all[i] = (gr[i] + hr[i]) * up;
-      l[i] = lse[at];
+      of[i] = rows[at];
       rel[i] = t >= 0 && far >= 0 && far < 32 * TN && ((far >> 2) & 1) == hi ? (int)far - 4 * hi : -1;
     }
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
-      // a row without weight has no gradient, whatever its logits are
-      const bool none = gr[i] == 0.f && hr[i] == 0.f;
-      float zt = 0.f;
-      if (rel[i] >= 0) {
-#pragma unroll
-        for (int j = 0; j < TN; ++j)
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (rel[i] == j * 32 + 8 * (e >> 2) + (e & 3)) zt = acc[i][j][e];
-        if constexpr (PL == 2) zt = zt * ux * uw;
-      }
+      const bool none = of[i].y == 0.f && of[i].z == 0.f;  // without weight: no gradient, whatever the logits are
 #pragma unroll
       for (int j = 0; j < TN; ++j)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           float z = acc[i][j][e];
           if constexpr (PL == 2) z = z * ux * uw;
-          acc[i][j][e] = none ? 0.f : exp_fast(z - l[i]) * all[i];
+          acc[i][j][e] = none ? 0.f : exp_fast(z - of[i].x) * of[i].y;
         }
-      // p - 1 of the target from its loss, which keeps the digits of 1 - p
       if (rel[i] >= 0 && !none) {
-        const float dt = (gr[i] * expm1f(-loss[c.m0 + TL::row_of(c, i)]) + hr[i] * exp_fast(zt - l[i])) * up;
 #pragma unroll
         for (int j = 0; j < TN; ++j)
 #pragma unroll
           for (int e = 0; e < 16; ++e)
-            if (rel[i] == j * 32 + 8 * (e >> 2) + (e & 3)) acc[i][j][e] = dt;
+            if (rel[i] == j * 32 + 8 * (e >> 2) + (e & 3)) acc[i][j][e] = of[i].z;
       }
       if (ragged) {
 #pragma unroll
@@ -334,6 +369,23 @@ struct EpiGrad {
   }
 };
 
+// What dx gets back of its targets' parts (rows null: nothing).
+template <typename TO>
+struct Lost {
+  const TO* w = nullptr;
+  int64_t ldw = 0, V = 0;
+  const void* targets = nullptr;
+  bool wide = false;
+  const float4* rows = nullptr;
+  // the factor, and the weights it applies to from column k on
+  __device__ __forceinline__ float of(int64_t row, int64_t k, const TO** at) const {
+    if (!rows) return 0.f;
+    const int64_t t = target_of(targets, wide, row, V);
+    *at = w + t * ldw + k;
+    return t < 0 ? 0.f : rows[row].w;
+  }
+};
+
 // acc times the inverse powers, as outputs or as fp32 parts of a sum.
 template <typename TO>
 struct EpiOut {
@@ -341,6 +393,7 @@ struct EpiOut {
   float* part;   // [splits][M][N], or null
   bool more;     // parts are added to what is there
   const float2 *pa, *pb;
+  Lost<TO> lost;
   template <class TL>
   __device__ __forceinline__ void form(const Args&, const Place&, typename TL::Acc&) const {}
   template <class TL>
@@ -367,10 +420,16 @@ struct EpiOut {
             }
             return;
           }
+          const TO* wt = nullptr;
+          const float back = lost.of(row, col, &wt);
           constexpr int W = 16 / sizeof(TO);  // a store
           struct V { TO e[W]; } o[8 / W];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) o[e / W].e[e % W] = from_f<TO>(v[e] * ua * ub);
+          for (int e = 0; e < 8; ++e) {
+            v[e] = v[e] * ua * ub;
+            if (back != 0.f && e < n) v[e] += back * to_f(wt[e]);
+            o[e / W].e[e % W] = from_f<TO>(v[e]);
+          }
           if (n == 8) {
 #pragma unroll
             for (int q = 0; q < 8 / W; ++q) put_past(out + at + q * W, o[q]);
@@ -383,28 +442,41 @@ struct EpiOut {
   }
 };
 
-// out = the parts' sum times the inverse powers.
+// out [R, K] = the parts' sum times the inverse powers, and what they lost.
 template <typename TO>
-__global__ void __launch_bounds__(256) sum_parts_kernel(const float* part, int splits, int64_t n, const float2* pa,
-                                                        const float2* pb, TO* out) {
+__global__ void __launch_bounds__(256) sum_parts_kernel(const float* part, int splits, int64_t n, int64_t K,
+                                                        const float2* pa, const float2* pb, Lost<TO> lost, TO* out) {
   const float ua = pa ? pa->y : 1.f, ub = pb ? pb->y : 1.f;
   const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
   if (i >= n) return;
-  if (i + 4 <= n && n % 4 == 0) {
+  const TO* wt = nullptr;
+  if (K % 4 == 0) {
     float4 a = *(const float4*)(part + i);
+#pragma unroll 8
     for (int s = 1; s < splits; ++s) {
       const float4 b = *(const float4*)(part + s * n + i);
       a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
     }
-    struct V { TO e[4]; } o = {from_f<TO>(a.x * ua * ub), from_f<TO>(a.y * ua * ub), from_f<TO>(a.z * ua * ub),
-                               from_f<TO>(a.w * ua * ub)};
+    float v[4] = {a.x * ua * ub, a.y * ua * ub, a.z * ua * ub, a.w * ua * ub};
+    const int64_t r = i / K;
+    const float back = lost.of(r, i - r * K, &wt);
+    struct V { TO e[4]; } o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (back != 0.f) v[e] += back * to_f(wt[e]);
+      o.e[e] = from_f<TO>(v[e]);
+    }
     __builtin_memcpy(out + i, &o, sizeof(o));
     return;
   }
   for (int64_t j = i; j < n && j < i + 4; ++j) {
     float a = part[j];
+#pragma unroll 8
     for (int s = 1; s < splits; ++s) a += part[s * n + j];
-    out[j] = from_f<TO>(a * ua * ub);
+    a = a * ua * ub;
+    const float back = lost.of(j / K, j % K, &wt);
+    if (back != 0.f) a += back * to_f(*wt);
+    out[j] = from_f<TO>(a);
   }
 }
 
@@ -420,64 +492,95 @@ struct Carver {
   }
 };
 
+
 bool direct(const void* p, int64_t ld, int64_t K) {
   return K % 8 == 0 && ld % 8 == 0 && ((uintptr_t)p & 15) == 0 && ld < (1 << 21);
 }
 
-// x [rows, K] as an operand: in place, or packed into the workspace.
+// The operands x and w as a product takes them: in place, packed into the
+// workspace, or (raw) w as the fp32 rows that it is.
 struct Packed {
   Operand o;
   float2* power = nullptr;
 };
+struct Both {
+  Packed x, w;
+};
 template <typename TI, typename T, int PL>
-Packed ready(const void* x, int64_t rows, int64_t K, int64_t ld, Carver& ws, hipStream_t s) {
-  Packed r;
-  if (PL == 1 && direct(x, ld, K)) {
-    r.o = {x, ld, 0};
-    return r;
-  }
-  const int64_t kp = (K + 31) / 32 * 32 * PL;
-  T* out = ws.take<T>((size_t)(rows * kp));
+Both ready(const LinearCE& a, bool raw, Carver& ws, hipStream_t s) {
+  Both b;
   float* part = nullptr;
-  if (PL == 2) {
-    part = ws.take<float>(kParts);
-    r.power = ws.take<float2>(1);
-  }
-  r.o = {out, kp, 0};
-  if (!ws.base) return r;
   if constexpr (PL == 2) {
-    hipLaunchKernelGGL(most_kernel, dim3(kParts), dim3(256), 0, s, (const float*)x, rows, K, ld, part);
-    check_launch("linear_cross_entropy");
+    part = ws.take<float>(2 * kParts);
+    b.x.power = ws.take<float2>(1);
+    b.w.power = ws.take<float2>(1);
+    if (ws.base) {
+      hipLaunchKernelGGL(most_kernel, dim3(kParts, 2), dim3(256), 0, s, Rows32{(const float*)a.x, a.R, a.K, a.ldx},
+                         Rows32{(const float*)a.w, a.V, a.K, a.ldw}, part);
+      check_launch("linear_cross_entropy");
+    }
   }
-  const int64_t chunks = rows * (kp / (8 * PL));
-  const unsigned blocks = (unsigned)std::min<int64_t>(blocks_for(chunks, 256), 4096);
-  hipLaunchKernelGGL((pack_kernel<TI, T, PL>), dim3(blocks), dim3(256), 0, s, (const TI*)x, rows, K, ld, part, r.power,
-                     out, kp);
-  check_launch("linear_cross_entropy");
-  return r;
+  auto pack = [&](Packed& p, const void* x, int64_t rows, int64_t ld, const float* mine, const float* other_part,
+                  float2* other) {
+    if (PL == 1 && direct(x, ld, a.K)) {
+      p.o = {x, ld, 0};
+      return;
+    }
+    const int64_t kp = (a.K + 31) / 32 * 32 * PL;
+    T* out = ws.take<T>((size_t)(rows * kp));
+    p.o = {out, kp, 0};
+    if (!ws.base) return;
+    const unsigned blocks = (unsigned)std::min<int64_t>(blocks_for(rows * (kp / (8 * PL)), 512), 4096);
+    hipLaunchKernelGGL((pack_kernel<TI, T, PL>), dim3(blocks), dim3(256), 0, s, (const TI*)x, rows, a.K, ld, mine,
+                       p.power, other_part, other, out, kp);
+    check_launch("linear_cross_entropy");
+  };
+  pack(b.x, a.x, a.R, a.ldx, part, part ? part + kParts : nullptr, raw ? b.w.power : nullptr);
+  if (raw) b.w.o = {a.w, 2 * a.ldw, 0};
+  else pack(b.w, a.w, a.V, a.ldw, part ? part + kParts : nullptr, nullptr, nullptr);
+  return b;
 }
 
-// Tiles: 256 x 256 (8 wavefronts), 128 x 128 (4), 32 x 128 (4).
-enum { kBig, kMid, kFew };
-int pick(int64_t M, int64_t N, int64_t splits, int cus) {
+// Tiles of 8 wavefronts: 256 x 256, 128 x 128, 64 x 128; of 4: 32 x 128.
+enum { kBig, kMid, kThin, kFew };
+// Forward in us, 256 / 128 / 64 / 32 rows a tile:
+//   1 x 50257 x 1280 fp16     35 / 25 / 25 / 24
+//   61 x 50257 x 1280 fp16    37 / 27 / 26 / 31
+//   509 x 50257 x 768 bf16    52 / 54 / 60       (394 and 1572 tiles)
+//   1111 x 10007 x 515 fp16   38 / 42 / 46       (200 and 711)
+//   1000 x 2000 x 512 bf16    22 / 12 / 11       (32 and 128)
+// A round of 128-wide tiles, two a compute unit, takes 0.53 times a round of
+// 256-wide ones.  (Splitting fp32 words takes registers that 256 x 256 does not
+// have.)
+int pick(int64_t M, int64_t N, bool raw, int cus) {
   if (M <= 32) return kFew;
-  return ceil_div(M, 256) * ceil_div(N, 256) * splits * 4 >= 3 * cus ? kBig : kMid;
+  if (M <= 64) return kThin;
+  const double big = (double)ceil_div(ceil_div(M, 256) * ceil_div(N, 256), cus);
+  const double mid = (double)ceil_div(ceil_div(M, 128) * ceil_div(N, 128), 2 * cus);
+  return !raw && big <= 0.53 * mid ? kBig : kMid;
 }
 int bn_of(int tile) { return tile == kBig ? 256 : 128; }
 
-template <typename T, int PL, bool AC, bool BC, class Epi>
+template <typename T, int PL, bool RAW, class Epi>
 void run(int tile, const Args& p, const Epi& e, hipStream_t s, const char* what) {
-  if (tile == kBig) launch<Tile<T, 4, 2, 2, 4, PL, AC, BC>>(p, e, s, what);
-  else if (tile == kMid) launch<Tile<T, 2, 2, 2, 2, PL, AC, BC>>(p, e, s, what);
-  else launch<Tile<T, 1, 1, 1, 4, PL, AC, BC>>(p, e, s, what);
+  if (tile == kBig && !RAW) launch<Tile<T, 4, 2, 2, 4, PL, false, false>>(p, e, s, what);
+  else if (tile == kMid) launch<Tile<T, 2, 1, 2, 4, PL, false, false, false, RAW>>(p, e, s, what);
+  else if (tile == kThin) launch<Tile<T, 1, 1, 2, 4, PL, false, false, false, RAW>>(p, e, s, what);
+  else launch<Tile<T, 1, 1, 1, 4, PL, false, false, false, RAW>>(p, e, s, what);
 }
 
 template <typename TI, typename T, int PL>
 size_t forward(const LinearCE& a, void* wsp, int cus, hipStream_t s) {
   const char* what = "linear_cross_entropy";
   Carver ws{(char*)wsp};
-  const Packed x = ready<TI, T, PL>(a.x, a.R, a.K, a.ldx, ws, s), w = ready<TI, T, PL>(a.w, a.V, a.K, a.ldw, ws, s);
-  const int tile = pick(a.R, a.V, 1, cus);
+  // fp32 words of few rows are split where they are multiplied (packed, each is
+  // written and read once more), by every block that multiplies them: 50257 x
+  // 768, us, packed / split at 20 rows 119 / 62, 61: 122 / 72, 255: 145 / 129,
+  // 1023: 311 / 345
+  const bool raw = PL == 2 && a.R <= 320 && a.K % 4 == 0 && a.ldw % 4 == 0 && ((uintptr_t)a.w & 15) == 0;
+  const Both b = ready<TI, T, PL>(a, raw, ws, s);
+  const Packed &x = b.x, &w = b.w;
+  const int tile = pick(a.R, a.V, raw, cus);
   const int64_t parts = ceil_div(a.V, bn_of(tile));
   float2* part = ws.take<float2>((size_t)(parts * a.R));
   float* zt = ws.take<float>((size_t)a.R);
@@ -486,7 +589,10 @@ size_t forward(const LinearCE& a, void* wsp, int cus, hipStream_t s) {
   p.a = x.o; p.b = w.o;
   p.M = a.R; p.N = a.V; p.K = a.K;
   const bool wide = a.idx_dt == DType::I64;
-  run<T, PL, false, false>(tile, p, EpiLoss{part, zt, a.targets, wide, x.power, w.power}, s, what);
+  p.b_power = w.power;
+  const EpiLoss e{part, zt, a.targets, wide, x.power, w.power};
+  if (PL == 2 && raw) run<T, PL, PL == 2>(tile, p, e, s, what);
+  else run<T, PL, false>(tile, p, e, s, what);
   const int rx = a.R >= 64 * cus ? 64 : a.R >= 16 * cus ? 16 : a.R >= 4 * cus ? 4 : 1;
   hipLaunchKernelGGL(loss_kernel, dim3(blocks_for(a.R, rx)), dim3(256), 0, s, part, parts, zt, a.targets, wide, a.R,
                      a.V, rx, a.loss, a.lse);
@@ -497,20 +603,53 @@ size_t forward(const LinearCE& a, void* wsp, int cus, hipStream_t s) {
 // Values of d that are held at once: 2^29 (1 GB of 16 bits).
 constexpr int64_t kHeld = (int64_t)1 << 29;
 
-// Parts of dx's sum over the words, with the blocks of dw beside them: the
-// least of what a compute unit has to do, in stages of 64 k (a block's start
-// and end count as 4, half of a last block's length as waiting, a part's
-// writing and reading back by its bytes).
-int dx_parts(int64_t xtiles, int64_t stages, int64_t wtiles, int64_t wstages, int64_t values, int slots) {
-  int best = 1;
+// When n1 blocks of l1 stages and then n2 of l2 have all ended, one after
+// another on `slots` places.
+double ends(int64_t n1, double l1, int64_t n2, double l2, int64_t slots) {
+  const double whole = (double)(n1 / slots) * l1;  // by then every place is free of whole rounds
+  const int64_t late = n1 % slots;                 // places that take one more of the first
+  const double least = late ? whole + l1 : whole;
+  auto fit = [&](double t) {
+    return (int64_t)((t - whole) / l2 + 1e-6) * (slots - late) + (int64_t)((t - whole - l1) / l2 + 1e-6) * late >= n2;
+  };
+  double t = least;
+  for (int64_t k = n2 / slots; !fit(t) && k <= n2 + 1; ++k) {
+    const double a = whole + (double)k * l2, b = whole + l1 + (double)k * l2;
+    if (a >= least && fit(a)) t = a;
+    else if (b >= least && fit(b)) t = b;
+  }
+  return t;
+}
+
+// The products dx (over the words, in parts) and dw of a piece in one launch:
+// tiles and parts by the time they end, in us.  A stage of 64 k takes 1.75 us in
+// 256 x 256 tiles, 0.95 in 128 x 128 ones (two blocks a compute unit); a block's
+// start and end count as 4 stages; parts are written and read back at 6 TB/s
+// and summed by a launch of their own.  us at 2 / 4 / 8 / 16 / 32 parts, 256:
+// 61 x 50257 x 1280 fp16 536 / 287 / 165 / 114 / 106, 2047 x 10007 x 768 bf16
+// 187 / 138 / 163 / 171 / 219; 128: 275 / 155 / 103 / 103 / 100, 135 / 138 / 148
+// / 163 / 201.
+struct Plan {
+  bool big;
+  int parts;
+};
+Plan plan_products(int64_t R, int64_t K, int64_t words, int ks, int cus) {
+  Plan best{false, 1};
   double least = 1e300;
-  for (int s = 1; s <= 64 && s * 4 <= std::max<int64_t>(stages, 4); ++s) {
-    const double len = (double)ceil_div(stages, s) + 4, last = std::min<double>(len, (double)wstages + 4);
-    const double work = ((double)xtiles * s * len + (double)wtiles * ((double)wstages + 4)) / slots;
-    const double t = std::max(work, len) + 0.5 * last + (s > 1 ? s * (double)values * 8 / 8e6 : 0);
-    if (t < least) {
-      least = t;
-      best = s;
+  const double rows_len = (double)ceil_div(R, ks) + 4;
+  const int64_t stages = ceil_div(words, ks);
+  for (int big = R > 32 ? 1 : 0; big >= 0; --big) {
+    const int64_t side = big ? 256 : 128, xside = R <= 32 ? 32 : side;
+    const int64_t xtiles = ceil_div(R, xside) * ceil_div(K, side), wtiles = ceil_div(words, side) * ceil_div(K, side);
+    for (int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48}) {
+      if (s > 1 && s * 4 > stages) break;
+      const double len = (double)ceil_div(stages, s) + 4;
+      const double t = ends(xtiles * s, len, wtiles, rows_len, big ? cus : 2 * cus) * (big ? 1.75 : 0.95) +
+                       (s > 1 ? 4 + s * (double)(R * K) * 8 / 6e6 : 0);
+      if (t < least) {
+        least = t;
+        best = {big != 0, s};
+      }
     }
   }
   return best;
@@ -520,7 +659,8 @@ template <typename TI, typename T, int PL>
 size_t backward(const LinearCE& a, void* wsp, int cus, hipStream_t s) {
   const char* what = "linear_cross_entropy_backward";
   Carver ws{(char*)wsp};
-  const Packed x = ready<TI, T, PL>(a.x, a.R, a.K, a.ldx, ws, s), w = ready<TI, T, PL>(a.w, a.V, a.K, a.ldw, ws, s);
+  const Both b = ready<TI, T, PL>(a, false, ws, s);
+  const Packed &x = b.x, &w = b.w;
   const bool wide = a.idx_dt == DType::I64;
   // pieces of the vocabulary, whole tiles of it
   const int64_t most = std::min<int64_t>(std::max<int64_t>(kHeld / PL / a.R / 256 * 256, 256), 1 << 19);
@@ -529,47 +669,44 @@ size_t backward(const LinearCE& a, void* wsp, int cus, hipStream_t s) {
   T* d = ws.take<T>((size_t)(a.R * ldd));
   constexpr bool scaled = !std::is_same<T, bf16_t>::value;
   float2* pg = scaled ? ws.take<float2>(1) : nullptr;
-  // both products of a piece in one launch: large tiles where they fill the
-  // chip at one block a compute unit
-  const bool big = a.R > 32 && ceil_div(len, 256) * ceil_div(a.K, 256) >= cus / 2;
-  const int64_t b = big ? 256 : 128, xb = a.R <= 32 ? 32 : b;
-  const int splits = dx_parts(ceil_div(a.R, xb) * ceil_div(a.K, b), ceil_div(len, 64 / PL),
-                              ceil_div(len, b) * ceil_div(a.K, b), ceil_div(a.R, 64 / PL), a.R * a.K, big ? cus : 2 * cus);
+  float4* rows = ws.take<float4>((size_t)a.R);
+  const Plan plan = plan_products(a.R, a.K, len, 64 / PL, cus);
+  const int splits = plan.parts;
   const bool parted = splits > 1 || pieces > 1;
   float* part = parted ? ws.take<float>((size_t)(splits * a.R * a.K)) : nullptr;
   if (!wsp) return ws.used;
-  if (scaled) {
-    hipLaunchKernelGGL(grad_power_kernel, dim3(1), dim3(1024), 0, s, a.g_loss, a.g_lse, a.R, pg);
-    check_launch(what);
-  }
+  hipLaunchKernelGGL((rows_kernel<T, PL>), dim3(blocks_for(a.R, 1024)), dim3(1024), 0, s, a.g_loss, a.g_lse, a.loss,
+                     a.lse, a.targets, wide, a.R, a.V, pg, rows);
+  check_launch(what);
+  const Lost<TI> lost{(const TI*)a.w, a.ldw, a.V, a.targets, wide, PL == 1 ? rows : nullptr};
   for (int64_t v0 = 0; v0 < a.V; v0 += each) {
     const int64_t n = std::min(each, a.V - v0);
     const Operand wp{(const T*)w.o.p + v0 * w.o.ld, w.o.ld, 0}, dp{d, ldd, 0};
     Args p;
     p.a = x.o; p.b = wp;
     p.M = a.R; p.N = n; p.K = a.K;
-    run<T, PL, false, false>(pick(a.R, n, 1, cus), p,
-                             EpiGrad<T>{d, ldd, v0, a.V, a.targets, wide, a.loss, a.lse, a.g_loss, a.g_lse, x.power,
-                                        w.power, pg}, s, what);
+    run<T, PL, false>(pick(a.R, n, false, cus), p,
+                      EpiGrad<T>{d, ldd, v0, a.V, a.targets, wide, rows, x.power, w.power}, s, what);
     Args px, pw;
     px.a = pw.a = dp;
     px.b = wp;
     px.M = a.R; px.N = a.K; px.K = n; px.splits = splits;
     pw.b = x.o;
     pw.M = n; pw.N = a.K; pw.K = a.R;
-    const EpiOut<TI> ex{(TI*)a.dx, part, v0 > 0, pg, w.power}, ew{(TI*)a.dw + v0 * a.K, nullptr, false, pg, x.power};
-    typedef Tile<T, 2, 2, 2, 2, PL, true, true> WMid;
-    if (big)
+    const EpiOut<TI> ex{(TI*)a.dx, part, v0 > 0, pg, w.power, lost},
+        ew{(TI*)a.dw + v0 * a.K, nullptr, false, pg, x.power, {}};
+    typedef Tile<T, 2, 2, 2, 2, PL, true, true> WFew;  // (of four wavefronts, as dx's)
+    if (plan.big)
       launch_pair<Tile<T, 4, 2, 2, 4, PL, false, true>, Tile<T, 4, 2, 2, 4, PL, true, true>>(px, ex, pw, ew, s, what);
     else if (a.R > 32)
-      launch_pair<Tile<T, 2, 2, 2, 2, PL, false, true>, WMid>(px, ex, pw, ew, s, what);
+      launch_pair<Tile<T, 2, 1, 2, 4, PL, false, true>, Tile<T, 2, 1, 2, 4, PL, true, true>>(px, ex, pw, ew, s, what);
     else
-      launch_pair<Tile<T, 1, 1, 1, 4, PL, false, true>, WMid>(px, ex, pw, ew, s, what);
+      launch_pair<Tile<T, 1, 1, 1, 4, PL, false, true>, WFew>(px, ex, pw, ew, s, what);
   }
   if (parted) {
     const int64_t n = a.R * a.K;
-    hipLaunchKernelGGL((sum_parts_kernel<TI>), dim3(blocks_for(n, 1024)), dim3(256), 0, s, part, splits, n, pg, w.power,
-                       (TI*)a.dx);
+    hipLaunchKernelGGL((sum_parts_kernel<TI>), dim3(blocks_for(n, 1024)), dim3(256), 0, s, part, splits, n, a.K, pg,
+                       w.power, lost, (TI*)a.dx);
     check_launch(what);
   }
   return ws.used;

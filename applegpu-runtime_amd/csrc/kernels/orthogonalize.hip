@@ -497,12 +497,25 @@ __device__ __forceinline__ f32x16 flat_product(const Flat& a, int ra, const Flat
   f32x16 high, cross;
 #pragma unroll
   for (int e = 0; e < 16; ++e) high[e] = cross[e] = 0.f;
-  for (int kk = 0; kk < k / 16; ++kk) {
-    const H8 ah = flat_read<AC>(a.high, a.ld, ra, kk, lane), al = flat_read<AC>(a.low, a.ld, ra, kk, lane);
-    const H8 bh = flat_read<BC>(b.high, b.ld, rb, kk, lane), bl = flat_read<BC>(b.low, b.ld, rb, kk, lane);
-    high = Mfma<half_t>::run(bh, ah, high);
-    cross = Mfma<half_t>::run(bl, ah, cross);
-    cross = Mfma<half_t>::run(bh, al, cross);
+  // the next step's fragments are read meanwhile
+  H8 f[2][4];
+  auto read = [&](int set, int kk) __attribute__((always_inline)) {
+    f[set][0] = flat_read<AC>(a.high, a.ld, ra, kk, lane);
+    f[set][1] = flat_read<AC>(a.low, a.ld, ra, kk, lane);
+    f[set][2] = flat_read<BC>(b.high, b.ld, rb, kk, lane);
+    f[set][3] = flat_read<BC>(b.low, b.ld, rb, kk, lane);
+  };
+  auto mul = [&](int set) __attribute__((always_inline)) {
+    high = Mfma<half_t>::run(f[set][2], f[set][0], high);
+    cross = Mfma<half_t>::run(f[set][3], f[set][0], cross);
+    cross = Mfma<half_t>::run(f[set][2], f[set][1], cross);
+  };
+  read(0, 0);
+  for (int kk = 0; kk < k / 16; kk += 2) {  // (an even number of steps)
+    read(1, kk + 1);
+    mul(0);
+    if (kk + 2 < k / 16) read(0, kk + 2);
+    mul(1);
   }
 #pragma unroll
   for (int e = 0; e < 16; ++e) high[e] += cross[e];
@@ -515,7 +528,7 @@ __device__ __forceinline__ void flat_put(const Flat& f, int row, int col, const 
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     h[e] = (_Float16)v[e];
-    l[e] = (_Float16)(fabsf((float)h[e]) < INFINITY ? v[e] - (float)h[e] : 0.f);
+    l[e] = (_Float16)(v[e] - (float)h[e]);
   }
   *(h4*)(f.high + row * f.ld + col) = h;
   *(h4*)(f.low + row * f.ld + col) = l;

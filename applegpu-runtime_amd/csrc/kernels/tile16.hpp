@@ -65,6 +65,7 @@ struct Args {
   int splits = 1, batches = 1;
   int stages = 0, per_split = 0;
   int group = 8;  // tile rows that share their columns' loads
+  const float2* b_power = nullptr;  // what fp32 rows of b are multiplied by before they are split (.x)
 };
 
 // An offset behind the end of every resource: what is copied from there is
@@ -90,7 +91,9 @@ __device__ __forceinline__ i16x4 read_transposed(const __attribute__((address_sp
 
 // One operand's part of a block: B rows (m) of it, L windows of 1 KB a
 // wavefront and stage.
-template <typename T, int B, int L, int PL, bool COLS>
+// RAW: rows of fp32 values, in the place of their planes (32 a stage; K and ld
+// multiples of 4, ld and offsets in 16-bit units all the same).
+template <typename T, int B, int L, int PL, bool COLS, bool RAW = false>
 struct Stream {
   static constexpr int KS = 64 / PL;                 // k of a stage
   static constexpr int CPR = COLS ? B * PL / 8 : 8;  // 16-byte chunks of a k row, or of a row's stage
@@ -111,7 +114,7 @@ struct Stream {
     k_rows = K;
     // values of a row from base on (rows: with the zeros up to a whole chunk,
     // or a whole group of planes)
-    width = COLS ? ld - m0 * PL : PL == 1 ? (K + 7) / 8 * 8 : (K + 31) / 32 * 64;
+    width = COLS ? ld - m0 * PL : PL == 1 ? (K + 7) / 8 * 8 : RAW ? K * 2 : (K + 31) / 32 * 64;
     if (!COLS) rows = resource(base, ((M - m0 - 1) * ld + width) * (int64_t)sizeof(T));
 #pragma unroll
     for (int q = 0; q < L; ++q) {
@@ -163,6 +166,23 @@ struct Stream {
   }
 };
 
+// 8 fp32 values of a row of a RAW stage (step kk of 16 k), and their planes.
+struct Raw8 { float e[8]; };
+__device__ __forceinline__ Raw8 read_raw(const half_t* from, int blk, int kk, int lane) {
+  const int r = blk * 32 + (lane & 31), c = 4 * kk + 2 * (lane >> 5), x = (r >> 1) & 7;
+  Raw8 v;
+  *(float4*)v.e = *(const float4*)(from + r * 64 + ((c ^ x) << 3));
+  *(float4*)(v.e + 4) = *(const float4*)(from + r * 64 + (((c + 1) ^ x) << 3));
+  return v;
+}
+__device__ __forceinline__ void split_raw(const Raw8& v, float power, Mfma<half_t>::vec& h, Mfma<half_t>::vec& l) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    h[e] = (_Float16)(v.e[e] * power);
+    l[e] = (_Float16)fmaf(v.e[e], power, -(float)h[e]);
+  }
+}
+
 // Where a block stands.
 struct Place {
   int64_t m0, n0;
@@ -170,20 +190,23 @@ struct Place {
   int wave, wm, wn, lane;
 };
 
-template <typename T_, int TM_, int TN_, int WM_, int WN_, int PL_, bool AC_, bool BC_, bool SYM_ = false>
+template <typename T_, int TM_, int TN_, int WM_, int WN_, int PL_, bool AC_, bool BC_, bool SYM_ = false,
+          bool RAW_ = false>
 struct Tile {
   typedef T_ T;
   static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, PL = PL_;
   static constexpr bool SYM = SYM_;  // tiles on and below the diagonal only
+  static constexpr bool RAW = RAW_;  // B is fp32 rows, split into planes in registers
   static constexpr int NW = WM * WN, BM = 32 * TM * WM, BN = 32 * TN * WN;
   static constexpr int KS = 64 / PL, KK = KS / 16;
   static constexpr int AW = BM / 8, BW = BN / 8, STAGE = (AW + BW) * 512;  // 16-bit values
   static constexpr int LDS = 2 * STAGE;
   static_assert(AW % NW == 0 && BW % NW == 0, "tile shape");
-  // the epilogue stages 32 rows of every wavefront in the second stage's place
-  static_assert(NW * 32 * 32 * TN * 4 <= STAGE * 2, "epilogue staging");
+  // the epilogue stages 32 rows of every wavefront in the operands' place
+  static_assert(NW * 32 * 32 * TN * 4 <= LDS * 2, "epilogue staging");
   typedef Stream<T, BM, AW / NW, PL, AC_> SA;
-  typedef Stream<T, BN, BW / NW, PL, BC_> SB;
+  typedef Stream<T, BN, BW / NW, PL, BC_, RAW> SB;
+  static_assert(!RAW || (PL == 2 && !BC_), "fp32 rows of a product of planes");
   typedef typename Mfma<T>::vec V8;
   typedef f32x16 Acc[TM][TN];
 
@@ -239,10 +262,15 @@ struct Tile {
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
     V8 fa[2][TM], fb[2][TN];
+    Raw8 raw[2][TN];
+    const float power = RAW ? p.b_power->x : 1.f;
     auto read = [&](int set, int st, int kk) __attribute__((always_inline)) {
       const T* from = lds + (st & 1) * STAGE;
 #pragma unroll
-      for (int j = 0; j < TN; ++j) fb[set][j] = SB::read(from + AW * 512, c.wn * TN + j, kk, 0, c.lane);
+      for (int j = 0; j < TN; ++j) {
+        if constexpr (RAW) raw[set][j] = read_raw((const half_t*)from + AW * 512, c.wn * TN + j, kk, c.lane);
+        else fb[set][j] = SB::read(from + AW * 512, c.wn * TN + j, kk, 0, c.lane);
+      }
 #pragma unroll
       for (int i = 0; i < TM; ++i) fa[set][i] = SA::read(from, c.wm * TM + i, kk, 0, c.lane);
     };
@@ -291,15 +319,24 @@ struct Tile {
       V8 la[TM], lb[TN];
       auto read_low = [&](int st, int kk) __attribute__((always_inline)) {
         const T* from = lds + (st & 1) * STAGE;
+        if constexpr (!RAW) {
 #pragma unroll
-        for (int j = 0; j < TN; ++j) lb[j] = SB::read(from + AW * 512, c.wn * TN + j, kk, 1, c.lane);
+          for (int j = 0; j < TN; ++j) lb[j] = SB::read(from + AW * 512, c.wn * TN + j, kk, 1, c.lane);
+        }
 #pragma unroll
         for (int i = 0; i < TM; ++i) la[i] = SA::read(from, c.wm * TM + i, kk, 1, c.lane);
+      };
+      auto split = [&](int set) __attribute__((always_inline)) {
+        if constexpr (RAW) {
+#pragma unroll
+          for (int j = 0; j < TN; ++j) split_raw(raw[set][j], power, fb[set][j], lb[j]);
+        }
       };
       for (int st = 0; st < nk; ++st) {
         __builtin_amdgcn_s_waitcnt(kReads);
         __builtin_amdgcn_sched_barrier(0);
         read_low(st, 0);
+        split(0);
         __builtin_amdgcn_sched_barrier(0);
         mul(fa[0], fb[0]);
         __builtin_amdgcn_sched_barrier(0);
@@ -309,6 +346,7 @@ struct Tile {
         mul(la, fb[0]);
         __builtin_amdgcn_sched_barrier(0);
         read_low(st, 1);
+        split(1);
         __builtin_amdgcn_sched_barrier(0);
         mul(fa[1], fb[1]);
         next(st);
@@ -378,8 +416,7 @@ struct Tile {
     }
   };
 
-  // Through this wavefront's own part of LDS (in the second stage's place), 32
-  // rows at a time: fr(row, column, v) for 8 columns of each row and, where
+  // Through this wavefront's own part of LDS, 32 rows at a time: fr(row, column, v) for 8 columns of each row and, where
   // `with` is true, fc(row, column, v) for 8 rows of each column (row, column:
   // of the product).  A row's 16-byte chunks are exchanged so that 16 rows at
   // one chunk cover all banks.  The loops stay rolled: unrolled, their
@@ -387,7 +424,7 @@ struct Tile {
   template <bool COLUMNS, class FR, class FC>
   static __device__ __forceinline__ void runs(const Place& c, T* lds, const Acc& acc, bool with, FR fr, FC fc) {
     constexpr int CN = 32 * TN, LPR = CN / 8, RPI = 64 / LPR;
-    float* ct = (float*)(lds + STAGE) + c.wave * 32 * CN;
+    float* ct = (float*)lds + c.wave * 32 * CN;
     const int l31 = c.lane & 31, hi = c.lane >> 5;
     auto at = [&](int r, int chunk) { return r * CN + ((TN == 1 ? chunk ^ ((r >> 1) & 7) : chunk ^ (r & 15)) << 2); };
 #pragma unroll
@@ -509,11 +546,7 @@ __device__ __forceinline__ void put_planes(T* row, int64_t col, const float (&v)
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     h.e[e] = from_f<T>(v[e]);
-    if constexpr (PL == 2) {
-      const float hf = to_f(h.e[e]);
-      // an infinity has no low half (inf - inf)
-      l.e[e] = from_f<T>(fabsf(hf) < INFINITY ? v[e] - hf : 0.f);
-    }
+    if constexpr (PL == 2) l.e[e] = from_f<T>(v[e] - to_f(h.e[e]));  // (an infinity's is NaN)
   }
   put_past(at, h);
   if constexpr (PL == 2) put_past(at + 32, l);
