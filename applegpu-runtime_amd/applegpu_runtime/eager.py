@@ -13,7 +13,7 @@ from ctypes import c_double, c_int64, c_uint32, c_uint64
 
 import numpy as np
 
-from ._native import lib, eager_error, DTYPE_CODES, CODE_DTYPES
+from ._native import lib, eager_error, ffi_error, DTYPE_CODES, CODE_DTYPES
 
 _ready = False
 
@@ -228,6 +228,30 @@ def sgd_sum_rows_(bias, g, alpha=1.0):
 def mse_loss_grad(out, y):
     """(mean((out - y)^2), d loss / d out) in one launch."""
     return op("mse_loss_grad", [out, y], nout=2)
+
+
+def linear_cross_entropy(x, w, targets):
+    """(loss, lse) of the logits x @ w^T over a vocabulary, which are not kept."""
+    return op("linear_cross_entropy", [x, w, targets], nout=2)
+
+
+def linear_cross_entropy_backward(grad_loss, x, w, targets, loss, lse, grad_lse=None):
+    """(dx, dw) of linear_cross_entropy, from the gradients of its outputs."""
+    ins = [grad_loss, x, w, targets, loss, lse] + ([grad_lse] if grad_lse is not None else [])
+    return op("linear_cross_entropy_backward", ins, nout=2)
+
+
+def muon_step_(weights, momenta, grads, lr=0.02, beta=0.95, weight_decay=0.0, nesterov=True, steps=5, eps=1e-7):
+    """An optimiser's step with orthogonalised updates, in place, on matrices
+    of one shape: momentum = beta momentum + grad, U = grad + beta momentum (or
+    the momentum), weight = (1 - lr weight_decay) weight - lr sqrt(max(1, rows /
+    columns)) orthogonalize(U)."""
+    if not len(weights) == len(momenta) == len(grads):
+        raise RuntimeError("muon_step: weights, momenta and gradients differ in number")
+    ids = [(c_uint64 * len(ts))(*[t.id for t in ts]) for ts in (weights, momenta, grads)]
+    if lib.applegpu_muon_step(*ids, len(weights), float(lr), float(beta), float(weight_decay), int(bool(nesterov)),
+                              int(steps), float(eps)) != 0:
+        raise RuntimeError(ffi_error())
 
 
 def synchronize():

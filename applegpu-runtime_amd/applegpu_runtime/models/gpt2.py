@@ -474,13 +474,10 @@ def gpt2_decode_step(model: dict, tokens, cache: KVCache):
     return logits, gpu.argmax(logits), lens
 
 
-def gpt2_score(model: dict, ids, top_k: int = 0):
-    """How likely each next token of a batch of texts [B, T] is: (logprobs,
-    entropy, lse), float32 [B, T] on the device, and with top_k also
-    (top_logprobs, top_ids) [B, T, top_k]; entry t is of token t + 1 given
-    those up to t (the last one's logprob, of no token, is 0).  Negative ids
-    are padding at the end of a text: they are read as token 0, which no
-    earlier position sees, and their log probabilities are 0."""
+def _text_hidden(model: dict, ids):
+    """(hidden states in front of the last layer_norm [B * T, d], ids of the next
+    tokens [B, T], -1 where there is none) of texts [B, T] with negative ids
+    as padding at their ends."""
     w = model["weights"]
     ids = np.asarray(ids, dtype=np.int32)
     if ids.ndim != 2 or ids.shape[1] < 1:
@@ -493,9 +490,42 @@ def gpt2_score(model: dict, ids, top_k: int = 0):
         gpu.embedding(w["transformer.wpe.weight"], gpu.from_numpy(np.tile(np.arange(T, dtype=np.int32), B)))
     for i in range(model["config"]["n_layer"]):
         x = _block(model, i, x, B, T, lambda i, q, k, v: gpu.attention_causal(q, k, v))
-    logits = _head(model, x, B * T)
     nxt = np.full((B, T), -1, np.int32)
     nxt[:, :-1] = ids[:, 1:]
+    return x, nxt
+
+
+def gpt2_loss(model: dict, ids, grads: bool = False):
+    """The cross entropy of each next token of a batch of texts [B, T] with
+    negative ids as padding at their ends, without the logits in memory (for
+    50257 words they are 100 KB a token in 16 bits): float32 [B, T] on the
+    device, entry t of token t + 1, 0 where there is none.  With grads, (loss,
+    d hidden [B, T, d], d wte [V, d]) of the tokens' mean loss: what the tied
+    head hands to the rest of the model and to its table."""
+    x, nxt = _text_hidden(model, ids)
+    B, T = nxt.shape
+    w = model["weights"]
+    x = gpu.layer_norm(x, w["transformer.ln_f.weight"], w["transformer.ln_f.bias"])
+    x = gpu.reshape(x, [B, T, x.shape[-1]])
+    t = gpu.from_numpy(nxt)
+    loss, lse = gpu.linear_cross_entropy(x, w["transformer.wte.weight"], t)
+    if not grads:
+        return loss
+    some = max(int(((nxt >= 0) & (nxt < model["config"]["vocab_size"])).sum()), 1)
+    g = gpu.full([B, T], 1.0 / some, "float32")
+    return (loss, *gpu.linear_cross_entropy_backward(g, x, w["transformer.wte.weight"], t, loss, lse))
+
+
+def gpt2_score(model: dict, ids, top_k: int = 0):
+    """How likely each next token of a batch of texts [B, T] is: (logprobs,
+    entropy, lse), float32 [B, T] on the device, and with top_k also
+    (top_logprobs, top_ids) [B, T, top_k]; entry t is of token t + 1 given
+    those up to t (the last one's logprob, of no token, is 0).  Negative ids
+    are padding at the end of a text: they are read as token 0, which no
+    earlier position sees, and their log probabilities are 0."""
+    x, nxt = _text_hidden(model, ids)
+    B, T = nxt.shape
+    logits = _head(model, x, B * T)
     return gpu.token_logprobs(gpu.reshape(logits, [B, T, logits.shape[-1]]), gpu.from_numpy(nxt), top_k=top_k)
 
 

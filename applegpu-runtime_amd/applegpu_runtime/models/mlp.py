@@ -45,13 +45,21 @@ def torch_default_init(sizes, seed=42):
 
 
 class EagerMLP:
-    """Linear -> ReLU -> ... -> Linear trained with MSE + SGD on the device."""
+    """Linear -> ReLU -> ... -> Linear trained with MSE + SGD on the device.
+    With optimizer="muon" the hidden layers' matrices (all but the last) take
+    orthogonalised updates of `muon_lr` instead, with momentum; biases and the
+    last layer keep SGD's."""
 
-    def __init__(self, params_np):
+    def __init__(self, params_np, optimizer: str = "sgd", muon_lr: float = 0.02, muon_beta: float = 0.95):
+        if optimizer not in ("sgd", "muon"):
+            raise ValueError(f"optimizer must be sgd or muon, got {optimizer!r}")
         E.init()
+        self.optimizer, self.muon_lr, self.muon_beta = optimizer, muon_lr, muon_beta
         self.params = [(E.from_numpy(np.asarray(w, np.float32)), E.from_numpy(np.asarray(b, np.float32)))
                        for w, b in params_np]
         self._one = E.from_numpy(np.ones((1,), np.float32))
+        self.momenta = [E.from_numpy(np.zeros(np.shape(w), np.float32)) for w, _ in params_np[:-1]] \
+            if optimizer == "muon" else []
 
     def forward(self, x):
         acts = [x]
@@ -64,6 +72,8 @@ class EagerMLP:
 
     def train_step(self, x, y, lr=0.01):
         """One forward + MSE + backward + SGD step; returns the loss tensor (on device)."""
+        if self.optimizer == "muon":
+            return self._muon_step(x, y, lr)
         n = len(self.params)
         if n == 2:
             # Linear -> ReLU -> Linear: one op (one launch at small sizes)
@@ -96,9 +106,8 @@ class EagerMLP:
             E.linear_backward_sgd_pair_(w1, b1, g, acts[1], w0, b0, x, -lr)
         return loss
 
-    def train_step_unfused(self, x, y, lr=0.01):
-        """The same step with every gradient materialised and one axpy per
-        parameter (the reference's aten sequence); kept for comparison."""
+    def _gradients(self, x, y):
+        """(loss, [(dw, db) of each layer]), every gradient materialised."""
         out, acts = self.forward(x)
         loss = E.mse_loss(out, y)
         g = E.mse_loss_backward(self._one, out, y)
@@ -111,9 +120,30 @@ class EagerMLP:
             grads[i] = (dw, db)
             if i > 0:
                 g = E.matmul_masked(g, w, False, False, acts[i])
+        return loss, grads
+
+    def train_step_unfused(self, x, y, lr=0.01):
+        """The same step with every gradient materialised and one axpy per
+        parameter (the reference's aten sequence); kept for comparison."""
+        loss, grads = self._gradients(x, y)
         for (w, b), (dw, db) in zip(self.params, grads):
             E.add_(w, dw, -lr)
             E.add_(b, db, -lr)
+        return loss
+
+    def _muon_step(self, x, y, lr):
+        loss, grads = self._gradients(x, y)
+        last = len(self.params) - 1
+        alike = {}
+        for i, (w, b) in enumerate(self.params):
+            E.add_(b, grads[i][1], -lr)
+            if i < last:
+                alike.setdefault(w.shape, []).append(i)
+            else:
+                E.add_(w, grads[i][0], -lr)
+        for layers in alike.values():   # matrices of one shape are stepped together
+            E.muon_step_([self.params[i][0] for i in layers], [self.momenta[i] for i in layers],
+                         [grads[i][0] for i in layers], self.muon_lr, self.muon_beta)
         return loss
 
     def numpy_params(self):

@@ -17,8 +17,8 @@
 //
 // Roundings: d is rounded once to the operands' 16 bits before its products,
 // as the logits' gradient of any 16-bit program is; fp16 (and the planes of
-// fp32) hold d times a power of two that takes the largest |g| + |h| to 2^13,
-// so that words of probability 2^-37 still count.  fp32 operands are scaled
+// fp32) hold d times a power of two that takes the largest of them to 2^13, so
+// that what is 2^-37 of it still counts.  fp32 operands are scaled
 // alike by their largest magnitude and split into fp16 planes (22 bits).
 #include "tile16.hpp"
 
@@ -268,12 +268,26 @@ __global__ void __launch_bounds__(256) loss_kernel(const float2* part, int64_t p
 
 // ── backward ──────────────────────────────────────────────────────────────
 // What a row of d is made of: {lse, weight of p, d of the target in 16 bits,
-// what that rounding lost}.  The first two of d hold the power of the largest
-// |g| + |h| (not for bf16, whose range needs none).  A row's largest part is its
-// target's, alone in its size, so its rounding would be dx's: dx gets back what
-// it lost times the target's weights (fp16, 30 rows: error of dx 3.3e-4, so
-// 2.2e-4; of dw, where a word's rows have errors of their own, 3e-4).  Every
-// block finds the power from all rows.
+// what that rounding lost}.  The weight and d hold the power of the largest |d|
+// that any row can have (not for bf16, whose range needs none): of words other
+// than the target |g + h| (1 - p_t), of all |h| where there is none.  A row's
+// largest part is its target's, alone in its size, so its rounding would be
+// dx's: dx gets back what it lost times the target's weights (fp16, 30 rows:
+// error of dx 3.3e-4, so 2.2e-4; of dw, where a word's rows have errors of
+// their own, 3e-4).  Every block finds the power from all rows.
+struct RowPart {
+  float g, h, dt, most;
+};
+__device__ __forceinline__ RowPart row_part(const float* g, const float* h, const float* loss, bool there, int64_t r) {
+  RowPart o;
+  o.g = there ? g[r] : 0.f;
+  o.h = h ? h[r] : 0.f;
+  // 1 - p of the target from its loss, which keeps its digits
+  const float left = there ? -expm1f(-loss[r]) : 1.f;
+  o.dt = there ? o.h * expf(-loss[r]) - o.g * left : 0.f;
+  o.most = fmaxf(finite_abs(o.dt), finite_abs((o.g + o.h) * left));
+  return o;
+}
 template <typename T, int PL>
 __global__ void __launch_bounds__(1024) rows_kernel(const float* g, const float* h, const float* loss, const float* lse,
                                                     const void* targets, bool wide, int64_t R, int64_t V, float2* power,
@@ -282,24 +296,22 @@ __global__ void __launch_bounds__(1024) rows_kernel(const float* g, const float*
   float up = 1.f;
   if constexpr (!std::is_same<T, bf16_t>::value) {
     float m = 0.f;
-    for (int64_t i = threadIdx.x; i < R; i += 1024) m = fmaxf(m, finite_abs(g[i]) + (h ? finite_abs(h[i]) : 0.f));
+    for (int64_t i = threadIdx.x; i < R; i += 1024)
+      m = fmaxf(m, row_part(g, h, loss, target_of(targets, wide, i, V) >= 0, i).most);
     const float2 pw = power_for(block_max(m, red));
     if (blockIdx.x == 0 && threadIdx.x == 0) *power = pw;
     up = pw.x;
   }
   const int64_t r = (int64_t)blockIdx.x * 1024 + threadIdx.x;
   if (r >= R) return;
-  const bool there = target_of(targets, wide, r, V) >= 0;
-  const float gr = there ? g[r] : 0.f, hr = h ? h[r] : 0.f;
-  // p - 1 of the target from its loss, which keeps the digits of 1 - p
-  const float dt = there ? gr * expm1f(-loss[r]) + hr * expf(-loss[r]) : 0.f;
-  float held = dt * up, lost = 0.f;
+  const RowPart o = row_part(g, h, loss, target_of(targets, wide, r, V) >= 0, r);
+  float held = o.dt * up, lost = 0.f;
   if constexpr (PL == 1) {
-    held = to_f(from_f<T>(dt * up));
-    lost = (dt * up - held) / up;
+    held = to_f(from_f<T>(o.dt * up));
+    lost = (o.dt * up - held) / up;
     if (!(fabsf(lost) < kInf)) lost = 0.f;
   }
-  rows[r] = make_float4(lse[r], (gr + hr) * up, held, lost);
+  rows[r] = make_float4(lse[r], (o.g + o.h) * up, held, lost);
 }
 
 // d of the tile's logits; zeros behind the words up to the row's end.  Formed

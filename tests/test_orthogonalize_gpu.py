@@ -90,3 +90,159 @@ def test_muon_step_vs_oracle(gpu, shape, dtype):
             _, norm, value = _bars(u, dtype)
             # U itself is float32's
             _check(dw[i].to_numpy(), want, rate * norm, rate * value + 2.0 ** -23 * np.abs(want).max(), HALF_STEP[dtype])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("steps", [1, 2, 3, 7])
+def test_steps(gpu, dtype, steps):
+    for shape in ((40, 30), (200, 300)):
+        g = _gradient(shape, dtype, seed=steps)
+        out = gpu.orthogonalize(_dev(gpu, g, dtype), steps=steps)
+        _check(out.to_numpy(), *_bars(g, dtype, steps=steps), HALF_STEP[dtype])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_singular_values_come_near_one(gpu, dtype):
+    g = _gradient((150, 400), dtype)
+    s = np.linalg.svd(gpu.orthogonalize(_dev(gpu, g, dtype)).to_numpy().astype(np.float64), compute_uv=False)
+    assert s.max() < 1.3 and np.median(s) > 0.6
+
+
+def test_views_and_sizes_of_values(gpu):
+    """A transposed or cut view is as its copy; the size of the values matters
+    by eps alone."""
+    for shape in ((50, 90), (300, 200)):
+        g = _gradient(shape, "float32")
+        want = gpu.orthogonalize(_dev(gpu, g)).to_numpy()
+        t = gpu.transpose(_dev(gpu, np.ascontiguousarray(g.T)))
+        np.testing.assert_array_equal(gpu.orthogonalize(t).to_numpy(), want)
+        wide = np.zeros((shape[0] + 3, shape[1] + 5), np.float32)
+        wide[2:-1, 3:-2] = g
+        cut = gpu.slice(gpu.slice(_dev(gpu, wide), 0, 2, 2 + shape[0]), 1, 3, 3 + shape[1])
+        np.testing.assert_array_equal(gpu.orthogonalize(cut).to_numpy(), want)
+        for scale in (2.0 ** -60, 2.0 ** 40, 2.0 ** 90):
+            got = gpu.orthogonalize(_dev(gpu, g * np.float32(scale)), eps=0.0).to_numpy()
+            same = gpu.orthogonalize(_dev(gpu, g), eps=0.0).to_numpy()
+            np.testing.assert_allclose(got, same, rtol=0, atol=2e-6 * np.abs(same).max())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(4, 30, 50), (3, 200, 300)])
+def test_zeros_and_what_is_not_finite_stay_in_their_matrix(gpu, dtype, shape):
+    g = _gradient(shape, dtype)
+    want = gpu.orthogonalize(_dev(gpu, g, dtype)).to_numpy()
+    bad = g.copy()
+    bad[0] = 0
+    bad[1, 3, 5] = np.nan
+    for eps in (1e-7, 0.0):
+        got = gpu.orthogonalize(_dev(gpu, bad, dtype), eps=eps).to_numpy()
+        assert (got[0] == 0).all() and np.isnan(got[1]).all() and np.isfinite(got[2:]).all()
+    np.testing.assert_array_equal(gpu.orthogonalize(_dev(gpu, bad, dtype)).to_numpy()[2:], want[2:])
+
+
+def test_nothing_to_do(gpu):
+    assert gpu.orthogonalize(gpu.zeros([0, 5, 7])).shape == [0, 5, 7]
+    assert gpu.orthogonalize(gpu.zeros([3, 0])).shape == [3, 0]
+    gpu.muon_step_([], [], [])
+
+
+@pytest.mark.parametrize("shape", [(20, 30), (130, 200)])
+def test_many_matrices_in_groups(gpu, shape):
+    """More matrices than a launch takes by their addresses: as one by one."""
+    n = 37
+    rng = np.random.default_rng(1)
+    w = rng.standard_normal((n, *shape)).astype(np.float32)
+    g = _gradient((n, *shape), "float32")
+    together = [[_dev(gpu, a) for a in v] for v in (w, np.zeros_like(w), g)]
+    gpu.muon_step_(*together, lr=0.1)
+    for i in (0, 31, 32, 36):
+        alone = [_dev(gpu, v[i]) for v in (w, np.zeros_like(w), g)]
+        gpu.muon_step_(*alone, lr=0.1)
+        np.testing.assert_array_equal(together[0][i].to_numpy(), alone[0].to_numpy())
+        np.testing.assert_array_equal(together[1][i].to_numpy(), alone[1].to_numpy())
+
+
+def test_odd_places_of_views(gpu):
+    """Weights, momenta and gradients that start at any element."""
+    for dtype in DTYPES:
+        for shape in ((24, 40), (160, 200)):
+            size = shape[0] * shape[1]
+            rng = np.random.default_rng(2)
+            flat = rng.standard_normal(3 * size + 9).astype(np.float32) * 1e-2
+            flat = few_bits.round_to(flat, dtype)
+            m = rng.standard_normal(size + 3).astype(np.float32) * 1e-2
+            d, dm = _dev(gpu, flat, dtype), _dev(gpu, m)
+            view = lambda t, at: gpu.reshape(gpu.slice(t, 0, at, at + size), list(shape))
+            w, g, mom = view(d, 1), view(d, size + 4), view(dm, 3)
+            gpu.muon_step_(w, mom, g, lr=0.1)
+            cut = [flat[1:1 + size].reshape(shape), m[3:].reshape(shape), flat[size + 4:2 * size + 4].reshape(shape)]
+            same = [_dev(gpu, cut[0], dtype), _dev(gpu, cut[1]), _dev(gpu, cut[2], dtype)]
+            gpu.muon_step_(*same, lr=0.1)
+            got = d.to_numpy()
+            np.testing.assert_array_equal(got[1:1 + size], same[0].to_numpy().reshape(-1))
+            np.testing.assert_array_equal(np.delete(got, np.arange(1, 1 + size)),
+                                          np.delete(flat, np.arange(1, 1 + size)))   # nothing beside it
+            np.testing.assert_array_equal(dm.to_numpy()[3:], same[1].to_numpy().reshape(-1))
+            np.testing.assert_array_equal(dm.to_numpy()[:3], m[:3])
+
+
+def test_what_was_asked_before_the_step_sees_the_weights_before(gpu):
+    rng = np.random.default_rng(3)
+    w, m, g = (rng.standard_normal((16, 24)).astype(np.float32) for _ in range(3))
+    dw, dm, dg = (_dev(gpu, a) for a in (w, m, g))
+    x = _dev(gpu, rng.standard_normal((4, 24)))
+    y = gpu.relu(gpu.matmul(x, gpu.transpose(dw)) + gpu.full([4, 16], 1.0))
+    mm = gpu.transpose(dm) + gpu.transpose(dm)
+    gpu.muon_step_(dw, dm, dg, lr=0.5)
+    after = dw.to_numpy()
+    assert not np.array_equal(after, w)
+    np.testing.assert_allclose(y.to_numpy(), np.maximum(x.to_numpy() @ w.T + 1, 0), rtol=1e-3, atol=1e-4)
+    np.testing.assert_array_equal(mm.to_numpy(), 2 * m.T)
+
+
+def test_refusals(gpu):
+    z = lambda *s, dtype="float32": gpu.zeros(list(s), dtype)
+    with pytest.raises(ValueError, match="at least 2D"):
+        gpu.orthogonalize(z(5))
+    with pytest.raises(ValueError, match="orthogonalize"):
+        gpu.orthogonalize(gpu.cast(z(5, 5), "int32"))
+    for steps in (0, -1, 101):
+        with pytest.raises(ValueError, match="steps"):
+            gpu.orthogonalize(z(5, 5), steps=steps)
+    for eps in (-1.0, float("nan"), float("inf")):
+        with pytest.raises(ValueError, match="eps"):
+            gpu.orthogonalize(z(5, 5), eps=eps)
+    a, b, c = z(4, 6), z(4, 6), z(4, 6)
+    for t in (a, b, c):
+        t.eval()
+    with pytest.raises(ValueError, match="weights, 2 momenta"):
+        gpu.muon_step_([a], [b, c], [c])
+    with pytest.raises(ValueError, match="one shape"):
+        gpu.muon_step_(a, z(6, 4), c)
+    with pytest.raises(ValueError, match="one shape"):
+        gpu.muon_step_([a, z(5, 5)], [b, z(5, 5)], [c, z(5, 5)])
+    with pytest.raises(ValueError, match="one shape"):
+        gpu.muon_step_(z(4), z(4), z(4))
+    with pytest.raises(ValueError, match="must be float32"):
+        gpu.muon_step_(z(4, 6, dtype="float16"), z(4, 6, dtype="float16"), z(4, 6, dtype="float16"))
+    with pytest.raises(ValueError, match="Dtype mismatch"):
+        gpu.muon_step_(z(4, 6, dtype="float16"), b, c)
+    with pytest.raises(ValueError, match="contiguous"):
+        gpu.muon_step_(gpu.transpose(z(6, 4)), b, c)
+    with pytest.raises(ValueError, match="share storage"):
+        gpu.muon_step_([a, a], [b, c], [z(4, 6), z(4, 6)])
+    with pytest.raises(ValueError, match="share storage"):
+        gpu.muon_step_(a, b, b)
+    with pytest.raises(ValueError, match="share storage"):
+        gpu.muon_step_(a, b, a)
+    whole = z(8, 6)
+    whole.eval()
+    with pytest.raises(ValueError, match="share storage"):
+        gpu.muon_step_(gpu.slice(whole, 0, 0, 4), b, gpu.slice(whole, 0, 3, 7))
+    for kw in (dict(lr=float("nan")), dict(beta=float("inf")), dict(weight_decay=float("nan"))):
+        with pytest.raises(ValueError, match="finite"):
+            gpu.muon_step_(a, b, c, **kw)
+    with pytest.raises(ValueError, match="expected GpuTensor"):
+        gpu.muon_step_(a, b, np.zeros((4, 6), np.float32))
+    assert (a.to_numpy() == 0).all()
+    gpu.muon_step_([a, z(4, 6)], [b, z(4, 6)], [c, c])   # one gradient for two weights is a read
