@@ -79,7 +79,8 @@ class _LinearCrossEntropy(torch.autograd.Function):
 def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor):
     """(loss, lse), float32 [...], of the logits x @ weight.T for x [..., K],
     weight [V, K] and int32 or int64 targets [...]; a target outside [0, V)
-    (ignore_index -100) has loss 0.  Differentiable in x and weight."""
+    (ignore_index -100) has loss 0.  Differentiable in x and weight for up to
+    2^20 rows."""
     return _LinearCrossEntropy.apply(x, weight, target)
 
 
@@ -118,4 +119,6 @@ class Muon(torch.optim.Optimizer):
                     if lib.applegpu_muon_step(*arrays, len(params), group["lr"], group["beta"], group["weight_decay"],
                                               int(group["nesterov"]), group["steps"], group["eps"]) != 0:
                         raise ValueError(ffi_error())
+                # autograd learns of writes from the tensors' versions
+                torch.autograd.graph.increment_version([*params, *(self.state[p]["momentum"] for p in params)])
         return loss

@@ -227,3 +227,31 @@ def test_torch_device(torch_dev):
         Muon([torch.nn.Parameter(torch.zeros(4))])
     with pytest.raises(ValueError, match="applegpu device"):
         linear_cross_entropy(x, w, t)
+
+
+def test_torch_step_is_seen_by_autograd(torch_dev):
+    """A product whose saved weights the optimiser has stepped since refuses its
+    backward pass, as behind any other write in place."""
+    torch = torch_dev
+    from applegpu_runtime.training import Muon
+    w = torch.nn.Parameter((torch.randn(8, 8) * 0.1).to("applegpu"))
+    x = torch.randn(4, 8).to("applegpu").requires_grad_()
+    y = (x @ w).sum()
+    w.grad = torch.randn(8, 8).to("applegpu")
+    before = w._version
+    Muon([w]).step()
+    assert w._version > before
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+def test_torch_without_rows(torch_dev):
+    """No rows: no losses, and gradients of zeros."""
+    torch = torch_dev
+    from applegpu_runtime.training import linear_cross_entropy
+    w = torch.randn(5, 8).to("applegpu").requires_grad_()
+    x = torch.randn(2, 8).to("applegpu")[:0].requires_grad_()
+    loss, lse = linear_cross_entropy(x, w, torch.zeros(2, dtype=torch.int64).to("applegpu")[:0])
+    assert loss.shape == lse.shape == (0,)
+    loss.sum().backward()
+    assert x.grad.shape == (0, 8) and not w.grad.cpu().any()
