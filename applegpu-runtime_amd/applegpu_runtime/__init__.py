@@ -712,8 +712,9 @@ def linear_cross_entropy_backward(grad_loss, x, weight, targets, loss, lse, grad
     loss and lse it returned.  The logits are formed again, in pieces of the
     vocabulary; their gradient is rounded to 16 bits before its products for
     16-bit operands, and for float16 and float32 ones counts down to 2^-37 of
-    the largest one in the call.  Rows whose target is outside [0, V) get lse's part only;
-    one without any weight gets zeros whatever its logits are."""
+    the largest one in the call.  Rows whose target is outside [0, V) get lse's
+    part only; one without any weight gets zeros whatever its logits are.  At
+    most 2^20 rows at once."""
     ins = [_t(grad_loss), _t(x), _t(weight), _t(targets), _t(loss), _t(lse)]
     return _op(b"linear_cross_entropy_backward", ins + ([_t(grad_lse)] if grad_lse is not None else []), nout=2)
 
@@ -721,9 +722,12 @@ def linear_cross_entropy_backward(grad_loss, x, weight, targets, loss, lse, grad
 def orthogonalize(g, steps=5, eps=1e-7):
     """The matrices of g [..., m, n] with their singular values taken towards 1
     by Newton-Schulz products: X = g / (|g|_F + eps), then `steps` times
-    A = X X^T, X = 3.4445 X + (-4.7750 A + 2.0315 A A) X.  Products are of 11
-    bits of each value for 16-bit matrices, of 22 for float32 ones, with
-    float32 sums; X itself is kept in float32.  A matrix of zeros stays one."""
+    A = X X^T, X = 3.4445 X + (-4.7750 A + 2.0315 A A) X.  Products have
+    float32 sums and count 22 bits of each value for float32 matrices, 11 for
+    bfloat16 ones and for float16 ones 11, then 22 in the last three steps; X
+    itself keeps 22 bits beside them (float32: all).  Small matrices and those of
+    a short side in float16 have 22 bits throughout.  A matrix of zeros stays
+    one."""
     return _op(b"orthogonalize", [_t(g)], f=(float(eps),), i=(int(steps),))
 
 

@@ -613,6 +613,7 @@ struct LinearCE {
 };
 constexpr int64_t kLinearCEFeatures = (int64_t)1 << 19;  // K
 constexpr int64_t kLinearCEWords = (int64_t)1 << 30;     // V
+constexpr int64_t kLinearCERows = (int64_t)1 << 20;      // R of the gradient: its 8 panels lie in one buffer resource
 size_t linear_ce_ws_bytes(const LinearCE& a, int cus);
 void linear_ce(const LinearCE& a, void* ws, int cus, hipStream_t s);
 // d = g_loss (p - [v = t]) + g_lse p with p = exp(z - lse); dx = d w, dw = d^T x.

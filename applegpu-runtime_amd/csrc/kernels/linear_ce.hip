@@ -314,12 +314,13 @@ __global__ void __launch_bounds__(1024) rows_kernel(const float* g, const float*
   rows[r] = make_float4(lse[r], (o.g + o.h) * up, held, lost);
 }
 
-// d of the tile's logits; zeros behind the words up to the row's end.  Formed
-// where the accumulators are, from the few rows that a lane has.
+// d of the tile's logits, in panels; zeros behind the words up to the last
+// panel's end.  Formed where the accumulators are, from the few rows that a lane
+// has.
 template <typename T>
 struct EpiGrad {
   T* d;
-  int64_t ldd;
+  int64_t panel, len;  // values of a panel; the piece's words
   int64_t v0, V;  // the piece's first word; all words
   const void* targets;
   bool wide;
@@ -375,7 +376,8 @@ struct EpiGrad {
     TL::template runs<false>(
         c, lds, acc, false,
         [&](int64_t row, int64_t col, float (&v)[8]) {
-          if (row < p.M && col * PL < ldd) put_planes<T, PL>(d + row * ldd, col, v);
+          constexpr int W = 64 / PL;  // words of a panel
+          if (row < p.M && col < (len + W - 1) / W * W) put_planes<T, PL>(d + col / W * panel + row * 64, col % W, v);
         },
         [](int64_t, int64_t, float (&)[8]) {});
   }
@@ -504,7 +506,6 @@ struct Carver {
   }
 };
 
-
 bool direct(const void* p, int64_t ld, int64_t K) {
   return K % 8 == 0 && ld % 8 == 0 && ((uintptr_t)p & 15) == 0 && ld < (1 << 21);
 }
@@ -573,12 +574,12 @@ int pick(int64_t M, int64_t N, bool raw, int cus) {
 }
 int bn_of(int tile) { return tile == kBig ? 256 : 128; }
 
-template <typename T, int PL, bool RAW, class Epi>
+template <typename T, int PL, Layout BL, class Epi>
 void run(int tile, const Args& p, const Epi& e, hipStream_t s, const char* what) {
-  if (tile == kBig && !RAW) launch<Tile<T, 4, 2, 2, 4, PL, false, false>>(p, e, s, what);
-  else if (tile == kMid) launch<Tile<T, 2, 1, 2, 4, PL, false, false, false, RAW>>(p, e, s, what);
-  else if (tile == kThin) launch<Tile<T, 1, 1, 2, 4, PL, false, false, false, RAW>>(p, e, s, what);
-  else launch<Tile<T, 1, 1, 1, 4, PL, false, false, false, RAW>>(p, e, s, what);
+  if (tile == kBig && BL == kRows) launch<Tile<T, 4, 2, 2, 4, PL, kRows, kRows>>(p, e, s, what);
+  else if (tile == kMid) launch<Tile<T, 2, 1, 2, 4, PL, kRows, BL>>(p, e, s, what);
+  else if (tile == kThin) launch<Tile<T, 1, 1, 2, 4, PL, kRows, BL>>(p, e, s, what);
+  else launch<Tile<T, 1, 1, 1, 4, PL, kRows, BL>>(p, e, s, what);
 }
 
 template <typename TI, typename T, int PL>
@@ -589,7 +590,8 @@ size_t forward(const LinearCE& a, void* wsp, int cus, hipStream_t s) {
   // written and read once more), by every block that multiplies them: 50257 x
   // 768, us, packed / split at 20 rows 119 / 62, 61: 122 / 72, 255: 145 / 129,
   // 1023: 311 / 345
-  const bool raw = PL == 2 && a.R <= 320 && a.K % 4 == 0 && a.ldw % 4 == 0 && ((uintptr_t)a.w & 15) == 0;
+  const bool raw = PL == 2 && a.R <= 320 && a.K % 4 == 0 && a.ldw % 4 == 0 && a.ldw < (1 << 20) &&
+                   ((uintptr_t)a.w & 15) == 0;
   const Both b = ready<TI, T, PL>(a, raw, ws, s);
   const Packed &x = b.x, &w = b.w;
   const int tile = pick(a.R, a.V, raw, cus);
@@ -603,8 +605,8 @@ size_t forward(const LinearCE& a, void* wsp, int cus, hipStream_t s) {
   const bool wide = a.idx_dt == DType::I64;
   p.b_power = w.power;
   const EpiLoss e{part, zt, a.targets, wide, x.power, w.power};
-  if (PL == 2 && raw) run<T, PL, PL == 2>(tile, p, e, s, what);
-  else run<T, PL, false>(tile, p, e, s, what);
+  if (PL == 2 && raw) run<T, PL, PL == 2 ? kRaw : kRows>(tile, p, e, s, what);
+  else run<T, PL, kRows>(tile, p, e, s, what);
   const int rx = a.R >= 64 * cus ? 64 : a.R >= 16 * cus ? 16 : a.R >= 4 * cus ? 4 : 1;
   hipLaunchKernelGGL(loss_kernel, dim3(blocks_for(a.R, rx)), dim3(256), 0, s, part, parts, zt, a.targets, wide, a.R,
                      a.V, rx, a.loss, a.lse);
@@ -675,10 +677,14 @@ size_t backward(const LinearCE& a, void* wsp, int cus, hipStream_t s) {
   const Packed &x = b.x, &w = b.w;
   const bool wide = a.idx_dt == DType::I64;
   // pieces of the vocabulary, whole tiles of it
-  const int64_t most = std::min<int64_t>(std::max<int64_t>(kHeld / PL / a.R / 256 * 256, 256), 1 << 19);
+  const int64_t most = std::max<int64_t>(kHeld / PL / a.R / 256 * 256, 256);
   const int64_t pieces = ceil_div(a.V, most), each = ceil_div(ceil_div(a.V, pieces), 256) * 256;
-  const int64_t len = std::min(each, a.V), ldd = (len + 31) / 32 * 32 * PL;
-  T* d = ws.take<T>((size_t)(a.R * ldd));
+  // d lies in panels of 128 bytes a row: dx reads it along its rows, dw down
+  // them, both in long runs (as rows as long as the piece / in panels, us: 8191 x
+  // 50257 x 768 bf16 2057 / 1993, 1023 x 50257 x 768 fp32 and 61 x 50257 x 1280
+  // fp16 within 1 % of one another)
+  const int64_t len = std::min(each, a.V), panel = a.R * 64;
+  T* d = ws.take<T>((size_t)(panel * ceil_div(len, 64 / PL)));
   constexpr bool scaled = !std::is_same<T, bf16_t>::value;
   float2* pg = scaled ? ws.take<float2>(1) : nullptr;
   float4* rows = ws.take<float4>((size_t)a.R);
@@ -693,12 +699,12 @@ size_t backward(const LinearCE& a, void* wsp, int cus, hipStream_t s) {
   const Lost<TI> lost{(const TI*)a.w, a.ldw, a.V, a.targets, wide, PL == 1 ? rows : nullptr};
   for (int64_t v0 = 0; v0 < a.V; v0 += each) {
     const int64_t n = std::min(each, a.V - v0);
-    const Operand wp{(const T*)w.o.p + v0 * w.o.ld, w.o.ld, 0}, dp{d, ldd, 0};
+    const Operand wp{(const T*)w.o.p + v0 * w.o.ld, w.o.ld, 0}, dp{d, panel, 0};
     Args p;
     p.a = x.o; p.b = wp;
     p.M = a.R; p.N = n; p.K = a.K;
-    run<T, PL, false>(pick(a.R, n, false, cus), p,
-                      EpiGrad<T>{d, ldd, v0, a.V, a.targets, wide, rows, x.power, w.power}, s, what);
+    run<T, PL, kRows>(pick(a.R, n, false, cus), p,
+                      EpiGrad<T>{d, panel, len, v0, a.V, a.targets, wide, rows, x.power, w.power}, s, what);
     Args px, pw;
     px.a = pw.a = dp;
     px.b = wp;
@@ -707,13 +713,13 @@ size_t backward(const LinearCE& a, void* wsp, int cus, hipStream_t s) {
     pw.M = n; pw.N = a.K; pw.K = a.R;
     const EpiOut<TI> ex{(TI*)a.dx, part, v0 > 0, pg, w.power, lost},
         ew{(TI*)a.dw + v0 * a.K, nullptr, false, pg, x.power, {}};
-    typedef Tile<T, 2, 2, 2, 2, PL, true, true> WFew;  // (of four wavefronts, as dx's)
+    typedef Tile<T, 2, 2, 2, 2, PL, kPanelCols, kCols> WFew;  // (of four wavefronts, as dx's)
     if (plan.big)
-      launch_pair<Tile<T, 4, 2, 2, 4, PL, false, true>, Tile<T, 4, 2, 2, 4, PL, true, true>>(px, ex, pw, ew, s, what);
+      launch_pair<Tile<T, 4, 2, 2, 4, PL, kPanelRows, kCols>, Tile<T, 4, 2, 2, 4, PL, kPanelCols, kCols>>(px, ex, pw, ew, s, what);
     else if (a.R > 32)
-      launch_pair<Tile<T, 2, 1, 2, 4, PL, false, true>, Tile<T, 2, 1, 2, 4, PL, true, true>>(px, ex, pw, ew, s, what);
+      launch_pair<Tile<T, 2, 1, 2, 4, PL, kPanelRows, kCols>, Tile<T, 2, 1, 2, 4, PL, kPanelCols, kCols>>(px, ex, pw, ew, s, what);
     else
-      launch_pair<Tile<T, 1, 1, 1, 4, PL, false, true>, WFew>(px, ex, pw, ew, s, what);
+      launch_pair<Tile<T, 1, 1, 1, 4, PL, kPanelRows, kCols>, WFew>(px, ex, pw, ew, s, what);
   }
   if (parted) {
     const int64_t n = a.R * a.K;

@@ -366,11 +366,11 @@ int pick(int64_t M, int64_t N, int64_t count, bool sym, int cus) {
   return tiles(128) * 8 >= 5 * cus ? kMid : kSmall;
 }
 
-template <int PL, bool AC, bool BC, bool SYM, class Epi>
+template <int PL, Layout AL, Layout BL, bool SYM, class Epi>
 void run(int tile, const Args& p, const Epi& e, hipStream_t s, const char* what) {
-  if (tile == kBig) launch<Tile<half_t, 4, 2, 2, 4, PL, AC, BC, SYM>>(p, e, s, what);
-  else if (tile == kMid) launch<Tile<half_t, 2, 1, 2, 4, PL, AC, BC, SYM>>(p, e, s, what);
-  else launch<Tile<half_t, 1, 1, 2, 2, PL, AC, BC, SYM>>(p, e, s, what);
+  if (tile == kBig) launch<Tile<half_t, 4, 2, 2, 4, PL, AL, BL, SYM>>(p, e, s, what);
+  else if (tile == kMid) launch<Tile<half_t, 2, 1, 2, 4, PL, AL, BL, SYM>>(p, e, s, what);
+  else launch<Tile<half_t, 1, 1, 2, 2, PL, AL, BL, SYM>>(p, e, s, what);
 }
 
 // fp16 planes of a step's factors.  What a step rounds is passed on by the
@@ -444,19 +444,19 @@ void step(const Orthogonalize& a, const Space& w, int i, int cus, hipStream_t s,
   p.M = p.N = side;
   p.K = tall ? m : n;
   const EpiGram<false> eg{nullptr, w.a, lda, side * lda};
-  if (tall) run<PL, true, true, true>(gram, p, eg, s, what);
-  else run<PL, false, false, true>(gram, p, eg, s, what);
+  if (tall) run<PL, kCols, kCols, true>(gram, p, eg, s, what);
+  else run<PL, kRows, kRows, true>(gram, p, eg, s, what);
   p.a = p.b = ao;
   p.K = side;
-  run<PL, false, false, true>(gram, p, EpiGram<true>{w.a, w.b, lda, side * lda}, s, what);
+  run<PL, kRows, kRows, true>(gram, p, EpiGram<true>{w.a, w.b, lda, side * lda}, s, what);
   p.M = m;
   p.N = n;
   p.a = tall ? xo : bo;
   p.b = tall ? bo : xo;
   const EpiUpdate<TO, F32, NEXT> eu{w.planes[i & 1], ld, w.keep, w.planes[(i + 1) & 1], row_of(n, NEXT), a.out,
                                     a.momentum, a.keep, a.rate};
-  if (tall) run<PL, false, false, false>(upd, p, eu, s, what);
-  else run<PL, false, true, false>(upd, p, eu, s, what);
+  if (tall) run<PL, kRows, kRows, false>(upd, p, eu, s, what);
+  else run<PL, kRows, kCols, false>(upd, p, eu, s, what);
 }
 
 // ── small matrices: everything in one block ───────────────────────────────

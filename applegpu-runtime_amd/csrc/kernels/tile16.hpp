@@ -2,7 +2,9 @@
 // acc[m][n] = sum over k of A(m, k) B(n, k), fp32 accumulation on
 // v_mfma_f32_32x32x16, with each operand in memory either as rows (k
 // contiguous) or as columns (row k holds every m), and either as plain values
-// or as two planes, the high and the low half of an fp32 value.
+// or as two planes, the high and the low half of an fp32 value.  A matrix that
+// one product reads as rows and another as columns can lie in panels of 128
+// bytes of every row, one panel after the other: both then read long runs.
 //
 //  - A block owns a BM x BN tile in stages of 64 16-bit values per row of an
 //    operand: 64 k of plain values, 32 k of both planes.  In memory the planes
@@ -64,7 +66,6 @@ struct Args {
   int tiles_m = 0, tiles_n = 0, tiles = 0;  // tiles: those that are computed
   int splits = 1, batches = 1;
   int stages = 0, per_split = 0;
-  int group = 8;  // tile rows that share their columns' loads
   const float2* b_power = nullptr;  // what fp32 rows of b are multiplied by before they are split (.x)
 };
 
@@ -89,12 +90,22 @@ __device__ __forceinline__ i16x4 read_transposed(const __attribute__((address_sp
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)p);
 }
 
+// How an operand lies in memory.
+enum Layout {
+  kRows,       // k contiguous, rows ld apart
+  kCols,       // k rows of every m, ld apart
+  kRaw,        // rows of fp32 values, split into planes in registers
+  kPanelRows,  // panels of 64 values of each row, ld apart; k along the panels
+  kPanelCols,  // the same, m along the panels and k down them
+};
+
 // One operand's part of a block: B rows (m) of it, L windows of 1 KB a
-// wavefront and stage.
-// RAW: rows of fp32 values, in the place of their planes (32 a stage; K and ld
-// multiples of 4, ld and offsets in 16-bit units all the same).
-template <typename T, int B, int L, int PL, bool COLS, bool RAW = false>
+// wavefront and stage.  kRaw: rows of fp32 values, in the place of their planes
+// (32 a stage; K and ld multiples of 4, ld and offsets in 16-bit units all the
+// same).
+template <typename T, int B, int L, int PL, Layout LAY>
 struct Stream {
+  static constexpr bool COLS = LAY == kCols || LAY == kPanelCols, PANEL = LAY == kPanelRows || LAY == kPanelCols;
   static constexpr int KS = 64 / PL;                 // k of a stage
   static constexpr int CPR = COLS ? B * PL / 8 : 8;  // 16-byte chunks of a k row, or of a row's stage
   const T* base;
@@ -110,21 +121,41 @@ struct Stream {
     lane = ln;
     first = w * L;
     ld = o.ld;
-    base = (const T*)o.p + b * o.batch + (COLS ? m0 * PL : m0 * ld);
     k_rows = K;
-    // values of a row from base on (rows: with the zeros up to a whole chunk,
-    // or a whole group of planes)
-    width = COLS ? ld - m0 * PL : PL == 1 ? (K + 7) / 8 * 8 : RAW ? K * 2 : (K + 31) / 32 * 64;
-    if (!COLS) rows = resource(base, ((M - m0 - 1) * ld + width) * (int64_t)sizeof(T));
+    if constexpr (PANEL) {
+      // whole panels a block: of its columns as many as the matrix has, of its
+      // rows each panel's from base on
+      static_assert(!COLS || B * PL % 64 == 0, "a block of panels");
+      base = (const T*)o.p + (COLS ? m0 * PL / 64 * ld : m0 * 64);
+      const int64_t panels = ((M - m0) * PL + 63) / 64;
+      width = !COLS ? (M - m0) * 64 : panels < B * PL / 64 ? panels * ld : B * PL / 64 * ld;
+    } else {
+      base = (const T*)o.p + b * o.batch + (COLS ? m0 * PL : m0 * ld);
+      // values of a row from base on (rows: with the zeros up to a whole chunk,
+      // or a whole group of planes)
+      width = COLS ? ld - m0 * PL : PL == 1 ? (K + 7) / 8 * 8 : LAY == kRaw ? K * 2 : (K + 31) / 32 * 64;
+      if (!COLS) rows = resource(base, ((M - m0 - 1) * ld + width) * (int64_t)sizeof(T));
+    }
 #pragma unroll
     for (int q = 0; q < L; ++q) {
-      const int i = (first + q) * 64 + lane;
-      const int r = i / CPR, c = i % CPR;
-      off[q] = (int)(r * ld * (int64_t)sizeof(T)) + (c ^ swz(r)) * 16;
+      const int i = (first + q) * 64 + lane, r = i / CPR, c = (i % CPR) ^ swz(r);
+      if constexpr (LAY == kPanelCols) off[q] = (int)((c / 8) * ld * (int64_t)sizeof(T)) + r * 128 + c % 8 * 16;
+      else off[q] = (int)(r * (PANEL ? 64 : ld) * (int64_t)sizeof(T)) + c * 16;
     }
   }
   __device__ __forceinline__ void issue(T* to, int st) const {
-    if constexpr (COLS) {
+    if constexpr (LAY == kPanelCols) {
+      // rows behind the last would be the next panel's first
+      const int64_t left = k_rows - (int64_t)st * KS, from = (int64_t)st * KS * 64;
+      const __amdgpu_buffer_rsrc_t src = resource(base + from, (width - from) * (int64_t)sizeof(T));
+#pragma unroll
+      for (int q = 0; q < L; ++q)
+        copy16(src, to + (first + q) * 512, ((first + q) * 64 + lane) / CPR < left ? off[q] : kBehind, 0);
+    } else if constexpr (LAY == kPanelRows) {
+      const __amdgpu_buffer_rsrc_t src = resource(base + (int64_t)st * ld, width * (int64_t)sizeof(T));
+#pragma unroll
+      for (int q = 0; q < L; ++q) copy16(src, to + (first + q) * 512, off[q], 0);
+    } else if constexpr (COLS) {
       const __amdgpu_buffer_rsrc_t src = resource(
           base + (int64_t)st * KS * ld, ((k_rows - (int64_t)st * KS - 1) * ld + width) * (int64_t)sizeof(T));
 #pragma unroll
@@ -190,13 +221,12 @@ struct Place {
   int wave, wm, wn, lane;
 };
 
-template <typename T_, int TM_, int TN_, int WM_, int WN_, int PL_, bool AC_, bool BC_, bool SYM_ = false,
-          bool RAW_ = false>
+template <typename T_, int TM_, int TN_, int WM_, int WN_, int PL_, Layout AL_, Layout BL_, bool SYM_ = false>
 struct Tile {
   typedef T_ T;
   static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, PL = PL_;
   static constexpr bool SYM = SYM_;  // tiles on and below the diagonal only
-  static constexpr bool RAW = RAW_;  // B is fp32 rows, split into planes in registers
+  static constexpr bool RAW = BL_ == kRaw;
   static constexpr int NW = WM * WN, BM = 32 * TM * WM, BN = 32 * TN * WN;
   static constexpr int KS = 64 / PL, KK = KS / 16;
   static constexpr int AW = BM / 8, BW = BN / 8, STAGE = (AW + BW) * 512;  // 16-bit values
@@ -204,9 +234,9 @@ struct Tile {
   static_assert(AW % NW == 0 && BW % NW == 0, "tile shape");
   // the epilogue stages 32 rows of every wavefront in the operands' place
   static_assert(NW * 32 * 32 * TN * 4 <= LDS * 2, "epilogue staging");
-  typedef Stream<T, BM, AW / NW, PL, AC_> SA;
-  typedef Stream<T, BN, BW / NW, PL, BC_, RAW> SB;
-  static_assert(!RAW || (PL == 2 && !BC_), "fp32 rows of a product of planes");
+  typedef Stream<T, BM, AW / NW, PL, AL_> SA;
+  typedef Stream<T, BN, BW / NW, PL, BL_> SB;
+  static_assert(!RAW || PL == 2, "fp32 rows of a product of planes");
   typedef typename Mfma<T>::vec V8;
   typedef f32x16 Acc[TM][TN];
 
@@ -231,8 +261,9 @@ struct Tile {
       c.tm = r;
       c.tn = t - r * (r + 1) / 2;
     } else {
-      const int per = p.group * p.tiles_n, g = t / per, first = g * p.group;
-      const int size = p.tiles_m - first < p.group ? p.tiles_m - first : p.group;
+      constexpr int kGroup = 8;  // tile rows that share their columns' loads
+      const int per = kGroup * p.tiles_n, g = t / per, first = g * kGroup;
+      const int size = p.tiles_m - first < kGroup ? p.tiles_m - first : kGroup;
       c.tm = first + (t % per) % size;
       c.tn = (t % per) / size;
     }
@@ -416,9 +447,9 @@ struct Tile {
     }
   };
 
-  // Through this wavefront's own part of LDS, 32 rows at a time: fr(row, column, v) for 8 columns of each row and, where
-  // `with` is true, fc(row, column, v) for 8 rows of each column (row, column:
-  // of the product).  A row's 16-byte chunks are exchanged so that 16 rows at
+  // Through this wavefront's own part of LDS, 32 rows at a time: fr(row, column,
+  // v) for 8 columns of each row and, where `with` is true, fc(row, column, v)
+  // for 8 rows of each column (row, column: of the product).  A row's 16-byte chunks are exchanged so that 16 rows at
   // one chunk cover all banks.  The loops stay rolled: unrolled, their
   // instructions come from memory once a launch and compute unit.
   template <bool COLUMNS, class FR, class FC>
@@ -504,8 +535,9 @@ int64_t blocks_of(Args& p, const char* what) {
   p.stages = (int)ceil_div(p.K, TL::KS);
   p.per_split = (int)ceil_div(p.stages, p.splits);
   const int64_t blocks = tiles * p.splits * p.batches;
-  // (a tile's rows lie within the 2 GiB that a buffer resource spans)
-  if (blocks < 1 || blocks >= (1LL << 30) || p.a.ld >= (1 << 21) || p.b.ld >= (1 << 21))
+  // (a tile's rows, or its panels, lie within the 2 GiB that a buffer resource
+  // spans)
+  if (blocks < 1 || blocks >= (1LL << 30) || p.a.ld >= (TL::SA::PANEL ? 1 << 27 : 1 << 21) || p.b.ld >= (1 << 21))
     fail("%s: a product of %lld x %lld x %lld in %d parts is too large", what, (long long)p.M, (long long)p.N,
          (long long)p.K, p.splits);
   p.tiles = (int)tiles;

@@ -2380,6 +2380,7 @@ std::vector<TensorP> linear_cross_entropy_backward(const TensorP& g_loss, const 
   a.g_lse = g_lse ? row("grad_lse", g_lse) : nullptr;
   a.loss = row("loss", loss);
   a.lse = row("lse", lse);
+  if (a.R > k::kLinearCERows) fail("%s: more than %lld rows at once", name, (long long)k::kLinearCERows);
   if (a.R == 0) return {alloc_out(x->dtype, x->dims()), full(x->dtype, weight->dims(), 0.f)};
   TensorP dx = alloc_out(x->dtype, x->dims()), dw = alloc_out(x->dtype, weight->dims());
   if (meta_mode()) return {dx, dw};

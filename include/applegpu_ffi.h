@@ -279,7 +279,8 @@ int32_t applegpu_kv_write_int8(uint64_t k_codes_id, uint64_t k_scales_id, uint64
  *     int64): loss and lse, float32 [...], of the logits x weight^T, which are
  *     not kept; a target outside [0, V) has loss 0.
  *   "linear_cross_entropy_backward" (grad_loss, x, weight, targets, loss, lse[,
- *     grad_lse]): the gradients of x and weight in their dtype.
+ *     grad_lse]): the gradients of x and weight in their dtype, of at most
+ *     2^20 rows at once.
  *   "orthogonalize" (g [..., m, n]; int steps, default 5; float eps, default
  *     1e-7): X = g / (|g| + eps), then steps times A = X X^T,
  *     X = a X + (b A + c A A) X, (a, b, c) = (3.4445, -4.7750, 2.0315). */

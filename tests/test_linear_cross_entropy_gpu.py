@@ -151,6 +151,30 @@ def test_views_and_lead_dims(gpu, dtype):
     np.testing.assert_allclose(one[0].to_numpy(), want[0][:1], rtol=1e-5, atol=1e-6)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_of_weights_far_apart(gpu, dtype):
+    """Columns out of rows of 2^21 values and more, which no tile's loads reach
+    across: as the contiguous ones."""
+    x, w, t = _case(3, 8, 4, dtype)
+    wide = gpu.zeros([4, (1 << 21) + 8], dtype)
+    part = gpu.slice(wide, 1, 16, 24)
+    gpu.blit_copy(_dev(gpu, w, dtype), part)
+    g = np.full(3, 0.5, np.float32)
+    dev = [_dev(gpu, x, dtype), part, gpu.from_numpy(t)]
+    got = _check_forward(gpu, x, w, t, dtype, gpu.linear_cross_entropy(*dev))
+    _check_backward(gpu, x, w, t, dtype, g, None, gpu.linear_cross_entropy_backward(_dev(gpu, g), *dev, *got))
+
+
+# d lies in groups of 64 words (32 for float32's planes): ends within, at and
+# just past a group and a tile of words, and of rows
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("R,V", [(32, 63), (33, 65), (63, 255), (64, 256), (65, 257), (129, 511), (256, 1025), (300, 32)])
+def test_gradient_at_the_edges_of_words_and_rows(gpu, R, V, dtype):
+    x, w, t = _case(R, 40, V, dtype, seed=9)
+    g = np.random.default_rng(V).random(R).astype(np.float32) / R
+    _check_backward(gpu, x, w, t, dtype, g, None)
+
+
 def test_no_rows(gpu):
     for dtype in DTYPES:
         x, w = gpu.zeros([0, 8], dtype), gpu.zeros([5, 8], dtype)
@@ -370,3 +394,8 @@ def test_refusals(gpu):
         gpu.linear_cross_entropy_backward(gpu.zeros([4]), x, w, t, loss, gpu.zeros([3]))
     with pytest.raises(ValueError, match="grad_lse must be float32"):
         gpu.linear_cross_entropy_backward(gpu.zeros([4]), x, w, t, loss, lse, grad_lse=gpu.zeros([2]))
+    rows = (1 << 20) + 1
+    many = gpu.zeros([rows])
+    with pytest.raises(ValueError, match="rows at once"):
+        gpu.linear_cross_entropy_backward(many, gpu.zeros([rows, 1]), gpu.zeros([2, 1]),
+                                          gpu.from_numpy(np.zeros(rows, np.int32)), many, many)
