@@ -642,7 +642,7 @@ struct Orthogonalize {
   float beta = 0.f, keep = 1.f, rate = 1.f;
 };
 constexpr int64_t kOrthoSide = (int64_t)1 << 19;  // m, n
-size_t orthogonalize_ws_bytes(const Orthogonalize& a);  // 0: none needed
+size_t orthogonalize_ws_bytes(const Orthogonalize& a, int cus);  // 0: none needed
 void orthogonalize(const Orthogonalize& a, void* ws, int cus, hipStream_t s);
 
 // o = x elementwise with dtype conversion, o written through the strides of

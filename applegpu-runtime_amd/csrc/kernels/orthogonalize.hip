@@ -8,7 +8,7 @@
 //                              each stored as its mirror image too
 //   poly    B = b A + c A A    symmetric too (A's rows are its columns)
 //   update  X = a X + B X      X read as columns, so no transpose is kept
-// with one launch each for all matrices of a batch.
+// with one launch each for all matrices of a batch (two, where tiles are cut).
 //
 // Precision: products are of fp16 with fp32 sums, of one plane or of two (22
 // bits), see planes_of.  All entries are at most about
@@ -349,28 +349,77 @@ struct EpiUpdate {
 
 // Square tiles of 256 (one block a compute unit), 128 (both 8 wavefronts) or 64
 // (4).  Large ones where they fill whole rounds of the chip, else the next size
-// that makes enough blocks.  Gram, poly and update in us, 256 / 128 / 64:
+// that makes enough blocks.  Gram, poly (both uncut) and update in us, 256 / 128
+// / 64:
 //   2 x 4096 x 4096 fp32      526/419/572  520/393/575  635/692/889  (272 and 512 tiles of 256)
 //   12 x 768 x 2304           56/28/30     32/13/14     83/66/74
 //   12 x 768 x 768            28/12/13     33/14/14     41/25/28
 //   1280 x 1280               36/14/9.5    42/15/10     50/20/16
 //   200 x 400                 22/9/6       18/7.5/5.4   20/8.4/5.5
 enum { kBig, kMid, kSmall };
-int pick(int64_t M, int64_t N, int64_t count, bool sym, int cus) {
-  auto tiles = [&](int64_t b) {
-    const int64_t m = ceil_div(M, b), n = ceil_div(N, b);
-    return (sym ? m * (m + 1) / 2 : m * n) * count;
-  };
-  const int64_t big = tiles(256);
+int pick(int64_t M, int64_t N, int64_t count, int cus) {
+  const int64_t big = ceil_div(M, 256) * ceil_div(N, 256) * count;
   if (big * 10 >= ceil_div(big, cus) * cus * 9) return kBig;
-  return tiles(128) * 8 >= 5 * cus ? kMid : kSmall;
+  return ceil_div(M, 128) * ceil_div(N, 128) * count * 8 >= 5 * cus ? kMid : kSmall;
 }
 
-template <int PL, Layout AL, Layout BL, bool SYM, class Epi>
+// The same of a symmetric product, whose tiles behind the last whole round of
+// the chip may be cut along k, their parts joined by a launch of its own.  By
+// the time its rounds take, in us: a stage 1.75 in tiles of 256 and 0.95 in
+// tiles of 128 (two planes: 2 and 1.3), a block's start and end 4 of them, the
+// parts' way through memory at 4 TB/s.  Blocks alone on their compute unit are
+// faster than that, so a cut has to win by 15 %.  Whole / cut, us:
+//   2 x 4096 x 4096 fp32              435 / 372 + 13   (256 tiles of 256 and 16 in 12 parts)
+//   4 x 1280 x 1280 over 5120 fp16    81 / 63 + 10     (220 tiles of 128 in 2 parts)
+//   of two planes                     162 / 121 + 17   (60 tiles of 256 in 4)
+//   4 x 1280 x 1280 over 1280 of two  49 / 40 + 15     (not cut)
+struct Cut {
+  int tile;
+  int splits;     // of the tiles from `whole` on
+  int64_t whole;
+  size_t bytes;   // of their parts
+};
+Cut cut(int64_t side, int64_t k, int64_t count, int planes, int cus) {
+  auto tiles = [&](int64_t b) {
+    const int64_t m = ceil_div(side, b);
+    return m * (m + 1) / 2 * count;
+  };
+  if (tiles(128) * 8 < 5 * cus) return {kSmall, 1, tiles(64), 0};
+  const int64_t stages = ceil_div(k, 64 / planes);
+  Cut best{kMid, 1, tiles(128), 0};
+  double least = 1e300;
+  for (int tile : {kBig, kMid}) {
+    const int64_t b = tile == kBig ? 256 : 128, all = tiles(b), slots = tile == kBig ? cus : 2 * cus;
+    const double stage = planes == 1 ? (tile == kBig ? 1.75 : 0.95) : (tile == kBig ? 2.0 : 1.3);
+    for (int s : {1, 2, 3, 4, 6, 8, 12, 16}) {
+      if (s > 1 && s * 4 > stages) break;
+      const int64_t whole = s > 1 ? all / slots * slots : all, rest = all - whole;
+      const size_t bytes = (size_t)(rest * s * b * b * 4);
+      const double t = ((double)ceil_div(whole, slots) * (double)(stages + 4) +
+                        (double)ceil_div(rest * s, slots) * (double)(ceil_div(stages, s) + 4)) * stage +
+                       (rest ? 6 + (double)bytes * 2 / 4e6 : 0);
+      if (t * (rest ? 1.15 : 1.0) < least) {
+        least = t * (rest ? 1.15 : 1.0);
+        best = {tile, s, whole, bytes};
+      }
+    }
+  }
+  return best;
+}
+
+template <int PL, Layout AL, Layout BL, class Epi>
 void run(int tile, const Args& p, const Epi& e, hipStream_t s, const char* what) {
-  if (tile == kBig) launch<Tile<half_t, 4, 2, 2, 4, PL, AL, BL, SYM>>(p, e, s, what);
-  else if (tile == kMid) launch<Tile<half_t, 2, 1, 2, 4, PL, AL, BL, SYM>>(p, e, s, what);
-  else launch<Tile<half_t, 1, 1, 2, 2, PL, AL, BL, SYM>>(p, e, s, what);
+  if (tile == kBig) launch<Tile<half_t, 4, 2, 2, 4, PL, AL, BL>>(p, e, s, what);
+  else if (tile == kMid) launch<Tile<half_t, 2, 1, 2, 4, PL, AL, BL>>(p, e, s, what);
+  else launch<Tile<half_t, 1, 1, 2, 2, PL, AL, BL>>(p, e, s, what);
+}
+template <int PL, Layout L, class Epi>
+void run_symmetric(const Cut& c, const Args& p, const Epi& e, float* part, hipStream_t s, const char* what) {
+  typedef Tile<half_t, 1, 1, 2, 2, PL, L, L, true> Small;
+  typedef Tile<half_t, 1, 1, 2, 2, PL, kRows, kRows, true> Join;
+  if (c.tile == kBig) launch_tail<Tile<half_t, 4, 2, 2, 4, PL, L, L, true>, Join>(p, e, c.whole, c.splits, part, s, what);
+  else if (c.tile == kMid) launch_tail<Tile<half_t, 2, 1, 2, 4, PL, L, L, true>, Join>(p, e, c.whole, c.splits, part, s, what);
+  else launch<Small>(p, e, s, what);
 }
 
 // fp16 planes of a step's factors.  What a step rounds is passed on by the
@@ -392,9 +441,10 @@ struct Space {
   double* part;
   Kept keep;
   half_t *planes[2], *a, *b;
+  float* split;
   size_t bytes;
 };
-Space space(const Orthogonalize& a, char* base) {
+Space space(const Orthogonalize& a, int cus, char* base) {
   Space w;
   size_t used = 0;
   auto take = [&](size_t n) {
@@ -410,6 +460,10 @@ Space space(const Orthogonalize& a, char* base) {
   for (auto& q : w.planes) q = (half_t*)take((size_t)(a.count * a.m * row_of(a.n, pl)) * 2);
   w.a = (half_t*)take((size_t)(a.count * side * row_of(side, pl)) * 2);
   w.b = (half_t*)take((size_t)(a.count * side * row_of(side, pl)) * 2);
+  size_t split = 0;
+  for (int planes : {planes_of(a, 0), pl})
+    for (int64_t k : {std::max(a.m, a.n), side}) split = std::max(split, cut(side, k, a.count, planes, cus).bytes);
+  w.split = (float*)take(split);
   w.bytes = used;
   return w;
 }
@@ -436,7 +490,7 @@ template <typename TO, bool F32, int PL, int NEXT>
 void step(const Orthogonalize& a, const Space& w, int i, int cus, hipStream_t s, const char* what) {
   const int64_t m = a.m, n = a.n, side = std::min(m, n), ld = row_of(n, PL), lda = row_of(side, PL);
   const bool tall = m > n;
-  const int gram = pick(side, side, a.count, true, cus), upd = pick(m, n, a.count, false, cus);
+  const int upd = pick(m, n, a.count, cus);
   const Operand xo{w.planes[i & 1], ld, m * ld}, ao{w.a, lda, side * lda}, bo{w.b, lda, side * lda};
   Args p;
   p.batches = (int)a.count;
@@ -444,26 +498,28 @@ void step(const Orthogonalize& a, const Space& w, int i, int cus, hipStream_t s,
   p.M = p.N = side;
   p.K = tall ? m : n;
   const EpiGram<false> eg{nullptr, w.a, lda, side * lda};
-  if (tall) run<PL, kCols, kCols, true>(gram, p, eg, s, what);
-  else run<PL, kRows, kRows, true>(gram, p, eg, s, what);
+  const Cut gram = cut(side, p.K, a.count, PL, cus);
+  if (tall) run_symmetric<PL, kCols>(gram, p, eg, w.split, s, what);
+  else run_symmetric<PL, kRows>(gram, p, eg, w.split, s, what);
   p.a = p.b = ao;
   p.K = side;
-  run<PL, kRows, kRows, true>(gram, p, EpiGram<true>{w.a, w.b, lda, side * lda}, s, what);
+  run_symmetric<PL, kRows>(cut(side, side, a.count, PL, cus), p, EpiGram<true>{w.a, w.b, lda, side * lda}, w.split, s,
+                           what);
   p.M = m;
   p.N = n;
   p.a = tall ? xo : bo;
   p.b = tall ? bo : xo;
   const EpiUpdate<TO, F32, NEXT> eu{w.planes[i & 1], ld, w.keep, w.planes[(i + 1) & 1], row_of(n, NEXT), a.out,
                                     a.momentum, a.keep, a.rate};
-  if (tall) run<PL, kRows, kRows, false>(upd, p, eu, s, what);
-  else run<PL, kRows, kCols, false>(upd, p, eu, s, what);
+  if (tall) run<PL, kRows, kRows>(upd, p, eu, s, what);
+  else run<PL, kRows, kCols>(upd, p, eu, s, what);
 }
 
 // ── small matrices: everything in one block ───────────────────────────────
 // A matrix of at most kSmallValues values (sides rounded up to 32), the shorter
 // side at most 128, stays in one block's LDS and registers from its norm to its
 // result: one launch where the products of a step would be three of 4.5 us each
-// (128 x 64 fp32, five steps: 73 us, so 17).  X and the Gram matrix (then the
+// (128 x 64 fp32, five steps: 73 us, so 27).  X and the Gram matrix (then the
 // polynomial in its place) are two fp16 planes each; a wavefront holds two 32 x
 // 32 tiles of X in fp32.
 constexpr int kSmallValues = 16384, kSmallWaves = 8;
@@ -678,7 +734,9 @@ void small(const Orthogonalize& a, hipStream_t s, const char* what) {
 
 }  // namespace
 
-size_t orthogonalize_ws_bytes(const Orthogonalize& a) { return small_ok(a) ? 0 : space(a, nullptr).bytes; }
+size_t orthogonalize_ws_bytes(const Orthogonalize& a, int cus) {
+  return small_ok(a) ? 0 : space(a, cus, nullptr).bytes;
+}
 
 void orthogonalize(const Orthogonalize& a, void* ws, int cus, hipStream_t s) {
   const char* what = a.momentum ? "muon_step" : "orthogonalize";
@@ -686,7 +744,7 @@ void orthogonalize(const Orthogonalize& a, void* ws, int cus, hipStream_t s) {
     AGPU_FLOAT_SWITCH(a.dt, small<T>(a, s, what));
     return;
   }
-  const Space w = space(a, (char*)ws);
+  const Space w = space(a, cus, (char*)ws);
   AGPU_FLOAT_SWITCH(a.dt, if (a.momentum) start<T, true>(a, w, s, what); else start<T, false>(a, w, s, what));
   const bool f32 = a.dt == DType::F32;
   for (int i = 0; i + 1 < a.steps; ++i) {

@@ -63,7 +63,8 @@ struct Operand {
 struct Args {
   Operand a, b;
   int64_t M = 0, N = 0, K = 0;
-  int tiles_m = 0, tiles_n = 0, tiles = 0;  // tiles: those that are computed
+  int tiles_m = 0, tiles_n = 0, tiles = 0;  // tiles: those that are computed of a matrix
+  int first = 0, some = 0;  // of all matrices' tiles, the launch's first and number (0: all)
   int splits = 1, batches = 1;
   int stages = 0, per_split = 0;
   const float2* b_power = nullptr;  // what fp32 rows of b are multiplied by before they are split (.x)
@@ -218,6 +219,7 @@ __device__ __forceinline__ void split_raw(const Raw8& v, float power, Mfma<half_
 struct Place {
   int64_t m0, n0;
   int tm, tn, split, batch;
+  int index;  // of the launch's tiles
   int wave, wm, wn, lane;
 };
 
@@ -243,16 +245,23 @@ struct Tile {
   // Blocks in an order that keeps neighbours on one XCD (its blocks are every
   // eighth), groups of `group` tile rows column by column.
   static __device__ __forceinline__ Place place(const Args& p, int block, int blocks) {
+    const int x = block & 7, each = blocks >> 3, more = blocks & 7;
+    const int id = x * each + (x < more ? x : more) + (block >> 3);
+    Place c = place_of(p, id % p.some);
+    c.split = id / p.some;
+    return c;
+  }
+  // The launch's tile `index`, not split.
+  static __device__ __forceinline__ Place place_of(const Args& p, int index) {
     Place c;
     c.lane = threadIdx.x & 63;
     c.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     c.wm = c.wave / WN;
     c.wn = c.wave % WN;
-    const int x = block & 7, each = blocks >> 3, more = blocks & 7;
-    const int id = x * each + (x < more ? x : more) + (block >> 3);
-    const int t = id % p.tiles, rest = id / p.tiles;
-    c.split = rest % p.splits;
-    c.batch = rest / p.splits;
+    c.index = index;
+    const int t = (p.first + index) % p.tiles;
+    c.split = 0;
+    c.batch = (p.first + index) / p.tiles;
     if constexpr (SYM) {
       // tile t of the triangle, row by row
       int r = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
@@ -519,7 +528,7 @@ __global__ void __launch_bounds__(64 * TL1::NW, waves_for(TL1::NW)) tile_pair_ke
   static_assert(TL1::NW == TL2::NW, "wavefronts of a block");
   constexpr int n = TL1::LDS > TL2::LDS ? TL1::LDS : TL2::LDS;
   __shared__ __attribute__((aligned(16))) typename TL1::T lds[n];
-  const int first = p1.tiles * p1.splits * p1.batches;
+  const int first = p1.some * p1.splits;
   if ((int)blockIdx.x < first) tile_block<TL1>(p1, e1, lds, blockIdx.x, first);
   else tile_block<TL2>(p2, e2, lds, blockIdx.x - first, gridDim.x - first);
 }
@@ -534,13 +543,14 @@ int64_t blocks_of(Args& p, const char* what) {
   const int64_t tiles = TL::SYM ? (int64_t)p.tiles_m * (p.tiles_m + 1) / 2 : (int64_t)p.tiles_m * p.tiles_n;
   p.stages = (int)ceil_div(p.K, TL::KS);
   p.per_split = (int)ceil_div(p.stages, p.splits);
-  const int64_t blocks = tiles * p.splits * p.batches;
+  const int64_t some = p.some ? p.some : tiles * p.batches, blocks = some * p.splits;
   // (a tile's rows, or its panels, lie within the 2 GiB that a buffer resource
   // spans)
   if (blocks < 1 || blocks >= (1LL << 30) || p.a.ld >= (TL::SA::PANEL ? 1 << 27 : 1 << 21) || p.b.ld >= (1 << 21))
     fail("%s: a product of %lld x %lld x %lld in %d parts is too large", what, (long long)p.M, (long long)p.N,
          (long long)p.K, p.splits);
   p.tiles = (int)tiles;
+  p.some = (int)some;
   return blocks;
 }
 
@@ -555,6 +565,83 @@ void launch_pair(Args p1, const E1& e1, Args p2, const E2& e2, hipStream_t s, co
   const int64_t blocks = blocks_of<TL1>(p1, what) + blocks_of<TL2>(p2, what);
   hipLaunchKernelGGL((tile_pair_kernel<TL1, E1, TL2, E2>), dim3((unsigned)blocks), dim3(64 * TL1::NW), 0, s, p1, e1, p2,
                      e2);
+  check_launch(what);
+}
+
+// A product whose last tiles, fewer than fill the chip, are split over k: the
+// tiles from p.some on in `splits` parts, which join_kernel sums in order.
+template <class TL, class Epi>
+__global__ void __launch_bounds__(64 * TL::NW, waves_for(TL::NW)) tail_kernel(Args p, Epi e, int splits, float* part) {
+  __shared__ __attribute__((aligned(16))) typename TL::T lds[TL::LDS];
+  const bool tail = (int)blockIdx.x >= p.some;
+  const int whole = p.some;
+  if (tail) {
+    p.first = whole;
+    p.some = (int)(gridDim.x - whole) / splits;
+    p.splits = splits;
+    p.per_split = (p.stages + splits - 1) / splits;
+  }
+  const Place c = TL::place(p, blockIdx.x - (tail ? whole : 0), tail ? gridDim.x - whole : whole);
+  typename TL::Acc acc;
+  TL::product(p, c, lds, acc);
+  if (!tail) {
+    e.template form<TL>(p, c, acc);
+    e.template store<TL>(p, c, lds, acc);
+    return;
+  }
+  float* to = part + ((int64_t)c.index * splits + c.split) * (TL::BM * TL::BN);
+  Place at = c;
+  at.m0 = at.n0 = 0;
+  TL::template runs<false>(
+      at, lds, acc, false,
+      [&](int64_t row, int64_t col, float (&v)[8]) {
+        float4* o = (float4*)(to + row * TL::BN + col);
+        o[0] = *(const float4*)v;
+        o[1] = *(const float4*)(v + 4);
+      },
+      [](int64_t, int64_t, float (&)[8]) {});
+}
+// The tiles of BIG that were split, from p.first on, in blocks of JT's shape.
+template <class BIG, class JT, class Epi>
+__global__ void __launch_bounds__(64 * JT::NW) join_kernel(Args p, Epi e, int splits, const float* part) {
+  __shared__ __attribute__((aligned(16))) typename JT::T lds[JT::LDS];
+  constexpr int ACROSS = BIG::BN / JT::BN, EACH = BIG::BM / JT::BM * ACROSS;
+  const int tile = blockIdx.x / EACH, m = blockIdx.x % EACH / ACROSS * JT::BM, n = blockIdx.x % ACROSS * JT::BN;
+  const Place big = BIG::place_of(p, tile);
+  Place c = JT::place_of(p, tile);
+  c.tm = big.tm;
+  c.tn = big.tn;
+  c.batch = big.batch;
+  c.m0 = big.m0 + m;
+  c.n0 = big.n0 + n;
+  if (c.m0 >= p.M || c.n0 >= p.N) return;
+  constexpr int64_t kTile = BIG::BM * BIG::BN;
+  const float* from = part + (int64_t)tile * splits * kTile + m * BIG::BN + n;
+  typename JT::Acc acc = {};
+  for (int s = 0; s < splits; ++s, from += kTile)
+    JT::fours(acc, [&](int i, int j, int g, float (&v)[4]) {
+      const float4 q = *(const float4*)(from + JT::row_of(c, i) * BIG::BN + JT::col_of(c, j, 4 * g));
+      v[0] += q.x; v[1] += q.y; v[2] += q.z; v[3] += q.w;
+    });
+  e.template form<JT>(p, c, acc);
+  e.template store<JT>(p, c, lds, acc);
+}
+// The first `whole` tiles as they are, those behind them split and joined; part
+// holds (tiles - whole) * splits tiles.
+template <class TL, class JT, class Epi>
+void launch_tail(Args p, const Epi& e, int64_t whole, int splits, float* part, hipStream_t s, const char* what) {
+  const int64_t all = blocks_of<TL>(p, what), rest = all - whole, blocks = whole + rest * splits;
+  constexpr int EACH = TL::BM / JT::BM * (TL::BN / JT::BN);
+  if (rest < 0 || blocks >= (1LL << 30) || rest * EACH >= (1LL << 30))
+    fail("%s: %lld tiles in %d parts", what, (long long)rest, splits);
+  p.some = (int)whole;
+  hipLaunchKernelGGL((tail_kernel<TL, Epi>), dim3((unsigned)blocks), dim3(64 * TL::NW), 0, s, p, e, splits, part);
+  check_launch(what);
+  if (rest == 0) return;
+  p.first = (int)whole;
+  p.some = (int)rest;
+  hipLaunchKernelGGL((join_kernel<TL, JT, Epi>), dim3((unsigned)(rest * EACH)), dim3(64 * JT::NW), 0, s, p, e, splits,
+                     part);
   check_launch(what);
 }
 

@@ -2401,8 +2401,19 @@ static void check_ortho(const char* name, int64_t m, int64_t n, int64_t steps, d
 // Matrices at once: as many as 4 GB of workspace hold, one at least.
 static int64_t ortho_group(k::Orthogonalize a, int64_t most) {
   a.count = 1;
-  const size_t each = std::max<size_t>(k::orthogonalize_ws_bytes(a), 1);
+  const size_t each = std::max<size_t>(k::orthogonalize_ws_bytes(a, rt().info().cu_count), 1);
   return std::max<int64_t>(1, std::min<int64_t>({most, (int64_t)(((size_t)4 << 30) / each), 65535}));
+}
+
+// The workspace of `all` matrices, `each` at a time: the last ones, fewer, may
+// be cut into more parts.
+static BufferP ortho_scratch(k::Orthogonalize a, int64_t all, int64_t each) {
+  const int cus = rt().info().cu_count;
+  a.count = each;
+  size_t bytes = k::orthogonalize_ws_bytes(a, cus);
+  a.count = all % each;
+  if (a.count) bytes = std::max(bytes, k::orthogonalize_ws_bytes(a, cus));
+  return bytes ? scratch(bytes) : nullptr;
 }
 
 TensorP orthogonalize(const TensorP& g, int64_t steps, float eps) {
@@ -2420,10 +2431,7 @@ TensorP orthogonalize(const TensorP& g, int64_t steps, float eps) {
   a.eps = eps;
   a.in.apart = a.out.apart = a.m * a.n;
   const int64_t all = g->numel() / a.in.apart, each = ortho_group(a, all);
-  a.count = each;
-  const size_t wsb = k::orthogonalize_ws_bytes(a);
-  BufferP ws;
-  if (wsb) ws = scratch(wsb);
+  const BufferP ws = ortho_scratch(a, all, each);
   for (int64_t i = 0; i < all; i += each) {
     a.count = std::min(each, all - i);
     const size_t at = (size_t)(i * a.in.apart) * dtype_size(g->dtype);
@@ -2483,10 +2491,7 @@ void muon_step_(const std::vector<TensorP>& w, const std::vector<TensorP>& mom, 
   a.keep = (float)(1.0 - o.lr * o.decay);
   a.rate = (float)(o.lr * std::sqrt(std::max(1.0, (double)a.m / (double)a.n)));
   const int64_t all = (int64_t)w.size(), each = ortho_group(a, std::min<int64_t>(all, k::kOrthoMats));
-  a.count = each;
-  const size_t wsb = k::orthogonalize_ws_bytes(a);
-  BufferP ws;
-  if (wsb) ws = scratch(wsb);
+  const BufferP ws = ortho_scratch(a, all, each);
   for (int64_t i = 0; i < all; i += each) {
     a.count = std::min(each, all - i);
     for (int64_t j = 0; j < a.count; ++j) {

@@ -71,6 +71,33 @@ def test_orthogonalize_vs_oracle(gpu, shape, dtype):
     _check(out.to_numpy(), *_bars(g, dtype), HALF_STEP[dtype])
 
 
+# products whose last tiles, or all of them, are cut along k and joined: of 128
+# and of 256 wide, of X and of the Gram matrix itself, ragged, from either side
+@pytest.mark.parametrize("shape,dtype,steps", [
+    ((90, 257, 1500), "bfloat16", 5), ((90, 900, 257), "float32", 5), ((27, 1500, 300), "float32", 5),
+    ((27, 300, 3000), "float16", 5), ((2300, 2300), "float32", 1), ((5700, 2850), "float32", 1)])
+def test_cut_products_vs_oracle(gpu, shape, dtype, steps):
+    g = _gradient(shape, dtype)
+    out = gpu.orthogonalize(_dev(gpu, g, dtype), steps=steps)
+    out, again = out.to_numpy(), gpu.orthogonalize(_dev(gpu, g, dtype), steps=steps).to_numpy()
+    np.testing.assert_array_equal(out, again)
+    some = [0, len(g) // 2, len(g) - 1] if g.ndim == 3 else ...
+    _check(out[some], *_bars(g[some], dtype, steps=steps), HALF_STEP[dtype])
+
+
+def test_cut_products_of_a_smaller_last_group(gpu):
+    """More matrices than a launch takes by their addresses: the last ones, fewer,
+    are cut elsewhere than the first."""
+    rng = np.random.default_rng(3)
+    n, shape = 40, (700, 2000)
+    g = [_gradient(shape, "float32", seed=i) for i in range(2)]
+    w, mom = [_dev(gpu, np.zeros(shape)) for _ in range(n)], [_dev(gpu, np.zeros(shape)) for _ in range(n)]
+    gpu.muon_step_(w, mom, [_dev(gpu, g[i % 2]) for i in range(n)], lr=1.0, beta=0.0)
+    bars = [_bars(a, "float32") for a in g]
+    for i in (0, 1, 31, 32, 39):
+        _check(-w[i].to_numpy(), *bars[i % 2], HALF_STEP["float32"])
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("shape", [(1, 1), (5, 9), (64, 128), (96, 40), (257, 130)])
 def test_muon_step_vs_oracle(gpu, shape, dtype):
