@@ -241,6 +241,11 @@ def linear_cross_entropy_backward(grad_loss, x, w, targets, loss, lse, grad_lse=
     return op("linear_cross_entropy_backward", ins, nout=2)
 
 
+def orthogonalize(g, steps=5, eps=1e-7):
+    """The matrices of g [..., m, n] with their singular values taken towards 1."""
+    return op("orthogonalize", [g], f=(float(eps),), i=(int(steps),))
+
+
 def muon_step_(weights, momenta, grads, lr=0.02, beta=0.95, weight_decay=0.0, nesterov=True, steps=5, eps=1e-7):
     """An optimiser's step with orthogonalised updates, in place, on matrices
     of one shape: momentum = beta momentum + grad, U = grad + beta momentum (or

@@ -85,6 +85,14 @@ def test_cut_products_vs_oracle(gpu, shape, dtype, steps):
     _check(out[some], *_bars(g[some], dtype, steps=steps), HALF_STEP[dtype])
 
 
+def test_eager_entry(gpu):
+    from applegpu_runtime import eager as E
+    E.init()
+    g = _gradient((3, 40, 70), "float32")
+    np.testing.assert_array_equal(E.orthogonalize(E.from_numpy(g.astype(np.float32)), steps=3).numpy(),
+                                  gpu.orthogonalize(_dev(gpu, g), steps=3).to_numpy())
+
+
 def test_cut_products_of_a_smaller_last_group(gpu):
     """More matrices than a launch takes by their addresses: the last ones, fewer,
     are cut elsewhere than the first."""
