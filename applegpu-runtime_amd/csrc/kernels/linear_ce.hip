@@ -456,7 +456,7 @@ struct EpiOut {
   }
 };
 
-// out [R, K] = the parts' sum times the inverse powers, and what they lost.  G
+// out [.., K] = the parts' sum times the inverse powers, and what they lost.  G
 // threads take the parts of 4 values in turn and their sums are added in order:
 // many parts behind one another are a chain of loads (32 parts of 61 x 1280, one
 // thread / eight: 10.4 / 6.5 us).
@@ -661,34 +661,42 @@ double ends(int64_t n1, double l1, int64_t n2, double l2, int64_t slots) {
   return t;
 }
 
-// The products dx (over the words, in parts) and dw of a piece in one launch:
-// tiles and parts by the time they end, in us.  A stage of 64 k takes 1.75 us in
+// The products dx (over the words, in parts) and dw (over the rows, in parts
+// where the vocabulary is one piece) in one launch: tiles and parts by the time
+// they end, in us.  A stage of 64 k takes 1.75 us in
 // 256 x 256 tiles, 0.95 in 128 x 128 ones (two blocks a compute unit); a block's
 // start and end count as 4 stages; parts are written and read back at 6 TB/s
 // and summed by a launch of their own.  us at 2 / 4 / 8 / 16 / 32 parts, 256:
 // 61 x 50257 x 1280 fp16 536 / 287 / 165 / 114 / 106, 2047 x 10007 x 768 bf16
 // 187 / 138 / 163 / 171 / 219; 128: 275 / 155 / 103 / 103 / 100, 135 / 138 / 148
-// / 163 / 201.
+// / 163 / 201.  The whole gradient with dw in one part / in those chosen: bf16,
+// 16384 x 100 x 768 206 / 57, 16384 x 5000 x 64 233 / 125; fp32, 4096 x 1000 x 64
+// 120 / 49.
 struct Plan {
   bool big;
-  int parts;
+  int parts, wparts;
 };
-Plan plan_products(int64_t R, int64_t K, int64_t words, int ks, int cus) {
-  Plan best{false, 1};
+Plan plan_products(int64_t R, int64_t K, int64_t words, bool one_piece, int ks, int cus) {
+  Plan best{false, 1, 1};
   double least = 1e300;
-  const double rows_len = (double)ceil_div(R, ks) + 4;
-  const int64_t stages = ceil_div(words, ks);
+  const int64_t stages = ceil_div(words, ks), row_stages = ceil_div(R, ks);
+  constexpr int kMany[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48};
+  auto join = [&](int parts, int64_t values) { return parts > 1 ? 4 + parts * (double)values * 8 / 6e6 : 0; };
   for (int big = R > 32 ? 1 : 0; big >= 0; --big) {
     const int64_t side = big ? 256 : 128, xside = R <= 32 ? 32 : side;
     const int64_t xtiles = ceil_div(R, xside) * ceil_div(K, side), wtiles = ceil_div(words, side) * ceil_div(K, side);
-    for (int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48}) {
-      if (s > 1 && s * 4 > stages) break;
-      const double len = (double)ceil_div(stages, s) + 4;
-      const double t = ends(xtiles * s, len, wtiles, rows_len, big ? cus : 2 * cus) * (big ? 1.75 : 0.95) +
-                       (s > 1 ? 4 + s * (double)(R * K) * 8 / 6e6 : 0);
-      if (t < least) {
-        least = t;
-        best = {big != 0, s};
+    for (int w : kMany) {
+      if (w > 1 && (!one_piece || w * 4 > row_stages)) break;
+      const double wlen = (double)ceil_div(row_stages, w) + 4;
+      for (int s : kMany) {
+        if (s > 1 && s * 4 > stages) break;
+        const double len = (double)ceil_div(stages, s) + 4;
+        const double t = ends(xtiles * s, len, wtiles * w, wlen, big ? cus : 2 * cus) * (big ? 1.75 : 0.95) +
+                         join(s, R * K) + join(w, words * K);
+        if (t < least) {
+          least = t;
+          best = {big != 0, s, w};
+        }
       }
     }
   }
@@ -714,10 +722,11 @@ size_t backward(const LinearCE& a, void* wsp, int cus, hipStream_t s) {
   constexpr bool scaled = !std::is_same<T, bf16_t>::value;
   float2* pg = scaled ? ws.take<float2>(1) : nullptr;
   float4* rows = ws.take<float4>((size_t)a.R);
-  const Plan plan = plan_products(a.R, a.K, len, 64 / PL, cus);
+  const Plan plan = plan_products(a.R, a.K, len, pieces == 1, 64 / PL, cus);
   const int splits = plan.parts;
   const bool parted = splits > 1 || pieces > 1;
   float* part = parted ? ws.take<float>((size_t)(splits * a.R * a.K)) : nullptr;
+  float* wpart = plan.wparts > 1 ? ws.take<float>((size_t)(plan.wparts * a.V * a.K)) : nullptr;
   if (!wsp) return ws.used;
   hipLaunchKernelGGL((rows_kernel<T, PL>), dim3(blocks_for(a.R, 1024)), dim3(1024), 0, s, a.g_loss, a.g_lse, a.loss,
                      a.lse, a.targets, wide, a.R, a.V, pg, rows);
@@ -736,9 +745,9 @@ size_t backward(const LinearCE& a, void* wsp, int cus, hipStream_t s) {
     px.b = wp;
     px.M = a.R; px.N = a.K; px.K = n; px.splits = splits;
     pw.b = x.o;
-    pw.M = n; pw.N = a.K; pw.K = a.R;
+    pw.M = n; pw.N = a.K; pw.K = a.R; pw.splits = plan.wparts;
     const EpiOut<TI> ex{(TI*)a.dx, part, v0 > 0, pg, w.power, lost},
-        ew{(TI*)a.dw + v0 * a.K, nullptr, false, pg, x.power, {}};
+        ew{(TI*)a.dw + v0 * a.K, wpart, false, pg, x.power, {}};
     typedef Tile<T, 2, 2, 2, 2, PL, kPanelCols, kCols> WFew;  // (of four wavefronts, as dx's)
     if (plan.big)
       launch_pair<Tile<T, 4, 2, 2, 4, PL, kPanelRows, kCols>, Tile<T, 4, 2, 2, 4, PL, kPanelCols, kCols>>(px, ex, pw, ew, s, what);
@@ -747,16 +756,17 @@ size_t backward(const LinearCE& a, void* wsp, int cus, hipStream_t s) {
     else
       launch_pair<Tile<T, 1, 1, 1, 4, PL, kPanelRows, kCols>, WFew>(px, ex, pw, ew, s, what);
   }
-  if (parted) {
-    const int64_t n = a.R * a.K;
-    auto sum = [&](auto kernel, int threads) {
-      hipLaunchKernelGGL(kernel, dim3(blocks_for(n * threads, 1024)), dim3(256), 0, s, part, splits, n, a.K, pg, w.power,
-                         lost, (TI*)a.dx);
+  auto sum = [&](const float* of, int parts, int64_t n, const float2* power, const Lost<TI>& back, void* out) {
+    auto go = [&](auto kernel, int threads) {
+      hipLaunchKernelGGL(kernel, dim3(blocks_for(n * threads, 1024)), dim3(256), 0, s, of, parts, n, a.K, pg, power, back,
+                         (TI*)out);
     };
-    if (splits >= 8) sum(sum_parts_kernel<TI, 8>, 8);
-    else sum(sum_parts_kernel<TI, 1>, 1);
+    if (parts >= 8) go(sum_parts_kernel<TI, 8>, 8);
+    else go(sum_parts_kernel<TI, 1>, 1);
     check_launch(what);
-  }
+  };
+  if (parted) sum(part, splits, a.R * a.K, w.power, lost, a.dx);
+  if (wpart) sum(wpart, plan.wparts, a.V * a.K, x.power, {}, a.dw);
   return ws.used;
 }
 

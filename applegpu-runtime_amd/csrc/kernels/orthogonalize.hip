@@ -366,13 +366,16 @@ int pick(int64_t M, int64_t N, int64_t count, int cus) {
 // The same of a symmetric product, whose tiles behind the last whole round of
 // the chip may be cut along k, their parts joined by a launch of its own.  By
 // the time its rounds take, in us: a stage 1.75 in tiles of 256 and 0.95 in
-// tiles of 128 (two planes: 2 and 1.3), a block's start and end 4 of them, the
-// parts' way through memory at 4 TB/s.  Blocks alone on their compute unit are
+// tiles of 128 (two planes: 2 and 1.3), 0.4 in tiles of 64 (0.5), of which four
+// blocks share a compute unit and which small products take; a block's start and
+// end 4 stages, the parts' way through memory at 4 TB/s.  Blocks alone on their compute unit are
 // faster than that, so a cut has to win by 15 %.  Whole / cut, us:
 //   2 x 4096 x 4096 fp32              435 / 372 + 13   (256 tiles of 256 and 16 in 12 parts)
 //   4 x 1280 x 1280 over 5120 fp16    81 / 63 + 10     (220 tiles of 128 in 2 parts)
 //   of two planes                     162 / 121 + 17   (60 tiles of 256 in 4)
 //   4 x 1280 x 1280 over 1280 of two  49 / 40 + 15     (not cut)
+// and all launches of a matrix in tiles of 64, bf16: 64 x 4096 211 / 118, 768 x
+// 2304 273 / 217, 16 x 100000 3844 / 320; fp32: 340 / 159, 480 / 321, 7976 / 364.
 struct Cut {
   int tile;
   int splits;     // of the tiles from `whole` on
@@ -384,14 +387,17 @@ Cut cut(int64_t side, int64_t k, int64_t count, int planes, int cus) {
     const int64_t m = ceil_div(side, b);
     return m * (m + 1) / 2 * count;
   };
-  if (tiles(128) * 8 < 5 * cus) return {kSmall, 1, tiles(64), 0};
+  const bool few = tiles(128) * 8 < 5 * cus;
   const int64_t stages = ceil_div(k, 64 / planes);
-  Cut best{kMid, 1, tiles(128), 0};
+  Cut best{};
   double least = 1e300;
-  for (int tile : {kBig, kMid}) {
-    const int64_t b = tile == kBig ? 256 : 128, all = tiles(b), slots = tile == kBig ? cus : 2 * cus;
-    const double stage = planes == 1 ? (tile == kBig ? 1.75 : 0.95) : (tile == kBig ? 2.0 : 1.3);
-    for (int s : {1, 2, 3, 4, 6, 8, 12, 16}) {
+  for (int tile : {kBig, kMid, kSmall}) {
+    if (few != (tile == kSmall)) continue;
+    const int64_t b = tile == kBig ? 256 : tile == kMid ? 128 : 64, all = tiles(b);
+    const int64_t slots = (tile == kBig ? 1 : tile == kMid ? 2 : 4) * cus;
+    static const double kStage[2][3] = {{1.75, 0.95, 0.4}, {2.0, 1.3, 0.5}};
+    const double stage = kStage[planes - 1][tile];
+    for (int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
       if (s > 1 && s * 4 > stages) break;
       const int64_t whole = s > 1 ? all / slots * slots : all, rest = all - whole;
       const size_t bytes = (size_t)(rest * s * b * b * 4);
@@ -415,11 +421,10 @@ void run(int tile, const Args& p, const Epi& e, hipStream_t s, const char* what)
 }
 template <int PL, Layout L, class Epi>
 void run_symmetric(const Cut& c, const Args& p, const Epi& e, float* part, hipStream_t s, const char* what) {
-  typedef Tile<half_t, 1, 1, 2, 2, PL, L, L, true> Small;
   typedef Tile<half_t, 1, 1, 2, 2, PL, kRows, kRows, true> Join;
   if (c.tile == kBig) launch_tail<Tile<half_t, 4, 2, 2, 4, PL, L, L, true>, Join>(p, e, c.whole, c.splits, part, s, what);
   else if (c.tile == kMid) launch_tail<Tile<half_t, 2, 1, 2, 4, PL, L, L, true>, Join>(p, e, c.whole, c.splits, part, s, what);
-  else launch<Small>(p, e, s, what);
+  else launch_tail<Tile<half_t, 1, 1, 2, 2, PL, L, L, true>, Join>(p, e, c.whole, c.splits, part, s, what);
 }
 
 // fp16 planes of a step's factors.  What a step rounds is passed on by the

@@ -175,6 +175,30 @@ def test_gradient_at_the_edges_of_words_and_rows(gpu, R, V, dtype):
     _check_backward(gpu, x, w, t, dtype, g, None)
 
 
+# few words and many rows: dw in parts
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("R,K,V", [(5000, 70, 30), (3001, 129, 200)])
+def test_gradient_of_few_words(gpu, R, K, V, dtype):
+    x, w, t = _case(R, K, V, dtype, seed=4)
+    g = np.random.default_rng(V).random(R).astype(np.float32) / R
+    got = _check_backward(gpu, x, w, t, dtype, g, None)
+    again = _check_backward(gpu, x, w, t, dtype, g, None)
+    for a, b in zip(got, again):
+        np.testing.assert_array_equal(a.to_numpy(), b.to_numpy())
+
+
+def test_most_rows(gpu):
+    x, w, t = _case(1 << 20, 8, 5, "float16", seed=6)
+    _check_backward(gpu, x, w, t, "float16", np.full(1 << 20, 2.0 ** -10, np.float32), None)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_many_words(gpu, dtype):
+    x, w, t = _case(2, 8, (1 << 21) + 3, dtype, seed=7)
+    _check_forward(gpu, x, w, t, dtype)
+    _check_backward(gpu, x, w, t, dtype, np.full(2, 0.5, np.float32), None)
+
+
 def test_no_rows(gpu):
     for dtype in DTYPES:
         x, w = gpu.zeros([0, 8], dtype), gpu.zeros([5, 8], dtype)
