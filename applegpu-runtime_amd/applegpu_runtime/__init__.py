@@ -711,8 +711,8 @@ def linear_cross_entropy_backward(grad_loss, x, weight, targets, loss, lse, grad
     gradients of its loss and lse (float32 [...]; grad_lse may be None) and the
     loss and lse it returned.  The logits are formed again, in pieces of the
     vocabulary; their gradient is rounded to 16 bits before its products for
-    16-bit operands, and for float16 and float32 ones counts down to 2^-37 of
-    the largest one in the call.  Rows whose target is outside [0, V) get lse's
+    16-bit operands and counts down to 2^-37 (bfloat16: 2^-139) of the largest
+    one in the call.  Rows whose target is outside [0, V) get lse's
     part only; one without any weight gets zeros whatever its logits are.  At
     most 2^20 rows at once."""
     ins = [_t(grad_loss), _t(x), _t(weight), _t(targets), _t(loss), _t(lse)]

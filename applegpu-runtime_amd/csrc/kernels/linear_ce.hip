@@ -16,10 +16,14 @@
 // order, and dw over the rows.  No sum goes through atomics.
 //
 // Roundings: d is rounded once to the operands' 16 bits before its products,
-// as the logits' gradient of any 16-bit program is; fp16 (and the planes of
-// fp32) hold d times a power of two that takes the largest of them to 2^13, so
-// that what is 2^-37 of it still counts.  fp32 operands are scaled
-// alike by their largest magnitude and split into fp16 planes (22 bits).
+// as the logits' gradient of any 16-bit program is, times a factor that takes
+// the largest of them to 255 2^6 (planes of fp32: a power of two, to 2^13 and
+// more), so that in fp16 what is 2^-37 of it still counts, in bf16 2^-139.  That
+// value has 8 bits: rows of one weight, whose targets' d are all nearly the
+// largest, are then held without an error that their sums would keep (96 rows
+// of weight 1.0035 in bf16: error of dw 3.6e-3 with a power of two, so 1.7e-3,
+// its own rounding).  fp32 operands are scaled by a power of two, from their
+// largest magnitude, and split into fp16 planes (22 bits).
 #include "tile16.hpp"
 
 namespace agpu {
@@ -268,13 +272,13 @@ __global__ void __launch_bounds__(256) loss_kernel(const float2* part, int64_t p
 
 // ── backward ──────────────────────────────────────────────────────────────
 // What a row of d is made of: {lse, weight of p, d of the target in 16 bits,
-// what that rounding lost}.  The weight and d hold the power of the largest |d|
-// that any row can have (not for bf16, whose range needs none): of words other
-// than the target |g + h| (1 - p_t), of all |h| where there is none.  A row's
+// what that rounding lost}.  The weight and d hold the factor from the largest
+// |d| that any row can have: of words other than the target |g + h| (1 - p_t),
+// of all |h| where there is none.  A row's
 // largest part is its target's, alone in its size, so its rounding would be
 // dx's: dx gets back what it lost times the target's weights (fp16, 30 rows:
 // error of dx 3.3e-4, so 2.2e-4; of dw, where a word's rows have errors of
-// their own, 3e-4).  Every block finds the power from all rows.
+// their own, 3e-4).  Every block finds the factor from all rows.
 struct RowPart {
   float g, h, dt, most;
 };
@@ -288,27 +292,33 @@ __device__ __forceinline__ RowPart row_part(const float* g, const float* h, cons
   o.most = fmaxf(finite_abs(o.dt), finite_abs((o.g + o.h) * left));
   return o;
 }
+__device__ __forceinline__ float2 factor_for(float most) {
+  constexpr float kLargest = 16320.f;  // 255 2^6
+  return most >= 0x1p-100f ? make_float2(kLargest / most, most / kLargest) : power_for(most);
+}
 template <typename T, int PL>
 __global__ void __launch_bounds__(1024) rows_kernel(const float* g, const float* h, const float* loss, const float* lse,
                                                     const void* targets, bool wide, int64_t R, int64_t V, float2* power,
                                                     float4* rows) {
   __shared__ float red[16];
-  float up = 1.f;
-  if constexpr (!std::is_same<T, bf16_t>::value) {
-    float m = 0.f;
-    for (int64_t i = threadIdx.x; i < R; i += 1024)
-      m = fmaxf(m, row_part(g, h, loss, target_of(targets, wide, i, V) >= 0, i).most);
-    const float2 pw = power_for(block_max(m, red));
-    if (blockIdx.x == 0 && threadIdx.x == 0) *power = pw;
-    up = pw.x;
+  float m = 0.f, top = 0.f;
+  for (int64_t i = threadIdx.x; i < R; i += 1024) {
+    const RowPart o = row_part(g, h, loss, target_of(targets, wide, i, V) >= 0, i);
+    m = fmaxf(m, o.most);
+    top = fmaxf(top, finite_abs(o.g + o.h));
   }
+  // (a weight of p times the factor stays finite where every row is certain)
+  m = fmaxf(block_max(m, red), block_max(top, red) * 0x1p-106f);
+  const float2 pw = PL == 1 ? factor_for(m) : power_for(m);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *power = pw;
+  const float up = pw.x;
   const int64_t r = (int64_t)blockIdx.x * 1024 + threadIdx.x;
   if (r >= R) return;
   const RowPart o = row_part(g, h, loss, target_of(targets, wide, r, V) >= 0, r);
   float held = o.dt * up, lost = 0.f;
   if constexpr (PL == 1) {
     held = to_f(from_f<T>(o.dt * up));
-    lost = (o.dt * up - held) / up;
+    lost = (o.dt * up - held) * pw.y;
     if (!(fabsf(lost) < kInf)) lost = 0.f;
   }
   rows[r] = make_float4(lse[r], (o.g + o.h) * up, held, lost);
@@ -719,8 +729,7 @@ size_t backward(const LinearCE& a, void* wsp, int cus, hipStream_t s) {
   // fp16 within 1 % of one another)
   const int64_t len = std::min(each, a.V), panel = a.R * 64;
   T* d = ws.take<T>((size_t)(panel * ceil_div(len, 64 / PL)));
-  constexpr bool scaled = !std::is_same<T, bf16_t>::value;
-  float2* pg = scaled ? ws.take<float2>(1) : nullptr;
+  float2* pg = ws.take<float2>(1);
   float4* rows = ws.take<float4>((size_t)a.R);
   const Plan plan = plan_products(a.R, a.K, len, pieces == 1, 64 / PL, cus);
   const int splits = plan.parts;

@@ -175,6 +175,45 @@ def test_gradient_at_the_edges_of_words_and_rows(gpu, R, V, dtype):
     _check_backward(gpu, x, w, t, dtype, g, None)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("gap", [80, 83, 86, 120])
+def test_all_but_certain_rows_of_large_weight(gpu, gap, dtype):
+    """1 - p of every target is about exp(-gap), down to nothing: gradients of
+    that size, finite whatever the weights.  Off by lse's rounding (gap 2^-24),
+    the exponent's (1.5 gap 2^-24) and exp2's below float32's normal range."""
+    x, w = np.full((3, 1), gap, np.float32), np.array([[1.0], [0.0]], np.float32)
+    t, g = np.zeros(3, np.int32), np.full(3, 1000, np.float32)
+    dev = [_dev(gpu, x, dtype), _dev(gpu, w, dtype), gpu.from_numpy(t)]
+    got = gpu.linear_cross_entropy_backward(_dev(gpu, g), *dev, *gpu.linear_cross_entropy(*dev))
+    for a, b in zip(got, O.linear_cross_entropy_backward(x, w, t, g, None)):
+        bar = (2 * HALF_STEP[dtype] + 4 * gap * 2.0 ** -24) * np.abs(b) + 3 * 1000 * gap * 2.0 ** -126
+        assert (np.abs(a.to_numpy() - b) <= bar + (2.0 ** -25 if dtype == "float16" else 0)).all()
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+def test_even_weights_are_not_rounded(gpu, dtype):
+    """Rows of one weight g have d = g (p - 1) of their targets alike, whose
+    rounding, the same in every row, no sum would take back: dw of a word that
+    is the target of some is off by its own rounding and by what p and the
+    other words' parts are rounded by, also for a g between two 16-bit values."""
+    R, K, V = 96, 64, 4096
+    u, rng = HALF_STEP[dtype], np.random.default_rng(5)
+    x = few_bits.round_to(rng.standard_normal((R, K)), dtype)
+    w = few_bits.round_to(rng.standard_normal((V, K)) * 2.0 ** -12, dtype)   # p is near 1 / V everywhere
+    t = (np.arange(R) % 24 * 7).astype(np.int32)
+    g = np.full(R, 1 + 0.9 * u, np.float32)
+    dev = [_dev(gpu, x, dtype), _dev(gpu, w, dtype), gpu.from_numpy(t)]
+    dw = gpu.linear_cross_entropy_backward(_dev(gpu, g), *dev, *gpu.linear_cross_entropy(*dev))[1].to_numpy()
+    want = O.linear_cross_entropy_backward(x, w, t, g, None)[1]
+    d = O.logit_gradients(x, w, t, g, None)
+    hit = d < 0
+    # targets' d lie within 2^-18 of the largest, which is held as it is: less
+    # than half a step of 16 bits below it, so they are held as the largest
+    assert 1 - d[hit].max() / d[hit].min() < 2.0 ** -18
+    err = (np.abs(d) * np.where(hit, 2.0 ** -18, 1.01 * u)).T @ np.abs(x).astype(np.float64)
+    assert (np.abs(dw - want) <= u * np.abs(want) * (1 + u) + err + 2.0 ** -20 * (np.abs(d).T @ np.abs(x))).all()
+
+
 # few words and many rows: dw in parts
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("R,K,V", [(5000, 70, 30), (3001, 129, 200)])
