@@ -274,11 +274,10 @@ __global__ void __launch_bounds__(256) loss_kernel(const float2* part, int64_t p
 // What a row of d is made of: {lse, weight of p, d of the target in 16 bits,
 // what that rounding lost}.  The weight and d hold the factor from the largest
 // |d| that any row can have: of words other than the target |g + h| (1 - p_t),
-// of all |h| where there is none.  A row's
-// largest part is its target's, alone in its size, so its rounding would be
-// dx's: dx gets back what it lost times the target's weights (fp16, 30 rows:
-// error of dx 3.3e-4, so 2.2e-4; of dw, where a word's rows have errors of
-// their own, 3e-4).  Every block finds the factor from all rows.
+// of all |h| where there is none.  A row's largest part is its target's, alone in
+// its size, so its rounding would be dx's: dx gets back what it lost times the
+// target's weights (fp16, 30 rows: error of dx 3.3e-4, so 2.2e-4), and dw likewise
+// where rows are few.  Every block finds the factor from all rows.
 struct RowPart {
   float g, h, dt, most;
 };
@@ -296,19 +295,48 @@ __device__ __forceinline__ float2 factor_for(float most) {
   constexpr float kLargest = 16320.f;  // 255 2^6
   return most >= 0x1p-100f ? make_float2(kLargest / most, most / kLargest) : power_for(most);
 }
+// The largest of rows' parts and weights: of many rows by blocks of 1024 first
+// (every block over all rows / in a launch of its own, whole gradients: 4096 x
+// 1000 x 64 bf16 36 / 37 us, 16384 x 256 x 128 48 / 38).
+struct Most {
+  float part, weight;
+};
+__device__ __forceinline__ Most most_of_rows(const float* g, const float* h, const float* loss, const void* targets,
+                                             bool wide, int64_t R, int64_t V, int64_t i, int64_t apart, float* red) {
+  Most m{0.f, 0.f};
+#pragma unroll 4
+  for (; i < R; i += apart) {
+    const RowPart o = row_part(g, h, loss, target_of(targets, wide, i, V) >= 0, i);
+    m.part = fmaxf(m.part, o.most);
+    m.weight = fmaxf(m.weight, finite_abs(o.g + o.h));
+  }
+  m.part = block_max(m.part, red);
+  m.weight = block_max(m.weight, red);
+  return m;
+}
+constexpr int kMostBlocks = 128;
+__global__ void __launch_bounds__(1024) rows_most_kernel(const float* g, const float* h, const float* loss,
+                                                         const void* targets, bool wide, int64_t R, int64_t V, Most* out) {
+  __shared__ float red[16];
+  const Most m = most_of_rows(g, h, loss, targets, wide, R, V, (int64_t)blockIdx.x * 1024 + threadIdx.x,
+                              (int64_t)gridDim.x * 1024, red);
+  if (threadIdx.x == 0) out[blockIdx.x] = m;
+}
+
 template <typename T, int PL>
 __global__ void __launch_bounds__(1024) rows_kernel(const float* g, const float* h, const float* loss, const float* lse,
                                                     const void* targets, bool wide, int64_t R, int64_t V, float2* power,
-                                                    float4* rows) {
+                                                    float4* rows, const Most* most, int mosts) {
   __shared__ float red[16];
-  float m = 0.f, top = 0.f;
-  for (int64_t i = threadIdx.x; i < R; i += 1024) {
-    const RowPart o = row_part(g, h, loss, target_of(targets, wide, i, V) >= 0, i);
-    m = fmaxf(m, o.most);
-    top = fmaxf(top, finite_abs(o.g + o.h));
+  Most all;
+  if (most) {
+    const Most mine = (int)threadIdx.x < mosts ? most[threadIdx.x] : Most{0.f, 0.f};
+    all = {block_max(mine.part, red), block_max(mine.weight, red)};
+  } else {
+    all = most_of_rows(g, h, loss, targets, wide, R, V, threadIdx.x, 1024, red);
   }
   // (a weight of p times the factor stays finite where every row is certain)
-  m = fmaxf(block_max(m, red), block_max(top, red) * 0x1p-106f);
+  const float m = fmaxf(all.part, all.weight * 0x1p-106f);
   const float2 pw = PL == 1 ? factor_for(m) : power_for(m);
   if (blockIdx.x == 0 && threadIdx.x == 0) *power = pw;
   const float up = pw.x;
@@ -409,17 +437,59 @@ struct Lost {
     return t < 0 ? 0.f : rows[row].w;
   }
 };
+// What dw gets back of its words' rows, in the units of the accumulators, for few
+// rows: there one row's rounding can be most of the error (1 to 5 rows in bf16: up
+// to 3.9e-3 beside the result's own 1.7e-3), where that of many evens out (61: 1.3
+// times the result's, 8191: 1.35) and looking the targets up takes 7 us of 102.
+constexpr int kFewRows = 32;
+template <typename TO>
+struct LostOfRows {
+  int count = 0;
+  const float4* rows = nullptr;
+  const TO* x = nullptr;
+  int64_t ldx = 0, v0 = 0;
+  const void* targets = nullptr;
+  bool wide = false;
+  const float2* up = nullptr;
+  template <class TL>
+  __device__ __forceinline__ void add(const Args& p, const Place& c, typename TL::Acc& acc) const {
+    const int64_t t = c.lane < count ? target_of(targets, wide, c.lane, v0 + p.M) : -1;
+    const int64_t far = t - v0 - c.m0 - c.wm * TL::TM * 32;
+    const int in = t >= 0 && far >= 0 && far < TL::TM * 32 ? (int)far : -1;
+    const int cols = (int)(p.N - c.n0);
+    for (uint64_t left = __ballot(in >= 0); left; left &= left - 1) {
+      const int r = __builtin_ctzll(left), word = __builtin_amdgcn_readlane(in, r);
+      const float back = rows[r].w * up->x;
+      if (back == 0.f || (c.lane & 31) != (word & 31)) continue;
+      const TO* at = x + r * ldx + c.n0;
+#pragma unroll
+      for (int i = 0; i < TL::TM; ++i)
+        if (word >> 5 == i) {
+#pragma unroll
+          for (int j = 0; j < TL::TN; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const int col = TL::col_of(c, j, e);  // (columns behind the last are not stored)
+              acc[i][j][e] += back * to_f(at[col < cols ? col : 0]);
+            }
+        }
+    }
+  }
+};
 
 // acc times the inverse powers, as outputs or as fp32 parts of a sum.
-template <typename TO>
+template <typename TO, bool FEW = false>
 struct EpiOut {
   TO* out;
   float* part;   // [splits][M][N], or null
   bool more;     // parts are added to what is there
   const float2 *pa, *pb;
   Lost<TO> lost;
+  LostOfRows<TO> back;
   template <class TL>
-  __device__ __forceinline__ void form(const Args&, const Place&, typename TL::Acc&) const {}
+  __device__ __forceinline__ void form(const Args& p, const Place& c, typename TL::Acc& acc) const {
+    if constexpr (FEW && TL::PL == 1) back.template add<TL>(p, c, acc);
+  }
   template <class TL>
   __device__ __forceinline__ void store(const Args& p, const Place& c, typename TL::T* lds, typename TL::Acc& acc) const {
     const float ua = pa ? pa->y : 1.f, ub = pb ? pb->y : 1.f;
@@ -731,14 +801,21 @@ size_t backward(const LinearCE& a, void* wsp, int cus, hipStream_t s) {
   T* d = ws.take<T>((size_t)(panel * ceil_div(len, 64 / PL)));
   float2* pg = ws.take<float2>(1);
   float4* rows = ws.take<float4>((size_t)a.R);
+  const int mosts = a.R > 4096 ? (int)std::min<int64_t>(ceil_div(a.R, 1024), kMostBlocks) : 0;
+  Most* most_of = mosts ? ws.take<Most>((size_t)mosts) : nullptr;
   const Plan plan = plan_products(a.R, a.K, len, pieces == 1, 64 / PL, cus);
   const int splits = plan.parts;
   const bool parted = splits > 1 || pieces > 1;
   float* part = parted ? ws.take<float>((size_t)(splits * a.R * a.K)) : nullptr;
   float* wpart = plan.wparts > 1 ? ws.take<float>((size_t)(plan.wparts * a.V * a.K)) : nullptr;
   if (!wsp) return ws.used;
+  if (mosts) {
+    hipLaunchKernelGGL(rows_most_kernel, dim3((unsigned)mosts), dim3(1024), 0, s, a.g_loss, a.g_lse, a.loss, a.targets,
+                       wide, a.R, a.V, most_of);
+    check_launch(what);
+  }
   hipLaunchKernelGGL((rows_kernel<T, PL>), dim3(blocks_for(a.R, 1024)), dim3(1024), 0, s, a.g_loss, a.g_lse, a.loss,
-                     a.lse, a.targets, wide, a.R, a.V, pg, rows);
+                     a.lse, a.targets, wide, a.R, a.V, pg, rows, most_of, mosts);
   check_launch(what);
   const Lost<TI> lost{(const TI*)a.w, a.ldw, a.V, a.targets, wide, PL == 1 ? rows : nullptr};
   for (int64_t v0 = 0; v0 < a.V; v0 += each) {
@@ -755,15 +832,18 @@ size_t backward(const LinearCE& a, void* wsp, int cus, hipStream_t s) {
     px.M = a.R; px.N = a.K; px.K = n; px.splits = splits;
     pw.b = x.o;
     pw.M = n; pw.N = a.K; pw.K = a.R; pw.splits = plan.wparts;
-    const EpiOut<TI> ex{(TI*)a.dx, part, v0 > 0, pg, w.power, lost},
-        ew{(TI*)a.dw + v0 * a.K, wpart, false, pg, x.power, {}};
+    const EpiOut<TI> ex{(TI*)a.dx, part, v0 > 0, pg, w.power, lost, {}},
+        ew{(TI*)a.dw + v0 * a.K, wpart, false, pg, x.power, {}, {}};
     typedef Tile<T, 2, 2, 2, 2, PL, kPanelCols, kCols> WFew;  // (of four wavefronts, as dx's)
     if (plan.big)
       launch_pair<Tile<T, 4, 2, 2, 4, PL, kPanelRows, kCols>, Tile<T, 4, 2, 2, 4, PL, kPanelCols, kCols>>(px, ex, pw, ew, s, what);
-    else if (a.R > 32)
+    else if (a.R > kFewRows)
       launch_pair<Tile<T, 2, 1, 2, 4, PL, kPanelRows, kCols>, Tile<T, 2, 1, 2, 4, PL, kPanelCols, kCols>>(px, ex, pw, ew, s, what);
     else
-      launch_pair<Tile<T, 1, 1, 1, 4, PL, kPanelRows, kCols>, WFew>(px, ex, pw, ew, s, what);
+      launch_pair<Tile<T, 1, 1, 1, 4, PL, kPanelRows, kCols>, WFew>(
+          px, ex, pw,
+          EpiOut<TI, true>{ew.out, nullptr, false, pg, x.power, {},
+                           {(int)a.R, rows, (const TI*)a.x, a.ldx, v0, a.targets, wide, pg}}, s, what);
   }
   auto sum = [&](const float* of, int parts, int64_t n, const float2* power, const Lost<TI>& back, void* out) {
     auto go = [&](auto kernel, int threads) {

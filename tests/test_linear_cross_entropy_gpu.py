@@ -214,6 +214,30 @@ def test_even_weights_are_not_rounded(gpu, dtype):
     assert (np.abs(dw - want) <= u * np.abs(want) * (1 + u) + err + 2.0 ** -20 * (np.abs(d).T @ np.abs(x))).all()
 
 
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("R,words", [(1, 1), (3, 1), (5, 5), (20, 7), (31, 31), (32, 2)])
+def test_few_rows_lose_nothing(gpu, R, words, dtype):
+    """dw of up to 32 rows is off by its own rounding and by what the parts of
+    words that are no targets are rounded by; the targets' parts, the largest,
+    are given back."""
+    K, V = 72, 4096
+    u, rng = HALF_STEP[dtype], np.random.default_rng(R + words)
+    x = few_bits.round_to(rng.standard_normal((R, K)), dtype)
+    w = few_bits.round_to(rng.standard_normal((V, K)) * 2.0 ** -12, dtype)
+    t = (rng.permutation(R) % words * 13).astype(np.int32)
+    t[rng.random(R) < 0.05] = -1
+    g = (rng.random(R) + 0.5).astype(np.float32)
+    dev = [_dev(gpu, x, dtype), _dev(gpu, w, dtype), gpu.from_numpy(t)]
+    dw = gpu.linear_cross_entropy_backward(_dev(gpu, g), *dev, *gpu.linear_cross_entropy(*dev))[1].to_numpy()
+    want = O.linear_cross_entropy_backward(x, w, t, g, None)[1]
+    d = O.logit_gradients(x, w, t, g, None)
+    err = (np.abs(d) * np.where(d < 0, 2.0 ** -20, 1.01 * u)).T @ np.abs(x).astype(np.float64)
+    # float16 values below 2^-14 are 2^-24 apart, not 2^-10 of themselves: words
+    # that are no targets have |dw| of g p |x| = 1e-6 here, rounded by up to 2^-25
+    tiny = 2.0 ** -25 if dtype == "float16" else 0.0
+    assert (np.abs(dw - want) <= u * np.abs(want) * (1 + u) + err + 2.0 ** -20 * (np.abs(d).T @ np.abs(x)) + tiny).all()
+
+
 # few words and many rows: dw in parts
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("R,K,V", [(5000, 70, 30), (3001, 129, 200)])
