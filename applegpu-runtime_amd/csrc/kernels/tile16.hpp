@@ -29,6 +29,7 @@
 #include <algorithm>
 
 #include "device.hpp"
+#include "extent.hpp"
 
 namespace agpu {
 namespace k {
@@ -111,6 +112,7 @@ struct Stream {
   static constexpr int CPR = COLS ? B * PL / 8 : 8;  // 16-byte chunks of a k row, or of a row's stage
   const T* base;
   int64_t ld, k_rows, width;
+  int64_t from, cols;  // kCols: the block's first column, all columns
   int off[L], first, lane;
   __amdgpu_buffer_rsrc_t rows;
 
@@ -132,9 +134,11 @@ struct Stream {
       width = !COLS ? (M - m0) * 64 : panels < B * PL / 64 ? panels * ld : B * PL / 64 * ld;
     } else {
       base = (const T*)o.p + b * o.batch + (COLS ? m0 * PL : m0 * ld);
-      // values of a row from base on (rows: with the zeros up to a whole chunk,
-      // or a whole group of planes)
-      width = COLS ? ld - m0 * PL : PL == 1 ? (K + 7) / 8 * 8 : LAY == kRaw ? K * 2 : (K + 31) / 32 * 64;
+      from = m0;
+      cols = M;
+      // values of a row, with the zeros up to a whole chunk or a whole group of
+      // planes
+      width = LAY == kRaw ? K * 2 : row_values(K, PL);
       if (!COLS) rows = resource(base, ((M - m0 - 1) * ld + width) * (int64_t)sizeof(T));
     }
 #pragma unroll
@@ -157,8 +161,9 @@ struct Stream {
 #pragma unroll
       for (int q = 0; q < L; ++q) copy16(src, to + (first + q) * 512, off[q], 0);
     } else if constexpr (COLS) {
-      const __amdgpu_buffer_rsrc_t src = resource(
-          base + (int64_t)st * KS * ld, ((k_rows - (int64_t)st * KS - 1) * ld + width) * (int64_t)sizeof(T));
+      const __amdgpu_buffer_rsrc_t src =
+          resource(base + (int64_t)st * KS * ld,
+                   extent_of_columns(k_rows - (int64_t)st * KS, cols, from, ld, PL) * (int64_t)sizeof(T));
 #pragma unroll
       for (int q = 0; q < L; ++q) copy16(src, to + (first + q) * 512, off[q], 0);
     } else {

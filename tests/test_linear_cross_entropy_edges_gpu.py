@@ -1,0 +1,52 @@
+"""Cross entropy of a linear layer and its gradient where operands are read in
+place out of larger tensors, and at values that are not ordinary; float64
+beside them."""
+import numpy as np
+import pytest
+
+from oracle import few_bits
+from oracle import training as O
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = ["float32", "float16", "bfloat16"]
+
+
+def _dev(gpu, a, dtype="float32"):
+    t = gpu.from_numpy(np.ascontiguousarray(a, np.float32))
+    return t if dtype == "float32" else gpu.cast(t, dtype)
+
+
+def _columns(gpu, a, dtype, ld, off):
+    """a as the columns from `off` on of rows of `ld` values that are not
+    numbers: the last one's storage ends with it where off + columns = ld."""
+    wide = np.full((a.shape[0], ld), np.nan, np.float32)
+    wide[:, off:off + a.shape[1]] = a
+    return gpu.slice(_dev(gpu, wide, dtype), 1, off, off + a.shape[1])
+
+
+# rows of 16-byte chunks, so that 16-bit operands are read where they are: few
+# features and more than a tile's columns, views that end with their rows
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("R,K,V,ld,off", [
+    (64, 64, 128, 128, 64), (8, 64, 1024, 512, 448), (128, 72, 256, 136, 64), (256, 264, 512, 1024, 760),
+    (300, 768, 1000, 2304, 768), (33, 520, 257, 1024, 504), (1, 8, 5, 16, 8)])
+def test_columns_of_wider_rows(gpu, R, K, V, ld, off, dtype):
+    rng = np.random.default_rng(R + K + V)
+    w = few_bits.round_to(rng.standard_normal((V, K)) * 3 / np.sqrt(K), dtype)
+    x = few_bits.round_to(rng.standard_normal((R, K)), dtype)
+    t = rng.integers(-1, V, R).astype(np.int32)
+    g = rng.random(R).astype(np.float32)
+
+    def all_of(a, b):
+        ti = gpu.from_numpy(t)
+        out = gpu.linear_cross_entropy(a, b, ti)
+        return [v.to_numpy() for v in (*out, *gpu.linear_cross_entropy_backward(_dev(gpu, g), a, b, ti, *out))]
+
+    plain = _dev(gpu, x, dtype), _dev(gpu, w, dtype)
+    want = all_of(*plain)
+    assert all(np.isfinite(v).all() for v in want)
+    views = _columns(gpu, x, dtype, ld, off), _columns(gpu, w, dtype, ld, off)
+    for a, b in ((views[0], plain[1]), (plain[0], views[1]), views):
+        for got, v in zip(all_of(a, b), want):
+            np.testing.assert_array_equal(got, v)
