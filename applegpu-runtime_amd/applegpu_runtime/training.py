@@ -98,6 +98,16 @@ class Muon(torch.optim.Optimizer):
                 if p.dim() != 2:
                     raise ValueError(f"Muon steps matrices, got a parameter of shape {tuple(p.shape)}")
 
+    def load_state_dict(self, state_dict):
+        """As of any optimiser; the momenta stay float32, as they were saved
+        (the base class casts state to its parameter's type)."""
+        super().load_state_dict(state_dict)
+        saved = state_dict["state"]
+        ids = [i for group in state_dict["param_groups"] for i in group["params"]]
+        for i, p in zip(ids, [p for group in self.param_groups for p in group["params"]]):
+            if "momentum" in saved.get(i, {}):
+                self.state[p]["momentum"] = saved[i]["momentum"].to(p.device, torch.float32, copy=True)
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
