@@ -81,7 +81,9 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     weight [V, K] and int32 or int64 targets [...]; a target outside [0, V)
     (ignore_index -100) has loss 0.  Differentiable in x and weight for up to
     2^20 rows."""
-    return _LinearCrossEntropy.apply(x, weight, target)
+    loss, lse = _LinearCrossEntropy.apply(x, weight, target)
+    # (the library's tensors have one dimension at least)
+    return (loss, lse) if target.dim() else (loss.reshape(()), lse.reshape(()))
 
 
 class Muon(torch.optim.Optimizer):

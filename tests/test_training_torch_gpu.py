@@ -102,6 +102,22 @@ def test_layouts(torch_dev, dtype):
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_one_row_without_a_row_dimension(torch_dev, dtype):
+    """x [K] and a target []: losses and gradients of their shapes."""
+    torch = torch_dev
+    from applegpu_runtime.training import linear_cross_entropy
+    x, w, t = _case(2, 24, 30, dtype)
+    xd, wd = (_to(torch, a, dtype).requires_grad_() for a in (x[1], w))
+    loss, lse = linear_cross_entropy(xd, wd, torch.tensor(int(t[1])).to("applegpu"))
+    assert loss.shape == lse.shape == ()
+    want = O.linear_cross_entropy(x[1:], w, t[1:])
+    np.testing.assert_allclose([loss.item(), lse.item()], [want[0][0], want[1][0]], rtol=1e-4)
+    (loss + lse * 0.5).backward()
+    assert xd.grad.shape == (24,)
+    _check_grads(x[1:], w, t[1:], dtype, np.ones(1), np.full(1, 0.5), (xd.grad[None], wd.grad))
+
+
 @pytest.mark.parametrize("lead", [(0,), (0, 3), (2, 0)])
 def test_tensors_of_no_rows(torch_dev, lead):
     """Tensors of no elements, with storages of none."""
