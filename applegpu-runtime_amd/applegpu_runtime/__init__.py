@@ -699,7 +699,7 @@ def linear_cross_entropy(x, weight, targets):
     sum exp(logits) and loss = lse - logits[target].  A target outside [0, V)
     (padding) has loss 0.  A nearly certain word's loss keeps its digits.  A
     row with a logit of NaN or +inf gives NaN, and so does a float32 x or weight
-    that is not finite.
+    that is not finite; logits beyond 2.3e38 count as infinite.
 
     Products are summed in float32; float32 operands count with 22 bits of
     each value, by magnitudes of at least 2^-27 of the operand's largest."""

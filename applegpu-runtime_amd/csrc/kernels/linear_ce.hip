@@ -257,7 +257,9 @@ __global__ void __launch_bounds__(256) loss_kernel(const float2* part, int64_t p
   } else {
     // log(exp z_t + the others), from the larger of the two
     const float z = zt[row], q = z * kLog2e;
-    if (q >= a.x) {
+    if (q == kInf) {
+      out = sum = kInf - q;  // an infinite sum has no certain word: NaN
+    } else if (q >= a.x) {
       out = log1pf(a.y * exp2f(fmaf(-z, kLog2e, a.x)));
       sum = z + out;
     } else {

@@ -50,3 +50,34 @@ def test_columns_of_wider_rows(gpu, R, K, V, ld, off, dtype):
     for a, b in ((views[0], plain[1]), (plain[0], views[1]), views):
         for got, v in zip(all_of(a, b), want):
             np.testing.assert_array_equal(got, v)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [1, 2, 40, 700])
+def test_an_infinite_logit_is_not_a_certain_word(gpu, dtype, V):
+    """One word of +inf: rows that see it have no loss and no sum, be it their
+    target, another word or the only one; rows that see it as -inf do without
+    it."""
+    word, K = V // 2, 16
+    rng = np.random.default_rng(V)
+    x = few_bits.round_to(rng.standard_normal((6, K)), dtype)
+    w = few_bits.round_to(rng.standard_normal((V, K)), dtype)
+    x[:, 0], w[word, 0] = [1, 2, 1, 0.5, -1, -2], np.inf
+    t = np.array([word, 0, -100, V - 1, 0, -100], np.int32)
+    loss, lse = (a.to_numpy() for a in gpu.linear_cross_entropy(_dev(gpu, x, dtype), _dev(gpu, w, dtype),
+                                                                gpu.from_numpy(t)))
+    assert np.isnan(lse[:4]).all() and np.isnan(loss[[0, 1, 3]]).all() and loss[2] == 0 and loss[5] == 0
+    if dtype != "float32" and word != 0:
+        want = O.linear_cross_entropy(x[4:], np.delete(w, word, 0), [0, -100])
+        np.testing.assert_allclose(lse[4:], want[1], rtol=1e-5, atol=1e-4)
+        np.testing.assert_allclose(loss[4:], want[0], rtol=1e-4, atol=1e-4)
+
+
+def test_products_past_float32_are_not_certain_words(gpu):
+    """bfloat16 operands whose one product overflows, as the target."""
+    x, w = np.zeros((2, 8), np.float32), np.eye(5, 8, dtype=np.float32)
+    x[0, 3], w[3, 3], x[1, 1] = 2.0 ** 100, 2.0 ** 100, 4.0
+    loss, lse = (a.to_numpy() for a in gpu.linear_cross_entropy(_dev(gpu, x, "bfloat16"), _dev(gpu, w, "bfloat16"),
+                                                                gpu.from_numpy(np.array([3, 1], np.int32))))
+    assert np.isnan(loss[0]) and np.isnan(lse[0])
+    np.testing.assert_allclose([loss[1], lse[1]], [np.log(4 + np.exp(4)) - 4, np.log(4 + np.exp(4))], rtol=1e-5)
