@@ -713,8 +713,9 @@ def linear_cross_entropy_backward(grad_loss, x, weight, targets, loss, lse, grad
     vocabulary; their gradient is rounded to 16 bits before its products for
     16-bit operands and counts down to 2^-37 (bfloat16: 2^-139) of the largest
     one in the call.  Rows whose target is outside [0, V) get lse's
-    part only; one without any weight gets zeros whatever its logits are.  At
-    most 2^20 rows at once."""
+    part only; one without any weight gets zeros whatever its logits and its
+    loss are, and has no part in dweight as long as its x is finite.  At most
+    2^20 rows at once."""
     ins = [_t(grad_loss), _t(x), _t(weight), _t(targets), _t(loss), _t(lse)]
     return _op(b"linear_cross_entropy_backward", ins + ([_t(grad_lse)] if grad_lse is not None else []), nout=2)
 

@@ -287,6 +287,8 @@ __device__ __forceinline__ RowPart row_part(const float* g, const float* h, cons
   RowPart o;
   o.g = there ? g[r] : 0.f;
   o.h = h ? h[r] : 0.f;
+  o.dt = o.most = 0.f;
+  if (o.g == 0.f && o.h == 0.f) return o;  // without weight: nothing, whatever its loss is
   // 1 - p of the target from its loss, which keeps its digits
   const float left = there ? -expm1f(-loss[r]) : 1.f;
   o.dt = there ? o.h * expf(-loss[r]) - o.g * left : 0.f;

@@ -81,3 +81,53 @@ def test_products_past_float32_are_not_certain_words(gpu):
                                                                 gpu.from_numpy(np.array([3, 1], np.int32))))
     assert np.isnan(loss[0]) and np.isnan(lse[0])
     np.testing.assert_allclose([loss[1], lse[1]], [np.log(4 + np.exp(4)) - 4, np.log(4 + np.exp(4))], rtol=1e-5)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("R,bad", [(20, 5), (33, 32), (300, 131), (5000, 4999)])
+def test_rows_without_weight_and_without_a_loss(gpu, R, bad, dtype):
+    """A row with a word as its target whose loss is not a number, left out by a
+    weight of 0: dx is zero there, and all else is as without the row."""
+    K, V = 24, 90
+    rng = np.random.default_rng(R)
+    x = few_bits.round_to(rng.standard_normal((R, K)), dtype)
+    w = few_bits.round_to(rng.standard_normal((V, K)), dtype)
+    t = rng.integers(0, V, R).astype(np.int32)
+    g, h = rng.random(R).astype(np.float32) / R, rng.standard_normal(R).astype(np.float32) / R
+    g[bad] = h[bad] = 0
+    dev = [_dev(gpu, x, dtype), _dev(gpu, w, dtype), gpu.from_numpy(t)]
+    good = [a.to_numpy() for a in gpu.linear_cross_entropy(*dev)]
+    for of_lse in (None, _dev(gpu, h)):
+        want = [a.to_numpy() for a in gpu.linear_cross_entropy_backward(_dev(gpu, g), *dev, *map(gpu.from_numpy, good),
+                                                                        grad_lse=of_lse)]
+        assert (want[0][bad] == 0).all()
+        for value in ((np.nan, np.nan), (np.nan, np.inf), (np.inf, np.inf), (np.inf, 3.0)):
+            loss, lse = (a.copy() for a in good)
+            loss[bad], lse[bad] = value
+            got = gpu.linear_cross_entropy_backward(_dev(gpu, g), *dev, _dev(gpu, loss), _dev(gpu, lse), grad_lse=of_lse)
+            for a, b in zip(got, want):
+                np.testing.assert_array_equal(a.to_numpy(), b)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16"])
+def test_a_row_that_overflows_is_left_out_by_its_weight(gpu, dtype):
+    """The same from the forward pass: finite values whose products overflow."""
+    rng = np.random.default_rng(1)
+    x = few_bits.round_to(rng.standard_normal((9, 16)), dtype)
+    w = few_bits.round_to(rng.standard_normal((50, 16)), dtype)
+    t, g = rng.integers(0, 50, 9).astype(np.int32), rng.random(9).astype(np.float32)
+    g[4] = 0
+
+    def run(x):
+        dev = [_dev(gpu, x, dtype), _dev(gpu, w, dtype), gpu.from_numpy(t)]
+        out = gpu.linear_cross_entropy(*dev)
+        return [a.to_numpy() for a in (*out, *gpu.linear_cross_entropy_backward(_dev(gpu, g), *dev, *out))]
+
+    want = run(x)
+    x[4] = few_bits.round_to(np.sign(x[4]) * 3e38, dtype)
+    loss, lse, dx, dw = run(x)
+    assert not np.isfinite(loss[4])
+    rest = np.arange(9) != 4
+    for a, b in ((loss[rest], want[0][rest]), (lse[rest], want[1][rest]), (dx[rest], want[2][rest]), (dw, want[3])):
+        np.testing.assert_allclose(a, b, rtol=1e-5, atol=1e-5 * np.abs(b).max())
+    assert (dx[4] == 0).all()
