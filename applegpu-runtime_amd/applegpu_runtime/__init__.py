@@ -698,11 +698,14 @@ def linear_cross_entropy(x, weight, targets):
     targets [...] (int32 or int64), (loss, lse), float32 [...], where lse = log
     sum exp(logits) and loss = lse - logits[target].  A target outside [0, V)
     (padding) has loss 0.  A nearly certain word's loss keeps its digits.  A
-    row with a logit of NaN or +inf gives NaN, and so does a float32 x or weight
-    that is not finite; logits beyond 2.3e38 count as infinite.
+    row with a logit of NaN or +inf gives NaN; logits beyond 2.3e38 count as
+    infinite.
 
-    Products are summed in float32; float32 operands count with 22 bits of
-    each value, by magnitudes of at least 2^-27 of the operand's largest."""
+    Products are summed in float32, one after another along K.  float32 operands
+    count with 22 bits of each value down to 2^-16 of the operand's largest, and
+    smaller ones in steps of 2^-38 of it; where the largest values of its rows
+    are more than 2^14 apart, or one is infinite, the call multiplies float32
+    values themselves, which takes two to four times as long."""
     return _op(b"linear_cross_entropy", [_t(x), _t(weight), _t(targets)], nout=2)
 
 
@@ -711,11 +714,12 @@ def linear_cross_entropy_backward(grad_loss, x, weight, targets, loss, lse, grad
     gradients of its loss and lse (float32 [...]; grad_lse may be None) and the
     loss and lse it returned.  The logits are formed again, in pieces of the
     vocabulary; their gradient is rounded to 16 bits before its products for
-    16-bit operands and counts down to 2^-37 (bfloat16: 2^-139) of the largest
-    one in the call.  Rows whose target is outside [0, V) get lse's
-    part only; one without any weight gets zeros whatever its logits and its
-    loss are, and has no part in dweight as long as its x is finite.  At most
-    2^20 rows at once."""
+    16-bit operands (the results' errors are 1.4 times those of one rounding of
+    the results alone) and counts down to 2^-37 (bfloat16: 2^-139) of the
+    largest one in the call, for float32 with 22 bits down to 2^-16 of it.  Rows
+    whose target is outside [0, V) get lse's part only; one without any weight
+    gets zeros whatever its logits and its loss are, and has no part in dweight
+    as long as its x is finite.  At most 2^20 rows at once."""
     ins = [_t(grad_loss), _t(x), _t(weight), _t(targets), _t(loss), _t(lse)]
     return _op(b"linear_cross_entropy_backward", ins + ([_t(grad_lse)] if grad_lse is not None else []), nout=2)
 

@@ -23,7 +23,8 @@
 // largest, are then held without an error that their sums would keep (96 rows
 // of weight 1.0035 in bf16: error of dw 3.6e-3 with a power of two, so 1.7e-3,
 // its own rounding).  fp32 operands are scaled by a power of two, from their
-// largest magnitude, and split into fp16 planes (22 bits).
+// largest magnitude, and split into fp16 planes (22 bits); where an operand's rows
+// lie too far apart for one power, its products are of the fp32 values themselves.
 #include "tile16.hpp"
 
 namespace agpu {
@@ -71,52 +72,123 @@ __device__ __forceinline__ float block_max(float v, float* red) {
   return v;
 }
 
-constexpr int kParts = 512;  // blocks of the largest magnitude's first pass
+constexpr int kParts = 512;  // blocks of the largest magnitudes' first pass
 struct Rows32 {
   const float* x;
   int64_t rows, n, ld;
+  int team;  // threads of a row: a power of two up to 64, or 256
 };
-// part[y][b] = the largest finite magnitude of every kParts-th run of operand y.
-__global__ void __launch_bounds__(256) most_kernel(Rows32 x0, Rows32 x1, float* part) {
+// Of a part of an operand's rows: the largest magnitude, and the least that is
+// any row's largest (rows of zeros aside).
+struct Span {
+  float most, least;
+};
+// part[y][b]: of the rows of operand y that block b has; infinite with an
+// infinity among them.  (50257 x 768: 28 us, 26 without the rows' own.)
+__global__ void __launch_bounds__(256) most_kernel(Rows32 x0, Rows32 x1, Span* part) {
   __shared__ float red[4];
   const Rows32 o = blockIdx.y ? x1 : x0;
-  float m = 0.f;
-  if (o.ld == o.n && o.n % 4 == 0 && ((uintptr_t)o.x & 15) == 0) {
-    const int64_t q = o.rows * o.n / 4;
-#pragma unroll 4
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < q; i += (int64_t)kParts * 256) {
-      const float4 v = ((const float4*)o.x)[i];
-      m = fmaxf(fmaxf(m, fmaxf(finite_abs(v.x), finite_abs(v.y))), fmaxf(finite_abs(v.z), finite_abs(v.w)));
-    }
+  const bool fours = o.n % 4 == 0 && o.ld % 4 == 0 && ((uintptr_t)o.x & 15) == 0;
+  auto size4 = [](float4 v) { return fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))); };
+  Span s{0.f, kInf};
+  if (o.rows == 1) {  // a row of its own scale, by all blocks
+    const int64_t first = (int64_t)blockIdx.x * 256 + threadIdx.x, apart = (int64_t)kParts * 256;
+    if (fours)
+      for (int64_t i = first * 4; i < o.n; i += apart * 4) s.most = fmaxf(s.most, size4(*(const float4*)(o.x + i)));
+    else
+      for (int64_t i = first; i < o.n; i += apart) s.most = fmaxf(s.most, fabsf(o.x[i]));
   } else {
-    for (int64_t r = blockIdx.x; r < o.rows; r += kParts)
-      for (int64_t i = threadIdx.x; i < o.n; i += 256) m = fmaxf(m, finite_abs(o.x[r * o.ld + i]));
+    const int team = o.team, member = threadIdx.x & (team - 1), each = 256 / team;
+    const int64_t apart = (int64_t)kParts * each;
+    constexpr int kAtOnce = 4;
+    for (int64_t r0 = (int64_t)blockIdx.x * each; r0 < o.rows; r0 += apart * kAtOnce) {
+      float m[kAtOnce] = {};
+      const float* at[kAtOnce];
+#pragma unroll
+      for (int q = 0; q < kAtOnce; ++q) {  // (the last row again behind it)
+        const int64_t r = r0 + threadIdx.x / team + q * apart;
+        at[q] = o.x + (r < o.rows ? r : o.rows - 1) * o.ld;
+      }
+      if (fours) {
+#pragma unroll 1
+        for (int64_t i = member * 4; i < o.n; i += team * 4)
+#pragma unroll
+          for (int q = 0; q < kAtOnce; ++q) m[q] = fmaxf(m[q], size4(*(const float4*)(at[q] + i)));
+      } else {
+        for (int64_t i = member; i < o.n; i += team)
+#pragma unroll
+          for (int q = 0; q < kAtOnce; ++q) m[q] = fmaxf(m[q], fabsf(at[q][i]));
+      }
+      for (int k = team == 256 ? 32 : team / 2; k; k >>= 1)
+#pragma unroll
+        for (int q = 0; q < kAtOnce; ++q) m[q] = fmaxf(m[q], __shfl_xor(m[q], k));
+#pragma unroll
+      for (int q = 0; q < kAtOnce; ++q) {
+        if (team == 256) m[q] = block_max(m[q], red);
+        s.most = fmaxf(s.most, m[q]);
+        if (m[q] > 0.f) s.least = fminf(s.least, m[q]);
+      }
+    }
   }
-  m = block_max(m, red);
-  if (threadIdx.x == 0) part[blockIdx.y * kParts + blockIdx.x] = m;
+  s.most = block_max(s.most, red);
+  s.least = -block_max(-s.least, red);
+  if (threadIdx.x == 0) part[blockIdx.y * kParts + blockIdx.x] = s;
 }
-// The power of kParts parts, for a block of 256.
-__device__ __forceinline__ float2 power_of_parts(const float* part, float* red) {
+// The operands' powers, and whether fp16 planes do not hold them: a row whose
+// largest value is 2^-14 of the operand's is held to 2^-24 of that value (the
+// low plane's smallest step is 2^-38 of the operand's largest), but beside a row
+// of 2^40 times the others nothing is left of them.  Where rows are further apart
+// than 2^14, or hold an infinity, products are of the fp32 values themselves and
+// the powers are 1.  (In planes / of the values, us: loss of 61 x 50257 x 1280
+// 101 / 231, of 1023 x 50257 x 768 313 / 962; gradients 307 / 558, 733 / 2738.)
+struct Scales {
+  float2 x, w;  // {2^s, 2^-s}
+  int full;
+};
+// From all parts, for a block of 256.
+__device__ __forceinline__ Scales scales_of(const Span* part) {
   static_assert(kParts == 512, "two parts a thread");
-  return power_for(block_max(fmaxf(part[threadIdx.x], part[threadIdx.x + 256]), red));
+  __shared__ Span red[2][4];
+  Span t[2];
+#pragma unroll
+  for (int y = 0; y < 2; ++y) {
+    const Span a = part[y * kParts + threadIdx.x], b = part[y * kParts + threadIdx.x + 256];
+    t[y] = {wave_max(fmaxf(a.most, b.most)), -wave_max(-fminf(a.least, b.least))};
+    if ((threadIdx.x & 63) == 0) red[y][threadIdx.x >> 6] = t[y];
+  }
+  __syncthreads();
+  Scales s;
+  s.full = 0;
+#pragma unroll
+  for (int y = 0; y < 2; ++y) {
+    Span a = red[y][0];
+#pragma unroll
+    for (int q = 1; q < 4; ++q) a = {fmaxf(a.most, red[y][q].most), fminf(a.least, red[y][q].least)};
+    if (!(a.most < kInf && a.most <= a.least * 0x1p14f)) s.full = 1;
+    (y ? s.w : s.x) = power_for(a.most);
+  }
+  if (s.full) s.x = s.w = make_float2(1.f, 1.f);
+  return s;
 }
 // Rows [rows, n] as 16-bit rows of ld values, zeros behind n: fp32 as planes of
-// x times its power of two (from part; and the other operand's power, where it
-// is asked for), 16-bit values as they are.
+// x times its power of two, 16-bit values as they are.  The first operand's
+// launch (with the parts) finds both powers and leaves them in *scales for what
+// follows.
 template <typename TI, typename T, int PL>
-__global__ void __launch_bounds__(256) pack_kernel(const TI* x, int64_t rows, int64_t n, int64_t ldi, const float* part,
-                                                   float2* power, const float* other_part, float2* other_power, T* out,
-                                                   int64_t ld) {
-  __shared__ float red[4];
+__global__ void __launch_bounds__(256) pack_kernel(const TI* x, int64_t rows, int64_t n, int64_t ldi, const Span* part,
+                                                   Scales* scales, T* out, int64_t ld) {
   float s = 1.f;
   if constexpr (PL == 2) {
-    const float2 pw = power_of_parts(part, red);
-    s = pw.x;
-    if (blockIdx.x == 0 && threadIdx.x == 0) *power = pw;
-    if (other_power && blockIdx.x == 0) {
-      const float2 o = power_of_parts(other_part, red);
-      if (threadIdx.x == 0) *other_power = o;
+    Scales c;
+    if (part) {
+      c = scales_of(part);
+      if (blockIdx.x == 0 && threadIdx.x == 0) *scales = c;
+      s = c.x.x;
+    } else {
+      c = *scales;
+      s = c.w.x;
     }
+    if (c.full) return;
   }
   const int chunks = (int)(ld / (8 * PL));
   const int64_t total = rows * chunks, apart = (int64_t)gridDim.x * 256;
@@ -160,13 +232,14 @@ struct EpiLoss {
   float* zt;
   const void* targets;
   bool wide;
-  const float2 *px, *pw;  // fp32: the operands' powers
+  const Scales* scales;  // fp32
+  static constexpr bool kFull = true;
   // the accumulators' first registers take a row's {c, s}
   template <class TL>
   __device__ __forceinline__ void form(const Args& p, const Place& c, typename TL::Acc& acc) const {
     constexpr int TM = TL::TM, TN = TL::TN;
     float ux = 1.f, uw = 1.f;
-    if constexpr (TL::PL == 2) { ux = px->y; uw = pw->y; }
+    if constexpr (TL::PL == 2) { ux = scales->x.y; uw = scales->w.y; }
     const int64_t cols = c.n0 + c.wn * 32 * TN;
     const bool ragged = cols + 32 * TN > p.N;
     const int hi = c.lane >> 5;
@@ -330,7 +403,7 @@ __global__ void __launch_bounds__(1024) rows_most_kernel(const float* g, const f
 template <typename T, int PL>
 __global__ void __launch_bounds__(1024) rows_kernel(const float* g, const float* h, const float* loss, const float* lse,
                                                     const void* targets, bool wide, int64_t R, int64_t V, float2* power,
-                                                    float4* rows, const Most* most, int mosts) {
+                                                    float4* rows, const Most* most, int mosts, const Scales* scales) {
   __shared__ float red[16];
   Most all;
   if (most) {
@@ -341,7 +414,7 @@ __global__ void __launch_bounds__(1024) rows_kernel(const float* g, const float*
   }
   // (a weight of p times the factor stays finite where every row is certain)
   const float m = fmaxf(all.part, all.weight * 0x1p-106f);
-  const float2 pw = PL == 1 ? factor_for(m) : power_for(m);
+  const float2 pw = PL == 1 ? factor_for(m) : scales->full ? make_float2(1.f, 1.f) : power_for(m);
   if (blockIdx.x == 0 && threadIdx.x == 0) *power = pw;
   const float up = pw.x;
   const int64_t r = (int64_t)blockIdx.x * 1024 + threadIdx.x;
@@ -367,12 +440,13 @@ struct EpiGrad {
   const void* targets;
   bool wide;
   const float4* rows;
-  const float2 *px, *pw;
+  const Scales* scales;  // fp32
+  static constexpr bool kFull = true;
   template <class TL>
   __device__ __forceinline__ void form(const Args& p, const Place& c, typename TL::Acc& acc) const {
     constexpr int PL = TL::PL, TM = TL::TM, TN = TL::TN;
     float ux = 1.f, uw = 1.f;
-    if constexpr (PL == 2) { ux = px->y; uw = pw->y; }
+    if constexpr (PL == 2) { ux = scales->x.y; uw = scales->w.y; }
     const int64_t cols = c.n0 + c.wn * 32 * TN;
     const bool ragged = cols + 32 * TN > p.N;
     const int hi = c.lane >> 5;
@@ -415,11 +489,21 @@ struct EpiGrad {
   template <class TL>
   __device__ __forceinline__ void store(const Args& p, const Place& c, typename TL::T* lds, typename TL::Acc& acc) const {
     constexpr int PL = TL::PL;
+    const bool full = PL == 2 && scales->full;  // (as they are: fp32 values take the planes' place)
     TL::template runs<false>(
         c, lds, acc, false,
         [&](int64_t row, int64_t col, float (&v)[8]) {
           constexpr int W = 64 / PL;  // words of a panel
-          if (row < p.M && col < (len + W - 1) / W * W) put_planes<T, PL>(d + col / W * panel + row * 64, col % W, v);
+          if (row >= p.M || col >= (len + W - 1) / W * W) return;
+          T* at = d + col / W * panel + row * 64;
+          if (full) {
+            struct alignas(16) V { float e[4]; } o[2];
+            __builtin_memcpy(o, v, 32);
+            put_past((float*)at + col % W, o[0]);
+            put_past((float*)at + col % W + 4, o[1]);
+          } else {
+            put_planes<T, PL>(at, col % W, v);
+          }
         },
         [](int64_t, int64_t, float (&)[8]) {});
   }
@@ -484,6 +568,7 @@ struct LostOfRows {
 // acc times the inverse powers, as outputs or as fp32 parts of a sum.
 template <typename TO, bool FEW = false>
 struct EpiOut {
+  static constexpr bool kFull = true;
   TO* out;
   float* part;   // [splits][M][N], or null
   bool more;     // parts are added to what is there
@@ -621,46 +706,52 @@ bool direct(const void* p, int64_t ld, int64_t K) {
 }
 
 // The operands x and w as a product takes them: in place, packed into the
-// workspace, or (raw) w as the fp32 rows that it is.
-struct Packed {
-  Operand o;
-  float2* power = nullptr;
-};
+// workspace, or (raw) w as the fp32 rows that it is; fp32: with their powers.
 struct Both {
-  Packed x, w;
+  Operand x, w;
+  Scales* scales = nullptr;
+  const float2 *px = nullptr, *pw = nullptr;
+  const int* full = nullptr;
 };
 template <typename TI, typename T, int PL>
 Both ready(const LinearCE& a, bool raw, Carver& ws, hipStream_t s) {
   Both b;
-  float* part = nullptr;
+  Span* part = nullptr;
   if constexpr (PL == 2) {
-    part = ws.take<float>(2 * kParts);
-    b.x.power = ws.take<float2>(1);
-    b.w.power = ws.take<float2>(1);
+    part = ws.take<Span>(2 * kParts);
+    b.scales = ws.take<Scales>(1);
     if (ws.base) {
-      hipLaunchKernelGGL(most_kernel, dim3(kParts, 2), dim3(256), 0, s, Rows32{(const float*)a.x, a.R, a.K, a.ldx},
-                         Rows32{(const float*)a.w, a.V, a.K, a.ldw}, part);
+      b.px = &b.scales->x;
+      b.pw = &b.scales->w;
+      b.full = &b.scales->full;
+      auto rows = [&](const void* x, int64_t rows, int64_t ld) {
+        int team = 256;
+        if (a.K <= 4096 && rows > 1)
+          for (team = 1; team < 64 && team * 4 < a.K;) team *= 2;
+        return Rows32{(const float*)x, rows, a.K, ld, team};
+      };
+      hipLaunchKernelGGL(most_kernel, dim3(kParts, 2), dim3(256), 0, s, rows(a.x, a.R, a.ldx), rows(a.w, a.V, a.ldw),
+                         part);
       check_launch("linear_cross_entropy");
     }
   }
-  auto pack = [&](Packed& p, const void* x, int64_t rows, int64_t ld, const float* mine, const float* other_part,
-                  float2* other) {
+  auto pack = [&](Operand& o, const void* x, int64_t rows, int64_t ld, const Span* parts) {
     if (PL == 1 && direct(x, ld, a.K)) {
-      p.o = {x, ld, 0};
+      o = {x, ld, 0};
       return;
     }
     const int64_t kp = (a.K + 31) / 32 * 32 * PL;
     T* out = ws.take<T>((size_t)(rows * kp));
-    p.o = {out, kp, 0};
+    o = {out, kp, 0};
     if (!ws.base) return;
     const unsigned blocks = (unsigned)std::min<int64_t>(blocks_for(rows * (kp / (8 * PL)), 512), 4096);
-    hipLaunchKernelGGL((pack_kernel<TI, T, PL>), dim3(blocks), dim3(256), 0, s, (const TI*)x, rows, a.K, ld, mine,
-                       p.power, other_part, other, out, kp);
+    hipLaunchKernelGGL((pack_kernel<TI, T, PL>), dim3(blocks), dim3(256), 0, s, (const TI*)x, rows, a.K, ld, parts,
+                       b.scales, out, kp);
     check_launch("linear_cross_entropy");
   };
-  pack(b.x, a.x, a.R, a.ldx, part, part ? part + kParts : nullptr, raw ? b.w.power : nullptr);
-  if (raw) b.w.o = {a.w, 2 * a.ldw, 0};
-  else pack(b.w, a.w, a.V, a.ldw, part ? part + kParts : nullptr, nullptr, nullptr);
+  pack(b.x, a.x, a.R, a.ldx, part);
+  if (raw) b.w = {a.w, 2 * a.ldw, 0};
+  else pack(b.w, a.w, a.V, a.ldw, nullptr);
   return b;
 }
 
@@ -692,6 +783,15 @@ void run(int tile, const Args& p, const Epi& e, hipStream_t s, const char* what)
   else launch<Tile<T, 1, 1, 1, 4, PL, kRows, BL>>(p, e, s, what);
 }
 
+// The fp32 operands of the logits of the words from v0 on, as they are.
+void full_rows(Args& p, const Both& b, const LinearCE& a, int64_t v0) {
+  p.full = b.full;
+  p.fa = (const float*)a.x;
+  p.lda = a.ldx;
+  p.fb = (const float*)a.w + v0 * a.ldw;
+  p.ldb = a.ldw;
+}
+
 template <typename TI, typename T, int PL>
 size_t forward(const LinearCE& a, void* wsp, int cus, hipStream_t s) {
   const char* what = "linear_cross_entropy";
@@ -703,18 +803,18 @@ size_t forward(const LinearCE& a, void* wsp, int cus, hipStream_t s) {
   const bool raw = PL == 2 && a.R <= 320 && a.K % 4 == 0 && a.ldw % 4 == 0 && a.ldw < (1 << 20) &&
                    ((uintptr_t)a.w & 15) == 0;
   const Both b = ready<TI, T, PL>(a, raw, ws, s);
-  const Packed &x = b.x, &w = b.w;
   const int tile = pick(a.R, a.V, raw, cus);
   const int64_t parts = ceil_div(a.V, bn_of(tile));
   float2* part = ws.take<float2>((size_t)(parts * a.R));
   float* zt = ws.take<float>((size_t)a.R);
   if (!wsp) return ws.used;
   Args p;
-  p.a = x.o; p.b = w.o;
+  p.a = b.x; p.b = b.w;
   p.M = a.R; p.N = a.V; p.K = a.K;
   const bool wide = a.idx_dt == DType::I64;
-  p.b_power = w.power;
-  const EpiLoss e{part, zt, a.targets, wide, x.power, w.power};
+  p.b_power = b.pw;
+  if (PL == 2) full_rows(p, b, a, 0);
+  const EpiLoss e{part, zt, a.targets, wide, b.scales};
   if (PL == 2 && raw) run<T, PL, PL == 2 ? kRaw : kRows>(tile, p, e, s, what);
   else run<T, PL, kRows>(tile, p, e, s, what);
   const int rx = a.R >= 64 * cus ? 64 : a.R >= 16 * cus ? 16 : a.R >= 4 * cus ? 4 : 1;
@@ -792,7 +892,6 @@ size_t backward(const LinearCE& a, void* wsp, int cus, hipStream_t s) {
   const char* what = "linear_cross_entropy_backward";
   Carver ws{(char*)wsp};
   const Both b = ready<TI, T, PL>(a, false, ws, s);
-  const Packed &x = b.x, &w = b.w;
   const bool wide = a.idx_dt == DType::I64;
   // pieces of the vocabulary, whole tiles of it
   const int64_t most = std::max<int64_t>(kHeld / PL / a.R / 256 * 256, 256);
@@ -819,25 +918,31 @@ size_t backward(const LinearCE& a, void* wsp, int cus, hipStream_t s) {
     check_launch(what);
   }
   hipLaunchKernelGGL((rows_kernel<T, PL>), dim3(blocks_for(a.R, 1024)), dim3(1024), 0, s, a.g_loss, a.g_lse, a.loss,
-                     a.lse, a.targets, wide, a.R, a.V, pg, rows, most_of, mosts);
+                     a.lse, a.targets, wide, a.R, a.V, pg, rows, most_of, mosts, b.scales);
   check_launch(what);
   const Lost<TI> lost{(const TI*)a.w, a.ldw, a.V, a.targets, wide, PL == 1 ? rows : nullptr};
   for (int64_t v0 = 0; v0 < a.V; v0 += each) {
     const int64_t n = std::min(each, a.V - v0);
-    const Operand wp{(const T*)w.o.p + v0 * w.o.ld, w.o.ld, 0}, dp{d, panel, 0};
+    const Operand wp{(const T*)b.w.p + v0 * b.w.ld, b.w.ld, 0}, dp{d, panel, 0};
     Args p;
-    p.a = x.o; p.b = wp;
+    p.a = b.x; p.b = wp;
     p.M = a.R; p.N = n; p.K = a.K;
+    if (PL == 2) full_rows(p, b, a, v0);
     run<T, PL, kRows>(pick(a.R, n, false, cus), p,
-                      EpiGrad<T>{d, panel, len, v0, a.V, a.targets, wide, rows, x.power, w.power}, s, what);
+                      EpiGrad<T>{d, panel, len, v0, a.V, a.targets, wide, rows, b.scales}, s, what);
     Args px, pw;
+    px.full = pw.full = p.full;
+    px.fa = pw.fa = (const float*)d;
+    px.lda = pw.lda = a.R * 32;
+    px.fb = p.fb; px.ldb = p.ldb;
+    pw.fb = p.fa; pw.ldb = p.lda;
     px.a = pw.a = dp;
     px.b = wp;
     px.M = a.R; px.N = a.K; px.K = n; px.splits = splits;
-    pw.b = x.o;
+    pw.b = b.x;
     pw.M = n; pw.N = a.K; pw.K = a.R; pw.splits = plan.wparts;
-    const EpiOut<TI> ex{(TI*)a.dx, part, v0 > 0, pg, w.power, lost, {}},
-        ew{(TI*)a.dw + v0 * a.K, wpart, false, pg, x.power, {}, {}};
+    const EpiOut<TI> ex{(TI*)a.dx, part, v0 > 0, pg, b.pw, lost, {}},
+        ew{(TI*)a.dw + v0 * a.K, wpart, false, pg, b.px, {}, {}};
     typedef Tile<T, 2, 2, 2, 2, PL, kPanelCols, kCols> WFew;  // (of four wavefronts, as dx's)
     if (plan.big)
       launch_pair<Tile<T, 4, 2, 2, 4, PL, kPanelRows, kCols>, Tile<T, 4, 2, 2, 4, PL, kPanelCols, kCols>>(px, ex, pw, ew, s, what);
@@ -846,7 +951,7 @@ size_t backward(const LinearCE& a, void* wsp, int cus, hipStream_t s) {
     else
       launch_pair<Tile<T, 1, 1, 1, 4, PL, kPanelRows, kCols>, WFew>(
           px, ex, pw,
-          EpiOut<TI, true>{ew.out, nullptr, false, pg, x.power, {},
+          EpiOut<TI, true>{ew.out, nullptr, false, pg, b.px, {},
                            {(int)a.R, rows, (const TI*)a.x, a.ldx, v0, a.targets, wide, pg}}, s, what);
   }
   auto sum = [&](const float* of, int parts, int64_t n, const float2* power, const Lost<TI>& back, void* out) {
@@ -858,8 +963,8 @@ size_t backward(const LinearCE& a, void* wsp, int cus, hipStream_t s) {
     else go(sum_parts_kernel<TI, 1>, 1);
     check_launch(what);
   };
-  if (parted) sum(part, splits, a.R * a.K, w.power, lost, a.dx);
-  if (wpart) sum(wpart, plan.wparts, a.V * a.K, x.power, {}, a.dw);
+  if (parted) sum(part, splits, a.R * a.K, b.pw, lost, a.dx);
+  if (wpart) sum(wpart, plan.wparts, a.V * a.K, b.px, {}, a.dw);
   return ws.used;
 }
 

@@ -184,6 +184,7 @@ __global__ void __launch_bounds__(256) start_kernel(Mats in, Mats mom, float bet
 // A (or B = b A + c A A) of a tile, and its mirror image.
 template <bool POLY>
 struct EpiGram {
+  static constexpr bool kFull = false;
   const half_t* a;  // POLY
   half_t* out;
   int64_t ld, batch;  // rows ld apart, matrices batch apart
@@ -235,6 +236,7 @@ struct EpiGram {
 // are not aligned.
 template <typename TO, bool F32, int NEXT>
 struct EpiUpdate {
+  static constexpr bool kFull = false;
   const half_t* from;  // the step's planes, rows ld apart
   int64_t ld;
   Kept keep;

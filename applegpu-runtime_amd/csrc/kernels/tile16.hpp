@@ -69,6 +69,12 @@ struct Args {
   int splits = 1, batches = 1;
   int stages = 0, per_split = 0;
   const float2* b_power = nullptr;  // what fp32 rows of b are multiplied by before they are split (.x)
+  // Products of planes whose epilogue allows it (kFull): where *full is not 0,
+  // the fp32 operands themselves instead, laid out as the layouts say, ld and
+  // panels counted in fp32 values.
+  const int* full = nullptr;
+  const float *fa = nullptr, *fb = nullptr;
+  int64_t lda = 0, ldb = 0;
 };
 
 // An offset behind the end of every resource: what is copied from there is
@@ -403,6 +409,75 @@ struct Tile {
     }
   }
 
+  // 4 fp32 values k .. k + 3 of an operand's row m, zeros from `end` on.
+  template <Layout LAY>
+  static __device__ __forceinline__ void fetch(const float* p, int64_t ld, int64_t m, int64_t k, int64_t end,
+                                               float (&v)[4]) {
+    if constexpr (LAY == kCols || LAY == kPanelCols) {
+      const float* at = LAY == kCols ? p + k * ld + m : p + (m >> 5) * ld + k * 32 + (m & 31);
+      const int64_t apart = LAY == kCols ? ld : 32;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) v[q] = k + q < end ? at[q * apart] : 0.f;
+    } else {
+      const float* at = LAY == kPanelRows ? p + (k >> 5) * ld + m * 32 + (k & 31) : p + m * ld + k;
+      if (k + 4 <= end) __builtin_memcpy(v, at, 16);  // (at any alignment)
+      else
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] = k + q < end ? at[q] : 0.f;
+    }
+  }
+  // The same product of the fp32 operands themselves (p.full), whatever their
+  // sizes: v_mfma_f32_32x32x2, whose lanes take 4 k of 8 in turn, straight from
+  // memory, the next 8 k under way meanwhile (1023 x 50257 x 768: 1730 us without,
+  // 962 with; planes 313).
+  static __device__ __forceinline__ void product_full(const Args& p, const Place& c, Acc& acc) {
+    const int64_t k0 = (int64_t)c.split * p.per_split * KS, past = k0 + (int64_t)p.per_split * KS;
+    const int64_t end = past < p.K ? past : p.K;
+    const int hi = c.lane >> 5;
+    int64_t am[TM], bn[TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      const int64_t m = c.m0 + (c.wm * TM + i) * 32 + (c.lane & 31);
+      am[i] = m < p.M ? m : p.M - 1;  // (rows behind the last are not stored)
+    }
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      const int64_t n = c.n0 + (c.wn * TN + j) * 32 + (c.lane & 31);
+      bn[j] = n < p.N ? n : p.N - 1;
+    }
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+    float a[2][TM][4], b[2][TN][4];
+    auto read = [&](int set, int64_t k) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < TM; ++i) fetch<AL_>(p.fa, p.lda, am[i], k + 4 * hi, end, a[set][i]);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) fetch<BL_>(p.fb, p.ldb, bn[j], k + 4 * hi, end, b[set][j]);
+    };
+    auto mul = [&](int set) __attribute__((always_inline)) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int j = 0; j < TN; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(b[set][j][q], a[set][i][q], acc[i][j], 0, 0, 0);
+    };
+    // (zeros from the end on)
+    read(0, k0);
+#pragma unroll 1
+    for (int64_t k = k0; k < end; k += 16) {
+      read(1, k + 8);
+      mul(0);
+      read(0, k + 16);
+      mul(1);
+    }
+  }
+
   // The accumulators hold C transposed: lane l, register e of a 32 x 32 tile
   // is row l % 32, column 8 (e / 4) + 4 (l / 32) + e % 4.
   static __device__ __forceinline__ int row_of(const Place& c, int i) { return (c.wm * TM + i) * 32 + (c.lane & 31); }
@@ -515,7 +590,10 @@ template <class TL, class Epi>
 __device__ __forceinline__ void tile_block(const Args& p, const Epi& e, typename TL::T* lds, int block, int blocks) {
   const Place c = TL::place(p, block, blocks);
   typename TL::Acc acc;
-  TL::product(p, c, lds, acc);
+  bool full = false;
+  if constexpr (TL::PL == 2 && Epi::kFull) full = *p.full != 0;
+  if (full) TL::product_full(p, c, acc);
+  else TL::product(p, c, lds, acc);
   e.template form<TL>(p, c, acc);
   e.template store<TL>(p, c, lds, acc);
 }

@@ -109,7 +109,7 @@ def test_rows_without_weight_and_without_a_loss(gpu, R, bad, dtype):
                 np.testing.assert_array_equal(a.to_numpy(), b)
 
 
-@pytest.mark.parametrize("dtype", ["bfloat16"])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 def test_a_row_that_overflows_is_left_out_by_its_weight(gpu, dtype):
     """The same from the forward pass: finite values whose products overflow."""
     rng = np.random.default_rng(1)
@@ -131,3 +131,97 @@ def test_a_row_that_overflows_is_left_out_by_its_weight(gpu, dtype):
     for a, b in ((loss[rest], want[0][rest]), (lse[rest], want[1][rest]), (dx[rest], want[2][rest]), (dw, want[3])):
         np.testing.assert_allclose(a, b, rtol=1e-5, atol=1e-5 * np.abs(b).max())
     assert (dx[4] == 0).all()
+
+
+# ── float32 operands whose rows are far apart ───────────────────────────────
+# Rows hold 22 bits of each value and no less than 2^-24 of the row's largest;
+# where rows are further apart than that allows, 24 bits.  Sums of K products:
+# one rounding each at most.
+def _far_logit_bar(x, w):
+    ax, aw = np.abs(x).astype(np.float64), np.abs(w).astype(np.float64)
+    held = 2.0 ** -24 * (ax.max(1)[:, None] * aw.sum(1)[None, :] + ax.sum(1)[:, None] * aw.max(1)[None, :])
+    return (x.shape[1] + 16) * 2.0 ** -24 * (ax @ aw.T) + 3 * 2.0 ** -22 * (ax @ aw.T) + held
+
+
+def _far_check(gpu, x, w, t, g, seen):
+    """Loss and gradient of the rows with weight, by the words in `seen` (the
+    others are ruled out: p is 0)."""
+    dev = [_dev(gpu, x), _dev(gpu, w), gpu.from_numpy(t)]
+    out = gpu.linear_cross_entropy(*dev)
+    dx, dw = (a.to_numpy().astype(np.float64) for a in gpu.linear_cross_entropy_backward(_dev(gpu, g), *dev, *out))
+    loss, lse = (a.to_numpy() for a in out)
+    rows = np.flatnonzero(g)
+    place = np.full(len(w), -100)
+    place[seen] = np.arange(len(seen))
+    xs, ws, ts = x[rows], w[seen], place[t[rows]]
+    want = O.linear_cross_entropy(xs, ws, ts)
+    z = _far_logit_bar(xs, ws)
+    top = z.max(1)
+    bar = 2 * top + 24 * 2.0 ** -20
+    assert (np.abs(loss[rows] - want[0]) <= bar * np.minimum(1.0, 2 * want[0]) * np.exp(2 * top) + 2.0 ** -23 * want[0]).all()
+    assert (np.abs(lse[rows] - want[1]) <= top + 21 * 2.0 ** -20 + 2.0 ** -23 * np.abs(want[1])).all()
+    rdx, rdw = O.linear_cross_entropy_backward(xs, ws, ts, g[rows])
+    d = np.abs(O.logit_gradients(xs, ws, ts, g[rows]))
+    d_err = d * (z + top[:, None] + 46 * 2.0 ** -20 + 2.0 ** -23 * np.abs(want[1])[:, None]) + 2.0 ** -37 * g.max()
+    ax, aw = np.abs(xs).astype(np.float64), np.abs(ws).astype(np.float64)
+    sums = (len(seen) + len(rows) + 48) * 2.0 ** -24 + 3 * 2.0 ** -22
+    # a value of an operand is off by at most 2^-24 of its row's largest
+    bx = d_err @ aw + sums * (d @ aw) + 2.0 ** -24 * (d @ aw.max(1))[:, None]
+    bw = d_err.T @ ax + sums * (d.T @ ax) + 2.0 ** -24 * (d.T @ ax.max(1))[:, None]
+    assert (np.abs(dx[rows] - rdx) <= bx).all()
+    assert (np.abs(dw[seen] - rdw) <= bw).all()
+    rest = np.setdiff1d(np.arange(len(w)), seen)
+    assert (dw[rest] == 0).all() and (dx[g == 0] == 0).all()
+
+
+FAR = [(1, 8, 5), (5, 33, 70), (40, 48, 300), (64, 100, 257), (200, 64, 1000), (330, 40, 600), (513, 129, 130), (3000, 20, 40)]
+
+
+@pytest.mark.parametrize("R,K,V", FAR)
+@pytest.mark.parametrize("far", [2.0 ** 13, 2.0 ** 20, 2.0 ** 27, 2.0 ** 40, 2.0 ** 100])
+def test_one_row_far_above_the_others(gpu, R, K, V, far):
+    """What a padding row holds takes nothing from the other rows."""
+    rng = np.random.default_rng(R + K)
+    x, w = rng.standard_normal((R + 1, K)).astype(np.float32), rng.standard_normal((V, K)).astype(np.float32)
+    t, g = rng.integers(0, V, R + 1).astype(np.int32), (rng.random(R + 1) / R + 0.01).astype(np.float32)
+    x[R // 2] *= np.float32(far)
+    t[R // 2], g[R // 2] = -100, 0
+    _far_check(gpu, x, w, t, g, np.arange(V))
+
+
+@pytest.mark.parametrize("R,K,V", FAR)
+@pytest.mark.parametrize("far", [2.0 ** 13, 2.0 ** 20, 2.0 ** 27, 2.0 ** 40, 2.0 ** 100])
+def test_one_word_far_below_the_others(gpu, R, K, V, far):
+    """A word that large values rule out in every row."""
+    rng = np.random.default_rng(R + K + 1)
+    x, w = rng.standard_normal((R, K)).astype(np.float32), rng.standard_normal((V + 1, K)).astype(np.float32)
+    t, g = rng.integers(0, V, R).astype(np.int32), (rng.random(R) / R + 0.01).astype(np.float32)
+    x[:, 0] = np.abs(x[:, 0]) + 0.5
+    w[V] = 0
+    w[V, 0] = -far
+    _far_check(gpu, x, w, t, g, np.arange(V))
+
+
+@pytest.mark.parametrize("R,K,V", FAR)
+def test_rows_far_below_the_others(gpu, R, K, V):
+    """Rows and words of 2^-30 of the others keep their bits."""
+    rng = np.random.default_rng(R + K + 2)
+    x, w = rng.standard_normal((R, K)).astype(np.float32), rng.standard_normal((V, K)).astype(np.float32)
+    t, g = rng.integers(0, V, R).astype(np.int32), (rng.random(R) / R + 0.01).astype(np.float32)
+    x[::3] *= np.float32(2.0 ** -30)
+    w[1::5] *= np.float32(2.0 ** -30)
+    _far_check(gpu, x, w, t, g, np.arange(V))
+
+
+@pytest.mark.parametrize("R", [3, 200, 400])
+def test_words_ruled_out_in_float32(gpu, R):
+    """A float32 weight row that gives -inf has no part in the sum either."""
+    rng = np.random.default_rng(R)
+    x, w = np.abs(rng.standard_normal((R, 16))).astype(np.float32) + 0.25, rng.standard_normal((40, 16)).astype(np.float32)
+    w[7] = -np.inf
+    t = np.where(np.arange(R) % 3 == 0, 7, np.where(np.arange(R) % 3 == 1, 8, -100)).astype(np.int32)
+    loss, lse = (a.to_numpy() for a in gpu.linear_cross_entropy(_dev(gpu, x), _dev(gpu, w), gpu.from_numpy(t)))
+    want = O.linear_cross_entropy(x, np.delete(w, 7, 0), np.where(t == 8, 7, -100))
+    np.testing.assert_allclose(lse, want[1], rtol=1e-6, atol=1e-5)
+    np.testing.assert_allclose(loss[t != 7], want[0][t != 7], rtol=1e-5, atol=1e-5)
+    assert np.isposinf(loss[t == 7]).all()
