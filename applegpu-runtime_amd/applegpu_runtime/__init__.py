@@ -698,8 +698,7 @@ def linear_cross_entropy(x, weight, targets):
     targets [...] (int32 or int64), (loss, lse), float32 [...], where lse = log
     sum exp(logits) and loss = lse - logits[target].  A target outside [0, V)
     (padding) has loss 0.  A nearly certain word's loss keeps its digits.  A
-    row with a logit of NaN or +inf gives NaN; logits beyond 2.3e38 count as
-    infinite.
+    row with a logit of NaN or +inf gives NaN.
 
     Products are summed in float32, one after another along K.  float32 operands
     count with 22 bits of each value down to 2^-16 of the operand's largest, and

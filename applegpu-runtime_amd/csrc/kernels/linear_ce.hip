@@ -39,13 +39,17 @@ constexpr float kInf = __builtin_inff();
 
 __device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 
-// A sum of exponentials as {c, s}: s 2^c, c the largest exponent; no term:
-// {-inf, 0}.  An exponent is z log2(e) - c in one fused operation, whatever c
-// was rounded to.
+// A sum of exponentials as {m, s}: s exp(m), m the largest logit; no term:
+// {-inf, 0}.
 __device__ __forceinline__ float2 join(float2 a, float2 b) {
   const float m = fmaxf(a.x, b.x), ref = m == -kInf ? 0.f : m;
-  return make_float2(m, a.y * __builtin_amdgcn_exp2f(a.x - ref) + b.y * __builtin_amdgcn_exp2f(b.x - ref));
+  return make_float2(m, a.y * exp_fast(a.x - ref) + b.y * exp_fast(b.x - ref));
 }
+// Logits past this are subtracted before they are multiplied by log2(e).  Up to
+// it z log2(e) - c is one fused operation, for c = m log2(e) rounded, and the sum
+// is multiplied by what c was rounded by (a step of c is 2^-3 here; it is 512 at
+// 2^33, and 2 to that power no number).
+constexpr float kFused = 0x1p20f;
 
 // ── powers of two that bring values into fp16's range ─────────────────────
 // {2^s, 2^-s} with the largest magnitude times 2^s in [2^13, 2^14); {1, 1}
@@ -234,7 +238,7 @@ struct EpiLoss {
   bool wide;
   const Scales* scales;  // fp32
   static constexpr bool kFull = true;
-  // the accumulators' first registers take a row's {c, s}
+  // the accumulators' first registers take a row's {m, s}
   template <class TL>
   __device__ __forceinline__ void form(const Args& p, const Place& c, typename TL::Acc& acc) const {
     constexpr int TM = TL::TM, TN = TL::TN;
@@ -280,12 +284,19 @@ struct EpiLoss {
       for (int e = 1; e < TN * 16; ++e) m = fmaxf(m, z[e]);
       m = fmaxf(m, __shfl_xor(m, 32));
       // (a NaN is no maximum but makes the sum NaN, and so does +inf)
-      m = m > -kInf ? m * kLog2e : -kInf;
-      const float ref = m > -kInf ? m : 0.f;
+      if (!(m > -kInf)) m = -kInf;
+      const bool large = m > -kInf && fabsf(m) > kFused, fused = m > -kInf && !large;
+      const float c2 = fused ? m * kLog2e : 0.f, lost = fused ? fmaf(m, kLog2e, -c2) : 0.f;
+      if (__any(large)) {
+        const float ref = large ? m : 0.f;
+#pragma unroll
+        for (int e = 0; e < TN * 16; ++e) z[e] -= ref;
+      }
       float s = 0.f;
 #pragma unroll
-      for (int e = 0; e < TN * 16; ++e) s += __builtin_amdgcn_exp2f(fmaf(z[e], kLog2e, -ref));
+      for (int e = 0; e < TN * 16; ++e) s += __builtin_amdgcn_exp2f(fmaf(z[e], kLog2e, -c2));
       s += __shfl_xor(s, 32);
+      s *= __builtin_amdgcn_exp2f(-lost);
       acc[i][0][0] = m;
       acc[i][0][1] = s;
     }
@@ -323,22 +334,21 @@ __global__ void __launch_bounds__(256) loss_kernel(const float2* part, int64_t p
     if (y < h) red[threadIdx.x] = a = join(a, red[threadIdx.x + h * rx]);
   }
   if (y != 0 || row >= R) return;
-  constexpr float kLn2 = 0.69314718055994531f;
   float out = 0.f, sum;
   if (target_of(targets, wide, row, V) < 0) {
-    sum = (a.x + log2f(a.y)) * kLn2;
+    sum = a.x + logf(a.y);
   } else {
     // log(exp z_t + the others), from the larger of the two
-    const float z = zt[row], q = z * kLog2e;
-    if (q == kInf) {
-      out = sum = kInf - q;  // an infinite sum has no certain word: NaN
-    } else if (q >= a.x) {
-      out = log1pf(a.y * exp2f(fmaf(-z, kLog2e, a.x)));
+    const float z = zt[row];
+    if (z == kInf) {
+      out = sum = kInf - z;  // an infinite sum has no certain word: NaN
+    } else if (z >= a.x) {
+      out = log1pf(a.y * expf(a.x - z));
       sum = z + out;
     } else {
-      const float others = log2f(a.y + exp2f(fmaf(z, kLog2e, -a.x)));
-      out = (fmaf(-z, kLog2e, a.x) + others) * kLn2;
-      sum = (a.x + others) * kLn2;
+      const float others = logf(a.y + expf(z - a.x));
+      out = (a.x - z) + others;
+      sum = a.x + others;
     }
   }
   loss[row] = out;
@@ -462,14 +472,27 @@ struct EpiGrad {
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
       const bool none = of[i].y == 0.f && of[i].z == 0.f;  // without weight: no gradient, whatever the logits are
+      auto p_times_weight = [&](float at, float most) {
+        float z = at;
+        if constexpr (PL == 2) z = z * ux * uw;
+        z -= of[i].x;
+        return exp_fast(z > most ? most : z) * of[i].y;
+      };
+      // a logit may pass a large sum by what either was rounded by, but p is no
+      // more than 1
+      const bool large = fabsf(of[i].x) > kFused;
+      if (__any(large)) {
+        const float most = large ? 0.f : kInf;
 #pragma unroll
-      for (int j = 0; j < TN; ++j)
+        for (int j = 0; j < TN; ++j)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float z = acc[i][j][e];
-          if constexpr (PL == 2) z = z * ux * uw;
-          acc[i][j][e] = none ? 0.f : exp_fast(z - of[i].x) * of[i].y;
-        }
+          for (int e = 0; e < 16; ++e) acc[i][j][e] = none ? 0.f : p_times_weight(acc[i][j][e], most);
+      } else {
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[i][j][e] = none ? 0.f : p_times_weight(acc[i][j][e], kInf);
+      }
       if (rel[i] >= 0 && !none) {
 #pragma unroll
         for (int j = 0; j < TN; ++j)

@@ -225,3 +225,66 @@ def test_words_ruled_out_in_float32(gpu, R):
     np.testing.assert_allclose(lse, want[1], rtol=1e-6, atol=1e-5)
     np.testing.assert_allclose(loss[t != 7], want[0][t != 7], rtol=1e-5, atol=1e-5)
     assert np.isposinf(loss[t == 7]).all()
+
+
+# ── logits that are large and finite ────────────────────────────────────────
+def _large(R, V, size, dtype, twice, seed):
+    """Operands whose logits are exact: up to `size` in most rows and a sixteenth
+    of it apart, ordinary in one.  The largest word is there twice or once."""
+    if dtype == "float16" and size > 2.0 ** 31:
+        size = 2.0 ** 29
+    root = 2.0 ** (np.floor(np.log2(size)) // 2)
+    rng = np.random.default_rng(seed)
+    x, w = np.zeros((R, 8)), np.zeros((V, 8))
+    x[:, 0] = root
+    w[:, 0] = root * rng.choice([-0.75, -0.5, -0.25, 0.0, 0.25, 0.5], V)
+    words = rng.permutation(V)
+    top, low = words[:2], words[2]
+    w[top if twice else top[:1], 0] = root
+    if not twice:
+        w[low, 0] = -root              # the one that is the largest of the row that looks the other way
+    x[R // 3, 0] = -root
+    x[R // 2, :2] = 0, 1.0             # a row of ordinary logits
+    w[:, 1] = rng.integers(-3, 4, V)
+    t = np.where(np.arange(R) % 3 == 0, top[0], rng.integers(0, V, R)).astype(np.int32)
+    return x.astype(np.float32), w.astype(np.float32), t, rng
+
+
+SIZES = [2.0 ** 15, 2.0 ** 21, 2.0 ** 24, 2.0 ** 31, 2.0 ** 60, 1e38]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("size", SIZES)
+@pytest.mark.parametrize("R,V", [(2, 3), (5, 900), (70, 300), (700, 130)])
+def test_large_logits(gpu, R, V, size, dtype):
+    """Losses and sums to their own rounding and that of the exponentials, 2^-20
+    (1 + |d|) for exponents of up to 6 (the logits are exact); where two words
+    share the largest, each has a loss of log 2."""
+    x, w, t, _ = _large(R, V, size, dtype, True, R + V)
+    loss, lse = (a.to_numpy() for a in gpu.linear_cross_entropy(_dev(gpu, x, dtype), _dev(gpu, w, dtype),
+                                                                gpu.from_numpy(t)))
+    want = O.linear_cross_entropy(x, w, t)
+    np.testing.assert_allclose(lse, want[1], rtol=2.0 ** -20, atol=7 * 2.0 ** -20)
+    np.testing.assert_allclose(loss, want[0], rtol=2.0 ** -20, atol=7 * 2.0 ** -20)
+    top = [r for r in range(0, R, 3) if x[r, 0] > 0]
+    np.testing.assert_allclose(loss[top], np.log(2), rtol=2.0 ** -19)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("size", SIZES)
+@pytest.mark.parametrize("R,V", [(2, 3), (5, 900), (70, 300), (700, 130)])
+def test_gradient_of_large_logits(gpu, R, V, size, dtype):
+    """One word is the largest by far: p is 0 or 1 but in the row of ordinary
+    logits, whose p is off by its exponent's and the sum's 7 2^-20 each; d and the
+    results are rounded once each."""
+    x, w, t, rng = _large(R, V, size, dtype, False, R + V)
+    g = (rng.random(R) + 0.5).astype(np.float32)
+    dev = [_dev(gpu, x, dtype), _dev(gpu, w, dtype), gpu.from_numpy(t)]
+    dx, dw = (a.to_numpy().astype(np.float64) for a in
+              gpu.linear_cross_entropy_backward(_dev(gpu, g), *dev, *gpu.linear_cross_entropy(*dev)))
+    d = O.logit_gradients(x, w, t, g)
+    half = {"float32": 2.0 ** -22, "float16": 2.0 ** -11, "bfloat16": 2.0 ** -8}[dtype]
+    tiny = 2.0 ** -25 if dtype == "float16" else 0.0
+    for got, want, of in ((dx, d @ w, np.abs(d) @ np.abs(w)), (dw, d.T @ x, np.abs(d).T @ np.abs(x))):
+        fits = np.abs(want) < {"float16": 65504.0}.get(dtype, 3.3e38)   # (a sum past the type is infinite)
+        assert (np.abs(got - want) <= of * (2 * half + 2.0 ** -16) + tiny)[fits].all()
