@@ -89,6 +89,7 @@ struct Arena {
   std::map<size_t, std::vector<Buffer*>> free;
   bool capturing = true;
   size_t bytes = 0;
+  uint64_t first_tensor = 0;  // ids from here on were given during the capture
 };
 
 struct PoolStats {
@@ -115,6 +116,8 @@ class Pool {
   void end_capture();
   void release_arena(Arena* a);
   bool capturing();
+  // The first tensor id given during the active capture; 0: there is none.
+  uint64_t capture_start();
 
  private:
   void release(Buffer* b);
@@ -200,7 +203,7 @@ class Runtime {
   size_t memory_usage();
   uint64_t find_by_data_ptr(const void* p);
   void replace(uint64_t id, TensorP t);
-  std::vector<TensorP> pending();        // the registered tensors that wait for their ops
+  std::vector<std::pair<uint64_t, TensorP>> pending();  // the registered tensors that wait for their ops
 
   std::recursive_mutex& big_lock() { return big_; }
 

@@ -326,7 +326,7 @@ int32_t applegpu_muon_step(const uint64_t* weight_ids, const uint64_t* momentum_
       written.push_back(w.back());
       written.push_back(m.back());
     }
-    eval_uses(written);
+    eval_uses("muon_step", written);
     ops::MuonStep o;
     o.lr = lr; o.beta = beta; o.decay = weight_decay; o.eps = eps;
     o.nesterov = nesterov != 0;

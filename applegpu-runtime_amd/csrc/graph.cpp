@@ -390,12 +390,13 @@ void eval_cache_uses(const std::vector<TensorP>& cache, bool appends_only) {
   eval_all(before);
 }
 
-void eval_uses(const std::vector<TensorP>& written) {
+void eval_uses(const char* name, const std::vector<TensorP>& written) {
   std::unordered_set<const Buffer*> bufs;
   for (const TensorP& t : written) bufs.insert(t->buf.get());
   std::unordered_map<const Node*, bool> seen;  // whether a node's values come from one of them
   std::vector<TensorP> roots;
-  for (const TensorP& t : Runtime::get().pending()) {
+  const uint64_t during = Runtime::get().pool().capture_start();
+  for (const auto& [id, t] : Runtime::get().pending()) {
     // a walk without recursion: a recorded chain can be long
     std::vector<std::pair<const Node*, size_t>> todo{{t->node.get(), 0}};
     while (!todo.empty()) {
@@ -416,7 +417,11 @@ void eval_uses(const std::vector<TensorP>& written) {
         else if (it->second) seen[n] = true;
       }
     }
-    if (seen[t->node.get()]) roots.push_back(t);
+    if (!seen[t->node.get()]) continue;
+    if (id < during)
+      fail("%s: tensor %llu, recorded before the graph capture, reads what is written; evaluate it first", name,
+           (unsigned long long)id);
+    roots.push_back(t);
   }
   if (!roots.empty()) eval_all(roots);
 }

@@ -52,8 +52,9 @@ std::vector<TensorP> record_op(int code, const std::vector<TensorP>& in, const s
 void eval_cache_uses(const std::vector<TensorP>& cache, bool appends_only);
 
 // Runs what was recorded and reads the storage of one of these tensors, which
-// are about to be written in place.
-void eval_uses(const std::vector<TensorP>& written);
+// `name` is about to write in place.  During a capture nothing runs: what was
+// recorded before it is refused.
+void eval_uses(const char* name, const std::vector<TensorP>& written);
 
 // Materialise a pending tensor (no-op when it already has storage).
 void eval(const TensorP& t);

@@ -276,6 +276,7 @@ void Pool::release(Buffer* b) {
 void Pool::begin_capture(Arena* a) {
   std::lock_guard<std::mutex> g(mu_);
   if (active_) fail("a graph capture is already active");
+  a->first_tensor = next_tensor_id();
   active_ = a;
 }
 
@@ -288,6 +289,11 @@ void Pool::end_capture() {
 bool Pool::capturing() {
   std::lock_guard<std::mutex> g(mu_);
   return active_ != nullptr;
+}
+
+uint64_t Pool::capture_start() {
+  std::lock_guard<std::mutex> g(mu_);
+  return active_ ? active_->first_tensor : 0;
 }
 
 void Pool::release_arena(Arena* a) {
@@ -496,11 +502,11 @@ void Runtime::replace(uint64_t id, TensorP t) {
   tensors_[id] = std::move(t);
 }
 
-std::vector<TensorP> Runtime::pending() {
+std::vector<std::pair<uint64_t, TensorP>> Runtime::pending() {
   std::lock_guard<std::mutex> g(reg_mu_);
-  std::vector<TensorP> r;
+  std::vector<std::pair<uint64_t, TensorP>> r;
   for (const auto& e : tensors_)
-    if (e.second->pending()) r.push_back(e.second);
+    if (e.second->pending()) r.emplace_back(e.first, e.second);
   return r;
 }
 

@@ -289,8 +289,9 @@ int32_t applegpu_kv_write_int8(uint64_t k_codes_id, uint64_t k_scales_id, uint64
  * one float dtype, momenta float32, all stored apart): momentum = beta momentum
  * + grad, U = grad + beta momentum (nesterov) or momentum, weight = (1 - lr
  * weight_decay) weight - lr sqrt(max(1, rows / cols)) orthogonalize(U).  What
- * was recorded on the weights or momenta is evaluated first.  Returns 0, or -1
- * with the error set. */
+ * was recorded on the weights or momenta is evaluated first; during a capture,
+ * what was recorded on them before it is an error.  Returns 0, or -1 with the
+ * error set. */
 int32_t applegpu_muon_step(const uint64_t* weight_ids, const uint64_t* momentum_ids, const uint64_t* grad_ids, uint32_t n,
                            double lr, double beta, double weight_decay, int32_t nesterov, int64_t steps, double eps);
 
