@@ -65,6 +65,21 @@ __device__ __forceinline__ void put_run(E* at, const Run<E>& r, int n) {
   }
 }
 
+// U times `pre` over `by` is X: |U| + eps, from the sum of U's squares, and a
+// power of two where that has no float32 or few bits of one.
+struct Norm {
+  float pre, by;
+};
+__device__ __forceinline__ Norm norm_of(double squares, float eps) {
+  const double root = sqrt(squares);
+  const float norm = (float)root + eps;
+  Norm n{1.f, norm > 0.f || norm != norm ? norm : 1.f};  // a matrix of zeros stays one
+  if (norm > 0.f && norm < 0x1p-100f) n.pre = 0x1p64f;
+  else if (norm == __builtin_inff() && root < __builtin_inf()) n.pre = 0x1p-64f;
+  if (n.pre != 1.f) n.by = (float)((root + (double)eps) * (double)n.pre);
+  return n;
+}
+
 constexpr int kNormParts = 128;  // blocks a matrix for its norm
 
 // Of matrix blockIdx.y: the sum of U's squares in kNormParts parts, and with
@@ -135,8 +150,7 @@ __global__ void __launch_bounds__(256) start_kernel(Mats in, Mats mom, float bet
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
   }
   __syncthreads();
-  const float norm = (float)sqrt(red[0] + red[1]) + eps;
-  const float by = norm > 0.f || norm != norm ? norm : 1.f;  // a matrix of zeros stays one
+  const Norm norm = norm_of(red[0] + red[1], eps);
   const int chunks = (int)(ld / (8 * PL));
   constexpr int kAtOnce = 2;
   const int64_t total = m * chunks, apart = (int64_t)gridDim.x * 256;
@@ -164,7 +178,7 @@ __global__ void __launch_bounds__(256) start_kernel(Mats in, Mats mom, float bet
       for (int e = 0; e < 8; ++e) {
         float u = to_f(gv[q].e[e]);
         if constexpr (MOM) u = nesterov ? u + beta * bv[q].e[e] : bv[q].e[e];
-        v[e] = u / by * kUnit;
+        v[e] = u * norm.pre / norm.by * kUnit;
       }
       put_planes<half_t, PL>(planes + r * ld, col[q], v);
       if constexpr (F32) {
@@ -646,12 +660,11 @@ __global__ void __launch_bounds__(64 * kSmallWaves, 2) small_kernel(Orthogonaliz
   sum = 0.0;
 #pragma unroll
   for (int w = 0; w < kSmallWaves; ++w) sum += red[w];
-  const float norm = (float)sqrt(sum) + a.eps;
-  const float by = norm > 0.f || norm != norm ? norm : 1.f;  // a matrix of zeros stays one
+  const Norm norm = norm_of(sum, a.eps);
 #pragma unroll
   for (int q = 0; q < 2; ++q)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) v[q][e] = v[q][e] / by * kUnit;
+    for (int e = 0; e < 16; ++e) v[q][e] = v[q][e] * norm.pre / norm.by * kUnit;
   auto put = [&](const Flat& f, const float (&w)[16], int t, int wide) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
