@@ -11,9 +11,10 @@
 // with one launch each for all matrices of a batch (two, where tiles are cut).
 //
 // Precision: products are of fp16 with fp32 sums, of one plane or of two (22
-// bits), see planes_of.  All entries are at most about
-// 1.3 in magnitude (singular values stay below 1.2), so X, A and B are held
-// times 2^14, where fp16 keeps 11 bits of everything down to 2^-28.  X itself
+// bits), see planes_of.  With singular values s of X below 1.2 the entries of X
+// and A stay below 1.2 and 1.5, those of B below 2.81 (b s^2 + c s^4 is -b^2 / 4c
+// at most in size, at s = 1.08): X, A and B are held times 2^14, where fp16 ends
+// at 4.0 and keeps 11 bits of everything down to 2^-28.  X itself
 // keeps more beside its planes, 22 bits for 16-bit matrices and fp32 for fp32
 // ones: a X is what carries the small singular values, multiplied by 3.4 in
 // each step, and would carry a rounding of X along (256 x 512 of rank 8 and 3 %
