@@ -742,9 +742,10 @@ def muon_step_(weights, momenta, grads, lr=0.02, beta=0.95, weight_decay=0.0, ne
     grad, U = grad + beta momentum (or the momentum, without nesterov), weight =
     (1 - lr weight_decay) weight - lr sqrt(max(1, m / n)) orthogonalize(U).
     Weights and gradients have one float dtype, momenta are float32; all are
-    stored apart.  What was asked of them before the step sees them as they
-    were, also where it is evaluated later; in a capture, what was asked of them
-    before it has to be evaluated first."""
+    stored apart.  What was computed from them before the step sees them as they
+    were, also where it is evaluated later (views share their values, packed
+    copies keep the old ones); in a capture, what was asked of them before it
+    has to be evaluated first."""
     def ids(t):
         t = [_t(x)._id for x in (t if isinstance(t, (list, tuple)) else [t])]
         return len(t), (c_uint64 * len(t))(*t)

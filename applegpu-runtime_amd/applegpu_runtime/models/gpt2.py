@@ -501,7 +501,8 @@ def gpt2_loss(model: dict, ids, grads: bool = False):
     50257 words they are 100 KB a token in 16 bits): float32 [B, T] on the
     device, entry t of token t + 1, 0 where there is none.  With grads, (loss,
     d hidden [B, T, d], d wte [V, d]) of the tokens' mean loss: what the tied
-    head hands to the rest of the model and to its table."""
+    head hands to the rest of the model and to its table.  The head's products
+    elsewhere may read packed copies of the table: see repack_table."""
     x, nxt = _text_hidden(model, ids)
     B, T = nxt.shape
     w = model["weights"]
@@ -514,6 +515,17 @@ def gpt2_loss(model: dict, ids, grads: bool = False):
     some = max(int(((nxt >= 0) & (nxt < model["config"]["vocab_size"])).sum()), 1)
     g = gpu.full([B, T], 1.0 / some, "float32")
     return (loss, *gpu.linear_cross_entropy_backward(g, x, w["transformer.wte.weight"], t, loss, lse))
+
+
+def repack_table(model: dict):
+    """Makes the packed copies of the token table (what load_model keeps beside
+    it for the head's products) anew, in place, after the table was written: a
+    step on it would otherwise be seen by the embedding and gpt2_loss alone."""
+    pk = model["packed"].get("transformer.wte.weight")
+    if pk is None:
+        return
+    wte = model["weights"]["transformer.wte.weight"]
+    gpu.blit_copy(gpu.pack_weight_x3(gpu.transpose(wte)) if pk[2] == "x3" else gpu.pack_weight(wte), pk[0])
 
 
 def gpt2_score(model: dict, ids, top_k: int = 0):
