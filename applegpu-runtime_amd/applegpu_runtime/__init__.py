@@ -714,7 +714,7 @@ def linear_cross_entropy_backward(grad_loss, x, weight, targets, loss, lse, grad
     loss and lse it returned.  The logits are formed again, in pieces of the
     vocabulary; their gradient is rounded to 16 bits before its products for
     16-bit operands (the results' errors are 1.4 times those of one rounding of
-    the results alone) and counts down to 2^-37 (bfloat16: 2^-139) of the
+    the results alone; operands cast to float32 avoid it) and counts down to 2^-37 (bfloat16: 2^-139) of the
     largest one in the call, for float32 with 22 bits down to 2^-16 of it.  Rows
     whose target is outside [0, V) get lse's part only; one without any weight
     gets zeros whatever its logits and its loss are, and has no part in dweight

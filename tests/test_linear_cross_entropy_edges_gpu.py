@@ -288,3 +288,47 @@ def test_gradient_of_large_logits(gpu, R, V, size, dtype):
     for got, want, of in ((dx, d @ w, np.abs(d) @ np.abs(w)), (dw, d.T @ x, np.abs(d).T @ np.abs(x))):
         fits = np.abs(want) < {"float16": 65504.0}.get(dtype, 3.3e38)   # (a sum past the type is infinite)
         assert (np.abs(got - want) <= of * (2 * half + 2.0 ** -16) + tiny)[fits].all()
+
+
+def test_eager_entries(gpu):
+    """The eager module's entries give the bits of the package's."""
+    from applegpu_runtime import eager as E
+    E.init()
+    rng = np.random.default_rng(8)
+    x, w = rng.standard_normal((9, 24)).astype(np.float32), rng.standard_normal((50, 24)).astype(np.float32)
+    t, g = rng.integers(-1, 50, 9).astype(np.int32), rng.random(9).astype(np.float32)
+    want = gpu.linear_cross_entropy(*map(gpu.from_numpy, (x, w, t)))
+    got = E.linear_cross_entropy(*map(E.from_numpy, (x, w, t)))
+    for a, b in zip(got, want):
+        np.testing.assert_array_equal(a.numpy(), b.to_numpy())
+    for h in (None, rng.standard_normal(9).astype(np.float32)):
+        a = E.linear_cross_entropy_backward(*map(E.from_numpy, (g, x, w, t)), *got, None if h is None else E.from_numpy(h))
+        b = gpu.linear_cross_entropy_backward(*map(gpu.from_numpy, (g, x, w, t)), *want,
+                                              grad_lse=None if h is None else gpu.from_numpy(h))
+        for u, v in zip(a, b):
+            np.testing.assert_array_equal(u.numpy(), v.to_numpy())
+    with pytest.raises(RuntimeError, match="differ in number"):
+        E.muon_step_([E.from_numpy(x)], [], [])
+    with pytest.raises(RuntimeError, match="must be float32 with one value a row"):
+        E.linear_cross_entropy_backward(*map(E.from_numpy, (g[:8], x, w, t)), *got)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_many_threads(gpu, dtype):
+    """Calls of several threads at once, with workspaces: the bits of one."""
+    from concurrent.futures import ThreadPoolExecutor
+    rng = np.random.default_rng(9)
+    x, w = rng.standard_normal((300, 64)).astype(np.float32), rng.standard_normal((2000, 64)).astype(np.float32)
+    t, g = rng.integers(-1, 2000, 300).astype(np.int32), rng.random(300).astype(np.float32)
+
+    def run(_):
+        dev = [_dev(gpu, x, dtype), _dev(gpu, w, dtype), gpu.from_numpy(t)]
+        out = gpu.linear_cross_entropy(*dev)
+        return [a.to_numpy() for a in (*out, *gpu.linear_cross_entropy_backward(_dev(gpu, g), *dev, *out),
+                                       gpu.orthogonalize(dev[1]))]
+
+    want = run(0)
+    with ThreadPoolExecutor(4) as pool:
+        for got in pool.map(run, range(12)):
+            for a, b in zip(got, want):
+                np.testing.assert_array_equal(a, b)
