@@ -730,9 +730,9 @@ def orthogonalize(g, steps=5, eps=1e-7):
     float32 sums and count 22 bits of each value for float32 matrices, 11 for
     bfloat16 ones and for float16 ones 11, then 22 in the last three steps; X
     itself keeps 22 bits beside them (float32: all).  Small matrices and those of
-    a short side in float16 have 22 bits throughout.  The result's errors beside
-    those of one rounding: 1.2 times in bfloat16.  A matrix of zeros stays
-    one."""
+    a short side in float16 have 22 bits throughout.  In bfloat16 the
+    result's errors are 1.2 times those of its own rounding; a float32 matrix
+    avoids it.  A matrix of zeros stays one."""
     return _op(b"orthogonalize", [_t(g)], f=(float(eps),), i=(int(steps),))
 
 
