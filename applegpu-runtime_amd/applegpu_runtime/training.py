@@ -83,7 +83,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     2^20 rows."""
     loss, lse = _LinearCrossEntropy.apply(x, weight, target)
     # (the library's tensors have one dimension at least)
-    return (loss, lse) if target.dim() else (loss.reshape(()), lse.reshape(()))
+    return (loss, lse) if x.dim() > 1 or target.dim() else (loss.reshape(()), lse.reshape(()))
 
 
 class Muon(torch.optim.Optimizer):

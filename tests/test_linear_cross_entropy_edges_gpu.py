@@ -227,6 +227,43 @@ def test_words_ruled_out_in_float32(gpu, R):
     assert np.isposinf(loss[t == 7]).all()
 
 
+@pytest.mark.parametrize("R,K,V", [(17000, 16, 17000), (2100, 72, 9000)])
+def test_many_rows_far_apart(gpu, R, K, V):
+    """Whole rounds of large tiles, and the vocabulary in pieces, with products of
+    the float32 values: a row of 2^40 times the others without weight, a third of
+    them of 2^-30, against float64 some rows at a time."""
+    import torch
+    rng = np.random.default_rng(R)
+    x, w = rng.standard_normal((R, K)).astype(np.float32), rng.standard_normal((V, K)).astype(np.float32)
+    t, g = rng.integers(0, V, R).astype(np.int32), rng.random(R).astype(np.float32)
+    x[::3] *= np.float32(2.0 ** -30)
+    x[R // 2] *= np.float32(2.0 ** 40)
+    t[R // 2] = -100
+    dev = [_dev(gpu, x), _dev(gpu, w), gpu.from_numpy(t)]
+    out = gpu.linear_cross_entropy(*dev)
+    dx, dw = (a.to_numpy().astype(np.float64) for a in gpu.linear_cross_entropy_backward(_dev(gpu, g), *dev, *out))
+    tw = torch.tensor(w, dtype=torch.float64)
+    loss, want_x, want_w = [], [], torch.zeros_like(tw)
+    for lo in range(0, R, 2048):
+        xi, ti = torch.tensor(x[lo:lo + 2048], dtype=torch.float64), torch.tensor(t[lo:lo + 2048]).long()
+        z = xi @ tw.t()
+        s = torch.logsumexp(z, 1)
+        there = ti >= 0
+        loss.append(torch.where(there, s - z.gather(1, ti.clamp(min=0)[:, None])[:, 0], 0.0))
+        d = torch.exp(z - s[:, None])
+        row = torch.arange(len(ti))[there]
+        d[row, ti[there]] -= 1.0
+        d *= torch.where(there, torch.tensor(g[lo:lo + 2048]).double(), 0.0)[:, None]
+        want_x.append(d @ tw)
+        want_w += d.t().contiguous() @ xi
+    np.testing.assert_allclose(out[0].to_numpy(), torch.cat(loss).numpy(), rtol=1e-5, atol=1e-5)
+    want_x = torch.cat(want_x).numpy()
+    # row by row: p's error, 46 2^-20 at most, and the sums'
+    bad = np.linalg.norm(dx - want_x, axis=1) > 1e-4 * np.linalg.norm(want_x, axis=1)
+    assert not bad.any()
+    assert np.linalg.norm(dw - want_w.numpy()) <= 1e-4 * np.linalg.norm(want_w.numpy())
+
+
 # ── logits that are large and finite ────────────────────────────────────────
 def _large(R, V, size, dtype, twice, seed):
     """Operands whose logits are exact: up to `size` in most rows and a sixteenth

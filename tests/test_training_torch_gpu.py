@@ -196,3 +196,41 @@ def test_a_run_goes_on_from_a_checkpoint(torch_dev, dtype, tmp_path):
         want = opt.state[p]["momentum"].cpu()
         assert torch.equal(want, from_file.state[a]["momentum"].cpu())
         assert torch.equal(want, from_device.state[b]["momentum"].cpu())
+
+
+def test_shapes_follow_x(torch_dev):
+    """A row with a row dimension keeps it, whatever its target's shape."""
+    torch = torch_dev
+    from applegpu_runtime.training import linear_cross_entropy
+    w = torch.randn(7, 8).to("applegpu")
+    one = torch.tensor(3).to("applegpu")
+    for x, t, shape in ((torch.randn(1, 8), one, (1,)), (torch.randn(8), one.reshape(1), (1,)), (torch.randn(8), one, ())):
+        loss, lse = linear_cross_entropy(x.to("applegpu"), w, t)
+        assert tuple(loss.shape) == tuple(lse.shape) == shape
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_nothing_is_left_behind(torch_dev, gpu, dtype):
+    """Losses, gradients and steps hand back all that they make, refused calls
+    too."""
+    torch = torch_dev
+    from applegpu_runtime.training import Muon, linear_cross_entropy
+    x, w, t = _case(12, 24, 30, dtype)
+    xd, ti = _to(torch, x, dtype).requires_grad_(), _to(torch, t, "int64")
+    p = torch.nn.Parameter(_to(torch, w, dtype))
+    opt = Muon([p], lr=0.01)
+
+    def step():
+        opt.zero_grad()
+        xd.grad = None
+        linear_cross_entropy(xd, p, ti)[0].sum().backward()
+        opt.step()
+        with pytest.raises(ValueError, match="does not match weight"):
+            linear_cross_entropy(xd, p[:, :5], ti)
+
+    for _ in range(3):
+        step()
+    count = gpu.tensor_count()
+    for _ in range(20):
+        step()
+    assert gpu.tensor_count() == count
