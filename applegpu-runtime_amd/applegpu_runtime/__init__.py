@@ -703,8 +703,9 @@ def linear_cross_entropy(x, weight, targets):
     Products are summed in float32, one after another along K.  float32 operands
     count with 22 bits of each value down to 2^-16 of the operand's largest, and
     smaller ones in steps of 2^-38 of it; where the largest values of its rows
-    are more than 2^14 apart, or one is infinite, the call multiplies float32
-    values themselves, which takes two to four times as long."""
+    are more than 2^14 apart, one is infinite or the largest of all is past 2^90
+    or below 2^-90, the call multiplies float32 values themselves, which takes
+    two to four times as long."""
     return _op(b"linear_cross_entropy", [_t(x), _t(weight), _t(targets)], nout=2)
 
 

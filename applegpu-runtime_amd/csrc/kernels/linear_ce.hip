@@ -142,8 +142,9 @@ __global__ void __launch_bounds__(256) most_kernel(Rows32 x0, Rows32 x1, Span* p
 // largest value is 2^-14 of the operand's is held to 2^-24 of that value (the
 // low plane's smallest step is 2^-38 of the operand's largest), but beside a row
 // of 2^40 times the others nothing is left of them.  Where rows are further apart
-// than 2^14, or hold an infinity, products are of the fp32 values themselves and
-// the powers are 1.  (In planes / of the values, us: loss of 61 x 50257 x 1280
+// than 2^14, or hold an infinity or nothing that a power and its inverse reach
+// (2^90: products of up to 2^47 times one operand's power stay finite), products
+// are of the fp32 values themselves and the powers are 1.  (In planes / of the values, us: loss of 61 x 50257 x 1280
 // 101 / 231, of 1023 x 50257 x 768 313 / 962; gradients 307 / 558, 733 / 2738.)
 struct Scales {
   float2 x, w;  // {2^s, 2^-s}
@@ -168,7 +169,7 @@ __device__ __forceinline__ Scales scales_of(const Span* part) {
     Span a = red[y][0];
 #pragma unroll
     for (int q = 1; q < 4; ++q) a = {fmaxf(a.most, red[y][q].most), fminf(a.least, red[y][q].least)};
-    if (!(a.most < kInf && a.most <= a.least * 0x1p14f)) s.full = 1;
+    if (!(a.most <= 0x1p90f && a.most <= a.least * 0x1p14f) || (a.most > 0.f && a.most < 0x1p-90f)) s.full = 1;
     (y ? s.w : s.x) = power_for(a.most);
   }
   if (s.full) s.x = s.w = make_float2(1.f, 1.f);
@@ -588,6 +589,12 @@ struct LostOfRows {
   }
 };
 
+// The inverse powers of a product's operands (null: 1), the smaller first: what is
+// between them is not past the result.
+__device__ __forceinline__ float2 unscale(const float2* pa, const float2* pb) {
+  const float a = pa ? pa->y : 1.f, b = pb ? pb->y : 1.f;
+  return make_float2(fminf(a, b), fmaxf(a, b));
+}
 // acc times the inverse powers, as outputs or as fp32 parts of a sum.
 template <typename TO, bool FEW = false>
 struct EpiOut {
@@ -604,7 +611,7 @@ struct EpiOut {
   }
   template <class TL>
   __device__ __forceinline__ void store(const Args& p, const Place& c, typename TL::T* lds, typename TL::Acc& acc) const {
-    const float ua = pa ? pa->y : 1.f, ub = pb ? pb->y : 1.f;
+    const float2 u = unscale(pa, pb);
     float* sums = part ? part + (int64_t)c.split * p.M * p.N : nullptr;
     TL::template runs<false>(
         c, lds, acc, false,
@@ -632,7 +639,7 @@ struct EpiOut {
           struct V { TO e[W]; } o[8 / W];
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            v[e] = v[e] * ua * ub;
+            v[e] = v[e] * u.x * u.y;
             if (back != 0.f && e < n) v[e] += back * to_f(wt[e]);
             o[e / W].e[e % W] = from_f<TO>(v[e]);
           }
@@ -688,8 +695,8 @@ __global__ void __launch_bounds__(256) sum_parts_kernel(const float* part, int s
     }
   }
   if (m <= 0) return;
-  const float ua = pa ? pa->y : 1.f, ub = pb ? pb->y : 1.f;
-  float v[4] = {a.x * ua * ub, a.y * ua * ub, a.z * ua * ub, a.w * ua * ub};
+  const float2 u = unscale(pa, pb);
+  float v[4] = {a.x * u.x * u.y, a.y * u.x * u.y, a.z * u.x * u.y, a.w * u.x * u.y};
   const TO* wt = nullptr;
   if (K % 4 == 0) {
     const int64_t r = i / K;

@@ -264,6 +264,33 @@ def test_many_rows_far_apart(gpu, R, K, V):
     assert np.linalg.norm(dw - want_w.numpy()) <= 1e-4 * np.linalg.norm(want_w.numpy())
 
 
+@pytest.mark.parametrize("R,K,V", [(5, 33, 70), (40, 48, 300), (330, 40, 600)])
+@pytest.mark.parametrize("size", [2.0 ** -124, 2.0 ** -115, 2.0 ** -100, 2.0 ** -80, 2.0 ** 80, 2.0 ** 100, 2.0 ** 115, 2.0 ** 124])
+def test_float32_of_the_ends(gpu, R, K, V, size):
+    """Operands near the ends of float32 whose products are ordinary."""
+    rng = np.random.default_rng(R + K + 3)
+    x = rng.uniform(0.5, 1.0, (R, K)).astype(np.float32) * rng.choice([-1, 1], (R, K)).astype(np.float32)
+    w = rng.uniform(0.5, 1.0, (V, K)).astype(np.float32) * rng.choice([-1, 1], (V, K)).astype(np.float32)
+    x, w = x * np.float32(size), w / np.float32(size)
+    t, g = rng.integers(0, V, R).astype(np.int32), (rng.random(R) / R + 0.01).astype(np.float32)
+    dev = [_dev(gpu, x), _dev(gpu, w), gpu.from_numpy(t)]
+    out = gpu.linear_cross_entropy(*dev)
+    loss, lse = (a.to_numpy() for a in out)
+    want = O.linear_cross_entropy(x, w, t)
+    z = _far_logit_bar(x, w).max(1)
+    bar = 2 * z + 24 * 2.0 ** -20
+    assert (np.abs(loss - want[0]) <= bar * np.minimum(1.0, 2 * want[0]) * np.exp(2 * z) + 2.0 ** -23 * want[0]).all()
+    assert (np.abs(lse - want[1]) <= z + 21 * 2.0 ** -20 + 2.0 ** -23 * np.abs(want[1])).all()
+    d = np.abs(O.logit_gradients(x, w, t, g))
+    d_err = d * (2 * z[:, None] + 46 * 2.0 ** -20 + 2.0 ** -23 * np.abs(want[1])[:, None]) + 2.0 ** -37 * g.max()
+    ax, aw = np.abs(x).astype(np.float64), np.abs(w).astype(np.float64)
+    sums = (R + V + 48) * 2.0 ** -24 + 3 * 2.0 ** -22 + 2.0 ** -24
+    got = gpu.linear_cross_entropy_backward(_dev(gpu, g), *dev, *out)
+    for a, b, e, s in zip(got, O.linear_cross_entropy_backward(x, w, t, g), (d_err @ aw, d_err.T @ ax), (d @ aw, d.T @ ax)):
+        # (results may lie below float32's normal range)
+        assert (np.abs(a.to_numpy() - b) <= e + sums * s + 2.0 ** -149 * 1024).all()
+
+
 # ── logits that are large and finite ────────────────────────────────────────
 def _large(R, V, size, dtype, twice, seed):
     """Operands whose logits are exact: up to `size` in most rows and a sixteenth
